@@ -79,6 +79,17 @@ SIGNATURES = {
     "cgnn_compressed_info": (_c_int, [_c_ptr, _c_ptr]),
     "cgnn_compressed_copy": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr]),
     "cgnn_compressed_destroy": (None, [_c_ptr]),
+    "cgnn_layer_norm": (_c_int, [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, ctypes.c_double, _c_int,
+                                 ctypes.c_double, ctypes.c_uint64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr]),
+    "cgnn_layer_norm_scratch_bytes": (_c_size, [_c_int, _c_i64, _c_i64]),
+    "cgnn_layer_norm_backward": (_c_int, [_c_int, _c_int, _c_i64, _c_i64, _c_i64] + [_c_ptr] * 6 +
+                                 [_c_int, ctypes.c_double, ctypes.c_uint64] + [_c_ptr] * 5 + [_c_size, _c_ptr]),
+    "cgnn_dropout": (_c_int, [_c_int, _c_i64, _c_ptr, _c_ptr, ctypes.c_double, ctypes.c_uint64, _c_ptr, _c_ptr, _c_ptr]),
+    "cgnn_cross_entropy_scratch_bytes": (_c_size, []),
+    "cgnn_cross_entropy": (_c_int, [_c_int, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr, _c_ptr, _c_ptr,
+                                    _c_ptr, _c_ptr, _c_size, _c_ptr]),
+    "cgnn_cross_entropy_backward": (_c_int, [_c_int, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr, _c_ptr,
+                                             _c_ptr, _c_int, _c_ptr, _c_ptr]),
 }
 
 _lib = None

@@ -629,6 +629,327 @@ Tensor transform_autograd(const Tensor &x_in, const Tensor &index, const Tensor 
 }
 
 // ---------------------------------------------------------------------------------------------
+// row operators of a training step: normalisation, dropout, loss
+// ---------------------------------------------------------------------------------------------
+int row_dtype(const Tensor &t, const char *what) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return CGNN_F32;
+        case at::kDouble: return CGNN_F64;
+        case at::kBFloat16: return CGNN_BF16;
+        case at::kHalf: return CGNN_F16;
+        default: TORCH_CHECK(false, what, ": only float32, float64, bfloat16 and float16 are supported");
+    }
+}
+
+Tensor dense(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
+
+at::ScalarType sum_type(const Tensor &t) { return t.scalar_type() == at::kDouble ? at::kDouble : at::kFloat; }
+
+// A matrix [rows, last dimension] over `t` whose rows may lie apart; anything else is made dense.
+struct Rows {
+    Tensor held;
+    int64_t rows, width, stride;
+    explicit Rows(const Tensor &t) : width(t.size(-1)) {
+        if (t.dim() == 2 && (t.stride(1) == 1 || width == 1) && t.stride(0) >= 0) {
+            held = t;
+            stride = t.stride(0);
+        } else {
+            held = t.contiguous();
+            stride = width;
+        }
+        rows = width ? held.numel() / width : 0;
+    }
+};
+
+// The engine lets the streams of a backward pass wait for those its leaves' gradients were first accumulated on.  While
+// a graph is captured that would be a wait on work outside the capture, which breaks it off (and ends the process where
+// the error meets a thread of the engine), so the call is refused before anything is recorded.
+void refuse_foreign_leaves(const char *what, at::TensorList inputs) {
+    if (!at::GradMode::is_enabled() || !capturing()) return;
+    for (const Tensor &t : inputs) {
+        if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+        const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+        if (!accumulator) continue;
+        const auto stream = accumulator->stream();
+        TORCH_CHECK(!stream || *stream == c10::cuda::getCurrentCUDAStream(t.get_device()).unwrap(), what,
+                    ": an eager graph over one of these leaves still lives, on another stream than the one being captured; "
+                    "drop its outputs before the capture, or build it on the capture's stream");
+    }
+}
+
+// The key of a dropout: a number, or one int64 on the device.  Neither given: a fresh one, inside a capture drawn by
+// the captured graph itself, so that every replay has another.
+struct Key {
+    uint64_t seed = 0;
+    Tensor on_device;
+    const int64_t *pointer() const { return on_device.defined() ? on_device.const_data_ptr<int64_t>() : nullptr; }
+};
+
+Key key_of(const char *what, double p, const c10::optional<int64_t> &seed, const c10::optional<Tensor> &seed_tensor,
+           const Tensor &like) {
+    TORCH_CHECK(p >= 0.0 && p < 1.0, "dropout probability must lie in [0, 1)");
+    Key key;
+    if (seed_tensor.has_value()) {
+        key.on_device = *seed_tensor;
+        TORCH_CHECK(key.on_device.device() == like.device() && key.on_device.scalar_type() == at::kLong &&
+                        key.on_device.numel() == 1,
+                    what, ": a seed in a tensor is one int64 on the input's device");
+    } else if (seed.has_value()) {
+        key.seed = (uint64_t)*seed;
+    } else if (p > 0.0) {
+        if (capturing())
+            key.on_device = at::randint(0, std::numeric_limits<int64_t>::max(), {1}, like.options().dtype(at::kLong).requires_grad(false));
+        else
+            key.seed = dropout_key();
+    }
+    return key;
+}
+
+struct NormSettings {
+    int dtype = 0, param_dtype = 0;
+    double eps = 0.0, p = 0.0;
+    bool relu = false;
+    uint64_t seed = 0;
+};
+
+struct LayerNormBackward : public Node {
+    SavedVariable x_, weight_, bias_, mean_, rstd_, key_;
+    NormSettings set;
+    at::TensorOptions param_options;
+    variable_list apply(variable_list &&grads) override {
+        Tensor dx, dw, db;
+        {
+            at::NoGradGuard no_grad;
+            const Tensor grad = materialized(*this, grads[0]).contiguous();
+            const c10::cuda::OptionalCUDAGuard guard(grad.device());
+            const Tensor x_in = x_.unpack(), weight = dense(weight_.unpack()), bias = dense(bias_.unpack());
+            const Tensor mean = mean_.unpack().contiguous(), rstd = rstd_.unpack().contiguous();
+            const Tensor key = dense(key_.unpack());
+            const Rows x(x_in);
+            const auto plain = grad.options().requires_grad(false);
+            if (task_should_compute_output(0)) dx = at::empty(x_in.sizes(), plain);
+            if (task_should_compute_output(1)) dw = at::empty({x.width}, param_options);
+            if (task_should_compute_output(2)) db = at::empty({x.width}, param_options);
+            Tensor scratch;
+            size_t bytes = 0;
+            if (dw.defined() || db.defined()) {
+                bytes = cgnn_layer_norm_scratch_bytes(set.dtype, x.rows, x.width);
+                scratch = at::empty({(int64_t)bytes}, plain.dtype(at::kByte));
+            }
+            check(cgnn_layer_norm_backward(set.dtype, set.param_dtype, x.rows, x.width, x.stride, data(x.held), data(weight),
+                                           data(bias), data(mean), data(rstd), data(grad), set.relu, set.p, set.seed,
+                                           static_cast<const int64_t *>(data(key)), data(dx), data(dw), data(db), data(scratch),
+                                           bytes, current_stream(grad)));
+        }
+        return first_order({dx, dw, db}, grads);
+    }
+    void release_variables() override {
+        for (SavedVariable *v : {&x_, &weight_, &bias_, &mean_, &rstd_, &key_}) v->reset_data();
+    }
+    std::string name() const override { return "CompressgnnLayerNormBackward"; }
+};
+
+Tensor layer_norm_autograd(const Tensor &x_in, const c10::optional<Tensor> &weight_in, const c10::optional<Tensor> &bias_in,
+                           double eps, bool relu, double p, const c10::optional<int64_t> &seed,
+                           const c10::optional<Tensor> &seed_tensor) {
+    const Tensor weight = weight_in.value_or(Tensor()), bias = bias_in.value_or(Tensor());
+    TORCH_CHECK(x_in.is_cuda() && x_in.dim() >= 1, "layer_norm: Expected a CUDA tensor of one dimension or more");
+    refuse_dual("the layer normalisation", {x_in, weight, bias});
+    NormSettings set;
+    set.dtype = set.param_dtype = row_dtype(x_in, "layer_norm");
+    const Tensor &either = weight.defined() ? weight : bias;
+    if (either.defined()) {
+        set.param_dtype = row_dtype(either, "layer_norm");
+        TORCH_CHECK(set.param_dtype == set.dtype || (x_in.element_size() == 2 && set.param_dtype == CGNN_F32),
+                    "layer_norm: weight and bias are of the input's type, or float32 beside a 16-bit one");
+    }
+    for (const Tensor &t : {weight, bias})
+        TORCH_CHECK(!t.defined() || (t.device() == x_in.device() && t.dim() == 1 && t.size(0) == x_in.size(-1) &&
+                                     t.scalar_type() == either.scalar_type()),
+                    "layer_norm: weight and bias are vectors over the last dimension, of one type and on the input's device");
+    TORCH_CHECK(eps >= 0.0, "layer_norm: eps must not be negative");
+    const c10::cuda::OptionalCUDAGuard guard(x_in.device());
+    const Key key = key_of("layer_norm", p, seed, seed_tensor, x_in);
+    refuse_foreign_leaves("layer_norm", {x_in, weight, bias});
+    set.eps = eps;
+    set.p = p;
+    set.relu = relu;
+    set.seed = key.seed;
+    const bool differentiated = torch::autograd::compute_requires_grad(x_in, weight, bias);
+    Tensor out, mean, rstd;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Rows x(x_in);
+        const Tensor w = dense(weight), b = dense(bias);
+        out = at::empty(x_in.sizes(), x_in.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+        if (differentiated) {
+            mean = at::empty({x.rows}, x_in.options().dtype(sum_type(x_in)).requires_grad(false));
+            rstd = at::empty_like(mean);
+        }
+        check(cgnn_layer_norm(set.dtype, set.param_dtype, x.rows, x.width, x.stride, data(x.held), data(w), data(b), eps, relu, p,
+                              key.seed, key.pointer(), data(out), data(mean), data(rstd), current_stream(x_in)));
+    }
+    if (differentiated) {
+        auto node = new_node<LayerNormBackward>();
+        node->set = set;
+        node->param_options = (either.defined() ? either : x_in).options().requires_grad(false);
+        node->x_ = SavedVariable(x_in, false);
+        node->weight_ = SavedVariable(weight, false);
+        node->bias_ = SavedVariable(bias, false);
+        node->mean_ = SavedVariable(mean, false);
+        node->rstd_ = SavedVariable(rstd, false);
+        node->key_ = SavedVariable(key.on_device, false);
+        node->set_next_edges(torch::autograd::collect_next_edges(x_in, weight, bias));
+        torch::autograd::set_history(out, node);
+    }
+    return out;
+}
+
+Tensor dropout_pass(const Tensor &x, const Tensor &residual, double p, uint64_t seed, const int64_t *device_seed) {
+    Tensor out = at::empty(x.sizes(), x.options().requires_grad(false));
+    check(cgnn_dropout(row_dtype(x, "dropout"), x.numel(), data(x), data(residual), p, seed, device_seed, data(out),
+                       current_stream(x)));
+    return out;
+}
+
+struct DropoutBackward : public Node {
+    SavedVariable key_;
+    double p = 0.0;
+    uint64_t seed = 0;
+    variable_list apply(variable_list &&grads) override {
+        Tensor dx, dresidual;
+        {
+            at::NoGradGuard no_grad;
+            const Tensor key = dense(key_.unpack());
+            const Tensor grad = materialized(*this, grads[0]);
+            const c10::cuda::OptionalCUDAGuard guard(grad.device());
+            if (task_should_compute_output(0))
+                dx = dropout_pass(grad.contiguous(), Tensor(), p, seed, static_cast<const int64_t *>(data(key)));
+            if (task_should_compute_output(1)) dresidual = grad;
+        }
+        return first_order({dx, dresidual}, grads);
+    }
+    void release_variables() override { key_.reset_data(); }
+    std::string name() const override { return "CompressgnnDropoutBackward"; }
+};
+
+Tensor dropout_autograd(const Tensor &x_in, double p, const c10::optional<Tensor> &residual_in, const c10::optional<int64_t> &seed,
+                        const c10::optional<Tensor> &seed_tensor) {
+    const Tensor residual = residual_in.value_or(Tensor());
+    TORCH_CHECK(x_in.is_cuda(), "dropout: Expected a CUDA tensor");
+    row_dtype(x_in, "dropout");
+    refuse_dual("the dropout", {x_in, residual});
+    TORCH_CHECK(!residual.defined() || (residual.device() == x_in.device() && residual.scalar_type() == x_in.scalar_type() &&
+                                        residual.sizes() == x_in.sizes()),
+                "dropout: the residual has the input's shape, type and device");
+    const c10::cuda::OptionalCUDAGuard guard(x_in.device());
+    const Key key = key_of("dropout", p, seed, seed_tensor, x_in);
+    refuse_foreign_leaves("dropout", {x_in, residual});
+    Tensor out;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        out = dropout_pass(x_in.contiguous(), dense(residual), p, key.seed, key.pointer());
+    }
+    if (torch::autograd::compute_requires_grad(x_in, residual)) {
+        auto node = new_node<DropoutBackward>();
+        node->p = p;
+        node->seed = key.seed;
+        node->key_ = SavedVariable(key.on_device, false);
+        node->set_next_edges(torch::autograd::collect_next_edges(x_in, residual));
+        torch::autograd::set_history(out, node);
+    }
+    return out;
+}
+
+// For a sum or a mean the forward pass has written the gradient for an incoming one (`unit_`).  The first backward pass
+// hands that array on, after a launch that computes it anew unless the incoming gradient is one; further passes over a
+// retained graph have an array of their own.
+struct CrossEntropyBackward : public Node {
+    SavedVariable logits_, target_, stats_, labelled_;
+    Tensor unit_;
+    int dtype = 0, reduction = 0;
+    int64_t ignore_index = 0;
+    variable_list apply(variable_list &&grads) override {
+        std::lock_guard<std::mutex> held(mutex_);
+        Tensor dlogits;
+        {
+            at::NoGradGuard no_grad;
+            const Tensor grad = materialized(*this, grads[0]).contiguous();
+            const c10::cuda::OptionalCUDAGuard guard(grad.device());
+            const Tensor logits = logits_.unpack(), target = target_.unpack().contiguous();
+            const Tensor stats = stats_.unpack().contiguous(), labelled = dense(labelled_.unpack());
+            const Rows z(logits);
+            const bool unit = unit_.defined() && !capturing();
+            if (unit) dlogits = std::move(unit_);
+            else dlogits = at::empty(logits.sizes(), logits.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+            unit_.reset();
+            check(cgnn_cross_entropy_backward(dtype, z.rows, z.width, z.stride, data(z.held), static_cast<const int64_t *>(data(target)),
+                                              ignore_index, reduction, data(stats), static_cast<const int64_t *>(data(labelled)),
+                                              data(grad), unit, data(dlogits), current_stream(grad)));
+        }
+        return first_order({dlogits}, grads);
+    }
+    void release_variables() override {
+        std::lock_guard<std::mutex> held(mutex_);
+        for (SavedVariable *v : {&logits_, &target_, &stats_, &labelled_}) v->reset_data();
+        unit_.reset();
+    }
+    std::string name() const override { return "CompressgnnCrossEntropyBackward"; }
+};
+
+Tensor cross_entropy_autograd(const Tensor &logits, const Tensor &target_in, int64_t ignore_index, int reduction) {
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.size(1) >= 1,
+                "cross_entropy: Expected a CUDA matrix [rows, classes] of class scores");
+    const int dtype = row_dtype(logits, "cross_entropy");
+    TORCH_CHECK(target_in.device() == logits.device() && target_in.scalar_type() == at::kLong && target_in.dim() == 1 &&
+                    target_in.size(0) == logits.size(0),
+                "cross_entropy: Expected one int64 class per row on the scores' device");
+    TORCH_CHECK(reduction >= CGNN_NONE && reduction <= CGNN_MEAN, "cross_entropy: unknown reduction");
+    refuse_dual("the cross entropy", {logits});
+    const c10::cuda::OptionalCUDAGuard guard(logits.device());
+    refuse_foreign_leaves("cross_entropy", {logits});
+    const bool differentiated = torch::autograd::compute_requires_grad(logits);
+    const Tensor target = target_in.contiguous();
+    Tensor loss, stats, labelled, unit;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Rows z(logits);
+        const auto plain = logits.options().requires_grad(false);
+        const auto sums = plain.dtype(sum_type(logits));
+        const bool reduced = reduction != CGNN_NONE;
+        if (reduced) loss = at::empty({}, sums);
+        else loss = at::empty({z.rows}, sums);
+        if (differentiated) stats = at::empty({z.rows, 2}, sums);
+        // (a captured backward pass may be replayed more than once per forward pass: it computes the gradient itself)
+        if (differentiated && reduced && !capturing())
+            unit = at::empty(logits.sizes(), plain.memory_format(at::MemoryFormat::Contiguous));
+        const int64_t bytes = reduced ? (int64_t)cgnn_cross_entropy_scratch_bytes() : 0;
+        Tensor scratch;
+        if (reduced) {
+            labelled = at::empty({1}, plain.dtype(at::kLong));
+            scratch = at::empty({bytes}, plain.dtype(at::kByte));
+        }
+        check(cgnn_cross_entropy(dtype, z.rows, z.width, z.stride, data(z.held), static_cast<const int64_t *>(data(target)),
+                                 ignore_index, reduction, data(loss), data(stats), data(unit),
+                                 static_cast<int64_t *>(data(labelled)), data(scratch), bytes, current_stream(logits)));
+    }
+    if (differentiated) {
+        auto node = new_node<CrossEntropyBackward>();
+        node->dtype = dtype;
+        node->reduction = reduction;
+        node->ignore_index = ignore_index;
+        node->logits_ = SavedVariable(logits, false);
+        node->target_ = SavedVariable(target, false);
+        node->stats_ = SavedVariable(stats, false);
+        node->labelled_ = SavedVariable(labelled, false);
+        node->unit_ = unit;
+        node->set_next_edges(torch::autograd::collect_next_edges(logits));
+        torch::autograd::set_history(loss, node);
+    }
+    return loss;
+}
+
+// ---------------------------------------------------------------------------------------------
 // assignment
 // ---------------------------------------------------------------------------------------------
 std::tuple<Tensor, Tensor, int64_t, PlanPtr> assign(const Tensor &x, const Tensor &planes, int bits, const Tensor &workspace) {
@@ -672,6 +993,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("mean", &mean_autograd, nogil());
     m.def("reconstruct", &reconstruct_autograd, nogil());
     m.def("transform", &transform_autograd, nogil());
+    m.def("layer_norm", &layer_norm_autograd, nogil());
+    m.def("dropout", &dropout_autograd, nogil());
+    m.def("cross_entropy", &cross_entropy_autograd, nogil());
     m.def("assign", &assign, nogil());
     m.def("matmul_tn", [](const Tensor &a, const Tensor &b) {
         TORCH_CHECK(a.is_cuda() && a.device() == b.device() && a.scalar_type() == b.scalar_type() && a.dim() == 2 &&

@@ -106,6 +106,7 @@ cudaError_t pool_alloc(void **ptr, size_t bytes, cudaStream_t stream) {
 
 namespace cgnn {
 int sample_status(int *out);  // cgnn_sample.cu
+int loss_status(int *out);    // cgnn_loss.cu
 }
 
 extern "C" {
@@ -123,7 +124,9 @@ int cgnn_device_status(int *status_out) {
     if (rc == CGNN_OK) rc = cgnn::cluster_status(&c);
     int d = 0;
     if (rc == CGNN_OK) rc = cgnn::sample_status(&d);  // defined in cgnn_sample.cu
-    *status_out = a | b | c | d;
+    int e = 0;
+    if (rc == CGNN_OK) rc = cgnn::loss_status(&e);
+    *status_out = a | b | c | d | e;
     return rc;
 }
 

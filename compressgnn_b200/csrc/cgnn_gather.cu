@@ -7,6 +7,7 @@
 // (the reference traps the GPU instead).
 #include <algorithm>
 
+#include "cgnn_philox.cuh"
 #include "cgnn_plan.h"
 
 #ifndef CGNN_EXPAND_WIDE
@@ -46,48 +47,10 @@ struct ExpandArgs {
     uint64_t seed = 0;
 };
 
-// Philox4x32 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011) with 7
-// rounds: four 32-bit words for the counter (element-vector index, 0) under the key `seed`.  Counter
-// based, so the words of an element do not depend on which thread produces them.
-__device__ __forceinline__ uint4 philox4x32_7(uint64_t counter, uint64_t seed) {
-    uint32_t c0 = (uint32_t)counter, c1 = (uint32_t)(counter >> 32), c2 = 0x243F6A88u, c3 = 0x85A308D3u;
-    uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
-#pragma unroll
-    for (int round = 0; round < 7; ++round) {
-        const uint32_t hi0 = __umulhi(0xD2511F53u, c0), lo0 = 0xD2511F53u * c0;
-        const uint32_t hi1 = __umulhi(0xCD9E8D57u, c2), lo1 = 0xCD9E8D57u * c2;
-        c0 = hi1 ^ c1 ^ k0;
-        c1 = lo1;
-        c2 = hi0 ^ c3 ^ k1;
-        c3 = lo0;
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
-    }
-    return make_uint4(c0, c1, c2, c3);
-}
-
-// Dropout of the VW values of the vector that starts at element `first` of the output (VW is 1, 2 or 4 and
-// divides `first`).  Element e takes word e % 4 of the Philox block counted e / 4, so the mask is a
-// function of (seed, element index) alone: the same whatever the element type or the kernel that writes it.
 template <typename T, int VW>
 __device__ __forceinline__ void drop_vector(Vec<T, VW> &y, int64_t first, uint32_t threshold, T keep_scale,
                                             uint64_t seed) {
-    static_assert(VW == 1 || VW == 2 || VW == 4, "a vector lies inside one block of four random words");
-    const uint4 r = philox4x32_7((uint64_t)first >> 2, seed);
-    if constexpr (VW == 4) {
-        const uint32_t word[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) y.v[k] = word[k] < threshold ? T(0) : y.v[k] * keep_scale;
-    } else if constexpr (VW == 2) {
-        const bool upper = (first & 2) != 0;
-        const uint32_t w0 = upper ? r.z : r.x, w1 = upper ? r.w : r.y;
-        y.v[0] = w0 < threshold ? T(0) : y.v[0] * keep_scale;
-        y.v[1] = w1 < threshold ? T(0) : y.v[1] * keep_scale;
-    } else {
-        const int at = (int)(first & 3);
-        const uint32_t w = at == 0 ? r.x : at == 1 ? r.y : at == 2 ? r.z : r.w;
-        y.v[0] = w < threshold ? T(0) : y.v[0] * keep_scale;
-    }
+    drop_values<T, VW>(y.v, first, threshold, keep_scale, seed);
 }
 
 // A group of LPR lanes expands LPR consecutive node rows per step: lane l reads index[r0 + l]
@@ -403,7 +366,7 @@ static int expand(int dtype, int64_t n, int64_t width, int64_t groups, const voi
     uint32_t threshold = 0;
     double keep_scale = 1.0;
     if (drop_p > 0.0) {
-        threshold = (uint32_t)std::min<double>(drop_p * 4294967296.0, 4294967295.0);
+        threshold = drop_threshold_of(drop_p);
         keep_scale = 1.0 / (1.0 - drop_p);
     }
     if (dtype == CGNN_F32) {

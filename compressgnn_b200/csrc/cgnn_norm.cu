@@ -1,0 +1,595 @@
+// Layer normalisation of the rows of a matrix, with the ReLU and the dropout that may follow it, both ways.
+//
+// Forward, per row x of `width` elements:  mu = mean(x), rstd = 1 / sqrt(mean((x - mu)^2) + eps), h = (x - mu) * rstd,
+// z = h * weight + bias, out = dropout(relu(z)).
+// Backward: g = the incoming gradient where out depends on z (times the dropout's factor), u = g * weight,
+// dx = rstd * (u - mean(u) - h * mean(u * h)), dweight = sum over the rows of g * h, dbias = sum of g.  h and z are
+// recomputed from x and the row's two statistics, the mask of the dropout from its key.
+//
+// Memory bounds both: a row is read once into the registers of its team and everything is computed from there, in
+// two passes over the registers (mean, then squared deviations: no cancellation).
+#include <algorithm>
+
+#include "cgnn_dropout.cuh"
+#include "cgnn_rows.cuh"
+
+namespace cgnn {
+
+constexpr int SMS = 148;
+constexpr int LONG_THREADS = 512;     // a block of the kernels that re-read their rows
+constexpr int COLUMN_ROWS = 512;      // least rows of a block of norm_columns_kernel
+
+template <typename T>
+struct NormArgs {
+    using A = Acc<T>;
+    const T *x;
+    int64_t rows, width, stride;  // x: elements from row to row
+    const void *weight, *bias;    // optional [width]
+    bool wide_params;             // they are fp32 beside a 16-bit x
+    int relu;
+    A eps;
+    Drop drop;
+    T *out;         // forward
+    A *mean, *rstd; // [rows]; forward: written unless null
+    const T *grad;  // backward: [rows, width]
+    T *dx;          // optional
+    A *partial;     // optional: [blocks, 2, width], sums of g * h and of g over a block's rows
+};
+
+// z of a row's elements: h * weight + bias.
+template <typename T, int VW>
+__device__ __forceinline__ void affine(const NormArgs<T> &a, const Acc<T> (&h)[VW], const Acc<T> (&w)[VW], const Acc<T> (&b)[VW],
+                                       Acc<T> (&z)[VW]) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) z[k] = fused(h[k], w[k], b[k]);
+}
+
+template <typename T, int VW>
+__device__ __forceinline__ void params_at(const NormArgs<T> &a, int64_t col, Acc<T> (&w)[VW], Acc<T> (&b)[VW]) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+        w[k] = Acc<T>(1);
+        b[k] = Acc<T>(0);
+    }
+    if (a.weight) load_params<T, VW>(a.weight, a.wide_params, col, w);
+    if (a.bias) load_params<T, VW>(a.bias, a.wide_params, col, b);
+}
+
+// relu and dropout of z (NaN stays NaN).
+template <typename T, int VW>
+__device__ __forceinline__ void follow(const NormArgs<T> &a, int64_t element, uint64_t key, Acc<T> (&z)[VW]) {
+    using A = Acc<T>;
+    if (a.relu)
+#pragma unroll
+        for (int k = 0; k < VW; ++k) z[k] = z[k] < A(0) ? A(0) : z[k];
+    if (a.drop.threshold) drop_values<A, VW>(z, element, a.drop.threshold, (A)a.drop.scale, key);
+}
+
+// The gradient of z from that of the output.
+template <typename T, int VW>
+__device__ __forceinline__ void unfollow(const NormArgs<T> &a, int64_t element, uint64_t key, const Acc<T> (&z)[VW],
+                                         Acc<T> (&g)[VW]) {
+    using A = Acc<T>;
+    if (a.drop.threshold) drop_values<A, VW>(g, element, a.drop.threshold, (A)a.drop.scale, key);
+    if (a.relu)
+#pragma unroll
+        for (int k = 0; k < VW; ++k) g[k] = z[k] <= A(0) ? A(0) : g[k];
+}
+
+template <int TEAM>
+constexpr int FORWARD_THREADS = TEAM > 32 ? TEAM : 256;
+template <int TEAM>
+constexpr int BACKWARD_THREADS = TEAM > 32 ? TEAM : 128;
+
+// The team's row, vector by vector; elements beyond the row are zero.
+template <typename T, int VW, int TEAM, int VPL>
+__device__ __forceinline__ void load_row(const T *row, int64_t width, int lane, Acc<T> (&v)[VPL][VW]) {
+    Vec<T, VW> raw[VPL];
+#pragma unroll
+    for (int p = 0; p < VPL; ++p) {
+        const int col = (p * TEAM + lane) * VW;
+        raw[p] = vec_zero<T, VW>();
+        if (col < width) raw[p] = vec_load<T, VW>(row + col);
+    }
+#pragma unroll
+    for (int p = 0; p < VPL; ++p) widen_all<T, VW>(raw[p], v[p]);
+}
+
+template <typename T, int VW, int TEAM, int VPL>
+__global__ void __launch_bounds__(FORWARD_THREADS<TEAM>) norm_kernel(const NormArgs<T> a) {
+    using A = Acc<T>;
+    constexpr int TEAMS = FORWARD_THREADS<TEAM> / TEAM;
+    __shared__ A shared[TEAMS * 2 * (TEAM > 32 ? TEAM / 32 : 1)];
+    const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
+    const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
+    int turn = 0;
+    const A inv = A(1) / (A)a.width;
+    for (int64_t r = (int64_t)blockIdx.x * TEAMS + team; r < a.rows; r += (int64_t)gridDim.x * TEAMS) {
+        A v[VPL][VW], s[1] = {A(0)};
+        load_row<T, VW, TEAM, VPL>(a.x + r * a.stride, a.width, lane, v);
+#pragma unroll
+        for (int p = 0; p < VPL; ++p)
+#pragma unroll
+            for (int k = 0; k < VW; ++k) s[0] += v[p][k];
+        team_sum<A, TEAM, 1>(s, shared, turn);
+        const A mean = s[0] * inv;
+        s[0] = A(0);
+#pragma unroll
+        for (int p = 0; p < VPL; ++p) {
+            const bool live = (p * TEAM + lane) * VW < a.width;
+#pragma unroll
+            for (int k = 0; k < VW; ++k) {
+                v[p][k] -= mean;
+                if (live) s[0] = fused(v[p][k], v[p][k], s[0]);
+            }
+        }
+        team_sum<A, TEAM, 1>(s, shared, turn);
+        const A rstd = inverse_root(fused(s[0], inv, a.eps));
+        if (a.mean && lane == 0) {
+            a.mean[r] = mean;
+            a.rstd[r] = rstd;
+        }
+#pragma unroll
+        for (int p = 0; p < VPL; ++p) {
+            const int col = (p * TEAM + lane) * VW;
+            if (col >= a.width) continue;
+            A w[VW], b[VW], z[VW];
+            params_at<T, VW>(a, col, w, b);
+#pragma unroll
+            for (int k = 0; k < VW; ++k) v[p][k] *= rstd;
+            affine<T, VW>(a, v[p], w, b, z);
+            follow<T, VW>(a, r * a.width + col, key, z);
+            vec_store<T, VW>(a.out + r * a.width + col, narrow_all<T, VW>(z));
+        }
+    }
+}
+
+// dx and a block's share of the parameters' gradients.  A lane keeps the same columns for all its rows, so their sums
+// stay in registers; teams of a warp, then the warps of the block, are added up in a fixed order at the end.
+template <typename T, int VW, int TEAM, int VPL>
+__global__ void __launch_bounds__(BACKWARD_THREADS<TEAM>) norm_backward_kernel(const NormArgs<T> a) {
+    using A = Acc<T>;
+    constexpr int THREADS = BACKWARD_THREADS<TEAM>, TEAMS = THREADS / TEAM, WARPS = THREADS / 32;
+    constexpr int COLUMNS = TEAM * VPL * VW;
+    __shared__ A shared[TEAM > 32 ? 4 * TEAM / 32 : 2 * COLUMNS];
+    const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
+    const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
+    int turn = 0;
+    const A inv = A(1) / (A)a.width;
+    A w[VPL][VW], dw[VPL][VW], db[VPL][VW];
+#pragma unroll
+    for (int p = 0; p < VPL; ++p) {
+        const int col = (p * TEAM + lane) * VW;
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+            w[p][k] = A(0);
+            dw[p][k] = db[p][k] = A(0);
+        }
+        if (col < a.width) {
+            A b[VW];
+            params_at<T, VW>(a, col, w[p], b);
+        }
+    }
+    for (int64_t r = (int64_t)blockIdx.x * TEAMS + team; r < a.rows; r += (int64_t)gridDim.x * TEAMS) {
+        A h[VPL][VW], g[VPL][VW], s[2] = {A(0), A(0)};
+        const A mean = a.mean[r], rstd = a.rstd[r];
+        load_row<T, VW, TEAM, VPL>(a.x + r * a.stride, a.width, lane, h);
+        load_row<T, VW, TEAM, VPL>(a.grad + r * a.width, a.width, lane, g);
+#pragma unroll
+        for (int p = 0; p < VPL; ++p) {
+            const int col = (p * TEAM + lane) * VW;
+            if (col >= a.width) continue;
+#pragma unroll
+            for (int k = 0; k < VW; ++k) h[p][k] = (h[p][k] - mean) * rstd;
+            A z[VW];
+            if (a.relu) {
+                A again[VW], b[VW];
+                params_at<T, VW>(a, col, again, b);
+                affine<T, VW>(a, h[p], w[p], b, z);
+            }
+            unfollow<T, VW>(a, r * a.width + col, key, z, g[p]);
+#pragma unroll
+            for (int k = 0; k < VW; ++k) {
+                dw[p][k] = fused(g[p][k], h[p][k], dw[p][k]);
+                db[p][k] += g[p][k];
+                g[p][k] *= w[p][k];
+                s[0] += g[p][k];
+                s[1] = fused(g[p][k], h[p][k], s[1]);
+            }
+        }
+        if (!a.dx) continue;
+        team_sum<A, TEAM, 2>(s, shared, turn);
+        const A c0 = s[0] * inv, c1 = s[1] * inv;
+#pragma unroll
+        for (int p = 0; p < VPL; ++p) {
+            const int col = (p * TEAM + lane) * VW;
+            if (col >= a.width) continue;
+            A d[VW];
+#pragma unroll
+            for (int k = 0; k < VW; ++k) d[k] = rstd * (g[p][k] - fused(h[p][k], c1, c0));
+            vec_store<T, VW>(a.dx + r * a.width + col, narrow_all<T, VW>(d));
+        }
+    }
+    if (!a.partial) return;
+    A *mine = a.partial + (int64_t)blockIdx.x * 2 * a.width;
+    if constexpr (TEAM <= 32) {
+#pragma unroll
+        for (int p = 0; p < VPL; ++p)
+#pragma unroll
+            for (int k = 0; k < VW; ++k)
+#pragma unroll
+                for (int off = TEAM; off < 32; off <<= 1) {
+                    dw[p][k] += __shfl_xor_sync(0xffffffffu, dw[p][k], off);
+                    db[p][k] += __shfl_xor_sync(0xffffffffu, db[p][k], off);
+                }
+        for (int warp = 0; warp < WARPS; ++warp) {
+            if ((int)(threadIdx.x >> 5) == warp && (threadIdx.x & 31) < TEAM)
+#pragma unroll
+                for (int p = 0; p < VPL; ++p)
+#pragma unroll
+                    for (int k = 0; k < VW; ++k) {
+                        A *at = shared + (p * TEAM + lane) * VW + k;
+                        at[0] = warp ? at[0] + dw[p][k] : dw[p][k];
+                        at[COLUMNS] = warp ? at[COLUMNS] + db[p][k] : db[p][k];
+                    }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < a.width; c += THREADS) {
+            mine[c] = shared[c];
+            mine[a.width + c] = shared[COLUMNS + c];
+        }
+    } else {
+#pragma unroll
+        for (int p = 0; p < VPL; ++p)
+#pragma unroll
+            for (int k = 0; k < VW; ++k) {
+                const int col = (p * TEAM + lane) * VW + k;
+                if (col < a.width) {
+                    mine[col] = dw[p][k];
+                    mine[a.width + col] = db[p][k];
+                }
+            }
+    }
+}
+
+// Rows too long for a team's registers: a block passes over its row again instead (it lies in L2 by then).
+template <typename T>
+__global__ void __launch_bounds__(LONG_THREADS) norm_long_kernel(const NormArgs<T> a) {
+    using A = Acc<T>;
+    __shared__ A shared[2 * LONG_THREADS / 32];
+    const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
+    int turn = 0;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T *row = a.x + r * a.stride;
+        A s[1] = {A(0)};
+        for (int64_t c = threadIdx.x; c < a.width; c += LONG_THREADS) s[0] += widen(row[c]);
+        team_sum<A, LONG_THREADS, 1>(s, shared, turn);
+        const A mean = s[0] / (A)a.width;
+        s[0] = A(0);
+        for (int64_t c = threadIdx.x; c < a.width; c += LONG_THREADS) {
+            const A d = widen(row[c]) - mean;
+            s[0] = fused(d, d, s[0]);
+        }
+        team_sum<A, LONG_THREADS, 1>(s, shared, turn);
+        const A rstd = inverse_root(s[0] / (A)a.width + a.eps);
+        if (a.mean && threadIdx.x == 0) {
+            a.mean[r] = mean;
+            a.rstd[r] = rstd;
+        }
+        for (int64_t c = threadIdx.x; c < a.width; c += LONG_THREADS) {
+            A h[1] = {(widen(row[c]) - mean) * rstd}, w[1], b[1], z[1];
+            params_at<T, 1>(a, c, w, b);
+            affine<T, 1>(a, h, w, b, z);
+            follow<T, 1>(a, r * a.width + c, key, z);
+            a.out[r * a.width + c] = narrow<T>(z[0]);
+        }
+    }
+}
+
+// One element of a long row on the way back: h and the gradient of z.
+template <typename T>
+__device__ __forceinline__ void long_element(const NormArgs<T> &a, int64_t r, int64_t c, Acc<T> mean, Acc<T> rstd, uint64_t key,
+                                             Acc<T> &h, Acc<T> &g, Acc<T> &weight) {
+    Acc<T> hat[1] = {(widen(a.x[r * a.stride + c]) - mean) * rstd}, grad[1] = {widen(a.grad[r * a.width + c])}, w[1], b[1], z[1];
+    params_at<T, 1>(a, c, w, b);
+    affine<T, 1>(a, hat, w, b, z);
+    unfollow<T, 1>(a, r * a.width + c, key, z, grad);
+    h = hat[0];
+    g = grad[0];
+    weight = w[0];
+}
+
+template <typename T>
+__global__ void __launch_bounds__(LONG_THREADS) norm_long_backward_kernel(const NormArgs<T> a) {
+    using A = Acc<T>;
+    __shared__ A shared[4 * LONG_THREADS / 32];
+    const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
+    int turn = 0;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const A mean = a.mean[r], rstd = a.rstd[r];
+        A s[2] = {A(0), A(0)}, h, g, w;
+        for (int64_t c = threadIdx.x; c < a.width; c += LONG_THREADS) {
+            long_element(a, r, c, mean, rstd, key, h, g, w);
+            s[0] = fused(g, w, s[0]);
+            s[1] = fused(g * w, h, s[1]);
+        }
+        team_sum<A, LONG_THREADS, 2>(s, shared, turn);
+        const A c0 = s[0] / (A)a.width, c1 = s[1] / (A)a.width;
+        for (int64_t c = threadIdx.x; c < a.width; c += LONG_THREADS) {
+            long_element(a, r, c, mean, rstd, key, h, g, w);
+            a.dx[r * a.width + c] = narrow<T>(rstd * (g * w - fused(h, c1, c0)));
+        }
+    }
+}
+
+// Sums over rows_per_block rows of g * h and g, a thread per column.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_columns_kernel(const NormArgs<T> a, int64_t rows_per_block) {
+    using A = Acc<T>;
+    const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= a.width) return;
+    const int64_t r0 = (int64_t)blockIdx.y * rows_per_block, r1 = min(a.rows, r0 + rows_per_block);
+    A dw = A(0), db = A(0), h, g, w;
+    for (int64_t r = r0; r < r1; ++r) {
+        long_element(a, r, c, a.mean[r], a.rstd[r], key, h, g, w);
+        dw = fused(g, h, dw);
+        db += g;
+    }
+    a.partial[(int64_t)blockIdx.y * 2 * a.width + c] = dw;
+    a.partial[((int64_t)blockIdx.y * 2 + 1) * a.width + c] = db;
+}
+
+// The blocks' shares added up in block order: column c of [dweight, dbias] by the lane c of a block of 32 warps, warp w
+// adding shares w, w + 32, ...
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_sums_kernel(const Acc<T> *partial, int64_t blocks, int64_t width, void *dweight,
+                                                         void *dbias, bool wide_params) {
+    using A = Acc<T>;
+    __shared__ A sums[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+    A s = A(0);
+    if (c < 2 * width)
+        for (int64_t b = warp; b < blocks; b += 32) s += partial[b * 2 * width + c];
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (warp || c >= 2 * width) return;
+#pragma unroll
+    for (int w = 1; w < 32; ++w) s += sums[w][lane];
+    void *to = c < width ? dweight : dbias;
+    if (!to) return;
+    const int64_t at = c < width ? c : c - width;
+    if (sizeof(T) == 2 && wide_params) static_cast<float *>(to)[at] = (float)s;
+    else static_cast<T *>(to)[at] = narrow<T>(s);
+}
+
+// ---------------------------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------------------------
+// Rows of `vectors` vectors: the least team that holds them.  f(team, vectors a lane) with both as constants.
+template <int N>
+struct Num {
+    static constexpr int value = N;
+};
+template <typename F>
+static int with_team(int64_t vectors, F &&f) {
+    if (vectors <= 2) return f(Num<2>(), Num<1>());
+    if (vectors <= 4) return f(Num<4>(), Num<1>());
+    if (vectors <= 8) return f(Num<8>(), Num<1>());
+    if (vectors <= 16) return f(Num<8>(), Num<2>());
+    if (vectors <= 32) return f(Num<8>(), Num<4>());
+    if (vectors <= 64) return f(Num<32>(), Num<2>());
+    if (vectors <= 128) return f(Num<32>(), Num<4>());
+    if (vectors <= 512) return f(Num<128>(), Num<4>());
+    return f(Num<512>(), Num<4>());
+}
+constexpr int64_t TEAM_VECTORS = 512 * 4;
+
+// Elements a vector holds: 16 bytes where rows and pointers allow, else one.
+template <typename T>
+constexpr int WIDEST = 16 / (int)sizeof(T);
+
+static bool vectors_fit(size_t item, int64_t width, int64_t stride, std::initializer_list<const void *> pointers) {
+    const int64_t n = 16 / (int64_t)item;
+    uintptr_t bits = 0;
+    for (const void *p : pointers) bits |= (uintptr_t)p;
+    return width % n == 0 && stride % n == 0 && (bits & 15) == 0;
+}
+
+template <typename T, int VW>
+static int forward_typed(const NormArgs<T> &a, cudaStream_t stream) {
+    return with_team(a.width / VW, [&](auto team, auto vpl) -> int {
+        constexpr int TEAM = decltype(team)::value, VPL = decltype(vpl)::value, THREADS = FORWARD_THREADS<TEAM>;
+        const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(a.rows, THREADS / TEAM), SMS * 8);
+        norm_kernel<T, VW, TEAM, VPL><<<blocks, THREADS, 0, stream>>>(a);
+        CGNN_LAUNCH_CHECK();
+        return CGNN_OK;
+    });
+}
+
+template <typename T>
+static int forward(const NormArgs<T> &a, cudaStream_t stream) {
+    constexpr int VW = WIDEST<T>;
+    if (vectors_fit(sizeof(T), a.width, a.stride, {a.x, a.out}) && a.width / VW <= TEAM_VECTORS)
+        return forward_typed<T, VW>(a, stream);
+    if (a.width <= TEAM_VECTORS) return forward_typed<T, 1>(a, stream);
+    norm_long_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, SMS * 4), LONG_THREADS, 0, stream>>>(a);
+    CGNN_LAUNCH_CHECK();
+    return CGNN_OK;
+}
+
+// Blocks of a backward launch, each of which leaves a partial row.
+template <int TEAM>
+static int64_t backward_blocks(int64_t rows) {
+    return std::min<int64_t>(ceil_div(rows, BACKWARD_THREADS<TEAM> / TEAM), TEAM > 128 ? SMS : SMS * 4);
+}
+
+static int64_t column_blocks(int64_t rows, int64_t width) {
+    return std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, COLUMN_ROWS), SMS * 8 / std::max<int64_t>(1, width / 256)));
+}
+
+// Partial rows of a backward pass, the most of the ways it may go.
+static int64_t partial_rows(size_t item, int64_t rows, int64_t width) {
+    int64_t most = 0;
+    for (int64_t vectors : {width / (int64_t)(16 / item), width}) {
+        if (vectors > TEAM_VECTORS)
+            most = std::max(most, column_blocks(rows, width));
+        else
+            with_team(vectors, [&](auto team, auto) -> int {
+                most = std::max(most, backward_blocks<decltype(team)::value>(rows));
+                return 0;
+            });
+    }
+    return most;
+}
+
+template <typename T, int VW>
+static int backward_typed(const NormArgs<T> &a, int64_t *blocks, cudaStream_t stream) {
+    return with_team(a.width / VW, [&](auto team, auto vpl) -> int {
+        constexpr int TEAM = decltype(team)::value, VPL = decltype(vpl)::value;
+        *blocks = backward_blocks<TEAM>(a.rows);
+        norm_backward_kernel<T, VW, TEAM, VPL><<<(unsigned)*blocks, BACKWARD_THREADS<TEAM>, 0, stream>>>(a);
+        CGNN_LAUNCH_CHECK();
+        return CGNN_OK;
+    });
+}
+
+template <typename T>
+static int backward(const NormArgs<T> &a, void *dweight, void *dbias, cudaStream_t stream) {
+    constexpr int VW = WIDEST<T>;
+    int64_t blocks = 0;
+    int rc = CGNN_OK;
+    if (vectors_fit(sizeof(T), a.width, a.stride, {a.x, a.grad, a.dx}) && a.width / VW <= TEAM_VECTORS) {
+        rc = backward_typed<T, VW>(a, &blocks, stream);
+    } else if (a.width <= TEAM_VECTORS) {
+        rc = backward_typed<T, 1>(a, &blocks, stream);
+    } else {
+        if (a.dx) {
+            norm_long_backward_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, SMS * 4), LONG_THREADS, 0, stream>>>(a);
+            CGNN_LAUNCH_CHECK();
+        }
+        if (a.partial) {
+            blocks = column_blocks(a.rows, a.width);
+            const int64_t each = ceil_div(a.rows, blocks);
+            blocks = ceil_div(a.rows, each);
+            norm_columns_kernel<T><<<dim3((unsigned)ceil_div(a.width, 256), (unsigned)blocks), 256, 0, stream>>>(a, each);
+            CGNN_LAUNCH_CHECK();
+        }
+    }
+    if (rc != CGNN_OK || !a.partial) return rc;
+    norm_sums_kernel<T><<<(unsigned)ceil_div(2 * a.width, 32), 1024, 0, stream>>>(a.partial, blocks, a.width, dweight, dbias,
+                                                                                  a.wide_params);
+    CGNN_LAUNCH_CHECK();
+    return CGNN_OK;
+}
+
+// What both directions are given, checked.
+struct NormCall {
+    int dtype, param_dtype;
+    int64_t rows, width, stride;
+    const void *x, *weight, *bias;
+    double p;
+};
+
+static int check_call(const char *what, const NormCall &c) {
+    CGNN_REQUIRE(c.dtype >= CGNN_F32 && c.dtype <= CGNN_F16, "%s: unknown dtype %d", what, c.dtype);
+    CGNN_REQUIRE((!c.weight && !c.bias) || c.param_dtype == c.dtype ||
+                     ((c.dtype == CGNN_BF16 || c.dtype == CGNN_F16) && c.param_dtype == CGNN_F32),
+                 "%s: weight and bias are of the matrix' type, or fp32 beside a 16-bit one", what);
+    CGNN_REQUIRE(c.rows >= 0 && c.width >= 0 && c.stride >= 0, "%s: negative size", what);
+    CGNN_REQUIRE(c.p >= 0.0 && c.p < 1.0, "%s: the drop probability must lie in [0, 1)", what);
+    CGNN_REQUIRE(c.width <= INT32_MAX / 2, "%s: rows of %lld elements are not supported", what, (long long)c.width);
+    return CGNN_OK;
+}
+
+template <typename T>
+static NormArgs<T> args_of(const NormCall &c, int relu, uint64_t seed, const int64_t *device_seed) {
+    NormArgs<T> a{};
+    a.x = (const T *)c.x;
+    a.rows = c.rows;
+    a.width = c.width;
+    a.stride = c.stride;
+    a.weight = c.weight;
+    a.bias = c.bias;
+    a.wide_params = c.param_dtype == CGNN_F32 && c.dtype != CGNN_F32;
+    a.relu = relu;
+    a.drop = Drop::of(c.p, seed, device_seed);
+    return a;
+}
+
+static size_t item_of(int dtype) { return dtype == CGNN_F64 ? 8 : dtype == CGNN_F32 ? 4 : 2; }
+static size_t acc_of(int dtype) { return dtype == CGNN_F64 ? 8 : 4; }
+
+}  // namespace cgnn
+
+using namespace cgnn;
+
+extern "C" {
+
+int cgnn_layer_norm(int dtype, int param_dtype, int64_t rows, int64_t width, int64_t stride, const void *x, const void *weight,
+                    const void *bias, double eps, int relu, double p, uint64_t seed, const int64_t *device_seed, void *out,
+                    void *mean, void *rstd, cgnn_stream_t stream) {
+    const NormCall c{dtype, param_dtype, rows, width, stride, x, weight, bias, p};
+    if (int rc = check_call("layer_norm", c)) return rc;
+    CGNN_REQUIRE((mean == nullptr) == (rstd == nullptr), "layer_norm: both statistics are written, or none");
+    if (rows == 0 || width == 0) return CGNN_OK;
+    CGNN_REQUIRE(x != nullptr && out != nullptr, "layer_norm: null pointer");
+    const auto run = [&](auto zero) -> int {
+        using T = decltype(zero);
+        NormArgs<T> a = args_of<T>(c, relu, seed, device_seed);
+        a.eps = (Acc<T>)eps;
+        a.out = (T *)out;
+        a.mean = (Acc<T> *)mean;
+        a.rstd = (Acc<T> *)rstd;
+        return forward<T>(a, (cudaStream_t)stream);
+    };
+    switch (dtype) {
+        case CGNN_F32: return run(0.0f);
+        case CGNN_F64: return run(0.0);
+        case CGNN_BF16: return run(__nv_bfloat16());
+        default: return run(__half());
+    }
+}
+
+size_t cgnn_layer_norm_scratch_bytes(int dtype, int64_t rows, int64_t width) {
+    if (dtype < CGNN_F32 || dtype > CGNN_F16 || rows <= 0 || width <= 0) return 0;
+    return (size_t)partial_rows(item_of(dtype), rows, width) * 2 * width * acc_of(dtype);
+}
+
+int cgnn_layer_norm_backward(int dtype, int param_dtype, int64_t rows, int64_t width, int64_t stride, const void *x,
+                             const void *weight, const void *bias, const void *mean, const void *rstd, const void *grad,
+                             int relu, double p, uint64_t seed, const int64_t *device_seed, void *dx, void *dweight,
+                             void *dbias, void *scratch, size_t scratch_bytes, cgnn_stream_t stream) {
+    const NormCall c{dtype, param_dtype, rows, width, stride, x, weight, bias, p};
+    if (int rc = check_call("layer_norm_backward", c)) return rc;
+    const size_t param = param_dtype == dtype ? item_of(dtype) : 4;
+    if (rows == 0 && width > 0) {  // sums of nothing
+        if (dweight) CGNN_CUDA(cudaMemsetAsync(dweight, 0, width * param, (cudaStream_t)stream));
+        if (dbias) CGNN_CUDA(cudaMemsetAsync(dbias, 0, width * param, (cudaStream_t)stream));
+    }
+    if (rows == 0 || width == 0 || (!dx && !dweight && !dbias)) return CGNN_OK;
+    CGNN_REQUIRE(x != nullptr && mean != nullptr && rstd != nullptr && grad != nullptr, "layer_norm_backward: null pointer");
+    CGNN_REQUIRE((!dweight && !dbias) || scratch != nullptr, "layer_norm_backward: null scratch");
+    if (dweight || dbias)
+        CGNN_REQUIRE(scratch_bytes >= cgnn_layer_norm_scratch_bytes(dtype, rows, width) && ((uintptr_t)scratch & 15) == 0,
+                     "layer_norm_backward: the scratch is too small or not 16-byte aligned");
+    const auto run = [&](auto zero) -> int {
+        using T = decltype(zero);
+        NormArgs<T> a = args_of<T>(c, relu, seed, device_seed);
+        a.mean = (Acc<T> *)mean;
+        a.rstd = (Acc<T> *)rstd;
+        a.grad = (const T *)grad;
+        a.dx = (T *)dx;
+        a.partial = dweight || dbias ? (Acc<T> *)scratch : nullptr;
+        return backward<T>(a, dweight, dbias, (cudaStream_t)stream);
+    };
+    switch (dtype) {
+        case CGNN_F32: return run(0.0f);
+        case CGNN_F64: return run(0.0);
+        case CGNN_BF16: return run(__nv_bfloat16());
+        default: return run(__half());
+    }
+}
+
+}  // extern "C"

@@ -106,6 +106,8 @@ class ShardedGNNLayer(torch.nn.Module):
         from .layer import Compressgnn_Cluster, Compressgnn_Reconstruct, KPropagate
         if not layer.use_transformation:
             raise ValueError("ShardedGNNLayer needs a layer built with use_transformation=True")
+        if layer.norm is not None:
+            raise ValueError("a normalised layer needs whole rows: it is not sharded by columns")
         self.group, self.shard_output = group, shard_output
         self.rank, self.world = dist.get_rank(group), dist.get_world_size(group)
         full = layer.cluster
@@ -155,6 +157,8 @@ class ShardedGCN(torch.nn.Module):
 
     def __init__(self, model, group=None):
         super().__init__()
+        if model.residual:
+            raise ValueError("a model with residual connections is not sharded by columns")
         last = len(model.layers) - 1
         self.group = group
         self.dropout = model.dropout
@@ -227,7 +231,8 @@ def place_model(model, in_features, group=None, min_features=MIN_SHARDED_FEATURE
     the same parameters and the same random stream everywhere, no collective).  A sharded module takes
     ``shard_columns(x, rank, world)``, a replica takes ``x``."""
     world = dist.get_world_size(group) if dist.is_initialized() else 1
-    if world > 1 and in_features >= min_features and in_features % world == 0:
+    whole_rows = getattr(model, "residual", False) or any(getattr(layer, "norm", None) is not None for layer in model.layers)
+    if world > 1 and in_features >= min_features and in_features % world == 0 and not whole_rows:
         return ShardedGCN(model, group), True
     return model, False
 

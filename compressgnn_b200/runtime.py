@@ -631,6 +631,61 @@ def cluster_reconstruct_backward(grad, index, output, groups, relu, plan=None,
     return (out, bias_grad) if return_bias_grad else out
 
 
+# -----------------------------------------------------------------------------------------
+# row operators of a training step (not in the reference, whose model calls torch here)
+# -----------------------------------------------------------------------------------------
+def _seed_args(seed):
+    """A dropout key as the binding takes it: (number or None, tensor or None)."""
+    if seed is None:
+        return None, None
+    if torch.is_tensor(seed):
+        return None, seed
+    seed = int(seed) & (2**64 - 1)
+    return seed - 2**64 if seed >= 2**63 else seed, None
+
+
+def layer_norm(input, weight=None, bias=None, eps=1e-5, activation=None, dropout=0.0, seed=None):
+    """``dropout(act((input - mean) / sqrt(var + eps) * weight + bias))`` over the last dimension, in one pass and
+    differentiable in ``input``, ``weight`` and ``bias``.
+
+    ``input``: float32, float64, bfloat16 or float16; rows of a matrix may lie apart.  ``weight`` and ``bias``: vectors of
+    the input's type, or float32 beside a 16-bit input; either may be None.  ``activation``: None or ``"relu"``.
+    ``dropout``: the probability of the dropout that follows; its mask is ``runtime.dropout``'s for the same ``seed``."""
+    _require(activation in (None, "relu"), "Supported activations: None, relu")
+    _require(torch.is_tensor(input) and input.is_cuda, "compressgnn_b200 runs on CUDA tensors only (no CPU normalisation path)")
+    return differentiable(ops().layer_norm, input, weight, bias, float(eps), activation == "relu", float(dropout),
+                          *_seed_args(seed))
+
+
+def dropout(input, p, residual=None, seed=None):
+    """``residual + dropout(input)``: elements are dropped with probability ``p`` in [0, 1), the others multiplied by
+    ``1 / (1 - p)``; ``residual`` may be None.  Differentiable; the mask is a function of ``(seed, element position)``,
+    the one ``cluster_reconstruct`` uses, and is computed again in the backward pass instead of being stored.
+
+    ``seed``: an int, or a CUDA tensor of one int64 that the kernels read when they run, so that a captured graph can be
+    given another one for each replay.  Without one every call draws a fresh key (from torch's host generator; inside a
+    capture, from the device's, again at every replay).  A dropped element is 0 whatever its value."""
+    _require(torch.is_tensor(input) and input.is_cuda, "compressgnn_b200 runs on CUDA tensors only (no CPU dropout path)")
+    return differentiable(ops().dropout, input, float(p), residual, *_seed_args(seed))
+
+
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+def cross_entropy(logits, target, ignore_index=-100, reduction="mean"):
+    """Softmax cross entropy of the class scores ``logits`` [rows, classes] with the classes ``target`` (int64 [rows]),
+    differentiable in ``logits``: what ``torch.nn.functional.cross_entropy`` computes, except that losses of 16-bit scores
+    are float32.
+
+    Rows whose target is ``ignore_index`` have no loss and a gradient of zeros; their scores are not read.  A target
+    that is no class is treated the same and recorded in ``device_status()``.  ``reduction="mean"`` divides by the
+    number of the other rows (NaN when there are none).  With ``"sum"`` and ``"mean"`` the forward pass writes the gradient as
+    well, so that the scores are read once a step: under ``torch.no_grad()`` it does not."""
+    _require(reduction in _REDUCTIONS, f"Supported reductions: {', '.join(_REDUCTIONS)}")
+    _require(torch.is_tensor(logits) and logits.is_cuda, "compressgnn_b200 runs on CUDA tensors only (no CPU loss path)")
+    return differentiable(ops().cross_entropy, logits, target, int(ignore_index), _REDUCTIONS[reduction])
+
+
 def device_status():
     """Read and clear the kernels' status word (synchronises the device)."""
     status = ctypes.c_int(0)

@@ -9,7 +9,10 @@
  * dtype: CGNN_F32 or CGNN_F64 (the reference dispatches both, ref:
  * src/runtime/csrc/sparse/cuda/spmm_gpu.cu:37).  All matrices are dense row-major with
  * row stride == width.  Index arrays handed to plan constructors may be 4 or 8 bytes wide;
- * plans keep private 32-bit copies.
+ * plans keep private 32-bit copies.  The row operators of a training step (cgnn_layer_norm, cgnn_dropout,
+ * cgnn_cross_entropy) also take CGNN_BF16 and CGNN_F16.
+ * The row operators of a training step (cgnn_layer_norm, cgnn_dropout, cgnn_cross_entropy) also take
+ * CGNN_BF16 and CGNN_F16.
  */
 #ifndef CGNN_B200_H
 #define CGNN_B200_H
@@ -24,7 +27,8 @@ extern "C" {
 typedef struct CUstream_st *cgnn_stream_t; /* a cudaStream_t */
 
 enum { CGNN_OK = 0, CGNN_ERR_INVALID = 1, CGNN_ERR_CUDA = 2, CGNN_ERR_CAPACITY = 3 };
-enum { CGNN_F32 = 0, CGNN_F64 = 1 };
+enum { CGNN_F32 = 0, CGNN_F64 = 1, CGNN_BF16 = 2, CGNN_F16 = 3 };
+enum { CGNN_NONE = 0, CGNN_SUM = 1, CGNN_MEAN = 2 }; /* reductions of cgnn_cross_entropy */
 
 int cgnn_version(void);
 const char *cgnn_last_error(void);
@@ -356,6 +360,57 @@ int cgnn_sample_hops_result(const cgnn_sample_graph *graph, int64_t batch, int h
                             const int64_t *fanouts, int64_t largest_degree, const int64_t sizes[2],
                             int32_t *first, const void *workspace, int64_t *samples_out,
                             int64_t *rows_out, int64_t *cols_out, cgnn_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Row operators of a training step: what stands between and behind the propagations.  They take fp32, fp64, bf16 and
+ * fp16 matrices; sums and statistics are fp32 (fp64 for fp64), results are rounded once.
+ *
+ * Dropout: element e of the (dense) output takes word e % 4 of the Philox4x32-7 block counted e / 4 under the key and
+ * is dropped when the word lies below p * 2^32; the others are multiplied by 1 / (1 - p).  It is the mask of
+ * cgnn_cluster_reconstruct_dropout.  The key is `seed`, or, when `device_seed` is not null, the value found there when
+ * the kernel runs (a captured graph draws another mask at every replay).  Nothing is stored: a backward pass
+ * takes the same p and key.
+ *
+ * cgnn_layer_norm: out[r,:] = dropout(act((x[r,:] - mean_r) * rstd_r * weight + bias)), rstd = 1 / sqrt(var + eps) with the
+ * biased variance, act = ReLU or nothing.  Row r of x begins at x + r * stride elements; out is dense.  weight and bias
+ * may be null; beside 16-bit matrices they may be fp32 (param_dtype).  mean and rstd ([rows], fp32 or fp64 like the sums)
+ * are what the backward pass reads; null when there is none.
+ * cgnn_layer_norm_backward: grad, dx: dense [rows, width]; dweight, dbias: [width] of param_dtype, added up in a fixed
+ * order; each of the three may be null.  scratch: cgnn_layer_norm_scratch_bytes(), 16-byte aligned, needed with
+ * dweight or dbias; its contents do not matter. */
+int cgnn_layer_norm(int dtype, int param_dtype, int64_t rows, int64_t width, int64_t stride, const void *x,
+                    const void *weight, const void *bias, double eps, int relu, double p, uint64_t seed,
+                    const int64_t *device_seed, void *out, void *mean, void *rstd, cgnn_stream_t stream);
+size_t cgnn_layer_norm_scratch_bytes(int dtype, int64_t rows, int64_t width);
+int cgnn_layer_norm_backward(int dtype, int param_dtype, int64_t rows, int64_t width, int64_t stride, const void *x,
+                             const void *weight, const void *bias, const void *mean, const void *rstd,
+                             const void *grad, int relu, double p, uint64_t seed, const int64_t *device_seed,
+                             void *dx, void *dweight, void *dbias, void *scratch, size_t scratch_bytes,
+                             cgnn_stream_t stream);
+
+/* out = residual + dropout(x) over n dense elements; residual may be null.  The backward pass is the same call on the
+ * gradient, without the residual (whose gradient is the incoming one). */
+int cgnn_dropout(int dtype, int64_t n, const void *x, const void *residual, double p, uint64_t seed,
+                 const int64_t *device_seed, void *out, cgnn_stream_t stream);
+
+/* Softmax cross entropy of logits[r,:] (row r begins at logits + r * stride elements) with the class target[r].
+ * A row whose target is ignore_index has no loss and a gradient of zeros; so has one whose target is no class, which
+ * also sets status bit 1.  Losses are fp32 (fp64 for fp64).
+ *   reduction   CGNN_NONE: loss[rows]; CGNN_SUM, CGNN_MEAN (over the rows with a class; NaN when there is none): one value
+ *   stats       [rows, 2], what the backward pass reads; may be null
+ *   grad        dense [rows, classes], the gradient for an incoming gradient of one; not with CGNN_NONE; may be null
+ *   labelled    one int64, written with CGNN_MEAN: the number of rows with a class
+ *   scratch     cgnn_cross_entropy_scratch_bytes(), 8-byte aligned, with CGNN_SUM and CGNN_MEAN
+ * Backward: upstream is one value, or one per row with CGNN_NONE, of the loss' type.  With holds_unit_gradient `grad` is what
+ * the forward call wrote: it is left alone when the incoming gradient is one, and computed anew otherwise. */
+size_t cgnn_cross_entropy_scratch_bytes(void);
+int cgnn_cross_entropy(int dtype, int64_t rows, int64_t classes, int64_t stride, const void *logits,
+                       const int64_t *target, int64_t ignore_index, int reduction, void *loss, void *stats,
+                       void *grad, int64_t *labelled, void *scratch, size_t scratch_bytes, cgnn_stream_t stream);
+int cgnn_cross_entropy_backward(int dtype, int64_t rows, int64_t classes, int64_t stride, const void *logits,
+                                const int64_t *target, int64_t ignore_index, int reduction, const void *stats,
+                                const int64_t *labelled, const void *upstream, int holds_unit_gradient, void *grad,
+                                cgnn_stream_t stream);
 
 #ifdef __cplusplus
 }
