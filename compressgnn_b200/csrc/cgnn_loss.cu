@@ -8,6 +8,7 @@
 // loss, from the copy of the row it holds anyway: the scores are read once a step, not twice.  Losses are added up in
 // fp64 and in a fixed order.
 #include <algorithm>
+#include <type_traits>
 
 #include <cooperative_groups.h>
 
@@ -56,7 +57,6 @@ struct LossArgs {
     const A *upstream;     // backward: one value, or one per row without reduction
     int skip_one;          // backward: `grad` holds the gradient for an incoming one already
     int dense;             // rows lie one behind the other from a 16-byte boundary on, in the scores and the gradient
-    uint32_t per_class;    // ceil(2^32 / classes): e / classes == umulhi(e, it) for the elements of a tile
 };
 
 // The class of a row, or -1 for a row without one.
@@ -69,22 +69,55 @@ __device__ __forceinline__ int64_t class_of(int64_t t, int64_t classes, int64_t 
     return t;
 }
 
-// e^x for x <= 0: 2^(x * log2(e)) by the special function unit; what lies below the normal numbers is zero.
-__device__ __forceinline__ float exponential(float x) {
+constexpr float LOG2_E = 1.4426950408889634f;
+// By the special function unit; what lies below the normal numbers is zero.
+__device__ __forceinline__ float power_of_two(float x) {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// e^x for x <= 0.
+__device__ __forceinline__ float exponential(float x) { return power_of_two(x * LOG2_E); }
 __device__ __forceinline__ double exponential(double x) { return exp(x); }
 __device__ __forceinline__ float logarithm(float x) { return logf(x); }
 __device__ __forceinline__ double logarithm(double x) { return log(x); }
 __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
 
-// One element of the gradient, the same arithmetic in every kernel.
+// The gradient of a score from its exponential, the same arithmetic in every kernel: scale = inv * share.
 template <typename A>
-__device__ __forceinline__ A slope(A z, A m, A inv, bool label, A share) {
-    return fused(exponential(z - m), inv, label ? A(-1) : A(0)) * share;
+__device__ __forceinline__ A slope(A e, A scale) { return e * scale; }
+template <typename A>
+__device__ __forceinline__ A slope_at_label(A e, A scale, A share) { return fused(e, scale, -share); }
+
+// The same of two scores at once: fp32 has instructions for pairs.
+__device__ __forceinline__ void exponentials(float &a, float &b, float m) {
+    const float2 d = __fadd2_rn(make_float2(a, b), make_float2(-m, -m));
+    const float2 e = __fmul2_rn(d, make_float2(LOG2_E, LOG2_E));
+    a = power_of_two(e.x);
+    b = power_of_two(e.y);
+}
+__device__ __forceinline__ void exponentials(double &a, double &b, double m) {
+    a = exponential(a - m);
+    b = exponential(b - m);
+}
+__device__ __forceinline__ void add_pair(float (&s)[2], float a, float b) {
+    const float2 two = __fadd2_rn(make_float2(s[0], s[1]), make_float2(a, b));
+    s[0] = two.x;
+    s[1] = two.y;
+}
+__device__ __forceinline__ void add_pair(double (&s)[2], double a, double b) {
+    s[0] += a;
+    s[1] += b;
+}
+__device__ __forceinline__ void slopes(float &a, float &b, float scale) {
+    const float2 two = __fmul2_rn(make_float2(a, b), make_float2(scale, scale));
+    a = two.x;
+    b = two.y;
+}
+__device__ __forceinline__ void slopes(double &a, double &b, double scale) {
+    a = slope(a, scale);
+    b = slope(b, scale);
 }
 
 // What a row's gradient is multiplied by: a mean's share is rounded once.
@@ -97,6 +130,31 @@ __device__ __forceinline__ void copy16(void *shared, const void *global, int byt
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(shared)), "l"(global),
                  "r"(bytes)
                  : "memory");
+}
+// Bulk copies (whole 16-byte vectors) report to a barrier in shared memory, for which threads wait with a limit.
+constexpr int WAIT_LIMIT = 1 << 20;
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void barrier_init(uint64_t *barrier, int arrivals) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(barrier)), "r"(arrivals) : "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint64_t *barrier, uint32_t bytes) {  // and arrive
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(barrier)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_copy(void *shared, const void *global, uint32_t bytes, uint64_t *barrier) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(shared_address(shared)),
+                 "l"(global), "r"(bytes), "r"(shared_address(barrier))
+                 : "memory");
+}
+__device__ __forceinline__ bool barrier_wait(uint64_t *barrier, uint32_t parity) {
+    for (int i = 0; i < WAIT_LIMIT; ++i) {
+        uint32_t done;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(done)
+                     : "r"(shared_address(barrier)), "r"(parity)
+                     : "memory");
+        if (done) return true;
+    }
+    return false;
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
@@ -162,27 +220,25 @@ __device__ __forceinline__ void finish(const LossArgs<T> &a, double total, int64
     *a.labelled = labelled;
 }
 
-// Columns lane, lane + LANES, ... of a row, beginning at `start` (a multiple of LANES) and around.
-template <int LANES, typename F>
-__device__ __forceinline__ void for_columns(int classes, int lane, int start, F &&f) {
-#pragma unroll 4
-    for (int c = lane + start; c < classes; c += LANES) f(c);
-    const int end = min(lane + start, classes);
-#pragma unroll 4
-    for (int c = lane; c < end; c += LANES) f(c);
-}
-
-// Rows of up to 1024 classes.  A block copies ROWS whole rows into shared memory as the 16-byte vectors they lie in, in
-// whatever way rows and vectors meet (47 classes: 188 bytes a row), leaving out vectors of unlabelled rows alone; LANES lanes
-// a row then pass over it three times (maximum, sum, gradient in place), and the gradient leaves by whole vectors.
-// The lanes of a warp begin at different columns, or rows of an even length would meet in the same banks.
-// CLUSTERED: the launch is one cluster, which counts the labelled rows and adds up the losses itself.
-template <typename T, int LANES, int ROWS, bool FORWARD, bool CLUSTERED>
-__global__ void __launch_bounds__(LANES *ROWS) loss_tile_kernel(const LossArgs<T> a) {
+// Rows of up to 768 classes.  A block copies ROWS whole rows into shared memory as the 16-byte vectors they lie in, in
+// whatever way rows and vectors meet (47 classes: 188 bytes a row): one bulk copy for each labelled row, while the tile
+// before is worked on.  LANES lanes then hold a row in registers, lane l the columns l, l + LANES, ...; the gradient takes
+// the row's place in shared memory and leaves by whole vectors.
+// What bounds it is instructions and their latency more than memory: 2.45 M x 47 in fp32 with 0.6 of the rows
+// labelled takes 171 us (DRAM 782 MB, 120 us); a lane group of 16 over registers loaded from DRAM took 375, three passes
+// over shared memory 301, one tile at a time 237.  HELD and the registers were tried together: 24 columns in
+// 64 registers 171, 24 in 80 176, 32 in 80 177, 32 in 64 193, 16 in 51 259.
+// AROUND: the lanes of a warp begin at different columns and go around, or rows of an even length would meet in the
+// same banks.  CLUSTERED: the launch is one cluster, which counts the labelled rows and adds up the losses itself.
+constexpr int HELD = 24;  // columns of a lane, at most
+template <typename T, int THREADS>
+constexpr int TILE_BLOCKS = (sizeof(T) == 8 ? 384 : 1024) / THREADS;  // to a multiprocessor, by their registers
+template <typename T, int LANES, int ROWS, bool AROUND, bool FORWARD, bool CLUSTERED>
+__global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS>) loss_tile_kernel(const LossArgs<T> a) {
     using A = Acc<T>;
     constexpr int THREADS = LANES * ROWS, VW = 16 / sizeof(T);
     extern __shared__ uint4 tile_vectors[];
-    __shared__ bool labelled_row[ROWS];
+    __shared__ uint64_t arrived[2];
     __shared__ double cluster_sum;
     __shared__ int cluster_count;
     if constexpr (!FORWARD) {
@@ -191,7 +247,7 @@ __global__ void __launch_bounds__(LANES *ROWS) loss_tile_kernel(const LossArgs<T
     if constexpr (FORWARD && !CLUSTERED) asm volatile("griddepcontrol.wait;" ::: "memory");
     T *tile = reinterpret_cast<T *>(tile_vectors);
     const int team = threadIdx.x / LANES, lane = threadIdx.x % LANES;
-    const int classes = (int)a.classes;
+    const int classes = (int)a.classes, held = (classes + LANES - 1) / LANES;
     const unsigned mask = team_mask<LANES>();
     int64_t labelled = 0;
     if constexpr (CLUSTERED) {
@@ -213,79 +269,140 @@ __global__ void __launch_bounds__(LANES *ROWS) loss_tile_kernel(const LossArgs<T
     A share = A(0);
     if (a.grad && (FORWARD || a.reduction != CGNN_NONE)) share = share_of(a, FORWARD ? 1.0 : (double)*a.upstream, labelled);
     double total = 0.0;
-    int start = 0;
-    if (LANES < 32 && (LANES > 1 || classes % 2 == 0)) start = team % ((classes + LANES - 1) / LANES) * LANES;
-    const auto row_of = [&](int e) { return classes == 1 ? e : (int)__umulhi((uint32_t)e, a.per_class); };
-    const int64_t tiles = (a.rows + ROWS - 1) / ROWS;
-    for (int64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
-        const int64_t r0 = i * ROWS, r = r0 + team;
-        const int n = (int)min((int64_t)ROWS, a.rows - r0) * classes;  // elements of the tile
-        const int64_t label = r < a.rows ? class_of(a.target[r], a.classes, a.ignore_index, FORWARD && lane == 0) : -1;
-        const int t = (int)label;
-        if (lane == 0) labelled_row[team] = t >= 0;
-        __syncthreads();
-        if (a.dense) {
-            const T *from = a.logits + r0 * a.classes;
-            for (int e = threadIdx.x * VW; e < n; e += THREADS * VW) {
-                const int last = row_of(min(e + VW, n) - 1);
-                bool any = false;
-                for (int row = row_of(e); row <= last; ++row) any |= labelled_row[row];
-                if (any) copy16(tile + e, from + e, min(16, (n - e) * (int)sizeof(T)));
-            }
-            copies_done();
-        } else {
-            for (int e = threadIdx.x; e < n; e += THREADS) {
-                const int row = row_of(e);
-                if (labelled_row[row]) tile[e] = a.logits[(r0 + row) * a.stride + (e - row * classes)];
+    // Register j of a lane has the column `lane + LANES * ((j + turn) % held)`; there_is(): one below `limit`.
+    const int turn = AROUND ? team % held : 0;
+    const auto column = [&](int j) { return AROUND ? lane + LANES * (j + turn >= held ? j + turn - held : j + turn) : lane + LANES * j; };
+    const auto there_is = [&](int j, int limit) { return AROUND ? j < held && column(j) < limit : LANES * j < limit - lane; };
+    const int tiles = (int)((a.rows + ROWS - 1) / ROWS);  // (below 2^31: the rows of more do not fit any memory)
+    // The team's row: the vectors that cover it, in one copy; one that it shares with the next row both may bring.  (The
+    // very last row may end inside a vector: its last elements are loaded one by one.)
+    const int first = team * classes / VW * VW, behind = (team + 1) * classes, last = (behind + VW - 1) / VW * VW;
+    const auto copy = [&](int i, bool wanted, int place, T *to) {
+        if (!a.dense) {
+            const T *from = a.logits + ((int64_t)i * ROWS + team) * a.stride;
+            if (wanted)
+                for (int c = lane; c < classes; c += LANES) to[team * classes + c] = from[c];
+        } else if (lane == 0) {
+            const T *from = a.logits + (int64_t)i * (ROWS * classes);
+            int end = last;
+            if (i == tiles - 1) end = min(last, (int)(a.rows - (int64_t)i * ROWS) * classes / VW * VW);
+            const uint32_t bytes = wanted && end > first ? (uint32_t)((end - first) * sizeof(T)) : 0u;
+            barrier_expect(&arrived[place], bytes);
+            if (bytes) bulk_copy(to + first, from + first, bytes, &arrived[place]);
+            if (wanted)
+                for (int e = max(end, first); e < behind; ++e) to[e] = from[e];
+        }
+    };
+    const auto label_of = [&](int i) {  // of the team's row of a tile
+        const int64_t r = (int64_t)i * ROWS + team;
+        return i < tiles && r < a.rows ? a.target[r] : a.ignore_index;
+    };
+    const auto class_or_none = [&](int64_t label) { return (int)class_of(label, a.classes, a.ignore_index, FORWARD && lane == 0); };
+    if (threadIdx.x == 0) {
+        barrier_init(&arrived[0], ROWS);
+        barrier_init(&arrived[1], ROWS);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    // While one tile is worked on the next one arrives, and the labels of the one after it.
+    T *here = tile, *there = tile + (ROWS * classes + VW - 1) / VW * VW;
+    int t = class_or_none(label_of(blockIdx.x)), round = 0;
+    int64_t label_next = label_of(blockIdx.x + gridDim.x);
+    if ((int)blockIdx.x < tiles) copy(blockIdx.x, t >= 0, 0, here);
+    for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++round) {
+        // (ordinary accesses to the other tile's place come before the copy into it)
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        const uint32_t parity = (uint32_t)(round >> 1) & 1u;
+        const bool late = a.dense && !barrier_wait(&arrived[round & 1], parity);
+        if (__syncthreads_or(late)) {  // the tile is here, and the one before it has left; or a copy did not arrive
+            if (threadIdx.x == 0) atomicOr(&g_loss_status, STATUS_WAIT_EXPIRED);
+            barrier_wait(&arrived[round & 1], parity);
+            return;
+        }
+        const int t_next = class_or_none(label_next);
+        if (i + (int)gridDim.x < tiles) copy(i + gridDim.x, t_next >= 0, (round & 1) ^ 1, there);
+        label_next = label_of(i + 2 * gridDim.x);
+        const int64_t r = (int64_t)i * ROWS + team;
+        const bool inside = i < tiles - 1 || r < a.rows;
+        T *const z = here + team * classes;
+        // A row without a label passes as one of scores of minus infinity with a share of zero.
+        const int read = t >= 0 ? classes : 0, written = inside ? classes : 0;
+        A v[HELD], m = -(A)INFINITY, other = m, inv = A(0), at_label = A(0);
+        if (t >= 0) at_label = widen(z[t]);
+#pragma unroll
+        for (int j = 0; j < HELD; j += 8) {
+            if (j >= held) break;
+#pragma unroll
+            for (int k = j; k < j + 8; ++k) {
+                v[k] = -(A)INFINITY;
+                if (there_is(k, read)) v[k] = widen(z[column(k)]);
+                if (FORWARD) (k & 1 ? other : m) = larger(k & 1 ? other : m, v[k]);
             }
         }
-        __syncthreads();
-        T *z = tile + team * classes;
-        if (t >= 0) {
-            A m = -(A)INFINITY, inv;
-            if constexpr (FORWARD) {
-                for_columns<LANES>(classes, lane, start, [&](int c) { m = larger(m, widen(z[c])); });
+        if constexpr (FORWARD) {
+            m = larger(m, other);
 #pragma unroll
-                for (int off = LANES / 2; off > 0; off >>= 1) m = larger(m, __shfl_xor_sync(mask, m, off));
-                A s = A(0);
-                for_columns<LANES>(classes, lane, start, [&](int c) { s += exponential(widen(z[c]) - m); });
+            for (int off = LANES / 2; off > 0; off >>= 1) m = larger(m, __shfl_xor_sync(mask, m, off));
+        } else if (t >= 0) {
+            m = a.stats[2 * r];
+            inv = a.stats[2 * r + 1];
+            if (a.reduction == CGNN_NONE) share = a.upstream[r];
+        }
+        if (t < 0) m = A(0);
+        A parts[2] = {A(0), A(0)};
 #pragma unroll
-                for (int off = LANES / 2; off > 0; off >>= 1) s += __shfl_xor_sync(mask, s, off);
-                inv = A(1) / s;
-                if (lane == 0) {
-                    // (the label's score and the largest one first: both may be large beside their difference)
-                    const A loss = logarithm(s) + (m - widen(z[t]));
-                    if (a.reduction == CGNN_NONE) a.loss[r] = loss;
-                    total += (double)loss;
-                    if (a.stats) {
-                        a.stats[2 * r] = m;
-                        a.stats[2 * r + 1] = inv;
-                    }
+        for (int j = 0; j < HELD; j += 8) {
+            if (j >= held) break;
+#pragma unroll
+            for (int k = j; k < j + 8; k += 2) {
+                exponentials(v[k], v[k + 1], m);
+                if (FORWARD) add_pair(parts, v[k], v[k + 1]);
+            }
+        }
+        A s = parts[0] + parts[1];
+        if constexpr (FORWARD) {
+#pragma unroll
+            for (int off = LANES / 2; off > 0; off >>= 1) s += __shfl_xor_sync(mask, s, off);
+            inv = A(1) / s;
+            if (lane == 0 && inside) {
+                // (the label's score and the largest one first: both may be large beside their difference)
+                const A loss = t >= 0 ? logarithm(s) + (m - at_label) : A(0);
+                if (a.reduction == CGNN_NONE) a.loss[r] = loss;
+                total += (double)loss;
+                if (a.stats) vec_store<A, 2>(a.stats + 2 * r, Vec<A, 2>{{m, inv}});
+            }
+        }
+        T *const now = here;
+        here = there;
+        there = now;
+        if (a.grad) {
+            const A scale = t >= 0 ? inv * share : A(0);
+            __syncwarp(mask);  // every lane has read its label's score ...
+#pragma unroll
+            for (int j = 0; j < HELD; j += 8) {
+                if (j >= held) break;
+#pragma unroll
+                for (int k = j; k < j + 8; k += 2) {
+                    slopes(v[k], v[k + 1], scale);
+                    if (there_is(k, written)) z[column(k)] = narrow<T>(v[k]);
+                    if (there_is(k + 1, written)) z[column(k + 1)] = narrow<T>(v[k + 1]);
                 }
-                __syncwarp(mask);
+            }
+            __syncwarp(mask);  // ... and written its columns
+            if (lane == 0 && t >= 0) z[t] = narrow<T>(slope_at_label(exponential(at_label - m), scale, share));
+            __syncthreads();
+            T *const to = a.grad + (int64_t)i * (ROWS * classes);
+            const int n = i < tiles - 1 ? ROWS * classes : (int)(a.rows - (int64_t)i * ROWS) * classes;
+            if (a.dense) {
+                const int whole = n / VW * VW;
+#pragma unroll 4
+                for (int e = threadIdx.x * VW; e < whole; e += THREADS * VW) vec_store<T, VW>(to + e, vec_load<T, VW>(now + e));
+                if (whole + (int)threadIdx.x < n) to[whole + threadIdx.x] = now[whole + threadIdx.x];
             } else {
-                m = a.stats[2 * r];
-                inv = a.stats[2 * r + 1];
-                if (a.reduction == CGNN_NONE) share = a.upstream[r];
+                for (int e = threadIdx.x; e < n; e += THREADS) to[e] = now[e];
             }
-            if (a.grad)
-                for_columns<LANES>(classes, lane, start, [&](int c) { z[c] = narrow<T>(slope<A>(widen(z[c]), m, inv, c == t, share)); });
-        } else if (r < a.rows) {
-            if (FORWARD && a.reduction == CGNN_NONE && lane == 0) a.loss[r] = A(0);
-            if (a.grad) for_columns<LANES>(classes, lane, start, [&](int c) { z[c] = narrow<T>(A(0)); });
         }
-        if (!a.grad) continue;
-        __syncthreads();
-        T *to = a.grad + r0 * a.classes;
-        if (a.dense) {
-            for (int e = threadIdx.x * VW; e < n; e += THREADS * VW) {
-                if (e + VW <= n) vec_store<T, VW>(to + e, vec_load<T, VW>(tile + e));
-                else
-                    for (int k = e; k < n; ++k) to[k] = tile[k];
-            }
-        } else {
-            for (int e = threadIdx.x; e < n; e += THREADS) to[e] = tile[e];
-        }
+        t = t_next;
     }
     if constexpr (FORWARD) {
         if (a.reduction == CGNN_NONE) return;
@@ -322,21 +439,207 @@ struct Cover {
         copy16(to + q, base + (int64_t)q * 16, min(16, (shift + classes) * (int)sizeof(T) - q * 16));
     }
     __device__ __forceinline__ int first(int q) const { return q * (16 / (int)sizeof(T)) - shift; }
+    // Elements of a copied vector that are not the row's become minus infinity.
+    __device__ __forceinline__ void clear(uint4 *in, int q) const {
+        T *v = reinterpret_cast<T *>(in + q);
+        for (int k = 0; k < 16 / (int)sizeof(T); ++k)
+            if ((unsigned)(first(q) + k) >= (unsigned)classes) v[k] = narrow<T>(-(Acc<T>)INFINITY);
+    }
 };
 
-// Rows of more classes: a block holds one row in shared memory.  A thread copies, reads and writes the same vectors
-// throughout, so that only the two sums over the block need barriers, and it fetches the next row's vector as soon as it is
-// done with this row's: one row is read while the other is written.
-template <typename T, int THREADS, bool FORWARD>
-__global__ void __launch_bounds__(THREADS) loss_row_kernel(const LossArgs<T> a) {
+// The largest element of a vector (pairs of 16-bit ones are compared as they are).
+template <typename T, int VW>
+__device__ __forceinline__ Acc<T> largest(const Vec<T, VW> &x) {
+    if constexpr (__is_same(T, __nv_bfloat16)) {
+        const __nv_bfloat162 *pairs = reinterpret_cast<const __nv_bfloat162 *>(&x);
+        const __nv_bfloat162 two = __hmax2(__hmax2(pairs[0], pairs[1]), __hmax2(pairs[2], pairs[3]));
+        return fmaxf(__low2float(two), __high2float(two));
+    } else if constexpr (__is_same(T, __half)) {
+        const __half2 *pairs = reinterpret_cast<const __half2 *>(&x);
+        const __half2 two = __hmax2(__hmax2(pairs[0], pairs[1]), __hmax2(pairs[2], pairs[3]));
+        return fmaxf(__low2float(two), __high2float(two));
+    } else {
+        Acc<T> m = widen(x.v[0]);
+#pragma unroll
+        for (int k = 1; k < VW; ++k) m = larger(m, widen(x.v[k]));
+        return m;
+    }
+}
+
+// e^(x - m) of fp32 sums as 2^(x * log2(e) - c), c = m * log2(e): one instruction before the special function.  The rounding
+// of c is common to all exponentials of one m, which are off by a factor of 2^(m * log2(e) - c); it is divided out of
+// their sum and of the scale they are multiplied by.  It stays near one for |m| below 2^20; other rows subtract first.
+__device__ __forceinline__ float from_offset(float m) { return power_of_two(fmaf(-m, LOG2_E, m * LOG2_E)); }  // 1 / that factor
+template <typename A>
+__device__ __forceinline__ bool is_steep(A m) {
+    return sizeof(A) == 8 || !(m < A(1048576) && m > A(-1048576));
+}
+
+// A row's largest score and 1 / sum e^(x - it), on every thread of the block.  vector(q) is vector q of the row's cover,
+// with minus infinity where it is not the row.  `turn` counts the calls: two sets of places in turn, so that one
+// barrier is enough.
+template <typename T, int THREADS, int BATCH, typename Vectors>
+__device__ __forceinline__ void row_statistics(Vectors &&vector, int vectors, int &turn, Acc<T> &m, Acc<T> &s) {
     using A = Acc<T>;
     constexpr int VW = 16 / sizeof(T), WARPS = THREADS / 32;
+    __shared__ A tops_of[2][WARPS], parts_of[2][WARPS];
+    A *const tops = tops_of[turn & 1], *const parts = parts_of[turn & 1];
+    ++turn;
+    m = -(A)INFINITY;
+    s = A(0);
+    bool steep = sizeof(A) == 8;
+    if constexpr (sizeof(A) == 4) {
+        // One pass with a running maximum of the thread, a batch of vectors at a time.
+        float2 two = make_float2(0.0f, 0.0f);
+        for (int q = threadIdx.x; q < vectors; q += BATCH * THREADS) {
+            Vec<T, VW> x[BATCH];
+            float top = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) x[b] = vector(q + b * THREADS < vectors ? q + b * THREADS : q);  // a thread's own
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) top = fmaxf(top, largest<T, VW>(x[b]));
+            if (top == -INFINITY) continue;  // (nothing to add; a NaN goes on)
+            steep |= is_steep(top);
+            if (top > m) {
+                const float down = power_of_two(fmaf(m, LOG2_E, -top * LOG2_E));
+                two.x *= down;
+                two.y *= down;
+                m = top;
+            }
+            const float2 base = make_float2(LOG2_E, LOG2_E), c = make_float2(-m * LOG2_E, -m * LOG2_E);
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                if (q + b * THREADS >= vectors) break;
+                float v[VW];
+                widen_all<T, VW>(x[b], v);
+#pragma unroll
+                for (int k = 0; k < VW; k += 2) {
+                    const float2 e = __ffma2_rn(make_float2(v[k], v[k + 1]), base, c);  // (two of them in one instruction)
+                    two = __fadd2_rn(make_float2(power_of_two(e.x), power_of_two(e.y)), two);
+                }
+            }
+        }
+        s = two.x + two.y;
+    }
+    // The threads' sums meet under the largest maximum; they are not used where a maximum is too large for them.
+    const A mine = m;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, off));
+    if constexpr (sizeof(A) == 4)
+        if (mine > -INFINITY) s *= from_offset(mine) * exponential(mine - m);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    if ((threadIdx.x & 31) == 0) {
+        tops[threadIdx.x >> 5] = m;
+        parts[threadIdx.x >> 5] = s;
+    }
+    if (!__syncthreads_or(steep)) {
+        m = tops[0];
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) m = larger(m, tops[w]);
+        s = A(0);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const A part = parts[w];  // (a warp without a score has none, and minus infinity for a maximum)
+            s += part == A(0) ? part : part * exponential(tops[w] - m);
+        }
+        return;
+    }
+    m = -(A)INFINITY;
+    for (int q = threadIdx.x; q < vectors; q += THREADS) m = larger(m, largest<T, VW>(vector(q)));
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, off));
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) m = larger(m, tops[w]);
+    s = A(0);
+    for (int q = threadIdx.x; q < vectors; q += THREADS) {
+        A v[VW];
+        widen_all<T, VW>(vector(q), v);
+#pragma unroll
+        for (int k = 0; k < VW; ++k) s += exponential(v[k] - m);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = s;
+    __syncthreads();
+    s = A(0);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) s += parts[w];
+}
+
+// The gradient of a vector of scores: e^(x - m) * scale, the label apart.
+template <typename T, bool STEEP>
+struct VectorSlope {
+    using A = Acc<T>;
+    static constexpr int VW = 16 / sizeof(T);
+    A m, scale, c;
+    __device__ __forceinline__ VectorSlope(A m_, A inv, A share) : m(m_), scale(inv * share), c(A(0)) {
+        if constexpr (!STEEP) {
+            scale *= from_offset(m);
+            c = m * LOG2_E;
+        }
+    }
+    __device__ __forceinline__ Vec<T, VW> operator()(const Vec<T, VW> &x) const {
+        A v[VW];
+        widen_all<T, VW>(x, v);
+        if constexpr (STEEP) {
+#pragma unroll
+            for (int k = 0; k < VW; ++k) v[k] = slope(exponential(v[k] - m), scale);
+        } else {
+#pragma unroll
+            for (int k = 0; k < VW; k += 2) {
+                const float2 e = __ffma2_rn(make_float2(v[k], v[k + 1]), make_float2(LOG2_E, LOG2_E), make_float2(-c, -c));
+                const float2 d = __fmul2_rn(make_float2(power_of_two(e.x), power_of_two(e.y)), make_float2(scale, scale));
+                v[k] = d.x;
+                v[k + 1] = d.y;
+            }
+        }
+        return narrow_all<T, VW>(v);
+    }
+    __device__ __forceinline__ T at_label(A x, A share) const {
+        if constexpr (STEEP) return narrow<T>(slope_at_label(exponential(x - m), scale, share));
+        else return narrow<T>(slope_at_label(power_of_two(fmaf(x, LOG2_E, -c)), scale, share));
+    }
+};
+template <typename T, typename F>
+__device__ __forceinline__ void with_slope(Acc<T> m, Acc<T> inv, Acc<T> share, F &&f) {
+    if constexpr (sizeof(T) == 8) {
+        f(VectorSlope<T, true>(m, inv, share));
+    } else {
+        if (is_steep(m)) f(VectorSlope<T, true>(m, inv, share));
+        else f(VectorSlope<T, false>(m, inv, share));
+    }
+}
+
+// A vector of the gradient to where it belongs, element by element where it is not whole.
+template <typename T>
+__device__ __forceinline__ void store_vector(T *out, int first, int classes, bool aligned, const Vec<T, 16 / sizeof(T)> &y) {
+    constexpr int VW = 16 / sizeof(T);
+    if (aligned && first >= 0 && first + VW <= classes) {
+        vec_store<T, VW>(out + first, y);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VW; ++k)
+            if ((unsigned)(first + k) < (unsigned)classes) out[first + k] = y.v[k];
+    }
+}
+
+// Rows of more classes: a block holds one row in shared memory.  A thread copies, reads and writes the same vectors
+// throughout, so that only the sums over the block need a barrier, and it fetches the next row's vector as soon as it is
+// done with this row's: one row is read while the other is written.  8192 x 50001 in bf16, 0.9 of the rows labelled: 333 us
+// (1.56 GB, 238 us at the copy rate); the special function unit is 56 % busy, issue slots 53 %, DRAM 47 %.
+template <typename T, int THREADS, bool FORWARD>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_row_kernel(const LossArgs<T> a) {
+    using A = Acc<T>;
+    constexpr int VW = 16 / sizeof(T);
     extern __shared__ uint4 row_vectors[];
-    __shared__ A maxima[WARPS], sums[WARPS];
     if constexpr (!FORWARD) {
         if (a.skip_one && *a.upstream == A(1)) return;
     }
     if constexpr (FORWARD) asm volatile("griddepcontrol.wait;" ::: "memory");
+    int turn = 0;
     int64_t labelled = 0;
     if (FORWARD && a.reduction != CGNN_NONE) labelled = labelled_rows<T, THREADS>(a);
     if (!FORWARD && a.reduction == CGNN_MEAN) labelled = *a.labelled;
@@ -344,6 +647,7 @@ __global__ void __launch_bounds__(THREADS) loss_row_kernel(const LossArgs<T> a) 
     if (a.grad && (FORWARD || a.reduction != CGNN_NONE)) share = share_of(a, FORWARD ? 1.0 : (double)*a.upstream, labelled);
     double total = 0.0;
     const int classes = (int)a.classes;
+    const auto vector = [&](int q) { return vec_load<T, VW>(reinterpret_cast<const T *>(row_vectors + q)); };
     const auto label_of = [&](int64_t r) {
         return r < a.rows ? (int)class_of(a.target[r], a.classes, a.ignore_index, FORWARD && threadIdx.x == 0) : -1;
     };
@@ -361,50 +665,15 @@ __global__ void __launch_bounds__(THREADS) loss_row_kernel(const LossArgs<T> a) 
         const Cover<T> row(a.logits + r * a.stride, a.classes), row_next(a.logits + (t_next >= 0 ? next : r) * a.stride, a.classes);
         A at_next = A(0);
         if (FORWARD && t_next >= 0 && threadIdx.x == 0) at_next = widen(a.logits[next * a.stride + t_next]);
-        A m = -(A)INFINITY, inv = A(0);
+        A m = A(0), inv = A(0);
         if (t >= 0) {
             copies_done();
             if constexpr (FORWARD) {
-                for (int q = threadIdx.x; q < row.vectors; q += THREADS) {
-                    A v[VW];
-                    widen_all<T, VW>(vec_load<T, VW>(reinterpret_cast<const T *>(row_vectors + q)), v);
-                    const int e = row.first(q);
-                    if (e >= 0 && e + VW <= classes) {
-#pragma unroll
-                        for (int k = 0; k < VW; ++k) m = larger(m, v[k]);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < VW; ++k)
-                            if ((unsigned)(e + k) < (unsigned)classes) m = larger(m, v[k]);
-                    }
-                }
-#pragma unroll
-                for (int off = 16; off > 0; off >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, off));
-                if ((threadIdx.x & 31) == 0) maxima[threadIdx.x >> 5] = m;
-                __syncthreads();
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) m = larger(m, maxima[w]);
-                A s = A(0);
-                for (int q = threadIdx.x; q < row.vectors; q += THREADS) {
-                    A v[VW];
-                    widen_all<T, VW>(vec_load<T, VW>(reinterpret_cast<const T *>(row_vectors + q)), v);
-                    const int e = row.first(q);
-                    if (e >= 0 && e + VW <= classes) {
-#pragma unroll
-                        for (int k = 0; k < VW; ++k) s += exponential(v[k] - m);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < VW; ++k)
-                            if ((unsigned)(e + k) < (unsigned)classes) s += exponential(v[k] - m);
-                    }
-                }
-#pragma unroll
-                for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-                if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;
-                __syncthreads();
-                s = A(0);
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) s += sums[w];
+                // what the first and the last vector hold beside the row counts for nothing
+                if (threadIdx.x == 0) row.clear(row_vectors, 0);
+                if ((row.vectors - 1) % THREADS == (int)threadIdx.x) row.clear(row_vectors, row.vectors - 1);
+                A s;
+                row_statistics<T, THREADS, 2>(vector, row.vectors, turn, m, s);
                 inv = A(1) / s;
                 if (threadIdx.x == 0) {
                     const A loss = logarithm(s) + (m - at_label);
@@ -426,31 +695,34 @@ __global__ void __launch_bounds__(THREADS) loss_row_kernel(const LossArgs<T> a) 
         // Out with this row, in with the next: the same vectors by the same thread.
         T *out = a.grad + r * a.classes;
         const bool aligned = ((uintptr_t)out & 15) == (uintptr_t)(row.shift * sizeof(T));
-        const int most = max(row.vectors, t_next >= 0 ? row_next.vectors : 0);
-        for (int q = threadIdx.x; q < most; q += THREADS) {
-            if (a.grad && q < row.vectors) {
-                A d[VW];
-                const int e = row.first(q);
-                if (t >= 0) {
-                    A v[VW];
-                    widen_all<T, VW>(vec_load<T, VW>(reinterpret_cast<const T *>(row_vectors + q)), v);
-#pragma unroll
-                    for (int k = 0; k < VW; ++k) d[k] = slope<A>(v[k], m, inv, e + k == t, share);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < VW; ++k) d[k] = A(0);
+        const int leaving = a.grad ? row.vectors : 0, entering = t_next >= 0 ? row_next.vectors : 0;
+        with_slope<T>(m, inv, share, [&](auto slopes) {
+            const auto pass = [&](int q) {  // any vector
+                if (q < leaving) store_vector<T>(out, row.first(q), classes, aligned, t >= 0 ? slopes(vector(q)) : vec_zero<T, VW>());
+                if (q < entering) row_next.copy(row_vectors, q);
+            };
+            // The label's element is written again below by the thread that has its vector.
+            const bool mine = t >= 0 && a.grad && (row.shift + t) / VW % THREADS == (int)threadIdx.x;
+            T label_slope = narrow<T>(A(0));
+            if (mine) label_slope = slopes.at_label(widen(reinterpret_cast<const T *>(row_vectors)[row.shift + t]), share);
+            int q = threadIdx.x;
+            if (t >= 0 && aligned && leaving && entering) {  // whole vectors on both sides, the usual case
+                if (q == 0) {
+                    pass(0);
+                    q = THREADS;
                 }
-                const Vec<T, VW> y = narrow_all<T, VW>(d);
-                if (aligned && e >= 0 && e + VW <= classes) {
-                    vec_store<T, VW>(out + e, y);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < VW; ++k)
-                        if ((unsigned)(e + k) < (unsigned)classes) out[e + k] = y.v[k];
+                const int inner = min(leaving, entering) - 1;
+                T *to = out + row.first(0);
+                const char *from = row_next.base;
+#pragma unroll 2
+                for (; q < inner; q += THREADS) {
+                    vec_store<T, VW>(to + q * VW, slopes(vector(q)));
+                    copy16(row_vectors + q, from + q * 16, 16);
                 }
             }
-            if (t_next >= 0 && q < row_next.vectors) row_next.copy(row_vectors, q);
-        }
+            for (; q < max(leaving, entering); q += THREADS) pass(q);
+            if (mine) out[t] = label_slope;
+        });
         r = next;
         t = t_next;
         at_label = at_next;
@@ -460,49 +732,45 @@ __global__ void __launch_bounds__(THREADS) loss_row_kernel(const LossArgs<T> a) 
     }
 }
 
-// Rows that shared memory does not hold: a block passes over its row again instead (the later times out of L2).
+// Rows that shared memory does not hold: read a second time for the gradient, out of L2.  (8192 x 50001 in bf16, which
+// it holds: 441 us this way, 333 with the row kept.)
 template <typename T, bool FORWARD>
-__global__ void __launch_bounds__(LONG_THREADS) loss_long_kernel(const LossArgs<T> a) {
+__global__ void __launch_bounds__(LONG_THREADS, sizeof(T) == 8 ? 1 : 2) loss_long_kernel(const LossArgs<T> a) {
     using A = Acc<T>;
-    constexpr int WARPS = LONG_THREADS / 32;
-    __shared__ A maxima[WARPS], sums[WARPS];
+    constexpr int VW = 16 / sizeof(T), BATCH = 4;
     if constexpr (!FORWARD) {
         if (a.skip_one && *a.upstream == A(1)) return;
     }
     if constexpr (FORWARD) asm volatile("griddepcontrol.wait;" ::: "memory");
+    int turn = 0;
     int64_t labelled = 0;
     if (FORWARD && a.reduction != CGNN_NONE) labelled = labelled_rows<T, LONG_THREADS>(a);
     if (!FORWARD && a.reduction == CGNN_MEAN) labelled = *a.labelled;
     A share = A(0);
     if (a.grad && (FORWARD || a.reduction != CGNN_NONE)) share = share_of(a, FORWARD ? 1.0 : (double)*a.upstream, labelled);
     double total = 0.0;
+    const int classes = (int)a.classes;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const int64_t t = class_of(a.target[r], a.classes, a.ignore_index, FORWARD && threadIdx.x == 0);
-        const T *row = a.logits + r * a.stride;
-        A m = -(A)INFINITY, inv = A(0);
+        const int t = (int)class_of(a.target[r], a.classes, a.ignore_index, FORWARD && threadIdx.x == 0);
+        const T *scores = a.logits + r * a.stride;
+        const Cover<T> row(scores, a.classes);
+        const auto vector = [&](int q) {
+            const int e = row.first(q);
+            if (e >= 0 && e + VW <= classes) return vec_load<T, VW>(reinterpret_cast<const T *>(row.base + (int64_t)q * 16));
+            Vec<T, VW> x;
+#pragma unroll
+            for (int k = 0; k < VW; ++k)
+                x.v[k] = (unsigned)(e + k) < (unsigned)classes ? scores[e + k] : narrow<T>(-(A)INFINITY);
+            return x;
+        };
+        A m = A(0), inv = A(0);
         if (t >= 0) {
             if constexpr (FORWARD) {
-#pragma unroll 8
-                for (int64_t c = threadIdx.x; c < a.classes; c += LONG_THREADS) m = larger(m, widen(row[c]));
-#pragma unroll
-                for (int off = 16; off > 0; off >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, off));
-                if ((threadIdx.x & 31) == 0) maxima[threadIdx.x >> 5] = m;
-                __syncthreads();
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) m = larger(m, maxima[w]);
-                A s = A(0);
-#pragma unroll 8
-                for (int64_t c = threadIdx.x; c < a.classes; c += LONG_THREADS) s += exponential(widen(row[c]) - m);
-#pragma unroll
-                for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-                if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;
-                __syncthreads();
-                s = A(0);
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) s += sums[w];
+                A s;
+                row_statistics<T, LONG_THREADS, BATCH>(vector, row.vectors, turn, m, s);
                 inv = A(1) / s;
                 if (threadIdx.x == 0) {
-                    const A loss = logarithm(s) + (m - widen(row[t]));
+                    const A loss = logarithm(s) + (m - widen(scores[t]));
                     if (a.reduction == CGNN_NONE) a.loss[r] = loss;
                     total += (double)loss;
                     if (a.stats) {
@@ -520,9 +788,25 @@ __global__ void __launch_bounds__(LONG_THREADS) loss_long_kernel(const LossArgs<
         }
         if (!a.grad) continue;
         T *out = a.grad + r * a.classes;
-#pragma unroll 8
-        for (int64_t c = threadIdx.x; c < a.classes; c += LONG_THREADS)
-            out[c] = narrow<T>(t >= 0 ? slope<A>(widen(row[c]), m, inv, c == t, share) : A(0));
+        const bool aligned = ((uintptr_t)out & 15) == (uintptr_t)(row.shift * sizeof(T));
+        if (t < 0) {
+            for (int q = threadIdx.x; q < row.vectors; q += LONG_THREADS)
+                store_vector<T>(out, row.first(q), classes, aligned, vec_zero<T, VW>());
+            continue;
+        }
+        with_slope<T>(m, inv, share, [&](auto slopes) {
+            for (int q = threadIdx.x; q < row.vectors; q += BATCH * LONG_THREADS) {
+                Vec<T, VW> x[BATCH];
+#pragma unroll
+                for (int b = 0; b < BATCH; ++b) x[b] = vector(q + b * LONG_THREADS < row.vectors ? q + b * LONG_THREADS : q);
+#pragma unroll
+                for (int b = 0; b < BATCH; ++b)
+                    if (q + b * LONG_THREADS < row.vectors)
+                        store_vector<T>(out, row.first(q + b * LONG_THREADS), classes, aligned, slopes(x[b]));
+            }
+            // (by the thread that has written the vector it lies in)
+            if ((row.shift + t) / VW % LONG_THREADS == (int)threadIdx.x) out[t] = slopes.at_label(widen(scores[t]), share);
+        });
     }
     if constexpr (FORWARD) {
         if (a.reduction != CGNN_NONE) finish<T, LONG_THREADS>(a, total, labelled);
@@ -534,11 +818,12 @@ __global__ void __launch_bounds__(LONG_THREADS) loss_long_kernel(const LossArgs<
 // ---------------------------------------------------------------------------------------------
 // follows: behind the launch that counts, which it may overlap until it waits; cluster: blocks of one cluster, or 1.
 template <typename T>
-static int launch(void (*kernel)(const LossArgs<T>), const LossArgs<T> &a, int64_t units, int threads, size_t shared, bool follows,
-                  int cluster, cudaStream_t stream) {
+static int launch(void (*kernel)(const LossArgs<T>), const LossArgs<T> &a, int64_t units, int threads, int blocks, size_t shared,
+                  bool follows, int cluster, cudaStream_t stream) {
     if (shared > 44 * 1024)  // (with the kernels' own variables no more than the 48 KB that need no leave)
         CGNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
-    const int64_t resident = std::min<int64_t>({16, (int64_t)(SHARED_MOST / (shared + 2048)), 2048 / threads});
+    // (no more than run at once: blocks that began when others end would double the time)
+    const int64_t resident = std::min<int64_t>(blocks, (int64_t)(SHARED_MOST / (shared + 2048)));
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(cluster > 1 ? (unsigned)cluster
                                       : (unsigned)std::max<int64_t>(1, std::min<int64_t>(units, SMS * std::max<int64_t>(1, resident))));
@@ -560,32 +845,41 @@ static int launch(void (*kernel)(const LossArgs<T>), const LossArgs<T> &a, int64
     return CGNN_OK;
 }
 
+// Whether rows of that many classes begin in too few banks for their lanes: words from row to row a multiple of two.
+static bool meet_in_banks(size_t item, int64_t classes) { return classes * item % 8 == 0; }
+
 template <typename T, int LANES, int ROWS, bool FORWARD>
 static int launch_tiles(const LossArgs<T> &a, bool follows, cudaStream_t stream) {
-    const size_t shared = (ROWS * a.classes * sizeof(T) + 15) / 16 * 16;
-    return launch<T>(loss_tile_kernel<T, LANES, ROWS, FORWARD, false>, a, ceil_div(a.rows, ROWS), LANES * ROWS, shared, follows, 1,
-                     stream);
+    const size_t shared = 2 * ((ROWS * a.classes * sizeof(T) + 15) / 16 * 16);
+    auto kernel = meet_in_banks(sizeof(T), a.classes) && LANES < 32 ? loss_tile_kernel<T, LANES, ROWS, (LANES < 32), FORWARD, false>
+                                                                    : loss_tile_kernel<T, LANES, ROWS, false, FORWARD, false>;
+    return launch<T>(kernel, a, ceil_div(a.rows, ROWS), LANES * ROWS, TILE_BLOCKS<T, LANES * ROWS>, shared, follows, 1, stream);
 }
 
 template <typename T, bool FORWARD>
 static int launch_rows(const LossArgs<T> &a, bool follows, cudaStream_t stream) {
-    if (a.classes <= 64) return launch_tiles<T, 1, 128, FORWARD>(a, follows, stream);
-    if (a.classes <= 256) return launch_tiles<T, 4, 32, FORWARD>(a, follows, stream);
-    if (a.classes <= 1024) return launch_tiles<T, 32, 8, FORWARD>(a, follows, stream);
+    if (a.classes <= HELD) return launch_tiles<T, 1, 128, FORWARD>(a, follows, stream);
+    if (a.classes <= 2 * HELD) return launch_tiles<T, 2, 64, FORWARD>(a, follows, stream);
+    if (a.classes <= 4 * HELD) return launch_tiles<T, 4, 32, FORWARD>(a, follows, stream);
+    if (a.classes <= 8 * HELD) return launch_tiles<T, 8, 16, FORWARD>(a, follows, stream);
+    if (a.classes <= 16 * HELD) return launch_tiles<T, 16, 8, FORWARD>(a, follows, stream);
+    if (a.classes <= 32 * HELD) return launch_tiles<T, 32, 8, FORWARD>(a, follows, stream);
     const size_t shared = (a.classes * sizeof(T) + 15) / 16 * 16 + 16;
-    if (shared <= 32 * 1024) return launch<T>(loss_row_kernel<T, 256, FORWARD>, a, a.rows, 256, shared, follows, 1, stream);
-    if (shared <= SHARED_MOST / 2 - 2048) return launch<T>(loss_row_kernel<T, 512, FORWARD>, a, a.rows, 512, shared, follows, 1, stream);
-    if (shared <= SHARED_MOST - 2048) return launch<T>(loss_row_kernel<T, 1024, FORWARD>, a, a.rows, 1024, shared, follows, 1, stream);
-    return launch<T>(loss_long_kernel<T, FORWARD>, a, a.rows, LONG_THREADS, 0, follows, 1, stream);
+    if (shared <= 32 * 1024) return launch<T>(loss_row_kernel<T, 256, FORWARD>, a, a.rows, 256, 4, shared, follows, 1, stream);
+    if (shared <= SHARED_MOST / 2 - 2048) return launch<T>(loss_row_kernel<T, 512, FORWARD>, a, a.rows, 512, 2, shared, follows, 1, stream);
+    if (shared <= SHARED_MOST - 2048) return launch<T>(loss_row_kernel<T, 1024, FORWARD>, a, a.rows, 1024, 1, shared, follows, 1, stream);
+    return launch<T>(loss_long_kernel<T, FORWARD>, a, a.rows, LONG_THREADS, sizeof(T) == 8 ? 1 : 2, 0, follows, 1, stream);
 }
 
 // One launch where a cluster does it all, else one that counts and one that computes.
 template <typename T>
 static int forward(LossArgs<T> a, cudaStream_t stream) {
     if (a.reduction == CGNN_NONE) return a.rows ? launch_rows<T, true>(a, false, stream) : CGNN_OK;
-    if (a.rows <= CLUSTER_ROWS && a.classes <= 64)
-        return launch<T>(loss_tile_kernel<T, 1, 128, true, true>, a, CLUSTER, 128, (128 * a.classes * sizeof(T) + 15) / 16 * 16, false,
-                         CLUSTER, stream);
+    if (a.rows <= CLUSTER_ROWS && a.classes <= HELD) {
+        auto kernel = meet_in_banks(sizeof(T), a.classes) ? loss_tile_kernel<T, 1, 128, true, true, true>
+                                                          : loss_tile_kernel<T, 1, 128, false, true, true>;
+        return launch<T>(kernel, a, CLUSTER, 128, 1, 2 * ((128 * a.classes * sizeof(T) + 15) / 16 * 16), false, CLUSTER, stream);
+    }
     a.count_blocks = a.reduction == CGNN_MEAN ? (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(a.rows, COUNT_THREADS), SMS)) : 1;
     loss_count_kernel<<<(unsigned)a.count_blocks, COUNT_THREADS, 0, stream>>>(
         a.target, a.reduction == CGNN_MEAN ? a.rows : 0, a.classes, a.ignore_index, a.scratch);
@@ -606,7 +900,6 @@ static LossArgs<T> args_of(int64_t rows, int64_t classes, int64_t stride, const 
     a.reduction = reduction;
     a.grad = (T *)grad;
     a.dense = (stride == classes || rows == 1) && (((uintptr_t)logits | (uintptr_t)grad) & 15) == 0;
-    a.per_class = (uint32_t)(((uint64_t)1 << 32) / (uint64_t)classes + 1);
     return a;
 }
 

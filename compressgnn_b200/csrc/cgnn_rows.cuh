@@ -36,17 +36,44 @@ __device__ __forceinline__ T narrow(Acc<T> x) {
     else return x;
 }
 
+// (16-bit types go in pairs: one conversion instruction packs two of them)
 template <typename T, int VW>
 __device__ __forceinline__ void widen_all(const Vec<T, VW> &x, Acc<T> (&y)[VW]) {
+    if constexpr (__is_same(T, __nv_bfloat16) && VW % 2 == 0) {
+        const uint32_t *pairs = reinterpret_cast<const uint32_t *>(&x);
 #pragma unroll
-    for (int k = 0; k < VW; ++k) y[k] = widen(x.v[k]);
+        for (int k = 0; k < VW; k += 2) {  // a bf16 is the upper half of the same number in fp32
+            y[k] = __uint_as_float(pairs[k / 2] << 16);
+            y[k + 1] = __uint_as_float(pairs[k / 2] & 0xffff0000u);
+        }
+    } else if constexpr (__is_same(T, __half) && VW % 2 == 0) {
+        const __half2 *pairs = reinterpret_cast<const __half2 *>(&x);
+#pragma unroll
+        for (int k = 0; k < VW; k += 2) {
+            const float2 two = __half22float2(pairs[k / 2]);
+            y[k] = two.x;
+            y[k + 1] = two.y;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VW; ++k) y[k] = widen(x.v[k]);
+    }
 }
 
 template <typename T, int VW>
 __device__ __forceinline__ Vec<T, VW> narrow_all(const Acc<T> (&y)[VW]) {
     Vec<T, VW> r;
+    if constexpr (__is_same(T, __nv_bfloat16) && VW % 2 == 0) {
 #pragma unroll
-    for (int k = 0; k < VW; ++k) r.v[k] = narrow<T>(y[k]);
+        for (int k = 0; k < VW; k += 2)
+            *reinterpret_cast<__nv_bfloat162 *>(&r.v[k]) = __floats2bfloat162_rn(y[k], y[k + 1]);
+    } else if constexpr (__is_same(T, __half) && VW % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < VW; k += 2) *reinterpret_cast<__half2 *>(&r.v[k]) = __floats2half2_rn(y[k], y[k + 1]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VW; ++k) r.v[k] = narrow<T>(y[k]);
+    }
     return r;
 }
 
