@@ -26,6 +26,7 @@ struct NormArgs {
     int64_t rows, width, stride;  // x: elements from row to row
     const void *weight, *bias;    // optional [width]
     bool wide_params;             // they are fp32 beside a 16-bit x
+    bool whole_params;            // they lie on 16-byte boundaries
     int relu;
     A eps;
     Drop drop;
@@ -36,14 +37,6 @@ struct NormArgs {
     A *partial;     // optional: [blocks, 2, width], sums of g * h and of g over a block's rows
 };
 
-// z of a row's elements: h * weight + bias.
-template <typename T, int VW>
-__device__ __forceinline__ void affine(const NormArgs<T> &a, const Acc<T> (&h)[VW], const Acc<T> (&w)[VW], const Acc<T> (&b)[VW],
-                                       Acc<T> (&z)[VW]) {
-#pragma unroll
-    for (int k = 0; k < VW; ++k) z[k] = fused(h[k], w[k], b[k]);
-}
-
 template <typename T, int VW>
 __device__ __forceinline__ void params_at(const NormArgs<T> &a, int64_t col, Acc<T> (&w)[VW], Acc<T> (&b)[VW]) {
 #pragma unroll
@@ -51,39 +44,29 @@ __device__ __forceinline__ void params_at(const NormArgs<T> &a, int64_t col, Acc
         w[k] = Acc<T>(1);
         b[k] = Acc<T>(0);
     }
-    if (a.weight) load_params<T, VW>(a.weight, a.wide_params, col, w);
-    if (a.bias) load_params<T, VW>(a.bias, a.wide_params, col, b);
+    if (a.weight) load_params<T, VW>(a.weight, a.wide_params, a.whole_params, col, w);
+    if (a.bias) load_params<T, VW>(a.bias, a.wide_params, a.whole_params, col, b);
 }
 
-// relu and dropout of z (NaN stays NaN).
-template <typename T, int VW>
-__device__ __forceinline__ void follow(const NormArgs<T> &a, int64_t element, uint64_t key, Acc<T> (&z)[VW]) {
-    using A = Acc<T>;
-    if (a.relu)
-#pragma unroll
-        for (int k = 0; k < VW; ++k) z[k] = z[k] < A(0) ? A(0) : z[k];
-    if (a.drop.threshold) drop_values<A, VW>(z, element, a.drop.threshold, (A)a.drop.scale, key);
-}
-
-// The gradient of z from that of the output.
-template <typename T, int VW>
-__device__ __forceinline__ void unfollow(const NormArgs<T> &a, int64_t element, uint64_t key, const Acc<T> (&z)[VW],
-                                         Acc<T> (&g)[VW]) {
-    using A = Acc<T>;
-    if (a.drop.threshold) drop_values<A, VW>(g, element, a.drop.threshold, (A)a.drop.scale, key);
-    if (a.relu)
-#pragma unroll
-        for (int k = 0; k < VW; ++k) g[k] = z[k] <= A(0) ? A(0) : g[k];
+// The dropout of a vector: by a verdict made before (of a row whose lanes have single elements), or by its own words.
+template <int VW, typename A>
+__device__ __forceinline__ void drop(const Drop &d, int64_t element, uint64_t key, bool decided, bool gone, A (&v)[VW]) {
+    if (!d.threshold) return;
+    if (decided) v[0] = gone ? A(0) : v[0] * (A)d.scale;
+    else drop_values<A, VW>(v, element, d.threshold, (A)d.scale, key);
 }
 
 template <int TEAM>
 constexpr int FORWARD_THREADS = TEAM > 32 ? TEAM : 256;
 template <int TEAM>
 constexpr int BACKWARD_THREADS = TEAM > 32 ? TEAM : 128;
+// Blocks of the backward kernel to a multiprocessor, by the registers that a lane's elements of so many words take.
+template <int TEAM, int WORDS>
+constexpr int BACKWARD_BLOCKS = std::max(1, (WORDS <= 4 ? 1024 : WORDS <= 8 ? 768 : WORDS <= 16 ? 512 : 256) / BACKWARD_THREADS<TEAM>);
 
 // The team's row, vector by vector; elements beyond the row are zero.
 template <typename T, int VW, int TEAM, int VPL>
-__device__ __forceinline__ void load_row(const T *row, int64_t width, int lane, Acc<T> (&v)[VPL][VW]) {
+__device__ __forceinline__ void load_row(const T *row, int width, int lane, Acc<T> (&v)[VPL][VW]) {
     Vec<T, VW> raw[VPL];
 #pragma unroll
     for (int p = 0; p < VPL; ++p) {
@@ -99,47 +82,61 @@ template <typename T, int VW, int TEAM, int VPL>
 __global__ void __launch_bounds__(FORWARD_THREADS<TEAM>) norm_kernel(const NormArgs<T> a) {
     using A = Acc<T>;
     constexpr int TEAMS = FORWARD_THREADS<TEAM> / TEAM;
-    __shared__ A shared[TEAMS * 2 * (TEAM > 32 ? TEAM / 32 : 1)];
-    const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
+    constexpr bool KEEP = VPL * VW <= 16;      // the parameters of a lane's columns stay in registers
+    constexpr bool VOTES = TEAM == 32 && VW == 1;  // a warp draws the words of its row together
+    constexpr int SUMS = VW % 2 == 0 ? 2 : 1;
+    __shared__ A shared[2 * (TEAM > 32 ? TEAM / 32 : 1)];
+    const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM, width = (int)a.width;
     const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
     int turn = 0;
     const A inv = A(1) / (A)a.width;
-    for (int64_t r = (int64_t)blockIdx.x * TEAMS + team; r < a.rows; r += (int64_t)gridDim.x * TEAMS) {
-        A v[VPL][VW], s[1] = {A(0)};
-        load_row<T, VW, TEAM, VPL>(a.x + r * a.stride, a.width, lane, v);
+    A w[KEEP ? VPL : 1][VW], b[KEEP ? VPL : 1][VW];
+    if constexpr (KEEP)
 #pragma unroll
         for (int p = 0; p < VPL; ++p)
+            if ((p * TEAM + lane) * VW < width) params_at<T, VW>(a, (p * TEAM + lane) * VW, w[p], b[p]);
+    for (int64_t r = (int64_t)blockIdx.x * TEAMS + team; r < a.rows; r += (int64_t)gridDim.x * TEAMS) {
+        A v[VPL][VW], two[SUMS] = {}, s[1];
+        load_row<T, VW, TEAM, VPL>(a.x + r * a.stride, width, lane, v);
+        uint32_t gone = 0;
+        if constexpr (VOTES)
+            if (a.drop.threshold) gone = dropped_of_row<VPL>(r * a.width, a.drop.threshold, key);
 #pragma unroll
-            for (int k = 0; k < VW; ++k) s[0] += v[p][k];
+        for (int p = 0; p < VPL; ++p) add(v[p], two);
+        s[0] = SUMS == 2 ? two[0] + two[SUMS - 1] : two[0];
         team_sum<A, TEAM, 1>(s, shared, turn);
         const A mean = s[0] * inv;
-        s[0] = A(0);
+        two[0] = two[SUMS - 1] = A(0);
 #pragma unroll
         for (int p = 0; p < VPL; ++p) {
-            const bool live = (p * TEAM + lane) * VW < a.width;
-#pragma unroll
-            for (int k = 0; k < VW; ++k) {
-                v[p][k] -= mean;
-                if (live) s[0] = fused(v[p][k], v[p][k], s[0]);
-            }
+            add_to_all(v[p], -mean);
+            if ((p * TEAM + lane) * VW < width) multiply_add(v[p], v[p], two);
         }
+        s[0] = SUMS == 2 ? two[0] + two[SUMS - 1] : two[0];
         team_sum<A, TEAM, 1>(s, shared, turn);
         const A rstd = inverse_root(fused(s[0], inv, a.eps));
         if (a.mean && lane == 0) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
         }
+        T *const out = a.out + r * a.width;
 #pragma unroll
         for (int p = 0; p < VPL; ++p) {
             const int col = (p * TEAM + lane) * VW;
-            if (col >= a.width) continue;
-            A w[VW], b[VW], z[VW];
-            params_at<T, VW>(a, col, w, b);
+            if (col >= width) continue;
+            A z[VW];
+            multiply_all(v[p], rstd);
+            if constexpr (KEEP) {
+                multiply_add_to(v[p], w[p], b[p], z);
+            } else {
+                params_at<T, VW>(a, col, w[0], b[0]);
+                multiply_add_to(v[p], w[0], b[0], z);
+            }
+            if (a.relu)  // (NaN stays NaN)
 #pragma unroll
-            for (int k = 0; k < VW; ++k) v[p][k] *= rstd;
-            affine<T, VW>(a, v[p], w, b, z);
-            follow<T, VW>(a, r * a.width + col, key, z);
-            vec_store<T, VW>(a.out + r * a.width + col, narrow_all<T, VW>(z));
+                for (int k = 0; k < VW; ++k) z[k] = z[k] < A(0) ? A(0) : z[k];
+            drop(a.drop, r * a.width + col, key, VOTES, gone >> p & 1u, z);
+            vec_store<T, VW>(out + col, narrow_all<T, VW>(z));
         }
     }
 }
@@ -147,12 +144,15 @@ __global__ void __launch_bounds__(FORWARD_THREADS<TEAM>) norm_kernel(const NormA
 // dx and a block's share of the parameters' gradients.  A lane keeps the same columns for all its rows, so their sums
 // stay in registers; teams of a warp, then the warps of the block, are added up in a fixed order at the end.
 template <typename T, int VW, int TEAM, int VPL>
-__global__ void __launch_bounds__(BACKWARD_THREADS<TEAM>) norm_backward_kernel(const NormArgs<T> a) {
+__global__ void __launch_bounds__(BACKWARD_THREADS<TEAM>, BACKWARD_BLOCKS<TEAM, VPL * VW * (int)sizeof(Acc<T>) / 4>) norm_backward_kernel(const NormArgs<T> a) {
     using A = Acc<T>;
     constexpr int THREADS = BACKWARD_THREADS<TEAM>, TEAMS = THREADS / TEAM, WARPS = THREADS / 32;
     constexpr int COLUMNS = TEAM * VPL * VW;
+    constexpr bool VOTES = TEAM == 32 && VW == 1;
+    constexpr int SUMS = VW % 2 == 0 ? 2 : 1;
     __shared__ A shared[TEAM > 32 ? 4 * TEAM / 32 : 2 * COLUMNS];
-    const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the launch that adds up the shares)
+    const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM, width = (int)a.width;
     const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
     int turn = 0;
     const A inv = A(1) / (A)a.width;
@@ -165,49 +165,57 @@ __global__ void __launch_bounds__(BACKWARD_THREADS<TEAM>) norm_backward_kernel(c
             w[p][k] = A(0);
             dw[p][k] = db[p][k] = A(0);
         }
-        if (col < a.width) {
+        if (col < width) {
             A b[VW];
             params_at<T, VW>(a, col, w[p], b);
         }
     }
     for (int64_t r = (int64_t)blockIdx.x * TEAMS + team; r < a.rows; r += (int64_t)gridDim.x * TEAMS) {
-        A h[VPL][VW], g[VPL][VW], s[2] = {A(0), A(0)};
+        A h[VPL][VW], g[VPL][VW], s0[SUMS] = {}, s1[SUMS] = {}, s[2];
         const A mean = a.mean[r], rstd = a.rstd[r];
-        load_row<T, VW, TEAM, VPL>(a.x + r * a.stride, a.width, lane, h);
-        load_row<T, VW, TEAM, VPL>(a.grad + r * a.width, a.width, lane, g);
+        load_row<T, VW, TEAM, VPL>(a.x + r * a.stride, width, lane, h);
+        load_row<T, VW, TEAM, VPL>(a.grad + r * a.width, width, lane, g);
+        uint32_t gone = 0;
+        if constexpr (VOTES)
+            if (a.drop.threshold) gone = dropped_of_row<VPL>(r * a.width, a.drop.threshold, key);
 #pragma unroll
         for (int p = 0; p < VPL; ++p) {
             const int col = (p * TEAM + lane) * VW;
-            if (col >= a.width) continue;
-#pragma unroll
-            for (int k = 0; k < VW; ++k) h[p][k] = (h[p][k] - mean) * rstd;
-            A z[VW];
+            if (col >= width) continue;
+            add_to_all(h[p], -mean);
+            multiply_all(h[p], rstd);
+            drop(a.drop, r * a.width + col, key, VOTES, gone >> p & 1u, g[p]);
             if (a.relu) {
-                A again[VW], b[VW];
+                A again[VW], b[VW], z[VW];
                 params_at<T, VW>(a, col, again, b);
-                affine<T, VW>(a, h[p], w[p], b, z);
-            }
-            unfollow<T, VW>(a, r * a.width + col, key, z, g[p]);
+                multiply_add_to(h[p], w[p], b, z);
 #pragma unroll
-            for (int k = 0; k < VW; ++k) {
-                dw[p][k] = fused(g[p][k], h[p][k], dw[p][k]);
-                db[p][k] += g[p][k];
-                g[p][k] *= w[p][k];
-                s[0] += g[p][k];
-                s[1] = fused(g[p][k], h[p][k], s[1]);
+                for (int k = 0; k < VW; ++k) g[p][k] = z[k] <= A(0) ? A(0) : g[p][k];
             }
+            multiply_add(g[p], h[p], dw[p]);
+            add(g[p], db[p]);
+            multiply_pairwise(g[p], w[p]);
+            add(g[p], s0);
+            multiply_add(g[p], h[p], s1);
         }
         if (!a.dx) continue;
+        s[0] = SUMS == 2 ? s0[0] + s0[SUMS - 1] : s0[0];
+        s[1] = SUMS == 2 ? s1[0] + s1[SUMS - 1] : s1[0];
         team_sum<A, TEAM, 2>(s, shared, turn);
         const A c0 = s[0] * inv, c1 = s[1] * inv;
+        T *const dx = a.dx + r * a.width;
 #pragma unroll
         for (int p = 0; p < VPL; ++p) {
             const int col = (p * TEAM + lane) * VW;
-            if (col >= a.width) continue;
-            A d[VW];
+            if (col >= width) continue;
+            // rstd * (u - (h * c1 + c0))
+            A minus_c1[VW];
 #pragma unroll
-            for (int k = 0; k < VW; ++k) d[k] = rstd * (g[p][k] - fused(h[p][k], c1, c0));
-            vec_store<T, VW>(a.dx + r * a.width + col, narrow_all<T, VW>(d));
+            for (int k = 0; k < VW; ++k) minus_c1[k] = -c1;
+            add_to_all(g[p], -c0);
+            multiply_add(h[p], minus_c1, g[p]);
+            multiply_all(g[p], rstd);
+            vec_store<T, VW>(dx + col, narrow_all<T, VW>(g[p]));
         }
     }
     if (!a.partial) return;
@@ -234,7 +242,7 @@ __global__ void __launch_bounds__(BACKWARD_THREADS<TEAM>) norm_backward_kernel(c
                     }
             __syncthreads();
         }
-        for (int c = threadIdx.x; c < a.width; c += THREADS) {
+        for (int c = threadIdx.x; c < width; c += THREADS) {
             mine[c] = shared[c];
             mine[a.width + c] = shared[COLUMNS + c];
         }
@@ -244,7 +252,7 @@ __global__ void __launch_bounds__(BACKWARD_THREADS<TEAM>) norm_backward_kernel(c
 #pragma unroll
             for (int k = 0; k < VW; ++k) {
                 const int col = (p * TEAM + lane) * VW + k;
-                if (col < a.width) {
+                if (col < width) {
                     mine[col] = dw[p][k];
                     mine[a.width + col] = db[p][k];
                 }
@@ -279,8 +287,9 @@ __global__ void __launch_bounds__(LONG_THREADS) norm_long_kernel(const NormArgs<
         for (int64_t c = threadIdx.x; c < a.width; c += LONG_THREADS) {
             A h[1] = {(widen(row[c]) - mean) * rstd}, w[1], b[1], z[1];
             params_at<T, 1>(a, c, w, b);
-            affine<T, 1>(a, h, w, b, z);
-            follow<T, 1>(a, r * a.width + c, key, z);
+            multiply_add_to(h, w, b, z);
+            if (a.relu && z[0] < A(0)) z[0] = A(0);
+            drop(a.drop, r * a.width + c, key, false, false, z);
             a.out[r * a.width + c] = narrow<T>(z[0]);
         }
     }
@@ -292,8 +301,9 @@ __device__ __forceinline__ void long_element(const NormArgs<T> &a, int64_t r, in
                                              Acc<T> &h, Acc<T> &g, Acc<T> &weight) {
     Acc<T> hat[1] = {(widen(a.x[r * a.stride + c]) - mean) * rstd}, grad[1] = {widen(a.grad[r * a.width + c])}, w[1], b[1], z[1];
     params_at<T, 1>(a, c, w, b);
-    affine<T, 1>(a, hat, w, b, z);
-    unfollow<T, 1>(a, r * a.width + c, key, z, grad);
+    multiply_add_to(hat, w, b, z);
+    drop(a.drop, r * a.width + c, key, false, false, grad);
+    if (a.relu && z[0] <= Acc<T>(0)) grad[0] = Acc<T>(0);
     h = hat[0];
     g = grad[0];
     weight = w[0];
@@ -350,7 +360,9 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(const Acc<T> *partial, 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     A s = A(0);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (c < 2 * width)
+#pragma unroll 4
         for (int64_t b = warp; b < blocks; b += 32) s += partial[b * 2 * width + c];
     sums[warp][lane] = s;
     __syncthreads();
@@ -367,24 +379,44 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(const Acc<T> *partial, 
 // ---------------------------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------------------------
-// Rows of `vectors` vectors: the least team that holds them.  f(team, vectors a lane) with both as constants.
+// Rows of `vectors` vectors of VW elements: the least team that holds them with at most 32 elements a lane.
+// f(team, vectors a lane) with both as constants.
 template <int N>
 struct Num {
     static constexpr int value = N;
 };
-template <typename F>
+template <int VW>
+constexpr int MOST_VPL = 32 / VW < 8 && VW > 1 ? 32 / VW : VW > 1 ? 8 : 32;
+template <int VW>
+constexpr int64_t TEAM_VECTORS = VW > 1 ? 256 * MOST_VPL<VW> : 1024;
+template <int VW, typename F>
 static int with_team(int64_t vectors, F &&f) {
     if (vectors <= 2) return f(Num<2>(), Num<1>());
     if (vectors <= 4) return f(Num<4>(), Num<1>());
     if (vectors <= 8) return f(Num<8>(), Num<1>());
     if (vectors <= 16) return f(Num<8>(), Num<2>());
-    if (vectors <= 32) return f(Num<8>(), Num<4>());
-    if (vectors <= 64) return f(Num<32>(), Num<2>());
-    if (vectors <= 128) return f(Num<32>(), Num<4>());
-    if (vectors <= 512) return f(Num<128>(), Num<4>());
-    return f(Num<512>(), Num<4>());
+    if constexpr (VW == 1) {
+        if (vectors <= 32) return f(Num<32>(), Num<1>());
+        if (vectors <= 64) return f(Num<32>(), Num<2>());
+        if (vectors <= 128) return f(Num<32>(), Num<4>());
+        if (vectors <= 256) return f(Num<32>(), Num<8>());
+        if (vectors <= 512) return f(Num<32>(), Num<16>());
+        return f(Num<32>(), Num<32>());
+    } else {
+        if (vectors <= 32) return f(Num<8>(), Num<4>());
+        if (vectors <= 64) return f(Num<16>(), Num<4>());
+        if (vectors <= 128) return f(Num<32>(), Num<4>());
+        if constexpr (MOST_VPL<VW> == 8) {
+            if (vectors <= 256) return f(Num<32>(), Num<8>());
+        } else {
+            if (vectors <= 256) return f(Num<128>(), Num<2>());
+        }
+        if (vectors <= 512) return f(Num<128>(), Num<4>());
+        if constexpr (MOST_VPL<VW> == 8)
+            if (vectors <= 1024) return f(Num<128>(), Num<8>());
+        return f(Num<256>(), Num<MOST_VPL<VW>>());
+    }
 }
-constexpr int64_t TEAM_VECTORS = 512 * 4;
 
 // Elements a vector holds: 16 bytes where rows and pointers allow, else one.
 template <typename T>
@@ -397,11 +429,23 @@ static bool vectors_fit(size_t item, int64_t width, int64_t stride, std::initial
     return width % n == 0 && stride % n == 0 && (bits & 15) == 0;
 }
 
+template <typename Kernel>
+static int resident_blocks(Kernel *kernel, int threads) {
+    int blocks = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, 0) != cudaSuccess) {
+        cudaGetLastError();
+        return 1;
+    }
+    return std::max(1, blocks);
+}
+
 template <typename T, int VW>
 static int forward_typed(const NormArgs<T> &a, cudaStream_t stream) {
-    return with_team(a.width / VW, [&](auto team, auto vpl) -> int {
+    return with_team<VW>(a.width / VW, [&](auto team, auto vpl) -> int {
         constexpr int TEAM = decltype(team)::value, VPL = decltype(vpl)::value, THREADS = FORWARD_THREADS<TEAM>;
-        const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(a.rows, THREADS / TEAM), SMS * 8);
+        // (no more than run at once: blocks that began when others end would double the time)
+        static const int resident = resident_blocks(norm_kernel<T, VW, TEAM, VPL>, THREADS);
+        const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(a.rows, THREADS / TEAM), SMS * resident);
         norm_kernel<T, VW, TEAM, VPL><<<blocks, THREADS, 0, stream>>>(a);
         CGNN_LAUNCH_CHECK();
         return CGNN_OK;
@@ -411,44 +455,48 @@ static int forward_typed(const NormArgs<T> &a, cudaStream_t stream) {
 template <typename T>
 static int forward(const NormArgs<T> &a, cudaStream_t stream) {
     constexpr int VW = WIDEST<T>;
-    if (vectors_fit(sizeof(T), a.width, a.stride, {a.x, a.out}) && a.width / VW <= TEAM_VECTORS)
+    if (vectors_fit(sizeof(T), a.width, a.stride, {a.x, a.out}) && a.width / VW <= TEAM_VECTORS<VW>)
         return forward_typed<T, VW>(a, stream);
-    if (a.width <= TEAM_VECTORS) return forward_typed<T, 1>(a, stream);
+    if (a.width <= TEAM_VECTORS<1>) return forward_typed<T, 1>(a, stream);
     norm_long_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, SMS * 4), LONG_THREADS, 0, stream>>>(a);
     CGNN_LAUNCH_CHECK();
     return CGNN_OK;
 }
 
-// Blocks of a backward launch, each of which leaves a partial row.
-template <int TEAM>
+// Blocks of a backward launch, each of which leaves a partial row: those that run at once.
+template <int TEAM, int WORDS>
 static int64_t backward_blocks(int64_t rows) {
-    return std::min<int64_t>(ceil_div(rows, BACKWARD_THREADS<TEAM> / TEAM), TEAM > 128 ? SMS : SMS * 4);
+    return std::min<int64_t>(ceil_div(rows, BACKWARD_THREADS<TEAM> / TEAM), SMS * BACKWARD_BLOCKS<TEAM, WORDS>);
 }
 
 static int64_t column_blocks(int64_t rows, int64_t width) {
     return std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, COLUMN_ROWS), SMS * 8 / std::max<int64_t>(1, width / 256)));
 }
 
-// Partial rows of a backward pass, the most of the ways it may go.
+// Partial rows of a backward pass by vectors of VW elements, or the most of the ways it may go.
+template <typename A, int VW>
+static int64_t partial_rows(int64_t rows, int64_t width) {
+    if (width / VW > TEAM_VECTORS<VW>) return column_blocks(rows, width);
+    int64_t blocks = 0;
+    with_team<VW>(width / VW, [&](auto team, auto vpl) -> int {
+        blocks = backward_blocks<decltype(team)::value, decltype(vpl)::value * VW * (int)sizeof(A) / 4>(rows);
+        return 0;
+    });
+    return blocks;
+}
 static int64_t partial_rows(size_t item, int64_t rows, int64_t width) {
-    int64_t most = 0;
-    for (int64_t vectors : {width / (int64_t)(16 / item), width}) {
-        if (vectors > TEAM_VECTORS)
-            most = std::max(most, column_blocks(rows, width));
-        else
-            with_team(vectors, [&](auto team, auto) -> int {
-                most = std::max(most, backward_blocks<decltype(team)::value>(rows));
-                return 0;
-            });
-    }
-    return most;
+    const int64_t single = item == 8 ? partial_rows<double, 1>(rows, width) : partial_rows<float, 1>(rows, width);
+    const int64_t vectors = item == 8   ? partial_rows<double, 2>(rows, width)
+                            : item == 4 ? partial_rows<float, 4>(rows, width)
+                                        : partial_rows<float, 8>(rows, width);
+    return std::max(single, vectors);
 }
 
 template <typename T, int VW>
 static int backward_typed(const NormArgs<T> &a, int64_t *blocks, cudaStream_t stream) {
-    return with_team(a.width / VW, [&](auto team, auto vpl) -> int {
+    return with_team<VW>(a.width / VW, [&](auto team, auto vpl) -> int {
         constexpr int TEAM = decltype(team)::value, VPL = decltype(vpl)::value;
-        *blocks = backward_blocks<TEAM>(a.rows);
+        *blocks = backward_blocks<TEAM, VPL * VW * (int)sizeof(Acc<T>) / 4>(a.rows);
         norm_backward_kernel<T, VW, TEAM, VPL><<<(unsigned)*blocks, BACKWARD_THREADS<TEAM>, 0, stream>>>(a);
         CGNN_LAUNCH_CHECK();
         return CGNN_OK;
@@ -460,9 +508,9 @@ static int backward(const NormArgs<T> &a, void *dweight, void *dbias, cudaStream
     constexpr int VW = WIDEST<T>;
     int64_t blocks = 0;
     int rc = CGNN_OK;
-    if (vectors_fit(sizeof(T), a.width, a.stride, {a.x, a.grad, a.dx}) && a.width / VW <= TEAM_VECTORS) {
+    if (vectors_fit(sizeof(T), a.width, a.stride, {a.x, a.grad, a.dx}) && a.width / VW <= TEAM_VECTORS<VW>) {
         rc = backward_typed<T, VW>(a, &blocks, stream);
-    } else if (a.width <= TEAM_VECTORS) {
+    } else if (a.width <= TEAM_VECTORS<1>) {
         rc = backward_typed<T, 1>(a, &blocks, stream);
     } else {
         if (a.dx) {
@@ -478,9 +526,17 @@ static int backward(const NormArgs<T> &a, void *dweight, void *dbias, cudaStream
         }
     }
     if (rc != CGNN_OK || !a.partial) return rc;
-    norm_sums_kernel<T><<<(unsigned)ceil_div(2 * a.width, 32), 1024, 0, stream>>>(a.partial, blocks, a.width, dweight, dbias,
-                                                                                  a.wide_params);
-    CGNN_LAUNCH_CHECK();
+    // Its blocks are there when the last of the launch before it end, and wait for them.
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)ceil_div(2 * a.width, 32));
+    config.blockDim = dim3(1024);
+    config.stream = stream;
+    cudaLaunchAttribute follows = {};
+    follows.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    follows.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &follows;
+    config.numAttrs = 1;
+    CGNN_CUDA(cudaLaunchKernelEx(&config, norm_sums_kernel<T>, (const Acc<T> *)a.partial, blocks, a.width, dweight, dbias, a.wide_params));
     return CGNN_OK;
 }
 
@@ -513,6 +569,7 @@ static NormArgs<T> args_of(const NormCall &c, int relu, uint64_t seed, const int
     a.weight = c.weight;
     a.bias = c.bias;
     a.wide_params = c.param_dtype == CGNN_F32 && c.dtype != CGNN_F32;
+    a.whole_params = (((uintptr_t)c.weight | (uintptr_t)c.bias) & 15) == 0;
     a.relu = relu;
     a.drop = Drop::of(c.p, seed, device_seed);
     return a;

@@ -51,6 +51,31 @@ __device__ __forceinline__ void drop_values(T (&y)[VW], int64_t first, uint32_t 
     }
 }
 
+// Which of the elements first + lane + 32 p of a row, p < VPL, a lane loses (bit p), for a whole warp together: a lane
+// draws the four words of one block, and votes hand each word's verdict to the lane whose element it is.  A lane alone
+// would draw a block for every element.
+template <int VPL>
+__device__ __forceinline__ uint32_t dropped_of_row(int64_t first, uint32_t threshold, uint64_t seed) {
+    constexpr int WINDOWS = (32 * VPL + 3 + 127) / 128;  // of 32 blocks; the row may begin inside a block
+    const int lane = threadIdx.x & 31, ahead = (int)(first & 3) + lane, word = ahead & 3;
+    uint32_t verdict[WINDOWS], gone = 0;
+#pragma unroll
+    for (int w = 0; w < WINDOWS; ++w) {
+        const uint4 r = philox4x32_7(((uint64_t)first >> 2) + 32 * w + lane, seed);
+        const uint32_t v0 = __ballot_sync(0xffffffffu, r.x < threshold), v1 = __ballot_sync(0xffffffffu, r.y < threshold);
+        const uint32_t v2 = __ballot_sync(0xffffffffu, r.z < threshold), v3 = __ballot_sync(0xffffffffu, r.w < threshold);
+        verdict[w] = word == 0 ? v0 : word == 1 ? v1 : word == 2 ? v2 : v3;
+    }
+#pragma unroll
+    for (int p = 0; p < VPL; ++p) {
+        const int at = 32 * (p % 4) + ahead;  // elements from the beginning of window p / 4
+        uint32_t bits = verdict[p / 4];
+        if (p % 4 == 3 && p / 4 + 1 < WINDOWS && at >= 128) bits = verdict[p / 4 + 1];
+        gone |= (bits >> ((at & 127) >> 2) & 1u) << p;
+    }
+    return gone;
+}
+
 // A probability as the bound its random words are compared with: an element is dropped when its word lies below.
 static inline uint32_t drop_threshold_of(double p) {
     const double bound = p * 4294967296.0;

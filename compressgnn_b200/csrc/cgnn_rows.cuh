@@ -77,18 +77,157 @@ __device__ __forceinline__ Vec<T, VW> narrow_all(const Acc<T> (&y)[VW]) {
     return r;
 }
 
-// VW parameters (weight or bias) from `at` on, of the matrix' type or, beside 16-bit matrices, fp32.
+// VW parameters (weight or bias) from `at` on, of the matrix' type or, beside 16-bit matrices, fp32.  whole: they lie on
+// 16-byte boundaries every VW.
 template <typename T, int VW>
-__device__ __forceinline__ void load_params(const void *params, bool wide, int64_t at, Acc<T> (&y)[VW]) {
-    if (sizeof(T) == 2 && wide) {
-        const float *p = static_cast<const float *>(params) + at;
+__device__ __forceinline__ void load_params(const void *params, bool wide, bool whole, int64_t at, Acc<T> (&y)[VW]) {
+    if constexpr (sizeof(T) == 2) {
+        if (wide) {
+            const float *p = static_cast<const float *>(params) + at;
+            if constexpr (VW % 4 == 0) {
+                if (whole) {
 #pragma unroll
-        for (int k = 0; k < VW; ++k) y[k] = (Acc<T>)__ldg(p + k);
+                    for (int k = 0; k < VW; k += 4) {
+                        const float4 four = *reinterpret_cast<const float4 *>(p + k);
+                        y[k] = four.x;
+                        y[k + 1] = four.y;
+                        y[k + 2] = four.z;
+                        y[k + 3] = four.w;
+                    }
+                    return;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < VW; ++k) y[k] = p[k];
+            return;
+        }
+    }
+    const T *p = static_cast<const T *>(params) + at;
+    if (whole) {
+        widen_all<T, VW>(vec_load<T, VW>(p), y);
     } else {
-        const T *p = static_cast<const T *>(params) + at;
 #pragma unroll
         for (int k = 0; k < VW; ++k) y[k] = widen(p[k]);
     }
+}
+
+// Arithmetic on a lane's vector.  fp32 has instructions for two numbers at once, which round like the single ones.
+template <int VW>
+__device__ __forceinline__ void add_to_all(float (&v)[VW], float a) {
+    if constexpr (VW % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < VW; k += 2) {
+            const float2 d = __fadd2_rn(make_float2(v[k], v[k + 1]), make_float2(a, a));
+            v[k] = d.x;
+            v[k + 1] = d.y;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VW; ++k) v[k] += a;
+    }
+}
+template <int VW>
+__device__ __forceinline__ void add_to_all(double (&v)[VW], double a) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) v[k] += a;
+}
+template <int VW>
+__device__ __forceinline__ void multiply_all(float (&v)[VW], float a) {
+    if constexpr (VW % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < VW; k += 2) {
+            const float2 d = __fmul2_rn(make_float2(v[k], v[k + 1]), make_float2(a, a));
+            v[k] = d.x;
+            v[k + 1] = d.y;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VW; ++k) v[k] *= a;
+    }
+}
+template <int VW>
+__device__ __forceinline__ void multiply_all(double (&v)[VW], double a) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) v[k] *= a;
+}
+template <int VW>
+__device__ __forceinline__ void multiply_pairwise(float (&v)[VW], const float (&w)[VW]) {
+    if constexpr (VW % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < VW; k += 2) {
+            const float2 d = __fmul2_rn(make_float2(v[k], v[k + 1]), make_float2(w[k], w[k + 1]));
+            v[k] = d.x;
+            v[k + 1] = d.y;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VW; ++k) v[k] *= w[k];
+    }
+}
+template <int VW>
+__device__ __forceinline__ void multiply_pairwise(double (&v)[VW], const double (&w)[VW]) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) v[k] *= w[k];
+}
+// s += a * b, element by element, a vector's elements by turns into the SUMS places of s (SUMS == VW: each its own).
+template <int VW, int SUMS>
+__device__ __forceinline__ void multiply_add(const float (&a)[VW], const float (&b)[VW], float (&s)[SUMS]) {
+    if constexpr (VW % 2 == 0 && SUMS % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < VW; k += 2) {
+            const float2 d = __ffma2_rn(make_float2(a[k], a[k + 1]), make_float2(b[k], b[k + 1]),
+                                        make_float2(s[k % SUMS], s[k % SUMS + 1]));
+            s[k % SUMS] = d.x;
+            s[k % SUMS + 1] = d.y;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VW; ++k) s[k % SUMS] = fmaf(a[k], b[k], s[k % SUMS]);
+    }
+}
+template <int VW, int SUMS>
+__device__ __forceinline__ void multiply_add(const double (&a)[VW], const double (&b)[VW], double (&s)[SUMS]) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) s[k % SUMS] = fma(a[k], b[k], s[k % SUMS]);
+}
+template <int VW, int SUMS>
+__device__ __forceinline__ void add(const float (&a)[VW], float (&s)[SUMS]) {
+    if constexpr (VW % 2 == 0 && SUMS % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < VW; k += 2) {
+            const float2 d = __fadd2_rn(make_float2(a[k], a[k + 1]), make_float2(s[k % SUMS], s[k % SUMS + 1]));
+            s[k % SUMS] = d.x;
+            s[k % SUMS + 1] = d.y;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VW; ++k) s[k % SUMS] += a[k];
+    }
+}
+template <int VW, int SUMS>
+__device__ __forceinline__ void add(const double (&a)[VW], double (&s)[SUMS]) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) s[k % SUMS] += a[k];
+}
+// z = h * w + b
+template <int VW>
+__device__ __forceinline__ void multiply_add_to(const float (&h)[VW], const float (&w)[VW], const float (&b)[VW], float (&z)[VW]) {
+    if constexpr (VW % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < VW; k += 2) {
+            const float2 d = __ffma2_rn(make_float2(h[k], h[k + 1]), make_float2(w[k], w[k + 1]), make_float2(b[k], b[k + 1]));
+            z[k] = d.x;
+            z[k + 1] = d.y;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VW; ++k) z[k] = fmaf(h[k], w[k], b[k]);
+    }
+}
+template <int VW>
+__device__ __forceinline__ void multiply_add_to(const double (&h)[VW], const double (&w)[VW], const double (&b)[VW], double (&z)[VW]) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) z[k] = fma(h[k], w[k], b[k]);
 }
 
 __device__ __forceinline__ float inverse_root(float x) { return rsqrtf(x); }
