@@ -6,6 +6,8 @@
 
 namespace cgnn {
 
+constexpr int SMS = 148;
+
 template <typename T>
 struct DropArgs {
     const T *x, *residual;  // residual: optional
@@ -14,66 +16,69 @@ struct DropArgs {
     Drop drop;
 };
 
-// A thread takes UNITS of VW elements (whole blocks of four random words), a block's threads side by side.  WIDE: the
-// arrays lie on 16-byte boundaries and move by vectors; otherwise element by element, with the same words.
-template <typename T, int VW, int UNITS, bool WIDE>
-__global__ void __launch_bounds__(256) dropout_kernel(const DropArgs<T> a) {
+// A block takes tiles of whole vectors, UNITS a thread, side by side; the elements behind the last tile and arrays that
+// do not lie on vector boundaries go element by element, a thread per block of four random words.
+template <typename T, int VW, int UNITS, bool ADDED>
+__global__ void __launch_bounds__(256) dropout_kernel(const DropArgs<T> a, int64_t tiles) {
     using A = Acc<T>;
-    const uint64_t key = a.drop.key();
+    Philox words(a.drop.key());
     const A scale = (A)a.drop.scale;
-    const int64_t step = (int64_t)blockDim.x * VW;
-    for (int64_t base = (int64_t)blockIdx.x * step * UNITS; base < a.n; base += (int64_t)gridDim.x * step * UNITS) {
-        const int64_t first = base + threadIdx.x * VW;
-        Vec<T, VW> x[UNITS], r[UNITS];
+    constexpr int TILE = 256 * VW * UNITS;
+    for (int64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
+        const T *const x = a.x + i * TILE, *const residual = ADDED ? a.residual + i * TILE : nullptr;
+        T *const out = a.out + i * TILE;
+        Vec<T, VW> v[UNITS], r[UNITS];
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
-            const int64_t at = first + u * step;
-            x[u] = r[u] = vec_zero<T, VW>();
-            if (WIDE && at + VW <= a.n) {
-                x[u] = vec_load<T, VW>(a.x + at);
-                if (a.residual) r[u] = vec_load<T, VW>(a.residual + at);
-            } else {
-#pragma unroll
-                for (int k = 0; k < VW; ++k)
-                    if (at + k < a.n) {
-                        x[u].v[k] = a.x[at + k];
-                        if (a.residual) r[u].v[k] = a.residual[at + k];
-                    }
-            }
+            const int at = (u * 256 + threadIdx.x) * VW;
+            v[u] = vec_load<T, VW>(x + at);
+            if (ADDED) r[u] = vec_load<T, VW>(residual + at);
         }
+        PhiloxRun run(words, (uint64_t)(i * (TILE / 4)), TILE / 4);
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
-            const int64_t at = first + u * step;
-            if (at >= a.n) break;
+            const int at = (u * 256 + threadIdx.x) * VW;
             A y[VW];
-            widen_all<T, VW>(x[u], y);
-            drop_values<A, VW>(y, at, a.drop.threshold, scale, key);
-            if (a.residual)
-#pragma unroll
-                for (int k = 0; k < VW; ++k) y[k] += widen(r[u].v[k]);
-            const Vec<T, VW> out = narrow_all<T, VW>(y);
-            if (WIDE && at + VW <= a.n) {
-                vec_store<T, VW>(a.out + at, out);
-            } else {
-#pragma unroll
-                for (int k = 0; k < VW; ++k)
-                    if (at + k < a.n) a.out[at + k] = out.v[k];
+            widen_all<T, VW>(v[u], y);
+            drop_blocks<A, VW>(y, (uint32_t)at / 4, a.drop.threshold, scale, run);
+            if (ADDED) {
+                A z[VW];
+                widen_all<T, VW>(r[u], z);
+                add(z, y);
             }
+            vec_store<T, VW>(out + at, narrow_all<T, VW>(y));
         }
     }
+    const int64_t done = tiles * TILE;
+    for (int64_t first = done + ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; first < a.n; first += (int64_t)gridDim.x * 256 * 4) {
+        const uint4 q = words((uint64_t)first >> 2);
+        const uint32_t word[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (first + k < a.n) {
+                A y = word[k] < a.drop.threshold ? A(0) : widen(a.x[first + k]) * scale;
+                if (ADDED) y += widen(a.residual[first + k]);
+                a.out[first + k] = narrow<T>(y);
+            }
+    }
+}
+
+template <typename T, bool ADDED>
+static int dropout_typed(const DropArgs<T> &a, cudaStream_t stream) {
+        constexpr int VW = sizeof(T) == 2 ? 8 : 4, UNITS = 4, TILE = 256 * VW * UNITS;
+    const bool vectors = (((uintptr_t)a.x | (uintptr_t)a.residual | (uintptr_t)a.out) & (sizeof(T) * VW - 1)) == 0;
+    const int64_t tiles = vectors ? a.n / TILE : 0, rest = ceil_div(a.n - tiles * TILE, 1024);
+    static const int resident = resident_blocks(dropout_kernel<T, VW, UNITS, ADDED>, 256);
+    const unsigned blocks = (unsigned)std::min<int64_t>(std::max(tiles, rest), SMS * resident);
+    dropout_kernel<T, VW, UNITS, ADDED><<<blocks, 256, 0, stream>>>(a, tiles);
+    CGNN_LAUNCH_CHECK();
+    return CGNN_OK;
 }
 
 template <typename T>
 static int dropout(int64_t n, const void *x, const void *residual, const Drop &drop, void *out, cudaStream_t stream) {
-    constexpr int VW = sizeof(T) == 2 ? 8 : 4, UNITS = 2;
     const DropArgs<T> a{(const T *)x, (const T *)residual, (T *)out, n, drop};
-    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n, 256 * VW * UNITS), 148 * 8);
-    if ((((uintptr_t)x | (uintptr_t)residual | (uintptr_t)out) & (sizeof(T) * VW - 1)) == 0)
-        dropout_kernel<T, VW, UNITS, true><<<blocks, 256, 0, stream>>>(a);
-    else
-        dropout_kernel<T, VW, UNITS, false><<<blocks, 256, 0, stream>>>(a);
-    CGNN_LAUNCH_CHECK();
-    return CGNN_OK;
+    return residual ? dropout_typed<T, true>(a, stream) : dropout_typed<T, false>(a, stream);
 }
 
 }  // namespace cgnn

@@ -50,7 +50,7 @@ struct ExpandArgs {
 template <typename T, int VW>
 __device__ __forceinline__ void drop_vector(Vec<T, VW> &y, int64_t first, uint32_t threshold, T keep_scale,
                                             uint64_t seed) {
-    drop_values<T, VW>(y.v, first, threshold, keep_scale, seed);
+    drop_values<T, VW>(y.v, first, threshold, keep_scale, [&](uint64_t counter) { return philox4x32_7(counter, seed); });
 }
 
 // A group of LPR lanes expands LPR consecutive node rows per step: lane l reads index[r0 + l]

@@ -26,7 +26,7 @@ struct NormArgs {
     int64_t rows, width, stride;  // x: elements from row to row
     const void *weight, *bias;    // optional [width]
     bool wide_params;             // they are fp32 beside a 16-bit x
-    bool whole_params;            // they lie on 16-byte boundaries
+    bool whole_params;            // they begin on 32-byte boundaries
     int relu;
     A eps;
     Drop drop;
@@ -48,13 +48,23 @@ __device__ __forceinline__ void params_at(const NormArgs<T> &a, int64_t col, Acc
     if (a.bias) load_params<T, VW>(a.bias, a.wide_params, a.whole_params, col, b);
 }
 
-// The dropout of a vector: by a verdict made before (of a row whose lanes have single elements), or by its own words.
+// The dropout of a vector of a row: by a verdict made before (of a row whose lanes have single elements), by the words of
+// whole blocks from the row's first one on, or by its own words.
 template <int VW, typename A>
-__device__ __forceinline__ void drop(const Drop &d, int64_t element, uint64_t key, bool decided, bool gone, A (&v)[VW]) {
-    if (!d.threshold) return;
+__device__ __forceinline__ void drop(const Drop &d, int64_t row_begin, int col, Philox &words, PhiloxRun &run, bool decided, bool gone,
+                                     A (&v)[VW]) {
     if (decided) v[0] = gone ? A(0) : v[0] * (A)d.scale;
-    else drop_values<A, VW>(v, element, d.threshold, (A)d.scale, key);
+    else if constexpr (VW % 4 == 0) drop_blocks<A, VW>(v, (uint32_t)col / 4, d.threshold, (A)d.scale, run);
+    else drop_values<A, VW>(v, row_begin + col, d.threshold, (A)d.scale, words);
 }
+
+// max(z, 0); NaN stays NaN.
+__device__ __forceinline__ float positive(float z) {
+    float y;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(z));
+    return y;
+}
+__device__ __forceinline__ double positive(double z) { return z < 0.0 ? 0.0 : z; }
 
 template <int TEAM>
 constexpr int FORWARD_THREADS = TEAM > 32 ? TEAM : 256;
@@ -62,32 +72,29 @@ template <int TEAM>
 constexpr int BACKWARD_THREADS = TEAM > 32 ? TEAM : 128;
 // Blocks of the backward kernel to a multiprocessor, by the registers that a lane's elements of so many words take.
 template <int TEAM, int WORDS>
-constexpr int BACKWARD_BLOCKS = std::max(1, (WORDS <= 4 ? 1024 : WORDS <= 8 ? 768 : WORDS <= 16 ? 512 : 256) / BACKWARD_THREADS<TEAM>);
+constexpr int BACKWARD_BLOCKS = std::max(1, (WORDS <= 4 ? 768 : WORDS <= 8 ? 512 : WORDS <= 16 ? 384 : 256) / BACKWARD_THREADS<TEAM>);
 
 // The team's row, vector by vector; elements beyond the row are zero.
 template <typename T, int VW, int TEAM, int VPL>
-__device__ __forceinline__ void load_row(const T *row, int width, int lane, Acc<T> (&v)[VPL][VW]) {
-    Vec<T, VW> raw[VPL];
+__device__ __forceinline__ void load_row(const T *row, int width, int lane, Vec<T, VW> (&raw)[VPL]) {
 #pragma unroll
     for (int p = 0; p < VPL; ++p) {
         const int col = (p * TEAM + lane) * VW;
         raw[p] = vec_zero<T, VW>();
         if (col < width) raw[p] = vec_load<T, VW>(row + col);
     }
-#pragma unroll
-    for (int p = 0; p < VPL; ++p) widen_all<T, VW>(raw[p], v[p]);
 }
 
-template <typename T, int VW, int TEAM, int VPL>
-__global__ void __launch_bounds__(FORWARD_THREADS<TEAM>) norm_kernel(const NormArgs<T> a) {
+template <typename T, int VW, int TEAM, int VPL, bool DROP>
+__global__ void __launch_bounds__(FORWARD_THREADS<TEAM>, 512 / FORWARD_THREADS<TEAM>) norm_kernel(const NormArgs<T> a) {
     using A = Acc<T>;
     constexpr int TEAMS = FORWARD_THREADS<TEAM> / TEAM;
-    constexpr bool KEEP = VPL * VW <= 16;      // the parameters of a lane's columns stay in registers
+        constexpr bool KEEP = VPL * VW <= 16;      // the parameters of a lane's columns stay in registers
     constexpr bool VOTES = TEAM == 32 && VW == 1;  // a warp draws the words of its row together
     constexpr int SUMS = VW % 2 == 0 ? 2 : 1;
     __shared__ A shared[2 * (TEAM > 32 ? TEAM / 32 : 1)];
     const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM, width = (int)a.width;
-    const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
+    Philox words(DROP ? a.drop.key() : 0);
     int turn = 0;
     const A inv = A(1) / (A)a.width;
     A w[KEEP ? VPL : 1][VW], b[KEEP ? VPL : 1][VW];
@@ -95,12 +102,20 @@ __global__ void __launch_bounds__(FORWARD_THREADS<TEAM>) norm_kernel(const NormA
 #pragma unroll
         for (int p = 0; p < VPL; ++p)
             if ((p * TEAM + lane) * VW < width) params_at<T, VW>(a, (p * TEAM + lane) * VW, w[p], b[p]);
-    for (int64_t r = (int64_t)blockIdx.x * TEAMS + team; r < a.rows; r += (int64_t)gridDim.x * TEAMS) {
+    // While a row is worked on the next one is on its way.
+    Vec<T, VW> raw[VPL];
+    const int64_t step = (int64_t)gridDim.x * TEAMS;
+    int64_t r = (int64_t)blockIdx.x * TEAMS + team;
+    if (r < a.rows) load_row<T, VW, TEAM, VPL>(a.x + r * a.stride, width, lane, raw);
+    for (; r < a.rows; r += step) {
         A v[VPL][VW], two[SUMS] = {}, s[1];
-        load_row<T, VW, TEAM, VPL>(a.x + r * a.stride, width, lane, v);
+#pragma unroll
+        for (int p = 0; p < VPL; ++p) widen_all<T, VW>(raw[p], v[p]);
+        if (r + step < a.rows) load_row<T, VW, TEAM, VPL>(a.x + (r + step) * a.stride, width, lane, raw);
         uint32_t gone = 0;
+        PhiloxRun run(words, (uint64_t)(r * a.width) >> 2, (uint32_t)width >> 2);
         if constexpr (VOTES)
-            if (a.drop.threshold) gone = dropped_of_row<VPL>(r * a.width, a.drop.threshold, key);
+            if (DROP) gone = dropped_of_row<VPL>(r * a.width, a.drop.threshold, words);
 #pragma unroll
         for (int p = 0; p < VPL; ++p) add(v[p], two);
         s[0] = SUMS == 2 ? two[0] + two[SUMS - 1] : two[0];
@@ -132,10 +147,10 @@ __global__ void __launch_bounds__(FORWARD_THREADS<TEAM>) norm_kernel(const NormA
                 params_at<T, VW>(a, col, w[0], b[0]);
                 multiply_add_to(v[p], w[0], b[0], z);
             }
-            if (a.relu)  // (NaN stays NaN)
+            if (a.relu)
 #pragma unroll
-                for (int k = 0; k < VW; ++k) z[k] = z[k] < A(0) ? A(0) : z[k];
-            drop(a.drop, r * a.width + col, key, VOTES, gone >> p & 1u, z);
+                for (int k = 0; k < VW; ++k) z[k] = positive(z[k]);
+            if (DROP) drop(a.drop, r * a.width, col, words, run, VOTES, gone >> p & 1u, z);
             vec_store<T, VW>(out + col, narrow_all<T, VW>(z));
         }
     }
@@ -143,7 +158,7 @@ __global__ void __launch_bounds__(FORWARD_THREADS<TEAM>) norm_kernel(const NormA
 
 // dx and a block's share of the parameters' gradients.  A lane keeps the same columns for all its rows, so their sums
 // stay in registers; teams of a warp, then the warps of the block, are added up in a fixed order at the end.
-template <typename T, int VW, int TEAM, int VPL>
+template <typename T, int VW, int TEAM, int VPL, bool DROP>
 __global__ void __launch_bounds__(BACKWARD_THREADS<TEAM>, BACKWARD_BLOCKS<TEAM, VPL * VW * (int)sizeof(Acc<T>) / 4>) norm_backward_kernel(const NormArgs<T> a) {
     using A = Acc<T>;
     constexpr int THREADS = BACKWARD_THREADS<TEAM>, TEAMS = THREADS / TEAM, WARPS = THREADS / 32;
@@ -153,7 +168,7 @@ __global__ void __launch_bounds__(BACKWARD_THREADS<TEAM>, BACKWARD_BLOCKS<TEAM, 
     __shared__ A shared[TEAM > 32 ? 4 * TEAM / 32 : 2 * COLUMNS];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the launch that adds up the shares)
     const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM, width = (int)a.width;
-    const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
+    Philox words(DROP ? a.drop.key() : 0);
     int turn = 0;
     const A inv = A(1) / (A)a.width;
     A w[VPL][VW], dw[VPL][VW], db[VPL][VW];
@@ -170,21 +185,38 @@ __global__ void __launch_bounds__(BACKWARD_THREADS<TEAM>, BACKWARD_BLOCKS<TEAM, 
             params_at<T, VW>(a, col, w[p], b);
         }
     }
-    for (int64_t r = (int64_t)blockIdx.x * TEAMS + team; r < a.rows; r += (int64_t)gridDim.x * TEAMS) {
+    // The next row of both matrices is on its way while one is worked on (without: 148 us for 139 of the 600,000 x 128 case).
+    Vec<T, VW> raw_x[VPL], raw_g[VPL];
+    A mean_next = A(0), rstd_next = A(0);
+    const int64_t step = (int64_t)gridDim.x * TEAMS;
+    const auto load = [&](int64_t r) {
+        mean_next = a.mean[r];
+        rstd_next = a.rstd[r];
+        load_row<T, VW, TEAM, VPL>(a.x + r * a.stride, width, lane, raw_x);
+        load_row<T, VW, TEAM, VPL>(a.grad + r * a.width, width, lane, raw_g);
+    };
+    int64_t r = (int64_t)blockIdx.x * TEAMS + team;
+    if (r < a.rows) load(r);
+    for (; r < a.rows; r += step) {
         A h[VPL][VW], g[VPL][VW], s0[SUMS] = {}, s1[SUMS] = {}, s[2];
-        const A mean = a.mean[r], rstd = a.rstd[r];
-        load_row<T, VW, TEAM, VPL>(a.x + r * a.stride, width, lane, h);
-        load_row<T, VW, TEAM, VPL>(a.grad + r * a.width, width, lane, g);
+        const A mean = mean_next, rstd = rstd_next;
+#pragma unroll
+        for (int p = 0; p < VPL; ++p) {
+            widen_all<T, VW>(raw_x[p], h[p]);
+            widen_all<T, VW>(raw_g[p], g[p]);
+        }
+        if (r + step < a.rows) load(r + step);
         uint32_t gone = 0;
+        PhiloxRun run(words, (uint64_t)(r * a.width) >> 2, (uint32_t)width >> 2);
         if constexpr (VOTES)
-            if (a.drop.threshold) gone = dropped_of_row<VPL>(r * a.width, a.drop.threshold, key);
+            if (DROP) gone = dropped_of_row<VPL>(r * a.width, a.drop.threshold, words);
 #pragma unroll
         for (int p = 0; p < VPL; ++p) {
             const int col = (p * TEAM + lane) * VW;
             if (col >= width) continue;
             add_to_all(h[p], -mean);
             multiply_all(h[p], rstd);
-            drop(a.drop, r * a.width + col, key, VOTES, gone >> p & 1u, g[p]);
+            if (DROP) drop(a.drop, r * a.width, col, words, run, VOTES, gone >> p & 1u, g[p]);
             if (a.relu) {
                 A again[VW], b[VW], z[VW];
                 params_at<T, VW>(a, col, again, b);
@@ -265,7 +297,7 @@ template <typename T>
 __global__ void __launch_bounds__(LONG_THREADS) norm_long_kernel(const NormArgs<T> a) {
     using A = Acc<T>;
     __shared__ A shared[2 * LONG_THREADS / 32];
-    const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
+    Philox words(a.drop.threshold ? a.drop.key() : 0);
     int turn = 0;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T *row = a.x + r * a.stride;
@@ -289,7 +321,7 @@ __global__ void __launch_bounds__(LONG_THREADS) norm_long_kernel(const NormArgs<
             params_at<T, 1>(a, c, w, b);
             multiply_add_to(h, w, b, z);
             if (a.relu && z[0] < A(0)) z[0] = A(0);
-            drop(a.drop, r * a.width + c, key, false, false, z);
+            if (a.drop.threshold) drop_values(z, r * a.width + c, a.drop.threshold, (A)a.drop.scale, words);
             a.out[r * a.width + c] = narrow<T>(z[0]);
         }
     }
@@ -297,12 +329,12 @@ __global__ void __launch_bounds__(LONG_THREADS) norm_long_kernel(const NormArgs<
 
 // One element of a long row on the way back: h and the gradient of z.
 template <typename T>
-__device__ __forceinline__ void long_element(const NormArgs<T> &a, int64_t r, int64_t c, Acc<T> mean, Acc<T> rstd, uint64_t key,
+__device__ __forceinline__ void long_element(const NormArgs<T> &a, int64_t r, int64_t c, Acc<T> mean, Acc<T> rstd, Philox &words,
                                              Acc<T> &h, Acc<T> &g, Acc<T> &weight) {
     Acc<T> hat[1] = {(widen(a.x[r * a.stride + c]) - mean) * rstd}, grad[1] = {widen(a.grad[r * a.width + c])}, w[1], b[1], z[1];
     params_at<T, 1>(a, c, w, b);
     multiply_add_to(hat, w, b, z);
-    drop(a.drop, r * a.width + c, key, false, false, grad);
+    if (a.drop.threshold) drop_values(grad, r * a.width + c, a.drop.threshold, (Acc<T>)a.drop.scale, words);
     if (a.relu && z[0] <= Acc<T>(0)) grad[0] = Acc<T>(0);
     h = hat[0];
     g = grad[0];
@@ -313,20 +345,20 @@ template <typename T>
 __global__ void __launch_bounds__(LONG_THREADS) norm_long_backward_kernel(const NormArgs<T> a) {
     using A = Acc<T>;
     __shared__ A shared[4 * LONG_THREADS / 32];
-    const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
+    Philox words(a.drop.threshold ? a.drop.key() : 0);
     int turn = 0;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const A mean = a.mean[r], rstd = a.rstd[r];
         A s[2] = {A(0), A(0)}, h, g, w;
         for (int64_t c = threadIdx.x; c < a.width; c += LONG_THREADS) {
-            long_element(a, r, c, mean, rstd, key, h, g, w);
+            long_element(a, r, c, mean, rstd, words, h, g, w);
             s[0] = fused(g, w, s[0]);
             s[1] = fused(g * w, h, s[1]);
         }
         team_sum<A, LONG_THREADS, 2>(s, shared, turn);
         const A c0 = s[0] / (A)a.width, c1 = s[1] / (A)a.width;
         for (int64_t c = threadIdx.x; c < a.width; c += LONG_THREADS) {
-            long_element(a, r, c, mean, rstd, key, h, g, w);
+            long_element(a, r, c, mean, rstd, words, h, g, w);
             a.dx[r * a.width + c] = narrow<T>(rstd * (g * w - fused(h, c1, c0)));
         }
     }
@@ -336,13 +368,13 @@ __global__ void __launch_bounds__(LONG_THREADS) norm_long_backward_kernel(const 
 template <typename T>
 __global__ void __launch_bounds__(256) norm_columns_kernel(const NormArgs<T> a, int64_t rows_per_block) {
     using A = Acc<T>;
-    const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
+    Philox words(a.drop.threshold ? a.drop.key() : 0);
     const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (c >= a.width) return;
     const int64_t r0 = (int64_t)blockIdx.y * rows_per_block, r1 = min(a.rows, r0 + rows_per_block);
     A dw = A(0), db = A(0), h, g, w;
     for (int64_t r = r0; r < r1; ++r) {
-        long_element(a, r, c, a.mean[r], a.rstd[r], key, h, g, w);
+        long_element(a, r, c, a.mean[r], a.rstd[r], words, h, g, w);
         dw = fused(g, h, dw);
         db += g;
     }
@@ -379,42 +411,52 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(const Acc<T> *partial, 
 // ---------------------------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------------------------
-// Rows of `vectors` vectors of VW elements: the least team that holds them with at most 32 elements a lane.
+// Rows of `vectors` vectors of VW elements: the least team that holds them with at most 16 elements a lane, whose
+// parameters then stay in registers.  (600,000 x 128 in fp32 and 100,000 x 768 in bf16, forward / backward with dropout: 96 / 139 and
+// 104 / 142 us; 8 elements: 111 / 227 and 110 / 162.)  Single elements are held by a warp, whose lanes draw random
+// words together.
 // f(team, vectors a lane) with both as constants.
 template <int N>
 struct Num {
     static constexpr int value = N;
 };
-template <int VW>
-constexpr int MOST_VPL = 32 / VW < 8 && VW > 1 ? 32 / VW : VW > 1 ? 8 : 32;
-template <int VW>
-constexpr int64_t TEAM_VECTORS = VW > 1 ? 256 * MOST_VPL<VW> : 1024;
-template <int VW, typename F>
+template <typename A>
+constexpr int ELEMENTS = 64 / sizeof(A);  // (8 of fp64)
+template <typename A, int VW>
+constexpr int64_t TEAM_VECTORS = VW > 1 ? 512 * ELEMENTS<A> / VW : 64 * ELEMENTS<A>;
+template <typename A, int VW, typename F>
 static int with_team(int64_t vectors, F &&f) {
     if (vectors <= 2) return f(Num<2>(), Num<1>());
     if (vectors <= 4) return f(Num<4>(), Num<1>());
     if (vectors <= 8) return f(Num<8>(), Num<1>());
-    if (vectors <= 16) return f(Num<8>(), Num<2>());
     if constexpr (VW == 1) {
+        if (vectors <= 16) return f(Num<8>(), Num<2>());
         if (vectors <= 32) return f(Num<32>(), Num<1>());
         if (vectors <= 64) return f(Num<32>(), Num<2>());
+        if (vectors <= 96) return f(Num<32>(), Num<3>());
         if (vectors <= 128) return f(Num<32>(), Num<4>());
+        if (vectors <= 192) return f(Num<32>(), Num<6>());
         if (vectors <= 256) return f(Num<32>(), Num<8>());
+        if (vectors <= 320) return f(Num<32>(), Num<10>());
+        if (vectors <= 384) return f(Num<32>(), Num<12>());
         if (vectors <= 512) return f(Num<32>(), Num<16>());
-        return f(Num<32>(), Num<32>());
-    } else {
-        if (vectors <= 32) return f(Num<8>(), Num<4>());
-        if (vectors <= 64) return f(Num<16>(), Num<4>());
-        if (vectors <= 128) return f(Num<32>(), Num<4>());
-        if constexpr (MOST_VPL<VW> == 8) {
-            if (vectors <= 256) return f(Num<32>(), Num<8>());
-        } else {
-            if (vectors <= 256) return f(Num<128>(), Num<2>());
+        if constexpr (sizeof(A) == 4) {
+            if (vectors <= 640) return f(Num<32>(), Num<20>());
+            if (vectors <= 768) return f(Num<32>(), Num<24>());
+            return f(Num<32>(), Num<32>());
         }
-        if (vectors <= 512) return f(Num<128>(), Num<4>());
-        if constexpr (MOST_VPL<VW> == 8)
-            if (vectors <= 1024) return f(Num<128>(), Num<8>());
-        return f(Num<256>(), Num<MOST_VPL<VW>>());
+        return CGNN_ERR_INVALID;  // (more are no team's: TEAM_VECTORS)
+    } else {
+        constexpr int VPL = ELEMENTS<A> / VW;
+        if constexpr (VPL > 2)
+            if (vectors <= 16) return f(Num<8>(), Num<2>());
+        if (vectors <= 8 * VPL) return f(Num<8>(), Num<VPL>());
+        if (vectors <= 16 * VPL) return f(Num<16>(), Num<VPL>());
+        if (vectors <= 32 * VPL) return f(Num<32>(), Num<VPL>());
+        if (vectors <= 64 * VPL) return f(Num<64>(), Num<VPL>());
+        if (vectors <= 128 * VPL) return f(Num<128>(), Num<VPL>());
+        if (vectors <= 256 * VPL) return f(Num<256>(), Num<VPL>());
+        return f(Num<512>(), Num<VPL>());
     }
 }
 
@@ -429,24 +471,16 @@ static bool vectors_fit(size_t item, int64_t width, int64_t stride, std::initial
     return width % n == 0 && stride % n == 0 && (bits & 15) == 0;
 }
 
-template <typename Kernel>
-static int resident_blocks(Kernel *kernel, int threads) {
-    int blocks = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, 0) != cudaSuccess) {
-        cudaGetLastError();
-        return 1;
-    }
-    return std::max(1, blocks);
-}
-
 template <typename T, int VW>
 static int forward_typed(const NormArgs<T> &a, cudaStream_t stream) {
-    return with_team<VW>(a.width / VW, [&](auto team, auto vpl) -> int {
+    return with_team<Acc<T>, VW>(a.width / VW, [&](auto team, auto vpl) -> int {
         constexpr int TEAM = decltype(team)::value, VPL = decltype(vpl)::value, THREADS = FORWARD_THREADS<TEAM>;
         // (no more than run at once: blocks that began when others end would double the time)
-        static const int resident = resident_blocks(norm_kernel<T, VW, TEAM, VPL>, THREADS);
-        const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(a.rows, THREADS / TEAM), SMS * resident);
-        norm_kernel<T, VW, TEAM, VPL><<<blocks, THREADS, 0, stream>>>(a);
+        static const int resident[2] = {resident_blocks(norm_kernel<T, VW, TEAM, VPL, false>, THREADS),
+                                        resident_blocks(norm_kernel<T, VW, TEAM, VPL, true>, THREADS)};
+        const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(a.rows, THREADS / TEAM), SMS * resident[a.drop.threshold != 0]);
+        if (a.drop.threshold) norm_kernel<T, VW, TEAM, VPL, true><<<blocks, THREADS, 0, stream>>>(a);
+        else norm_kernel<T, VW, TEAM, VPL, false><<<blocks, THREADS, 0, stream>>>(a);
         CGNN_LAUNCH_CHECK();
         return CGNN_OK;
     });
@@ -455,9 +489,9 @@ static int forward_typed(const NormArgs<T> &a, cudaStream_t stream) {
 template <typename T>
 static int forward(const NormArgs<T> &a, cudaStream_t stream) {
     constexpr int VW = WIDEST<T>;
-    if (vectors_fit(sizeof(T), a.width, a.stride, {a.x, a.out}) && a.width / VW <= TEAM_VECTORS<VW>)
+    if (vectors_fit(sizeof(T), a.width, a.stride, {a.x, a.out}) && a.width / VW <= TEAM_VECTORS<Acc<T>, VW>)
         return forward_typed<T, VW>(a, stream);
-    if (a.width <= TEAM_VECTORS<1>) return forward_typed<T, 1>(a, stream);
+    if (a.width <= TEAM_VECTORS<Acc<T>, 1>) return forward_typed<T, 1>(a, stream);
     norm_long_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, SMS * 4), LONG_THREADS, 0, stream>>>(a);
     CGNN_LAUNCH_CHECK();
     return CGNN_OK;
@@ -476,9 +510,9 @@ static int64_t column_blocks(int64_t rows, int64_t width) {
 // Partial rows of a backward pass by vectors of VW elements, or the most of the ways it may go.
 template <typename A, int VW>
 static int64_t partial_rows(int64_t rows, int64_t width) {
-    if (width / VW > TEAM_VECTORS<VW>) return column_blocks(rows, width);
+    if (width / VW > TEAM_VECTORS<A, VW>) return column_blocks(rows, width);
     int64_t blocks = 0;
-    with_team<VW>(width / VW, [&](auto team, auto vpl) -> int {
+    with_team<A, VW>(width / VW, [&](auto team, auto vpl) -> int {
         blocks = backward_blocks<decltype(team)::value, decltype(vpl)::value * VW * (int)sizeof(A) / 4>(rows);
         return 0;
     });
@@ -494,10 +528,11 @@ static int64_t partial_rows(size_t item, int64_t rows, int64_t width) {
 
 template <typename T, int VW>
 static int backward_typed(const NormArgs<T> &a, int64_t *blocks, cudaStream_t stream) {
-    return with_team<VW>(a.width / VW, [&](auto team, auto vpl) -> int {
+    return with_team<Acc<T>, VW>(a.width / VW, [&](auto team, auto vpl) -> int {
         constexpr int TEAM = decltype(team)::value, VPL = decltype(vpl)::value;
         *blocks = backward_blocks<TEAM, VPL * VW * (int)sizeof(Acc<T>) / 4>(a.rows);
-        norm_backward_kernel<T, VW, TEAM, VPL><<<(unsigned)*blocks, BACKWARD_THREADS<TEAM>, 0, stream>>>(a);
+        if (a.drop.threshold) norm_backward_kernel<T, VW, TEAM, VPL, true><<<(unsigned)*blocks, BACKWARD_THREADS<TEAM>, 0, stream>>>(a);
+        else norm_backward_kernel<T, VW, TEAM, VPL, false><<<(unsigned)*blocks, BACKWARD_THREADS<TEAM>, 0, stream>>>(a);
         CGNN_LAUNCH_CHECK();
         return CGNN_OK;
     });
@@ -508,9 +543,9 @@ static int backward(const NormArgs<T> &a, void *dweight, void *dbias, cudaStream
     constexpr int VW = WIDEST<T>;
     int64_t blocks = 0;
     int rc = CGNN_OK;
-    if (vectors_fit(sizeof(T), a.width, a.stride, {a.x, a.grad, a.dx}) && a.width / VW <= TEAM_VECTORS<VW>) {
+    if (vectors_fit(sizeof(T), a.width, a.stride, {a.x, a.grad, a.dx}) && a.width / VW <= TEAM_VECTORS<Acc<T>, VW>) {
         rc = backward_typed<T, VW>(a, &blocks, stream);
-    } else if (a.width <= TEAM_VECTORS<1>) {
+    } else if (a.width <= TEAM_VECTORS<Acc<T>, 1>) {
         rc = backward_typed<T, 1>(a, &blocks, stream);
     } else {
         if (a.dx) {
@@ -569,7 +604,7 @@ static NormArgs<T> args_of(const NormCall &c, int relu, uint64_t seed, const int
     a.weight = c.weight;
     a.bias = c.bias;
     a.wide_params = c.param_dtype == CGNN_F32 && c.dtype != CGNN_F32;
-    a.whole_params = (((uintptr_t)c.weight | (uintptr_t)c.bias) & 15) == 0;
+    a.whole_params = (((uintptr_t)c.weight | (uintptr_t)c.bias) & 31) == 0;
     a.relu = relu;
     a.drop = Drop::of(c.p, seed, device_seed);
     return a;

@@ -5,6 +5,8 @@
 // Elements are widened on arrival: sums and statistics are fp32 for the 16-bit types and fp32, fp64 for fp64.
 #pragma once
 
+#include <algorithm>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -77,23 +79,20 @@ __device__ __forceinline__ Vec<T, VW> narrow_all(const Acc<T> (&y)[VW]) {
     return r;
 }
 
-// VW parameters (weight or bias) from `at` on, of the matrix' type or, beside 16-bit matrices, fp32.  whole: they lie on
-// 16-byte boundaries every VW.
+// VW parameters (weight or bias) from `at` on, of the matrix' type or, beside 16-bit matrices, fp32.  whole: they begin on
+// a 32-byte boundary.
 template <typename T, int VW>
 __device__ __forceinline__ void load_params(const void *params, bool wide, bool whole, int64_t at, Acc<T> (&y)[VW]) {
     if constexpr (sizeof(T) == 2) {
         if (wide) {
             const float *p = static_cast<const float *>(params) + at;
-            if constexpr (VW % 4 == 0) {
+            if constexpr (VW == 8) {
                 if (whole) {
-#pragma unroll
-                    for (int k = 0; k < VW; k += 4) {
-                        const float4 four = *reinterpret_cast<const float4 *>(p + k);
-                        y[k] = four.x;
-                        y[k + 1] = four.y;
-                        y[k + 2] = four.z;
-                        y[k + 3] = four.w;
-                    }
+                    // In one instruction: two of 16 bytes would each touch every other half line.  (volatile: an address may
+                    // be good under the caller's conditions only, and a plain asm may be moved before them)
+                    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                        : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]), "=f"(y[4]), "=f"(y[5]), "=f"(y[6]), "=f"(y[7])
+                        : "l"(p));
                     return;
                 }
             }
@@ -266,6 +265,18 @@ __device__ __forceinline__ void team_sum(A (&s)[N], A *shared, int &turn) {
             for (int w = 0; w < WARPS; ++w) s[n] += mine[n * WARPS + w];
         }
     }
+}
+
+// Blocks of a kernel that run at once on a multiprocessor, for launches that walk their work in strides: blocks that begin
+// when others end would double the time.
+template <typename Kernel>
+static int resident_blocks(Kernel *kernel, int threads) {
+    int blocks = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, 0) != cudaSuccess) {
+        cudaGetLastError();
+        return 1;
+    }
+    return std::max(1, blocks);
 }
 
 }  // namespace cgnn
