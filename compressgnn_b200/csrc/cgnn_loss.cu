@@ -57,6 +57,7 @@ struct LossArgs {
     const A *upstream;     // backward: one value, or one per row without reduction
     int skip_one;          // backward: `grad` holds the gradient for an incoming one already
     int dense;             // rows lie one behind the other from a 16-byte boundary on, in the scores and the gradient
+    int whole_tiles;       // dense and narrow: a tile comes in one copy, unlabelled rows and all
 };
 
 // The class of a row, or -1 for a row without one.
@@ -269,10 +270,20 @@ __global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS>) los
     A share = A(0);
     if (a.grad && (FORWARD || a.reduction != CGNN_NONE)) share = share_of(a, FORWARD ? 1.0 : (double)*a.upstream, labelled);
     double total = 0.0;
-    // Register j of a lane has the column `lane + LANES * ((j + turn) % held)`; there_is(): one below `limit`.
-    const int turn = AROUND ? team % held : 0;
-    const auto column = [&](int j) { return AROUND ? lane + LANES * (j + turn >= held ? j + turn - held : j + turn) : lane + LANES * j; };
-    const auto there_is = [&](int j, int limit) { return AROUND ? j < held && column(j) < limit : LANES * j < limit - lane; };
+    // Register j of a lane has the column `lane + LANES * ((j + turn) % held)`, but for the lanes behind the last column.
+    const int turn = AROUND ? team % held : 0, wrap = held - turn;
+    const int missing = lane + LANES * (held - 1) < classes ? -1 : (AROUND ? wrap - 1 : held - 1);
+    // (`phase` keeps the compiler from holding the addresses of one pass for the next: they do not fit the registers)
+    struct Columns {
+        int begin, again, wrap;
+        __device__ __forceinline__ int operator()(int j) const { return (AROUND && j >= wrap ? again : begin) + LANES * j; }
+    };
+    const auto phase = [&] {
+        Columns c{lane + LANES * turn, lane - LANES * wrap, wrap};
+        if (AROUND) asm volatile("" : "+r"(c.begin), "+r"(c.again), "+r"(c.wrap));
+        return c;
+    };
+    const auto there_is = [&](int j, int count) { return j < count && j != missing; };
     const int tiles = (int)((a.rows + ROWS - 1) / ROWS);  // (below 2^31: the rows of more do not fit any memory)
     // The team's row: the vectors that cover it, in one copy; one that it shares with the next row both may bring.  (The
     // very last row may end inside a vector: its last elements are loaded one by one.)
@@ -282,6 +293,14 @@ __global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS>) los
             const T *from = a.logits + ((int64_t)i * ROWS + team) * a.stride;
             if (wanted)
                 for (int c = lane; c < classes; c += LANES) to[team * classes + c] = from[c];
+        } else if (a.whole_tiles) {
+            const T *from = a.logits + (int64_t)i * (ROWS * classes);
+            const int n = i < tiles - 1 ? ROWS * classes : (int)(a.rows - (int64_t)i * ROWS) * classes, whole = n / VW * VW;
+            if (threadIdx.x == 0) {
+                barrier_expect(&arrived[place], (uint32_t)(whole * sizeof(T)));
+                if (whole) bulk_copy(to, from, (uint32_t)(whole * sizeof(T)), &arrived[place]);
+            }
+            if (whole + (int)threadIdx.x < n) to[whole + threadIdx.x] = from[whole + threadIdx.x];
         } else if (lane == 0) {
             const T *from = a.logits + (int64_t)i * (ROWS * classes);
             int end = last;
@@ -299,8 +318,8 @@ __global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS>) los
     };
     const auto class_or_none = [&](int64_t label) { return (int)class_of(label, a.classes, a.ignore_index, FORWARD && lane == 0); };
     if (threadIdx.x == 0) {
-        barrier_init(&arrived[0], ROWS);
-        barrier_init(&arrived[1], ROWS);
+        barrier_init(&arrived[0], a.whole_tiles ? 1 : ROWS);
+        barrier_init(&arrived[1], a.whole_tiles ? 1 : ROWS);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -326,7 +345,8 @@ __global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS>) los
         const bool inside = i < tiles - 1 || r < a.rows;
         T *const z = here + team * classes;
         // A row without a label passes as one of scores of minus infinity with a share of zero.
-        const int read = t >= 0 ? classes : 0, written = inside ? classes : 0;
+        const int read = t >= 0 ? held : 0, written = inside ? held : 0;
+        const Columns column = phase();
         A v[HELD], m = -(A)INFINITY, other = m, inv = A(0), at_label = A(0);
         if (t >= 0) at_label = widen(z[t]);
 #pragma unroll
@@ -378,6 +398,7 @@ __global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS>) los
         if (a.grad) {
             const A scale = t >= 0 ? inv * share : A(0);
             __syncwarp(mask);  // every lane has read its label's score ...
+            const Columns column = phase();
 #pragma unroll
             for (int j = 0; j < HELD; j += 8) {
                 if (j >= held) break;
@@ -865,7 +886,9 @@ static int launch_rows(const LossArgs<T> &a, bool follows, cudaStream_t stream) 
     if (a.classes <= 16 * HELD) return launch_tiles<T, 16, 8, FORWARD>(a, follows, stream);
     if (a.classes <= 32 * HELD) return launch_tiles<T, 32, 8, FORWARD>(a, follows, stream);
     const size_t shared = (a.classes * sizeof(T) + 15) / 16 * 16 + 16;
-    if (shared <= 32 * 1024) return launch<T>(loss_row_kernel<T, 256, FORWARD>, a, a.rows, 256, 4, shared, follows, 1, stream);
+    if (shared <= 8 * 1024) return launch<T>(loss_row_kernel<T, 64, FORWARD>, a, a.rows, 64, 16, shared, follows, 1, stream);
+    if (shared <= 20 * 1024) return launch<T>(loss_row_kernel<T, 128, FORWARD>, a, a.rows, 128, 8, shared, follows, 1, stream);
+    if (shared <= 48 * 1024) return launch<T>(loss_row_kernel<T, 256, FORWARD>, a, a.rows, 256, 4, shared, follows, 1, stream);
     if (shared <= SHARED_MOST / 2 - 2048) return launch<T>(loss_row_kernel<T, 512, FORWARD>, a, a.rows, 512, 2, shared, follows, 1, stream);
     if (shared <= SHARED_MOST - 2048) return launch<T>(loss_row_kernel<T, 1024, FORWARD>, a, a.rows, 1024, 1, shared, follows, 1, stream);
     return launch<T>(loss_long_kernel<T, FORWARD>, a, a.rows, LONG_THREADS, sizeof(T) == 8 ? 1 : 2, 0, follows, 1, stream);
@@ -900,6 +923,9 @@ static LossArgs<T> args_of(int64_t rows, int64_t classes, int64_t stride, const 
     a.reduction = reduction;
     a.grad = (T *)grad;
     a.dense = (stride == classes || rows == 1) && (((uintptr_t)logits | (uintptr_t)grad) & 15) == 0;
+    // (a row of 96 bytes shares half of the 64-byte pieces it lies in, and small copies cost ten cycles each: 8.6 M x 7 with a
+    // copy for every row 298 us)
+    a.whole_tiles = a.dense && classes * (int64_t)sizeof(T) <= 96;
     return a;
 }
 
