@@ -74,12 +74,20 @@ constexpr int BACKWARD_THREADS = TEAM > 32 ? TEAM : 128;
 template <int TEAM, int WORDS>
 constexpr int BACKWARD_BLOCKS = std::max(1, (WORDS <= 4 ? 768 : WORDS <= 8 ? 512 : WORDS <= 16 ? 384 : 256) / BACKWARD_THREADS<TEAM>);
 
+// First column of a lane's vector p.  The warps of a large team that holds single elements have runs of columns, so that
+// each can draw the random words of its own.
+template <int VW, int TEAM, int VPL>
+__device__ __forceinline__ int column_of(int lane, int p) {
+    if constexpr (VW == 1 && TEAM > 32) return ((lane / 32) * VPL + p) * 32 + lane % 32;
+    else return (p * TEAM + lane) * VW;
+}
+
 // The team's row, vector by vector; elements beyond the row are zero.
 template <typename T, int VW, int TEAM, int VPL>
 __device__ __forceinline__ void load_row(const T *row, int width, int lane, Vec<T, VW> (&raw)[VPL]) {
 #pragma unroll
     for (int p = 0; p < VPL; ++p) {
-        const int col = (p * TEAM + lane) * VW;
+        const int col = column_of<VW, TEAM, VPL>(lane, p);
         raw[p] = vec_zero<T, VW>();
         if (col < width) raw[p] = vec_load<T, VW>(row + col);
     }
@@ -90,7 +98,7 @@ __global__ void __launch_bounds__(FORWARD_THREADS<TEAM>, 512 / FORWARD_THREADS<T
     using A = Acc<T>;
     constexpr int TEAMS = FORWARD_THREADS<TEAM> / TEAM;
         constexpr bool KEEP = VPL * VW <= 16;      // the parameters of a lane's columns stay in registers
-    constexpr bool VOTES = TEAM == 32 && VW == 1;  // a warp draws the words of its row together
+    constexpr bool VOTES = TEAM >= 32 && VW == 1;  // a warp draws the words of its columns together
     constexpr int SUMS = VW % 2 == 0 ? 2 : 1;
     __shared__ A shared[2 * (TEAM > 32 ? TEAM / 32 : 1)];
     const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM, width = (int)a.width;
@@ -101,7 +109,7 @@ __global__ void __launch_bounds__(FORWARD_THREADS<TEAM>, 512 / FORWARD_THREADS<T
     if constexpr (KEEP)
 #pragma unroll
         for (int p = 0; p < VPL; ++p)
-            if ((p * TEAM + lane) * VW < width) params_at<T, VW>(a, (p * TEAM + lane) * VW, w[p], b[p]);
+            if (column_of<VW, TEAM, VPL>(lane, p) < width) params_at<T, VW>(a, column_of<VW, TEAM, VPL>(lane, p), w[p], b[p]);
     // While a row is worked on the next one is on its way.
     Vec<T, VW> raw[VPL];
     const int64_t step = (int64_t)gridDim.x * TEAMS;
@@ -115,7 +123,7 @@ __global__ void __launch_bounds__(FORWARD_THREADS<TEAM>, 512 / FORWARD_THREADS<T
         uint32_t gone = 0;
         PhiloxRun run(words, (uint64_t)(r * a.width) >> 2, (uint32_t)width >> 2);
         if constexpr (VOTES)
-            if (DROP) gone = dropped_of_row<VPL>(r * a.width, a.drop.threshold, words);
+            if (DROP) gone = dropped_of_row<VPL>(r * a.width + lane / 32 * (32 * VPL), a.drop.threshold, words);
 #pragma unroll
         for (int p = 0; p < VPL; ++p) add(v[p], two);
         s[0] = SUMS == 2 ? two[0] + two[SUMS - 1] : two[0];
@@ -125,7 +133,7 @@ __global__ void __launch_bounds__(FORWARD_THREADS<TEAM>, 512 / FORWARD_THREADS<T
 #pragma unroll
         for (int p = 0; p < VPL; ++p) {
             add_to_all(v[p], -mean);
-            if ((p * TEAM + lane) * VW < width) multiply_add(v[p], v[p], two);
+            if (column_of<VW, TEAM, VPL>(lane, p) < width) multiply_add(v[p], v[p], two);
         }
         s[0] = SUMS == 2 ? two[0] + two[SUMS - 1] : two[0];
         team_sum<A, TEAM, 1>(s, shared, turn);
@@ -137,7 +145,7 @@ __global__ void __launch_bounds__(FORWARD_THREADS<TEAM>, 512 / FORWARD_THREADS<T
         T *const out = a.out + r * a.width;
 #pragma unroll
         for (int p = 0; p < VPL; ++p) {
-            const int col = (p * TEAM + lane) * VW;
+            const int col = column_of<VW, TEAM, VPL>(lane, p);
             if (col >= width) continue;
             A z[VW];
             multiply_all(v[p], rstd);
@@ -163,7 +171,7 @@ __global__ void __launch_bounds__(BACKWARD_THREADS<TEAM>, BACKWARD_BLOCKS<TEAM, 
     using A = Acc<T>;
     constexpr int THREADS = BACKWARD_THREADS<TEAM>, TEAMS = THREADS / TEAM, WARPS = THREADS / 32;
     constexpr int COLUMNS = TEAM * VPL * VW;
-    constexpr bool VOTES = TEAM == 32 && VW == 1;
+    constexpr bool VOTES = TEAM >= 32 && VW == 1;
     constexpr int SUMS = VW % 2 == 0 ? 2 : 1;
     __shared__ A shared[TEAM > 32 ? 4 * TEAM / 32 : 2 * COLUMNS];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the launch that adds up the shares)
@@ -174,7 +182,7 @@ __global__ void __launch_bounds__(BACKWARD_THREADS<TEAM>, BACKWARD_BLOCKS<TEAM, 
     A w[VPL][VW], dw[VPL][VW], db[VPL][VW];
 #pragma unroll
     for (int p = 0; p < VPL; ++p) {
-        const int col = (p * TEAM + lane) * VW;
+        const int col = column_of<VW, TEAM, VPL>(lane, p);
 #pragma unroll
         for (int k = 0; k < VW; ++k) {
             w[p][k] = A(0);
@@ -209,10 +217,10 @@ __global__ void __launch_bounds__(BACKWARD_THREADS<TEAM>, BACKWARD_BLOCKS<TEAM, 
         uint32_t gone = 0;
         PhiloxRun run(words, (uint64_t)(r * a.width) >> 2, (uint32_t)width >> 2);
         if constexpr (VOTES)
-            if (DROP) gone = dropped_of_row<VPL>(r * a.width, a.drop.threshold, words);
+            if (DROP) gone = dropped_of_row<VPL>(r * a.width + lane / 32 * (32 * VPL), a.drop.threshold, words);
 #pragma unroll
         for (int p = 0; p < VPL; ++p) {
-            const int col = (p * TEAM + lane) * VW;
+            const int col = column_of<VW, TEAM, VPL>(lane, p);
             if (col >= width) continue;
             add_to_all(h[p], -mean);
             multiply_all(h[p], rstd);
@@ -238,7 +246,7 @@ __global__ void __launch_bounds__(BACKWARD_THREADS<TEAM>, BACKWARD_BLOCKS<TEAM, 
         T *const dx = a.dx + r * a.width;
 #pragma unroll
         for (int p = 0; p < VPL; ++p) {
-            const int col = (p * TEAM + lane) * VW;
+            const int col = column_of<VW, TEAM, VPL>(lane, p);
             if (col >= width) continue;
             // rstd * (u - (h * c1 + c0))
             A minus_c1[VW];
@@ -283,7 +291,7 @@ __global__ void __launch_bounds__(BACKWARD_THREADS<TEAM>, BACKWARD_BLOCKS<TEAM, 
         for (int p = 0; p < VPL; ++p)
 #pragma unroll
             for (int k = 0; k < VW; ++k) {
-                const int col = (p * TEAM + lane) * VW + k;
+                const int col = column_of<VW, TEAM, VPL>(lane, p) + k;
                 if (col < width) {
                     mine[col] = dw[p][k];
                     mine[a.width + col] = db[p][k];
@@ -423,7 +431,7 @@ struct Num {
 template <typename A>
 constexpr int ELEMENTS = 64 / sizeof(A);  // (8 of fp64)
 template <typename A, int VW>
-constexpr int64_t TEAM_VECTORS = VW > 1 ? 512 * ELEMENTS<A> / VW : 64 * ELEMENTS<A>;
+constexpr int64_t TEAM_VECTORS = VW > 1 || sizeof(A) == 4 ? 512 * ELEMENTS<A> / VW : 512;
 template <typename A, int VW, typename F>
 static int with_team(int64_t vectors, F &&f) {
     if (vectors <= 2) return f(Num<2>(), Num<1>());
@@ -443,7 +451,10 @@ static int with_team(int64_t vectors, F &&f) {
         if constexpr (sizeof(A) == 4) {
             if (vectors <= 640) return f(Num<32>(), Num<20>());
             if (vectors <= 768) return f(Num<32>(), Num<24>());
-            return f(Num<32>(), Num<32>());
+            if (vectors <= 1024) return f(Num<32>(), Num<32>());
+            if (vectors <= 2048) return f(Num<128>(), Num<16>());
+            if (vectors <= 4096) return f(Num<256>(), Num<16>());
+            return f(Num<512>(), Num<16>());
         }
         return CGNN_ERR_INVALID;  // (more are no team's: TEAM_VECTORS)
     } else {
@@ -460,15 +471,16 @@ static int with_team(int64_t vectors, F &&f) {
     }
 }
 
-// Elements a vector holds: 16 bytes where rows and pointers allow, else one.
+// Elements a vector holds: 16 bytes where rows and pointers allow, 8 where only those fit (not of fp64), else one.
+// (600,000 x 100 in bf16: 84 us by single elements forward.)
 template <typename T>
 constexpr int WIDEST = 16 / (int)sizeof(T);
 
-static bool vectors_fit(size_t item, int64_t width, int64_t stride, std::initializer_list<const void *> pointers) {
-    const int64_t n = 16 / (int64_t)item;
+// Whether rows are whole vectors of n elements, in their places too.
+static bool vectors_fit(size_t item, int64_t n, int64_t width, int64_t stride, std::initializer_list<const void *> pointers) {
     uintptr_t bits = 0;
     for (const void *p : pointers) bits |= (uintptr_t)p;
-    return width % n == 0 && stride % n == 0 && (bits & 15) == 0;
+    return width % n == 0 && stride % n == 0 && bits % (n * item) == 0;
 }
 
 template <typename T, int VW>
@@ -489,8 +501,10 @@ static int forward_typed(const NormArgs<T> &a, cudaStream_t stream) {
 template <typename T>
 static int forward(const NormArgs<T> &a, cudaStream_t stream) {
     constexpr int VW = WIDEST<T>;
-    if (vectors_fit(sizeof(T), a.width, a.stride, {a.x, a.out}) && a.width / VW <= TEAM_VECTORS<Acc<T>, VW>)
-        return forward_typed<T, VW>(a, stream);
+    const auto fit = [&](int64_t n) { return vectors_fit(sizeof(T), n, a.width, a.stride, {a.x, a.out}); };
+    if (fit(VW) && a.width / VW <= TEAM_VECTORS<Acc<T>, VW>) return forward_typed<T, VW>(a, stream);
+    if constexpr (VW > 2)
+        if (fit(VW / 2) && a.width / (VW / 2) <= TEAM_VECTORS<Acc<T>, VW / 2>) return forward_typed<T, VW / 2>(a, stream);
     if (a.width <= TEAM_VECTORS<Acc<T>, 1>) return forward_typed<T, 1>(a, stream);
     norm_long_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, SMS * 4), LONG_THREADS, 0, stream>>>(a);
     CGNN_LAUNCH_CHECK();
@@ -519,11 +533,9 @@ static int64_t partial_rows(int64_t rows, int64_t width) {
     return blocks;
 }
 static int64_t partial_rows(size_t item, int64_t rows, int64_t width) {
-    const int64_t single = item == 8 ? partial_rows<double, 1>(rows, width) : partial_rows<float, 1>(rows, width);
-    const int64_t vectors = item == 8   ? partial_rows<double, 2>(rows, width)
-                            : item == 4 ? partial_rows<float, 4>(rows, width)
-                                        : partial_rows<float, 8>(rows, width);
-    return std::max(single, vectors);
+    if (item == 8) return std::max(partial_rows<double, 1>(rows, width), partial_rows<double, 2>(rows, width));
+    const int64_t most = std::max({partial_rows<float, 1>(rows, width), partial_rows<float, 2>(rows, width), partial_rows<float, 4>(rows, width)});
+    return item == 4 ? most : std::max(most, partial_rows<float, 8>(rows, width));
 }
 
 template <typename T, int VW>
@@ -543,8 +555,11 @@ static int backward(const NormArgs<T> &a, void *dweight, void *dbias, cudaStream
     constexpr int VW = WIDEST<T>;
     int64_t blocks = 0;
     int rc = CGNN_OK;
-    if (vectors_fit(sizeof(T), a.width, a.stride, {a.x, a.grad, a.dx}) && a.width / VW <= TEAM_VECTORS<Acc<T>, VW>) {
+    const auto fit = [&](int64_t n) { return vectors_fit(sizeof(T), n, a.width, a.stride, {a.x, a.grad, a.dx}); };
+    if (fit(VW) && a.width / VW <= TEAM_VECTORS<Acc<T>, VW>) {
         rc = backward_typed<T, VW>(a, &blocks, stream);
+    } else if (VW > 2 && fit(VW / 2) && a.width / (VW / 2) <= TEAM_VECTORS<Acc<T>, VW / 2>) {
+        rc = backward_typed<T, VW / 2>(a, &blocks, stream);
     } else if (a.width <= TEAM_VECTORS<Acc<T>, 1>) {
         rc = backward_typed<T, 1>(a, &blocks, stream);
     } else {
