@@ -705,6 +705,10 @@ Key key_of(const char *what, double p, const c10::optional<int64_t> &seed, const
     return key;
 }
 
+void *second_row(const Tensor &t) {
+    return t.defined() && t.numel() ? static_cast<char *>(t.data_ptr()) + t.size(1) * t.element_size() : nullptr;
+}
+
 struct NormSettings {
     int dtype = 0, param_dtype = 0;
     double eps = 0.0, p = 0.0;
@@ -713,7 +717,7 @@ struct NormSettings {
 };
 
 struct LayerNormBackward : public Node {
-    SavedVariable x_, weight_, bias_, mean_, rstd_, key_;
+    SavedVariable x_, weight_, bias_, statistics_, key_;
     NormSettings set;
     at::TensorOptions param_options;
     variable_list apply(variable_list &&grads) override {
@@ -723,7 +727,7 @@ struct LayerNormBackward : public Node {
             const Tensor grad = materialized(*this, grads[0]).contiguous();
             const c10::cuda::OptionalCUDAGuard guard(grad.device());
             const Tensor x_in = x_.unpack(), weight = dense(weight_.unpack()), bias = dense(bias_.unpack());
-            const Tensor mean = mean_.unpack().contiguous(), rstd = rstd_.unpack().contiguous();
+            const Tensor statistics = statistics_.unpack().contiguous();  // [2, rows]: means, then 1 / deviations
             const Tensor key = dense(key_.unpack());
             const Rows x(x_in);
             const auto plain = grad.options().requires_grad(false);
@@ -737,14 +741,14 @@ struct LayerNormBackward : public Node {
                 scratch = at::empty({(int64_t)bytes}, plain.dtype(at::kByte));
             }
             check(cgnn_layer_norm_backward(set.dtype, set.param_dtype, x.rows, x.width, x.stride, data(x.held), data(weight),
-                                           data(bias), data(mean), data(rstd), data(grad), set.relu, set.p, set.seed,
+                                           data(bias), data(statistics), second_row(statistics), data(grad), set.relu, set.p, set.seed,
                                            static_cast<const int64_t *>(data(key)), data(dx), data(dw), data(db), data(scratch),
                                            bytes, current_stream(grad)));
         }
         return first_order({dx, dw, db}, grads);
     }
     void release_variables() override {
-        for (SavedVariable *v : {&x_, &weight_, &bias_, &mean_, &rstd_, &key_}) v->reset_data();
+        for (SavedVariable *v : {&x_, &weight_, &bias_, &statistics_, &key_}) v->reset_data();
     }
     std::string name() const override { return "CompressgnnLayerNormBackward"; }
 };
@@ -776,18 +780,15 @@ Tensor layer_norm_autograd(const Tensor &x_in, const c10::optional<Tensor> &weig
     set.relu = relu;
     set.seed = key.seed;
     const bool differentiated = torch::autograd::compute_requires_grad(x_in, weight, bias);
-    Tensor out, mean, rstd;
+    Tensor out, statistics;
     {
         at::AutoDispatchBelowADInplaceOrView below;
         const Rows x(x_in);
         const Tensor w = dense(weight), b = dense(bias);
         out = at::empty(x_in.sizes(), x_in.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
-        if (differentiated) {
-            mean = at::empty({x.rows}, x_in.options().dtype(sum_type(x_in)).requires_grad(false));
-            rstd = at::empty_like(mean);
-        }
+        if (differentiated) statistics = at::empty({2, x.rows}, x_in.options().dtype(sum_type(x_in)).requires_grad(false));
         check(cgnn_layer_norm(set.dtype, set.param_dtype, x.rows, x.width, x.stride, data(x.held), data(w), data(b), eps, relu, p,
-                              key.seed, key.pointer(), data(out), data(mean), data(rstd), current_stream(x_in)));
+                              key.seed, key.pointer(), data(out), data(statistics), second_row(statistics), current_stream(x_in)));
     }
     if (differentiated) {
         auto node = new_node<LayerNormBackward>();
@@ -796,8 +797,7 @@ Tensor layer_norm_autograd(const Tensor &x_in, const c10::optional<Tensor> &weig
         node->x_ = SavedVariable(x_in, false);
         node->weight_ = SavedVariable(weight, false);
         node->bias_ = SavedVariable(bias, false);
-        node->mean_ = SavedVariable(mean, false);
-        node->rstd_ = SavedVariable(rstd, false);
+        node->statistics_ = SavedVariable(statistics, false);
         node->key_ = SavedVariable(key.on_device, false);
         node->set_next_edges(torch::autograd::collect_next_edges(x_in, weight, bias));
         torch::autograd::set_history(out, node);
@@ -861,37 +861,40 @@ Tensor dropout_autograd(const Tensor &x_in, double p, const c10::optional<Tensor
     return out;
 }
 
+constexpr int64_t LABELLED_BYTES = 16;
+
 // For a sum or a mean the forward pass has written the gradient for an incoming one (`unit_`).  The first backward pass
 // hands that array on, after a launch that computes it anew unless the incoming gradient is one; further passes over a
 // retained graph have an array of their own.
 struct CrossEntropyBackward : public Node {
-    SavedVariable logits_, target_, stats_, labelled_;
+    SavedVariable logits_, target_, held_;  // held_: the number of labelled rows, and each row's statistics
     Tensor unit_;
     int dtype = 0, reduction = 0;
     int64_t ignore_index = 0;
     variable_list apply(variable_list &&grads) override {
-        std::lock_guard<std::mutex> held(mutex_);
+        std::lock_guard<std::mutex> guard_of_node(mutex_);
         Tensor dlogits;
         {
             at::NoGradGuard no_grad;
             const Tensor grad = materialized(*this, grads[0]).contiguous();
             const c10::cuda::OptionalCUDAGuard guard(grad.device());
             const Tensor logits = logits_.unpack(), target = target_.unpack().contiguous();
-            const Tensor stats = stats_.unpack().contiguous(), labelled = dense(labelled_.unpack());
+            const Tensor held_bytes = held_.unpack().contiguous();
+            char *const held = static_cast<char *>(data(held_bytes));
             const Rows z(logits);
             const bool unit = unit_.defined() && !capturing();
             if (unit) dlogits = std::move(unit_);
             else dlogits = at::empty(logits.sizes(), logits.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
             unit_.reset();
             check(cgnn_cross_entropy_backward(dtype, z.rows, z.width, z.stride, data(z.held), static_cast<const int64_t *>(data(target)),
-                                              ignore_index, reduction, data(stats), static_cast<const int64_t *>(data(labelled)),
+                                              ignore_index, reduction, held + LABELLED_BYTES, reinterpret_cast<const int64_t *>(held),
                                               data(grad), unit, data(dlogits), current_stream(grad)));
         }
         return first_order({dlogits}, grads);
     }
     void release_variables() override {
-        std::lock_guard<std::mutex> held(mutex_);
-        for (SavedVariable *v : {&logits_, &target_, &stats_, &labelled_}) v->reset_data();
+        std::lock_guard<std::mutex> guard_of_node(mutex_);
+        for (SavedVariable *v : {&logits_, &target_, &held_}) v->reset_data();
         unit_.reset();
     }
     std::string name() const override { return "CompressgnnCrossEntropyBackward"; }
@@ -910,7 +913,7 @@ Tensor cross_entropy_autograd(const Tensor &logits, const Tensor &target_in, int
     refuse_foreign_leaves("cross_entropy", {logits});
     const bool differentiated = torch::autograd::compute_requires_grad(logits);
     const Tensor target = target_in.contiguous();
-    Tensor loss, stats, labelled, unit;
+    Tensor loss, held, unit;
     {
         at::AutoDispatchBelowADInplaceOrView below;
         const Rows z(logits);
@@ -919,19 +922,22 @@ Tensor cross_entropy_autograd(const Tensor &logits, const Tensor &target_in, int
         const bool reduced = reduction != CGNN_NONE;
         if (reduced) loss = at::empty({}, sums);
         else loss = at::empty({z.rows}, sums);
-        if (differentiated) stats = at::empty({z.rows, 2}, sums);
         // (a captured backward pass may be replayed more than once per forward pass: it computes the gradient itself)
         if (differentiated && reduced && !capturing())
             unit = at::empty(logits.sizes(), plain.memory_format(at::MemoryFormat::Contiguous));
-        const int64_t bytes = reduced ? (int64_t)cgnn_cross_entropy_scratch_bytes() : 0;
-        Tensor scratch;
-        if (reduced) {
-            labelled = at::empty({1}, plain.dtype(at::kLong));
-            scratch = at::empty({bytes}, plain.dtype(at::kByte));
+        // one allocation: the number of labelled rows, the rows' statistics, and what the launches hand each other
+        const int64_t stats_bytes = differentiated ? 2 * z.rows * (int64_t)sums.dtype().itemsize() : 0;
+        const int64_t scratch_begin = (LABELLED_BYTES + stats_bytes + 15) / 16 * 16;
+        const int64_t scratch_bytes = reduced ? (int64_t)cgnn_cross_entropy_scratch_bytes() : 0;
+        char *place = nullptr;
+        if (reduced || differentiated) {
+            held = at::empty({scratch_begin + scratch_bytes}, plain.dtype(at::kByte));
+            place = static_cast<char *>(data(held));
         }
         check(cgnn_cross_entropy(dtype, z.rows, z.width, z.stride, data(z.held), static_cast<const int64_t *>(data(target)),
-                                 ignore_index, reduction, data(loss), data(stats), data(unit),
-                                 static_cast<int64_t *>(data(labelled)), data(scratch), bytes, current_stream(logits)));
+                                 ignore_index, reduction, data(loss), stats_bytes ? place + LABELLED_BYTES : nullptr, data(unit),
+                                 reinterpret_cast<int64_t *>(place), place ? place + scratch_begin : nullptr, scratch_bytes,
+                                 current_stream(logits)));
     }
     if (differentiated) {
         auto node = new_node<CrossEntropyBackward>();
@@ -940,8 +946,7 @@ Tensor cross_entropy_autograd(const Tensor &logits, const Tensor &target_in, int
         node->ignore_index = ignore_index;
         node->logits_ = SavedVariable(logits, false);
         node->target_ = SavedVariable(target, false);
-        node->stats_ = SavedVariable(stats, false);
-        node->labelled_ = SavedVariable(labelled, false);
+        node->held_ = SavedVariable(held, false);
         node->unit_ = unit;
         node->set_next_edges(torch::autograd::collect_next_edges(logits));
         torch::autograd::set_history(loss, node);
