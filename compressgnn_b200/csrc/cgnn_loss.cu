@@ -929,11 +929,12 @@ static LossArgs<T> args_of(int64_t rows, int64_t classes, int64_t stride, const 
     return a;
 }
 
-static int check_call(const char *what, int dtype, int64_t rows, int64_t classes, int64_t stride, int reduction) {
+static int check_call(const char *what, int dtype, int64_t rows, int64_t classes, int64_t stride, int reduction, const void *stats) {
     CGNN_REQUIRE(dtype >= CGNN_F32 && dtype <= CGNN_F16, "%s: unknown dtype %d", what, dtype);
     CGNN_REQUIRE(reduction >= CGNN_NONE && reduction <= CGNN_MEAN, "%s: unknown reduction %d", what, reduction);
     CGNN_REQUIRE(rows >= 0 && stride >= 0, "%s: negative size", what);
     CGNN_REQUIRE(classes >= 1 && classes <= INT32_MAX / 2, "%s: %lld classes are not supported", what, (long long)classes);
+    CGNN_REQUIRE(((uintptr_t)stats & (dtype == CGNN_F64 ? 15 : 7)) == 0, "%s: the statistics are pairs on their own boundaries", what);
     return CGNN_OK;
 }
 
@@ -948,7 +949,7 @@ size_t cgnn_cross_entropy_scratch_bytes(void) { return sizeof(LossScratch); }
 int cgnn_cross_entropy(int dtype, int64_t rows, int64_t classes, int64_t stride, const void *logits, const int64_t *target,
                        int64_t ignore_index, int reduction, void *loss, void *stats, void *grad, int64_t *labelled, void *scratch,
                        size_t scratch_bytes, cgnn_stream_t stream_) {
-    if (int rc = check_call("cross_entropy", dtype, rows, classes, stride, reduction)) return rc;
+    if (int rc = check_call("cross_entropy", dtype, rows, classes, stride, reduction, stats)) return rc;
     const cudaStream_t stream = (cudaStream_t)stream_;
     CGNN_REQUIRE(reduction != CGNN_NONE || grad == nullptr, "cross_entropy: the gradient of unreduced losses takes their gradients");
     CGNN_REQUIRE(loss != nullptr || (reduction == CGNN_NONE && rows == 0), "cross_entropy: null loss");
@@ -978,7 +979,7 @@ int cgnn_cross_entropy_backward(int dtype, int64_t rows, int64_t classes, int64_
                                 const int64_t *target, int64_t ignore_index, int reduction, const void *stats,
                                 const int64_t *labelled, const void *upstream, int holds_unit_gradient, void *grad,
                                 cgnn_stream_t stream) {
-    if (int rc = check_call("cross_entropy_backward", dtype, rows, classes, stride, reduction)) return rc;
+    if (int rc = check_call("cross_entropy_backward", dtype, rows, classes, stride, reduction, stats)) return rc;
     if (rows == 0) return CGNN_OK;
     CGNN_REQUIRE(logits != nullptr && target != nullptr && stats != nullptr && upstream != nullptr && grad != nullptr &&
                      (reduction != CGNN_MEAN || labelled != nullptr),

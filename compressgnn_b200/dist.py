@@ -225,14 +225,18 @@ class ShardedGCN(torch.nn.Module):
 MIN_SHARDED_FEATURES = 512
 
 
+def needs_whole_rows(model):
+    """Whether a model has what cannot be sharded by columns: normalised layers or residual connections."""
+    return getattr(model, "residual", False) or any(getattr(layer, "norm", None) is not None for layer in model.layers)
+
+
 def place_model(model, in_features, group=None, min_features=MIN_SHARDED_FEATURES):
     """``(module, sharded)``: a ``ShardedGCN`` over ``model`` when the input is wide enough for column
-    sharding to pay, else ``model`` itself, to be run as a replica on every rank (the full feature matrix,
+    sharding to pay and the model allows it, else ``model`` itself, to be run as a replica on every rank (the full feature matrix,
     the same parameters and the same random stream everywhere, no collective).  A sharded module takes
     ``shard_columns(x, rank, world)``, a replica takes ``x``."""
     world = dist.get_world_size(group) if dist.is_initialized() else 1
-    whole_rows = getattr(model, "residual", False) or any(getattr(layer, "norm", None) is not None for layer in model.layers)
-    if world > 1 and in_features >= min_features and in_features % world == 0 and not whole_rows:
+    if world > 1 and in_features >= min_features and in_features % world == 0 and not needs_whole_rows(model):
         return ShardedGCN(model, group), True
     return model, False
 

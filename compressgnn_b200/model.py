@@ -49,8 +49,8 @@ class GNNLayer(torch.nn.Module):
         transformation path it runs inside the reconstruct kernel, behind a normalisation inside its kernel.
         ``residual``: added to the layer's output, in the pass of the dropout when there is one."""
         if residual is not None:
-            x = self(x, edge_index, edge_weight, vertex_cnt, rule_cnt)
-            return _native.dropout(x, dropout, residual) if dropout else x + residual
+            out = GNNLayer.forward(self, x, edge_index, edge_weight, vertex_cnt, rule_cnt)
+            return _native.dropout(out, dropout, residual) if dropout else out + residual
         x = self.P(x=x, edge_index=edge_index, edge_weight=edge_weight, vertex_cnt=vertex_cnt, rule_cnt=rule_cnt)
         if self.norm is not None:
             return self.norm(self._transform(x, None, 0.0), dropout)

@@ -397,9 +397,9 @@ int cgnn_dropout(int dtype, int64_t n, const void *x, const void *residual, doub
  * A row whose target is ignore_index has no loss and a gradient of zeros; so has one whose target is no class, which
  * also sets status bit 1.  Losses are fp32 (fp64 for fp64).
  *   reduction   CGNN_NONE: loss[rows]; CGNN_SUM, CGNN_MEAN (over the rows with a class; NaN when there is none): one value
- *   stats       [rows, 2], what the backward pass reads; may be null
+ *   stats       [rows, 2] on a boundary of such a pair, what the backward pass reads; may be null
  *   grad        dense [rows, classes], the gradient for an incoming gradient of one; not with CGNN_NONE; may be null
- *   labelled    one int64, written with CGNN_MEAN: the number of rows with a class
+ *   labelled    one int64, with CGNN_SUM and CGNN_MEAN: the number of rows with a class (0 with CGNN_SUM)
  *   scratch     cgnn_cross_entropy_scratch_bytes(), 8-byte aligned, with CGNN_SUM and CGNN_MEAN
  * Backward: upstream is one value, or one per row with CGNN_NONE, of the loss' type.  With holds_unit_gradient `grad` is what
  * the forward call wrote: it is left alone when the incoming gradient is one, and computed anew otherwise. */

@@ -63,6 +63,14 @@ def test_column_sharding_refuses_whole_row_models():
         dist.ShardedGCN(GCN(8, 3, use_transformation=True, residual=True))
 
 
+def test_placement_looks_into_a_model_only_where_it_would_shard_it():
+    from compressgnn_b200 import dist
+    anything = torch.nn.Linear(4, 4)
+    assert dist.place_model(anything, 4096) == (anything, False)
+    assert dist.needs_whole_rows(GCN(8, 3, norm="layer")) and dist.needs_whole_rows(GCN(8, 3, residual=True))
+    assert not dist.needs_whole_rows(GCN(8, 3))
+
+
 HUGE = 2**30
 
 
@@ -81,8 +89,8 @@ def _dropout(dtype=0, n=4, x=64, p=0.5, out=64):
 
 
 def _loss(dtype=0, rows=4, classes=8, stride=8, logits=64, target=64, reduction=2, loss=64, grad=None, labelled=64, scratch=64,
-          room=1 << 20):
-    return _lib.lib().cgnn_cross_entropy(dtype, rows, classes, stride, logits, target, -100, reduction, loss, None, grad, labelled,
+          room=1 << 20, stats=None):
+    return _lib.lib().cgnn_cross_entropy(dtype, rows, classes, stride, logits, target, -100, reduction, loss, stats, grad, labelled,
                                          scratch, room, None)
 
 
@@ -107,7 +115,8 @@ REFUSED = [
     (_loss, dict(classes=0), b"not supported"), (_loss, dict(classes=HUGE), b"not supported"),
     (_loss, dict(logits=None), b"null pointer"), (_loss, dict(target=None), b"null pointer"), (_loss, dict(loss=None), b"null loss"),
     (_loss, dict(labelled=None), b"count"), (_loss, dict(scratch=None), b"scratch"), (_loss, dict(room=8), b"too small"),
-    (_loss, dict(scratch=68), b"8-byte"), (_loss, dict(reduction=0, grad=64), b"unreduced"),
+    (_loss, dict(scratch=68), b"8-byte"), (_loss, dict(stats=68), b"boundaries"), (_loss, dict(dtype=1, stats=72), b"boundaries"),
+    (_loss_backward, dict(stats=68), b"boundaries"), (_loss, dict(reduction=0, grad=64), b"unreduced"),
     (_loss_backward, dict(dtype=4), b"unknown dtype"), (_loss_backward, dict(stats=None), b"null pointer"),
     (_loss_backward, dict(labelled=None), b"null pointer"), (_loss_backward, dict(upstream=None), b"null pointer"),
 ]

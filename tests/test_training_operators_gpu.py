@@ -3,7 +3,10 @@
 Tolerances count roundings.  ``U`` is half a step of the operator's sums (2^-24, for fp64 2^-53), ``half_step`` that of the
 result's type; a sum of n terms whose longest chain is c has an error of at most c * U * sum|terms|."""
 import math
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -766,6 +769,44 @@ def test_a_capture_over_leaves_of_a_living_eager_graph_is_refused():
     assert all(torch.equal(u, v) for u, v in zip(out, step(x, w, b, target, 5)))
 
 
+FIRST_CALLS_IN_A_CAPTURE = """
+import torch
+from compressgnn_b200 import runtime as rt
+x = torch.randn(300, 130, device="cuda", dtype=torch.float64, requires_grad=True)
+target = torch.arange(300, device="cuda") % 130
+side = torch.cuda.Stream()
+torch.cuda.synchronize()
+recorded = torch.cuda.CUDAGraph()
+with torch.cuda.graph(recorded, stream=side):
+    loss = rt.cross_entropy(rt.dropout(rt.layer_norm(x, dropout=0.2, seed=3), 0.1, seed=4), target)
+    dx, = torch.autograd.grad(loss, x)
+recorded.replay()
+torch.cuda.synchronize()
+again = rt.cross_entropy(rt.dropout(rt.layer_norm(x, dropout=0.2, seed=3), 0.1, seed=4), target)
+assert torch.equal(again, loss) and torch.equal(torch.autograd.grad(again, x)[0], dx)
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS_IN_A_CAPTURE], cwd=Path(__file__).resolve().parents[1],
+                          capture_output=True, text=True, timeout=240)
+    assert done.returncode == 0 and done.stdout.strip() == "same", done.stderr[-2000:]
+
+
+def test_masks_beyond_the_lower_half_of_the_counter():
+    """Blocks of four words beyond 2^32 of them, and a row that lies on both sides: 2^34 elements (32 GiB of fp16 out, the
+    rows in share their memory)."""
+    p, key, width = 0.5, 2**40 + 9, 4100
+    rows = 2**34 // width + 3
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    x = rand(1, width, dtype=F16).expand(rows, width)
+    y = rt.layer_norm(x, None, torch.full((width,), 30.0, dtype=F16, device="cuda"), dropout=p, seed=key)
+    for r in (0, 2**34 // width - 1, 2**34 // width, rows - 1):
+        assert torch.equal(y[r] != 0, kept((width,), p, key, r * width)), r
+
+
 # ---------------------------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------------------------
@@ -835,6 +876,13 @@ def test_modules():
     assert torch.equal(got, rt.cross_entropy(rt.dropout(h, 0.4, x, seed=keys[1]), target, reduction="sum"))
     got.backward()
     assert all(p.grad is not None for p in norm.parameters()) and x.grad is not None
+    # a layer's hooks run once, with a residual stream too
+    from compressgnn_b200.model import GNNLayer
+    data, seen = graph_data(), []
+    layer = GNNLayer(24, 24, activation="relu", norm="layer").cuda()
+    layer.register_forward_hook(lambda module, given, out: seen.append(out))
+    out = layer(data.x, data.edge_index, residual=data.x)
+    assert len(seen) == 1 and torch.equal(out, layer(data.x, data.edge_index) + data.x)
     drop.eval()
     assert torch.equal(drop(h, residual=x), h + x) and LayerNorm(8, bias=False).bias is None
 
