@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <mutex>
 #include <tuple>
 #include <vector>
@@ -665,9 +666,10 @@ struct Rows {
 // a graph is captured that would be a wait on work outside the capture, which breaks it off (and ends the process where
 // the error meets a thread of the engine), so the call is refused before anything is recorded.
 void refuse_foreign_leaves(const char *what, at::TensorList inputs) {
-    if (!at::GradMode::is_enabled() || !capturing()) return;
+    const auto concerned = [](const Tensor &t) { return t.defined() && t.requires_grad() && t.is_leaf(); };
+    if (!at::GradMode::is_enabled() || std::none_of(inputs.begin(), inputs.end(), concerned) || !capturing()) return;
     for (const Tensor &t : inputs) {
-        if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+        if (!concerned(t)) continue;
         const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
         if (!accumulator) continue;
         const auto stream = accumulator->stream();

@@ -226,7 +226,7 @@ __device__ __forceinline__ void finish(const LossArgs<T> &a, double total, int64
 // before is worked on.  LANES lanes then hold a row in registers, lane l the columns l, l + LANES, ...; the gradient takes
 // the row's place in shared memory and leaves by whole vectors.
 // What bounds it is instructions and their latency more than memory: 2.45 M x 47 in fp32 with 0.6 of the rows
-// labelled takes 171 us (DRAM 782 MB, 120 us); a lane group of 16 over registers loaded from DRAM took 375, three passes
+// labelled takes 172 us (DRAM 782 MB, 120 us); a lane group of 16 over registers loaded from DRAM took 375, three passes
 // over shared memory 301, one tile at a time 237.  HELD and the registers were tried together: 24 columns in
 // 64 registers 171, 24 in 80 176, 32 in 80 177, 32 in 64 193, 16 in 51 259.
 // AROUND: the lanes of a warp begin at different columns and go around, or rows of an even length would meet in the
