@@ -29,7 +29,6 @@ constexpr int SMS = 148;
 constexpr int LOSS_BLOCKS = SMS * 16;       // most blocks of a launch, each of which leaves a partial sum
 constexpr int COUNT_THREADS = 1024;
 constexpr int CLUSTER = 8;                  // blocks of the launch that does a small case alone
-constexpr int64_t CLUSTER_ROWS = 4096;
 constexpr size_t SHARED_MOST = 227 * 1024;  // of a block
 constexpr int LONG_THREADS = 512;
 
@@ -53,6 +52,7 @@ struct LossArgs {
     A *loss;               // forward: [rows] without reduction, else one value
     LossScratch *scratch;  // forward with reduction
     int count_blocks;      // forward, mean: entries of scratch->counts
+    int clustered;         // forward with reduction: the launch is one cluster, which counts and adds up itself
     T *grad;               // optional in the forward pass
     const A *upstream;     // backward: one value, or one per row without reduction
     int skip_one;          // backward: `grad` holds the gradient for an incoming one already
@@ -187,24 +187,52 @@ __global__ void __launch_bounds__(COUNT_THREADS) loss_count_kernel(const int64_t
     if (blockIdx.x == 0) scratch->ticket = 0;
 }
 
-// The number of labelled rows, on every thread of a block of the launch behind that one.
+// The number of labelled rows, on every thread of a block: from the launch before, or counted by the cluster that the
+// launch is.
 template <typename T, int THREADS>
 __device__ __forceinline__ int64_t labelled_rows(const LossArgs<T> &a) {
+    namespace cg = cooperative_groups;
     __shared__ int64_t all;
     if (a.reduction != CGNN_MEAN) return 0;
     int64_t mine = 0;
-    for (int b = threadIdx.x; b < a.count_blocks; b += THREADS) mine += a.scratch->counts[b];
+    if (a.clustered) {
+        for (int64_t r = (int64_t)blockIdx.x * THREADS + threadIdx.x; r < a.rows; r += CLUSTER * THREADS)
+            mine += class_of(a.target[r], a.classes, a.ignore_index, false) >= 0;
+    } else {
+        for (int b = threadIdx.x; b < a.count_blocks; b += THREADS) mine += a.scratch->counts[b];
+    }
     mine = block_sum<THREADS>(mine);
     if (threadIdx.x == 0) all = mine;
-    __syncthreads();
-    return all;
+    if (!a.clustered) {
+        __syncthreads();
+        return all;
+    }
+    cg::this_cluster().sync();
+    mine = 0;
+    for (int b = 0; b < CLUSTER; ++b) mine += *cg::this_cluster().map_shared_rank(&all, b);
+    return mine;
 }
 
-// The end of a reduced loss: a block leaves its sum, and the last one to do so adds all of them up in block order.
+// The end of a reduced loss: a block leaves its sum, and the last one to do so adds all of them up in block order; the
+// blocks of a cluster leave them in their shared memory.
 template <typename T, int THREADS>
 __device__ __forceinline__ void finish(const LossArgs<T> &a, double total, int64_t labelled) {
+    namespace cg = cooperative_groups;
     __shared__ bool last;
+    __shared__ double here;
     total = block_sum<THREADS>(total);
+    if (a.clustered) {
+        if (threadIdx.x == 0) here = total;
+        cg::this_cluster().sync();
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            double s = 0.0;
+            for (int b = 0; b < CLUSTER; ++b) s += *cg::this_cluster().map_shared_rank(&here, b);
+            *a.loss = (Acc<T>)(a.reduction == CGNN_MEAN ? s / (double)labelled : s);
+            *a.labelled = labelled;
+        }
+        cg::this_cluster().sync();  // a block's shared memory is read until here
+        return;
+    }
     if (threadIdx.x == 0) {
         a.scratch->partial[blockIdx.x] = total;
         __threadfence();
@@ -230,43 +258,27 @@ __device__ __forceinline__ void finish(const LossArgs<T> &a, double total, int64
 // over shared memory 301, one tile at a time 237.  HELD and the registers were tried together: 24 columns in
 // 64 registers 171, 24 in 80 176, 32 in 80 177, 32 in 64 193, 16 in 51 259.
 // AROUND: the lanes of a warp begin at different columns and go around, or rows of an even length would meet in the
-// same banks.  CLUSTERED: the launch is one cluster, which counts the labelled rows and adds up the losses itself.
+// same banks.
 constexpr int HELD = 24;  // columns of a lane, at most
 template <typename T, int THREADS>
 constexpr int TILE_BLOCKS = (sizeof(T) == 8 ? 384 : 1024) / THREADS;  // to a multiprocessor, by their registers
-template <typename T, int LANES, int ROWS, bool AROUND, bool FORWARD, bool CLUSTERED>
+template <typename T, int LANES, int ROWS, bool AROUND, bool FORWARD>
 __global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS>) loss_tile_kernel(const LossArgs<T> a) {
     using A = Acc<T>;
     constexpr int THREADS = LANES * ROWS, VW = 16 / sizeof(T);
     extern __shared__ uint4 tile_vectors[];
     __shared__ uint64_t arrived[2];
-    __shared__ double cluster_sum;
-    __shared__ int cluster_count;
     if constexpr (!FORWARD) {
         if (a.skip_one && *a.upstream == A(1)) return;
     }
-    if constexpr (FORWARD && !CLUSTERED) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if constexpr (FORWARD) asm volatile("griddepcontrol.wait;" ::: "memory");
     T *tile = reinterpret_cast<T *>(tile_vectors);
     const int team = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     const int classes = (int)a.classes, held = (classes + LANES - 1) / LANES;
     const unsigned mask = team_mask<LANES>();
     int64_t labelled = 0;
-    if constexpr (CLUSTERED) {
-        namespace cg = cooperative_groups;
-        if (a.reduction == CGNN_MEAN) {
-            int mine = 0;
-            for (int64_t r = (int64_t)blockIdx.x * THREADS + threadIdx.x; r < a.rows; r += CLUSTER * THREADS)
-                mine += class_of(a.target[r], a.classes, a.ignore_index, false) >= 0;
-            mine = block_sum<THREADS>(mine);
-            if (threadIdx.x == 0) cluster_count = mine;
-            cg::this_cluster().sync();
-            for (int b = 0; b < CLUSTER; ++b) labelled += *cg::this_cluster().map_shared_rank(&cluster_count, b);
-        }
-    } else if (FORWARD && a.reduction != CGNN_NONE) {
-        labelled = labelled_rows<T, THREADS>(a);
-    } else if (!FORWARD && a.reduction == CGNN_MEAN) {
-        labelled = *a.labelled;
-    }
+    if (FORWARD && a.reduction != CGNN_NONE) labelled = labelled_rows<T, THREADS>(a);
+    if (!FORWARD && a.reduction == CGNN_MEAN) labelled = *a.labelled;
     A share = A(0);
     if (a.grad && (FORWARD || a.reduction != CGNN_NONE)) share = share_of(a, FORWARD ? 1.0 : (double)*a.upstream, labelled);
     double total = 0.0;
@@ -426,22 +438,7 @@ __global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS>) los
         t = t_next;
     }
     if constexpr (FORWARD) {
-        if (a.reduction == CGNN_NONE) return;
-        if constexpr (CLUSTERED) {
-            namespace cg = cooperative_groups;
-            total = block_sum<THREADS>(total);
-            if (threadIdx.x == 0) cluster_sum = total;
-            cg::this_cluster().sync();
-            if (blockIdx.x == 0 && threadIdx.x == 0) {
-                double s = 0.0;
-                for (int b = 0; b < CLUSTER; ++b) s += *cg::this_cluster().map_shared_rank(&cluster_sum, b);
-                *a.loss = (A)(a.reduction == CGNN_MEAN ? s / (double)labelled : s);
-                *a.labelled = labelled;
-            }
-            cg::this_cluster().sync();  // a block's shared memory is read until here
-        } else {
-            finish<T, THREADS>(a, total, labelled);
-        }
+        if (a.reduction != CGNN_NONE) finish<T, THREADS>(a, total, labelled);
     }
 }
 
@@ -837,31 +834,43 @@ __global__ void __launch_bounds__(LONG_THREADS, sizeof(T) == 8 ? 1 : 2) loss_lon
 // ---------------------------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------------------------
-// follows: behind the launch that counts, which it may overlap until it waits; cluster: blocks of one cluster, or 1.
+// Units of work of a call (tiles or rows) that one cluster does alone, saving the launch that counts: as many rounds of its
+// blocks take no longer than that launch.
+constexpr int64_t CLUSTER_TILES = 4 * CLUSTER, CLUSTER_LONG_ROWS = CLUSTER;
+
+// units: of work; blocks: to a multiprocessor, by their registers.  follows: a reduced forward pass, which one cluster does
+// where that is enough for the units, and which otherwise stands behind the launch that counts and may overlap it until it
+// waits.
 template <typename T>
-static int launch(void (*kernel)(const LossArgs<T>), const LossArgs<T> &a, int64_t units, int threads, int blocks, size_t shared,
-                  bool follows, int cluster, cudaStream_t stream) {
+static int launch(void (*kernel)(LossArgs<T>), LossArgs<T> a, int64_t units, int64_t cluster_units, int threads, int blocks,
+                  size_t shared, bool follows, cudaStream_t stream) {
     if (shared > 44 * 1024)  // (with the kernels' own variables no more than the 48 KB that need no leave)
         CGNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+    a.clustered = follows && units <= cluster_units;
+    if (follows && !a.clustered) {
+        a.count_blocks = a.reduction == CGNN_MEAN ? (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(a.rows, COUNT_THREADS), SMS)) : 1;
+        loss_count_kernel<<<(unsigned)a.count_blocks, COUNT_THREADS, 0, stream>>>(
+            a.target, a.reduction == CGNN_MEAN ? a.rows : 0, a.classes, a.ignore_index, a.scratch);
+        CGNN_LAUNCH_CHECK();
+    }
     // (no more than run at once: blocks that began when others end would double the time)
-    const int64_t resident = std::min<int64_t>(blocks, (int64_t)(SHARED_MOST / (shared + 2048)));
+    const int64_t resident = SMS * std::max<int64_t>(1, std::min<int64_t>(blocks, (int64_t)(SHARED_MOST / (shared + 2048))));
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(cluster > 1 ? (unsigned)cluster
-                                      : (unsigned)std::max<int64_t>(1, std::min<int64_t>(units, SMS * std::max<int64_t>(1, resident))));
+    config.gridDim = dim3(a.clustered ? (unsigned)CLUSTER : (unsigned)std::max<int64_t>(1, std::min<int64_t>(units, resident)));
     config.blockDim = dim3((unsigned)threads);
     config.dynamicSmemBytes = shared;
     config.stream = stream;
     cudaLaunchAttribute attribute = {};
-    if (cluster > 1) {
+    if (a.clustered) {
         attribute.id = cudaLaunchAttributeClusterDimension;
-        attribute.val.clusterDim.x = (unsigned)cluster;
+        attribute.val.clusterDim.x = (unsigned)CLUSTER;
         attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
     } else {
         attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attribute.val.programmaticStreamSerializationAllowed = 1;
     }
     config.attrs = &attribute;
-    config.numAttrs = follows || cluster > 1 ? 1 : 0;
+    config.numAttrs = follows ? 1 : 0;
     CGNN_CUDA(cudaLaunchKernelEx(&config, kernel, a));
     return CGNN_OK;
 }
@@ -872,11 +881,17 @@ static bool meet_in_banks(size_t item, int64_t classes) { return classes * item 
 template <typename T, int LANES, int ROWS, bool FORWARD>
 static int launch_tiles(const LossArgs<T> &a, bool follows, cudaStream_t stream) {
     const size_t shared = 2 * ((ROWS * a.classes * sizeof(T) + 15) / 16 * 16);
-    auto kernel = meet_in_banks(sizeof(T), a.classes) && LANES < 32 ? loss_tile_kernel<T, LANES, ROWS, (LANES < 32), FORWARD, false>
-                                                                    : loss_tile_kernel<T, LANES, ROWS, false, FORWARD, false>;
-    return launch<T>(kernel, a, ceil_div(a.rows, ROWS), LANES * ROWS, TILE_BLOCKS<T, LANES * ROWS>, shared, follows, 1, stream);
+    auto kernel = meet_in_banks(sizeof(T), a.classes) && LANES < 32 ? loss_tile_kernel<T, LANES, ROWS, (LANES < 32), FORWARD>
+                                                                    : loss_tile_kernel<T, LANES, ROWS, false, FORWARD>;
+    return launch<T>(kernel, a, ceil_div(a.rows, ROWS), CLUSTER_TILES, LANES * ROWS, TILE_BLOCKS<T, LANES * ROWS>, shared, follows, stream);
 }
 
+template <typename T, int THREADS, bool FORWARD>
+static int launch_long_rows(const LossArgs<T> &a, size_t shared, bool follows, cudaStream_t stream) {
+    return launch<T>(loss_row_kernel<T, THREADS, FORWARD>, a, a.rows, CLUSTER_LONG_ROWS, THREADS, 1024 / THREADS, shared, follows, stream);
+}
+
+// follows: a reduced forward pass.
 template <typename T, bool FORWARD>
 static int launch_rows(const LossArgs<T> &a, bool follows, cudaStream_t stream) {
     if (a.classes <= HELD) return launch_tiles<T, 1, 128, FORWARD>(a, follows, stream);
@@ -885,28 +900,19 @@ static int launch_rows(const LossArgs<T> &a, bool follows, cudaStream_t stream) 
     if (a.classes <= 8 * HELD) return launch_tiles<T, 8, 16, FORWARD>(a, follows, stream);
     if (a.classes <= 16 * HELD) return launch_tiles<T, 16, 8, FORWARD>(a, follows, stream);
     if (a.classes <= 32 * HELD) return launch_tiles<T, 32, 8, FORWARD>(a, follows, stream);
+    // (60 M scores of 1000 classes with their gradient: 271 us by blocks of 256 threads, 119 by blocks of 64)
     const size_t shared = (a.classes * sizeof(T) + 15) / 16 * 16 + 16;
-    if (shared <= 8 * 1024) return launch<T>(loss_row_kernel<T, 64, FORWARD>, a, a.rows, 64, 16, shared, follows, 1, stream);
-    if (shared <= 20 * 1024) return launch<T>(loss_row_kernel<T, 128, FORWARD>, a, a.rows, 128, 8, shared, follows, 1, stream);
-    if (shared <= 48 * 1024) return launch<T>(loss_row_kernel<T, 256, FORWARD>, a, a.rows, 256, 4, shared, follows, 1, stream);
-    if (shared <= SHARED_MOST / 2 - 2048) return launch<T>(loss_row_kernel<T, 512, FORWARD>, a, a.rows, 512, 2, shared, follows, 1, stream);
-    if (shared <= SHARED_MOST - 2048) return launch<T>(loss_row_kernel<T, 1024, FORWARD>, a, a.rows, 1024, 1, shared, follows, 1, stream);
-    return launch<T>(loss_long_kernel<T, FORWARD>, a, a.rows, LONG_THREADS, sizeof(T) == 8 ? 1 : 2, 0, follows, 1, stream);
+    if (shared <= 8 * 1024) return launch_long_rows<T, 64, FORWARD>(a, shared, follows, stream);
+    if (shared <= 20 * 1024) return launch_long_rows<T, 128, FORWARD>(a, shared, follows, stream);
+    if (shared <= 48 * 1024) return launch_long_rows<T, 256, FORWARD>(a, shared, follows, stream);
+    if (shared <= SHARED_MOST / 2 - 2048) return launch_long_rows<T, 512, FORWARD>(a, shared, follows, stream);
+    if (shared <= SHARED_MOST - 2048) return launch_long_rows<T, 1024, FORWARD>(a, shared, follows, stream);
+    return launch<T>(loss_long_kernel<T, FORWARD>, a, a.rows, CLUSTER_LONG_ROWS, LONG_THREADS, sizeof(T) == 8 ? 1 : 2, 0, follows, stream);
 }
 
-// One launch where a cluster does it all, else one that counts and one that computes.
 template <typename T>
-static int forward(LossArgs<T> a, cudaStream_t stream) {
+static int forward(const LossArgs<T> &a, cudaStream_t stream) {
     if (a.reduction == CGNN_NONE) return a.rows ? launch_rows<T, true>(a, false, stream) : CGNN_OK;
-    if (a.rows <= CLUSTER_ROWS && a.classes <= HELD) {
-        auto kernel = meet_in_banks(sizeof(T), a.classes) ? loss_tile_kernel<T, 1, 128, true, true, true>
-                                                          : loss_tile_kernel<T, 1, 128, false, true, true>;
-        return launch<T>(kernel, a, CLUSTER, 128, 1, 2 * ((128 * a.classes * sizeof(T) + 15) / 16 * 16), false, CLUSTER, stream);
-    }
-    a.count_blocks = a.reduction == CGNN_MEAN ? (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(a.rows, COUNT_THREADS), SMS)) : 1;
-    loss_count_kernel<<<(unsigned)a.count_blocks, COUNT_THREADS, 0, stream>>>(
-        a.target, a.reduction == CGNN_MEAN ? a.rows : 0, a.classes, a.ignore_index, a.scratch);
-    CGNN_LAUNCH_CHECK();
     return launch_rows<T, true>(a, true, stream);
 }
 

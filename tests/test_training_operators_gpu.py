@@ -423,6 +423,18 @@ def test_loss_rows(rows):
             check_loss(logits, target, reduction, what=f"{rows}x{classes} {reduction}")
 
 
+@pytest.mark.parametrize("classes", [5, 40, 90, 172, 380, 600, 1000, 4000, 20000, 60000, 130000])
+def test_loss_around_the_sizes_of_one_cluster(classes):
+    """Calls that one cluster does alone, those just too large for it, and the same losses as rows of a larger call."""
+    for dtype in (F32, BF16, F64):
+        for rows in (1, 8, 9, 33) if classes > 768 else (1, 8, 9, 250, 300, 1100, 4096, 4100):
+            if rows * classes > 3_000_000:
+                continue
+            logits, target = loss_case(rows, classes, dtype)
+            for reduction in ("mean", "sum"):
+                check_loss(logits.detach(), target, reduction, what=f"{dtype} {rows}x{classes} {reduction}")
+
+
 @pytest.mark.parametrize("dtype", [F32, F16])
 def test_loss_with_an_incoming_gradient(dtype):
     for classes in (7, 47, 64, 2000):
