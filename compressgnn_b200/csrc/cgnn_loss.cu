@@ -254,16 +254,17 @@ __device__ __forceinline__ void finish(const LossArgs<T> &a, double total, int64
 // before is worked on.  LANES lanes then hold a row in registers, lane l the columns l, l + LANES, ...; the gradient takes
 // the row's place in shared memory and leaves by whole vectors.
 // What bounds it is instructions and their latency more than memory: 2.45 M x 47 in fp32 with 0.6 of the rows
-// labelled takes 172 us (DRAM 782 MB, 120 us); a lane group of 16 over registers loaded from DRAM took 375, three passes
-// over shared memory 301, one tile at a time 237.  HELD and the registers were tried together: 24 columns in
-// 64 registers 171, 24 in 80 176, 32 in 80 177, 32 in 64 193, 16 in 51 259.
+// labelled takes 170 us (DRAM 782 MB, 120 us); a lane group of 16 over registers loaded from DRAM took 375, three passes
+// over shared memory 301, one tile at a time 237.  Columns a lane, registers and time were tried together: 48 in 102 registers
+// 170, 48 in 85 181, 24 in 64 172 to 179, 24 in 80 176, 32 in 80 177, 32 in 64 193, 16 in 51 259.
 // AROUND: the lanes of a warp begin at different columns and go around, or rows of an even length would meet in the
 // same banks.
-constexpr int HELD = 24;  // columns of a lane, at most
-template <typename T, int THREADS>
-constexpr int TILE_BLOCKS = (sizeof(T) == 8 ? 384 : 1024) / THREADS;  // to a multiprocessor, by their registers
-template <typename T, int LANES, int ROWS, bool AROUND, bool FORWARD>
-__global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS>) loss_tile_kernel(const LossArgs<T> a) {
+constexpr int HELD = 24;  // columns of a lane, or twice as many
+template <typename T, int THREADS, int COLUMNS>
+constexpr int TILE_BLOCKS = (COLUMNS > HELD ? (sizeof(T) == 8 ? 256 : 640) : sizeof(T) == 8 ? 384 : 1024) / THREADS;  // to a
+// multiprocessor, by their registers
+template <typename T, int LANES, int ROWS, int COLUMNS, bool AROUND, bool FORWARD>
+__global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS, COLUMNS>) loss_tile_kernel(const LossArgs<T> a) {
     using A = Acc<T>;
     constexpr int THREADS = LANES * ROWS, VW = 16 / sizeof(T);
     extern __shared__ uint4 tile_vectors[];
@@ -359,10 +360,10 @@ __global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS>) los
         // A row without a label passes as one of scores of minus infinity with a share of zero.
         const int read = t >= 0 ? held : 0, written = inside ? held : 0;
         const Columns column = phase();
-        A v[HELD], m = -(A)INFINITY, other = m, inv = A(0), at_label = A(0);
+        A v[COLUMNS], m = -(A)INFINITY, other = m, inv = A(0), at_label = A(0);
         if (t >= 0) at_label = widen(z[t]);
 #pragma unroll
-        for (int j = 0; j < HELD; j += 8) {
+        for (int j = 0; j < COLUMNS; j += 8) {
             if (j >= held) break;
 #pragma unroll
             for (int k = j; k < j + 8; ++k) {
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS>) los
         if (t < 0) m = A(0);
         A parts[2] = {A(0), A(0)};
 #pragma unroll
-        for (int j = 0; j < HELD; j += 8) {
+        for (int j = 0; j < COLUMNS; j += 8) {
             if (j >= held) break;
 #pragma unroll
             for (int k = j; k < j + 8; k += 2) {
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS>) los
             __syncwarp(mask);  // every lane has read its label's score ...
             const Columns column = phase();
 #pragma unroll
-            for (int j = 0; j < HELD; j += 8) {
+            for (int j = 0; j < COLUMNS; j += 8) {
                 if (j >= held) break;
 #pragma unroll
                 for (int k = j; k < j + 8; k += 2) {
@@ -878,12 +879,12 @@ static int launch(void (*kernel)(LossArgs<T>), LossArgs<T> a, int64_t units, int
 // Whether rows of that many classes begin in too few banks for their lanes: words from row to row a multiple of two.
 static bool meet_in_banks(size_t item, int64_t classes) { return classes * item % 8 == 0; }
 
-template <typename T, int LANES, int ROWS, bool FORWARD>
+template <typename T, int LANES, int ROWS, bool FORWARD, int COLUMNS = HELD>
 static int launch_tiles(const LossArgs<T> &a, bool follows, cudaStream_t stream) {
     const size_t shared = 2 * ((ROWS * a.classes * sizeof(T) + 15) / 16 * 16);
-    auto kernel = meet_in_banks(sizeof(T), a.classes) && LANES < 32 ? loss_tile_kernel<T, LANES, ROWS, (LANES < 32), FORWARD>
-                                                                    : loss_tile_kernel<T, LANES, ROWS, false, FORWARD>;
-    return launch<T>(kernel, a, ceil_div(a.rows, ROWS), CLUSTER_TILES, LANES * ROWS, TILE_BLOCKS<T, LANES * ROWS>, shared, follows, stream);
+    auto kernel = meet_in_banks(sizeof(T), a.classes) && LANES < 32 ? loss_tile_kernel<T, LANES, ROWS, COLUMNS, (LANES < 32), FORWARD>
+                                                                    : loss_tile_kernel<T, LANES, ROWS, COLUMNS, false, FORWARD>;
+    return launch<T>(kernel, a, ceil_div(a.rows, ROWS), CLUSTER_TILES, LANES * ROWS, TILE_BLOCKS<T, LANES * ROWS, COLUMNS>, shared, follows, stream);
 }
 
 template <typename T, int THREADS, bool FORWARD>
@@ -894,11 +895,22 @@ static int launch_long_rows(const LossArgs<T> &a, size_t shared, bool follows, c
 // follows: a reduced forward pass.
 template <typename T, bool FORWARD>
 static int launch_rows(const LossArgs<T> &a, bool follows, cudaStream_t stream) {
+    // (Forward by twice the columns a lane, where a row has that many: less work around a row for each of its columns, but
+    // fewer threads.  60 M scores with their gradient, 24 and 48 columns a lane, us: 50 classes 150 and 128, 64 121 and 106, 192
+    // 98 and 92; in bf16 47 classes 85 and 69, 349 84 and 71, but 768 72 and 85.  Backward by twice the columns: 47 classes
+    // 95 and 108.)
     if (a.classes <= HELD) return launch_tiles<T, 1, 128, FORWARD>(a, follows, stream);
-    if (a.classes <= 2 * HELD) return launch_tiles<T, 2, 64, FORWARD>(a, follows, stream);
-    if (a.classes <= 4 * HELD) return launch_tiles<T, 4, 32, FORWARD>(a, follows, stream);
-    if (a.classes <= 8 * HELD) return launch_tiles<T, 8, 16, FORWARD>(a, follows, stream);
-    if (a.classes <= 16 * HELD) return launch_tiles<T, 16, 8, FORWARD>(a, follows, stream);
+    if constexpr (FORWARD) {
+        if (a.classes <= 2 * HELD) return launch_tiles<T, 1, 128, FORWARD, 2 * HELD>(a, follows, stream);
+        if (a.classes <= 4 * HELD) return launch_tiles<T, 2, 64, FORWARD, 2 * HELD>(a, follows, stream);
+        if (a.classes <= 8 * HELD) return launch_tiles<T, 4, 32, FORWARD, 2 * HELD>(a, follows, stream);
+        if (a.classes <= 16 * HELD) return launch_tiles<T, 8, 16, FORWARD, 2 * HELD>(a, follows, stream);
+    } else {
+        if (a.classes <= 2 * HELD) return launch_tiles<T, 2, 64, FORWARD>(a, follows, stream);
+        if (a.classes <= 4 * HELD) return launch_tiles<T, 4, 32, FORWARD>(a, follows, stream);
+        if (a.classes <= 8 * HELD) return launch_tiles<T, 8, 16, FORWARD>(a, follows, stream);
+        if (a.classes <= 16 * HELD) return launch_tiles<T, 16, 8, FORWARD>(a, follows, stream);
+    }
     if (a.classes <= 32 * HELD) return launch_tiles<T, 32, 8, FORWARD>(a, follows, stream);
     // (60 M scores of 1000 classes with their gradient: 271 us by blocks of 256 threads, 119 by blocks of 64)
     const size_t shared = (a.classes * sizeof(T) + 15) / 16 * 16 + 16;
