@@ -1,7 +1,7 @@
 // Softmax cross entropy of class scores over the labelled nodes, with the gradient of the scores.
 //
 // Row i with label t:  loss_i = lse(z_i) - z_i[t],  dz_i = (softmax(z_i) - onehot(t)) * share_i.  A row whose label is
-// `ignore_index` has no loss and a gradient of zeros, and its scores are not read; a label that is no class is treated
+// `ignore_index` has no loss and a gradient of zeros, whatever its scores are; a label that is no class is treated
 // the same and sets a status bit.  share_i is the incoming gradient, for a mean over the number of labelled rows.
 //
 // Memory bounds it.  For a sum or a mean the forward pass writes the gradient for an incoming gradient of one beside the
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS, COLU
     A share = A(0);
     if (a.grad && (FORWARD || a.reduction != CGNN_NONE)) share = share_of(a, FORWARD ? 1.0 : (double)*a.upstream, labelled);
     double total = 0.0;
-    // Register j of a lane has the column `lane + LANES * ((j + turn) % held)`, but for the lanes behind the last column.
+    // Register j of a lane has the column `lane + LANES * ((j + turn) % held)`, where there is one.
     const int turn = AROUND ? team % held : 0, wrap = held - turn;
     const int missing = lane + LANES * (held - 1) < classes ? -1 : (AROUND ? wrap - 1 : held - 1);
     // (`phase` keeps the compiler from holding the addresses of one pass for the next: they do not fit the registers)

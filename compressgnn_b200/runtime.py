@@ -677,7 +677,7 @@ def cross_entropy(logits, target, ignore_index=-100, reduction="mean"):
     differentiable in ``logits``: what ``torch.nn.functional.cross_entropy`` computes, except that losses of 16-bit scores
     are float32.
 
-    Rows whose target is ``ignore_index`` have no loss and a gradient of zeros; their scores are not read.  A target
+    Rows whose target is ``ignore_index`` have no loss and a gradient of zeros, whatever their scores are.  A target
     that is no class is treated the same and recorded in ``device_status()``.  ``reduction="mean"`` divides by the
     number of the other rows (NaN when there are none).  With ``"sum"`` and ``"mean"`` the forward pass writes the gradient as
     well, so that the scores are read once a step: under ``torch.no_grad()`` it does not."""
