@@ -100,7 +100,7 @@ template <typename T, int VW, int TEAM, int VPL, bool DROP>
 __global__ void __launch_bounds__(FORWARD_THREADS<TEAM>, 512 / FORWARD_THREADS<TEAM>) norm_kernel(const NormArgs<T> a) {
     using A = Acc<T>;
     constexpr int TEAMS = FORWARD_THREADS<TEAM> / TEAM;
-        constexpr bool KEEP = VPL * VW <= 16;      // the parameters of a lane's columns stay in registers
+    constexpr bool KEEP = VPL * VW <= 16;          // the parameters of a lane's columns stay in registers
     constexpr bool VOTES = TEAM >= 32 && VW == 1;  // a warp draws the words of its columns together
     constexpr int SUMS = VW % 2 == 0 ? 2 : 1;
     __shared__ A shared[2 * (TEAM > 32 ? TEAM / 32 : 1)];
