@@ -485,9 +485,10 @@ __device__ __forceinline__ Acc<T> largest(const Vec<T, VW> &x) {
     }
 }
 
-// e^(x - m) of fp32 sums as 2^(x * log2(e) - c), c = m * log2(e): one instruction before the special function.  The rounding
-// of c is common to all exponentials of one m, which are off by a factor of 2^(m * log2(e) - c); it is divided out of
-// their sum and of the scale they are multiplied by.  It stays near one for |m| below 2^20; other rows subtract first.
+// e^(x - m) of fp32 sums as 2^(x * log2(e) - c), c = m * log2(e) rounded: one instruction before the special function.  All
+// exponentials of one m are off by the same factor of 2^(m * log2(e) - c), which is divided out of their sum and of the scale
+// they are multiplied by; a sum goes over to another m by the difference of the two rounded c's, and then has that one's
+// factor.  The factor stays near one for |m| below 2^20; other rows subtract first.
 __device__ __forceinline__ float from_offset(float m) { return power_of_two(fmaf(-m, LOG2_E, m * LOG2_E)); }  // 1 / that factor
 template <typename A>
 __device__ __forceinline__ bool is_steep(A m) {
@@ -510,6 +511,7 @@ __device__ __forceinline__ void row_statistics(Vectors &&vector, int vectors, in
     if constexpr (sizeof(A) == 4) {
         // One pass with a running maximum of the thread, a batch of vectors at a time.
         float2 two = make_float2(0.0f, 0.0f);
+        float offset = -INFINITY;  // m * log2(e), rounded
         for (int q = threadIdx.x; q < vectors; q += BATCH * THREADS) {
             Vec<T, VW> x[BATCH];
             float top = -INFINITY;
@@ -520,12 +522,13 @@ __device__ __forceinline__ void row_statistics(Vectors &&vector, int vectors, in
             if (top == -INFINITY) continue;  // (nothing to add; a NaN goes on)
             steep |= is_steep(top);
             if (top > m) {
-                const float down = power_of_two(fmaf(m, LOG2_E, -top * LOG2_E));
+                const float raised = __fmul_rn(top, LOG2_E), down = power_of_two(offset - raised);
                 two.x *= down;
                 two.y *= down;
                 m = top;
+                offset = raised;
             }
-            const float2 base = make_float2(LOG2_E, LOG2_E), c = make_float2(-m * LOG2_E, -m * LOG2_E);
+            const float2 base = make_float2(LOG2_E, LOG2_E), c = make_float2(-offset, -offset);
 #pragma unroll
             for (int b = 0; b < BATCH; ++b) {
                 if (q + b * THREADS >= vectors) break;

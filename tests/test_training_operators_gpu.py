@@ -499,6 +499,23 @@ def test_loss_of_large_scores():
             check_loss(logits, target, "mean", what=f"{scale} {classes}")
 
 
+@pytest.mark.parametrize("rising", [False, True])
+@pytest.mark.parametrize("classes", [47, 768, 769, 1000, 1025, 4097, 50001, 130000])
+def test_loss_of_scores_far_from_zero(classes, rising):
+    """An offset that all scores of a row share, which changes neither the loss nor the gradient of a row's scores as they are
+    stored; rising ones give a thread a larger score in every step.  The bounds are those of any scores: a distance from the
+    row's largest score is exact to the type's rounding whatever the two have in common."""
+    for dtype, offsets in ((F32, (3e3, -3e3, 1e5, 3e5, -3e5, 9e5, 2e6)), (F16, (3e2, -3e3)), (F64, (3e5,)), (BF16, (3e2,))):
+        for offset in offsets:
+            logits, target = loss_case(5, classes, dtype, seed=7)
+            logits = (logits.double() + offset).to(dtype)
+            if rising:
+                logits = logits.sort(1).values
+            target[1] = classes // 2
+            for reduction in ("mean", "none"):
+                check_loss(logits.detach().clone(), target, reduction, what=f"{dtype} {classes} {offset} {reduction}")
+
+
 def test_loss_without_labels():
     logits, target = loss_case(40, 7)
     target[:] = IGNORED
