@@ -466,21 +466,29 @@ struct Cover {
     }
 };
 
-// The largest element of a vector (pairs of 16-bit ones are compared as they are).
+// NaN where either is.
+__device__ __forceinline__ float larger_or_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ double larger_or_nan(double a, double b) { return a != a || a > b ? a : b; }
+
+// The largest element of a vector, NaN where it holds one (pairs of 16-bit ones are compared as they are).
 template <typename T, int VW>
 __device__ __forceinline__ Acc<T> largest(const Vec<T, VW> &x) {
     if constexpr (__is_same(T, __nv_bfloat16)) {
         const __nv_bfloat162 *pairs = reinterpret_cast<const __nv_bfloat162 *>(&x);
-        const __nv_bfloat162 two = __hmax2(__hmax2(pairs[0], pairs[1]), __hmax2(pairs[2], pairs[3]));
-        return fmaxf(__low2float(two), __high2float(two));
+        const __nv_bfloat162 two = __hmax2_nan(__hmax2_nan(pairs[0], pairs[1]), __hmax2_nan(pairs[2], pairs[3]));
+        return larger_or_nan(__low2float(two), __high2float(two));
     } else if constexpr (__is_same(T, __half)) {
         const __half2 *pairs = reinterpret_cast<const __half2 *>(&x);
-        const __half2 two = __hmax2(__hmax2(pairs[0], pairs[1]), __hmax2(pairs[2], pairs[3]));
-        return fmaxf(__low2float(two), __high2float(two));
+        const __half2 two = __hmax2_nan(__hmax2_nan(pairs[0], pairs[1]), __hmax2_nan(pairs[2], pairs[3]));
+        return larger_or_nan(__low2float(two), __high2float(two));
     } else {
         Acc<T> m = widen(x.v[0]);
 #pragma unroll
-        for (int k = 1; k < VW; ++k) m = larger(m, widen(x.v[k]));
+        for (int k = 1; k < VW; ++k) m = larger_or_nan(m, widen(x.v[k]));
         return m;
     }
 }
@@ -518,9 +526,9 @@ __device__ __forceinline__ void row_statistics(Vectors &&vector, int vectors, in
 #pragma unroll
             for (int b = 0; b < BATCH; ++b) x[b] = vector(q + b * THREADS < vectors ? q + b * THREADS : q);  // a thread's own
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b) top = fmaxf(top, largest<T, VW>(x[b]));
-            if (top == -INFINITY) continue;  // (nothing to add; a NaN goes on)
-            steep |= is_steep(top);
+            for (int b = 0; b < BATCH; ++b) top = larger_or_nan(top, largest<T, VW>(x[b]));
+            if (top == -INFINITY) continue;  // (nothing to add)
+            steep |= is_steep(top);          // (so is a NaN: the passes below carry it into the sum)
             if (top > m) {
                 const float raised = __fmul_rn(top, LOG2_E), down = power_of_two(offset - raised);
                 two.x *= down;

@@ -492,6 +492,27 @@ def test_loss_of_masked_classes(classes):
     assert torch.isfinite(got).all() and not got[4].any()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("classes", [7, 47, 384, 768, 769, 1000, 1025, 5000, 50001, 130000])
+def test_loss_of_a_score_that_is_no_number(classes, dtype):
+    """A NaN makes its row's loss and gradient NaN wherever it stands: among ordinary scores, and as the one class beside
+    the label that is not masked.  The other rows keep their values."""
+    for place in (0, 3, classes // 2, classes - 1):
+        for masked in (False, True):
+            logits, target = loss_case(6, classes, dtype, seed=place)
+            target[1], target[4] = (place + classes // 3) % classes, place
+            for row in (1, 4):
+                if masked:
+                    label = logits[row, target[row]].item()
+                    logits[row] = -math.inf
+                    logits[row, target[row]] = label
+                logits[row, place] = math.nan
+            for reduction in ("none", "sum", "mean"):
+                check_loss(logits.detach().clone(), target, reduction, what=f"{dtype} {classes} {place} {masked} {reduction}")
+            each = rt.cross_entropy(logits, target, reduction="none")
+            assert each.isnan().tolist() == [False, True, False, False, True, False]
+
+
 def test_loss_of_large_scores():
     for scale in (100.0, 1e4):
         for classes in (7, 1000, 3000):
