@@ -30,6 +30,7 @@ constexpr int LOSS_BLOCKS = SMS * 16;       // most blocks of a launch, each of 
 constexpr int COUNT_THREADS = 1024;
 constexpr int CLUSTER = 8;                  // blocks of the launch that does a small case alone
 constexpr size_t SHARED_MOST = 227 * 1024;  // of a block
+constexpr size_t DYNAMIC_MOST = SHARED_MOST - 2048;  // of it beside the kernels' own variables
 constexpr int LONG_THREADS = 512;
 
 // What the launches of one call hand each other.
@@ -856,8 +857,10 @@ constexpr int64_t CLUSTER_TILES = 4 * CLUSTER, CLUSTER_LONG_ROWS = CLUSTER;
 template <typename T>
 static int launch(void (*kernel)(LossArgs<T>), LossArgs<T> a, int64_t units, int64_t cluster_units, int threads, int blocks,
                   size_t shared, bool follows, cudaStream_t stream) {
-    if (shared > 44 * 1024)  // (with the kernels' own variables no more than the 48 KB that need no leave)
-        CGNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+    // (With the kernels' own variables no more than 48 KB need no leave.  The leave belongs to the kernel, and another thread may
+    // be between its own and its launch: it is always the same.)
+    if (shared > 44 * 1024)
+        CGNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DYNAMIC_MOST));
     a.clustered = follows && units <= cluster_units;
     if (follows && !a.clustered) {
         a.count_blocks = a.reduction == CGNN_MEAN ? (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(a.rows, COUNT_THREADS), SMS)) : 1;
@@ -929,7 +932,7 @@ static int launch_rows(const LossArgs<T> &a, bool follows, cudaStream_t stream) 
     if (shared <= 20 * 1024) return launch_long_rows<T, 128, FORWARD>(a, shared, follows, stream);
     if (shared <= 48 * 1024) return launch_long_rows<T, 256, FORWARD>(a, shared, follows, stream);
     if (shared <= SHARED_MOST / 2 - 2048) return launch_long_rows<T, 512, FORWARD>(a, shared, follows, stream);
-    if (shared <= SHARED_MOST - 2048) return launch_long_rows<T, 1024, FORWARD>(a, shared, follows, stream);
+    if (shared <= DYNAMIC_MOST) return launch_long_rows<T, 1024, FORWARD>(a, shared, follows, stream);
     return launch<T>(loss_long_kernel<T, FORWARD>, a, a.rows, CLUSTER_LONG_ROWS, LONG_THREADS, sizeof(T) == 8 ? 1 : 2, 0, follows, stream);
 }
 

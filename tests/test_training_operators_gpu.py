@@ -728,6 +728,33 @@ def test_steps_on_streams_and_threads():
         assert all(torch.equal(u, v) for u, v in zip(a, b))
 
 
+def test_calls_of_several_threads_with_rows_of_several_lengths():
+    """Calls whose kernels are one and the same and take different amounts of shared memory, from two threads at once."""
+    for dtype, lengths in ((BF16, (30000, 50001)), (F32, (720, 768)), (F32, (13000, 25000))):
+        cases = []
+        for classes in lengths:
+            logits, target = loss_case(40, classes, dtype)
+            cases.append((logits, target, rt.cross_entropy(logits, target)))
+        torch.cuda.synchronize()
+        failures = []
+
+        def work(logits, target, want):
+            try:
+                with torch.cuda.stream(torch.cuda.Stream()):
+                    for _ in range(1500):
+                        got = rt.cross_entropy(logits, target)
+                    assert torch.equal(got, want)
+            except Exception as e:  # (an assertion in a thread ends the thread alone)
+                failures.append(e)
+
+        threads = [threading.Thread(target=work, args=case) for case in cases]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not failures, failures
+
+
 def test_captured_steps():
     """A step captured twice, replayed in turn, each time with another key and other features."""
     graphs = []
