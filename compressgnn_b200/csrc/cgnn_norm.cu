@@ -600,13 +600,14 @@ struct NormCall {
     int64_t rows, width, stride;
     const void *x, *weight, *bias;
     double p;
+    bool with_params;  // something of param_dtype is read or written
 };
 
 static int check_call(const char *what, const NormCall &c) {
     CGNN_REQUIRE(c.dtype >= CGNN_F32 && c.dtype <= CGNN_F16, "%s: unknown dtype %d", what, c.dtype);
-    CGNN_REQUIRE((!c.weight && !c.bias) || c.param_dtype == c.dtype ||
+    CGNN_REQUIRE(!c.with_params || c.param_dtype == c.dtype ||
                      ((c.dtype == CGNN_BF16 || c.dtype == CGNN_F16) && c.param_dtype == CGNN_F32),
-                 "%s: weight and bias are of the matrix' type, or fp32 beside a 16-bit one", what);
+                 "%s: weight, bias and their gradients are of the matrix' type, or fp32 beside a 16-bit one", what);
     CGNN_REQUIRE(c.rows >= 0 && c.width >= 0 && c.stride >= 0, "%s: negative size", what);
     CGNN_REQUIRE(c.p >= 0.0 && c.p < 1.0, "%s: the drop probability must lie in [0, 1)", what);
     CGNN_REQUIRE(c.width <= INT32_MAX / 2, "%s: rows of %lld elements are not supported", what, (long long)c.width);
@@ -641,7 +642,7 @@ extern "C" {
 int cgnn_layer_norm(int dtype, int param_dtype, int64_t rows, int64_t width, int64_t stride, const void *x, const void *weight,
                     const void *bias, double eps, int relu, double p, uint64_t seed, const int64_t *device_seed, void *out,
                     void *mean, void *rstd, cgnn_stream_t stream) {
-    const NormCall c{dtype, param_dtype, rows, width, stride, x, weight, bias, p};
+    const NormCall c{dtype, param_dtype, rows, width, stride, x, weight, bias, p, weight || bias};
     if (int rc = check_call("layer_norm", c)) return rc;
     CGNN_REQUIRE((mean == nullptr) == (rstd == nullptr), "layer_norm: both statistics are written, or none");
     if (rows == 0 || width == 0) return CGNN_OK;
@@ -672,7 +673,7 @@ int cgnn_layer_norm_backward(int dtype, int param_dtype, int64_t rows, int64_t w
                              const void *weight, const void *bias, const void *mean, const void *rstd, const void *grad,
                              int relu, double p, uint64_t seed, const int64_t *device_seed, void *dx, void *dweight,
                              void *dbias, void *scratch, size_t scratch_bytes, cgnn_stream_t stream) {
-    const NormCall c{dtype, param_dtype, rows, width, stride, x, weight, bias, p};
+    const NormCall c{dtype, param_dtype, rows, width, stride, x, weight, bias, p, weight || bias || dweight || dbias};
     if (int rc = check_call("layer_norm_backward", c)) return rc;
     const size_t param = param_dtype == dtype ? item_of(dtype) : 4;
     if (rows == 0 && width > 0) {  // sums of nothing

@@ -130,6 +130,20 @@ def test_argument_errors_of_the_c_entries(which):
     assert message in _lib.lib().cgnn_last_error(), _lib.lib().cgnn_last_error()
 
 
+def test_gradients_of_parameters_have_a_type_of_their_own_only_beside_16_bits():
+    """Without a weight and a bias too: the sums would be written in the matrix' type behind arrays of a narrower one."""
+    def call(dtype, params, rows=4, dweight=64, dbias=None):
+        return _lib.lib().cgnn_layer_norm_backward(dtype, params, rows, 8, 8, 64, None, None, 64, 64, 64, 0, 0.0, 0, None, 64, dweight,
+                                                   dbias, 64, 1 << 20, None)
+    for dtype, params in ((1, 0), (0, 2), (1, 3), (2, 3), (2, 1), (0, 7)):
+        for rows in (4, 0):
+            for wanted in (dict(), dict(dweight=None, dbias=64)):
+                assert call(dtype, params, rows, **wanted) == 1, (dtype, params, rows)
+                assert b"matrix' type" in _lib.lib().cgnn_last_error()
+    # (where nothing has the type it is not looked at)
+    assert call(1, 0, rows=0, dweight=None) == 0
+
+
 def test_empty_calls_do_nothing():
     assert _norm(rows=0, x=None, out=None) == 0 and _norm(width=0, x=None, out=None) == 0
     assert _dropout(n=0, x=None, out=None) == 0
