@@ -86,6 +86,7 @@ SIGNATURES = {
                                  [_c_int, ctypes.c_double, ctypes.c_uint64] + [_c_ptr] * 5 + [_c_size, _c_ptr]),
     "cgnn_dropout": (_c_int, [_c_int, _c_i64, _c_ptr, _c_ptr, ctypes.c_double, ctypes.c_uint64, _c_ptr, _c_ptr, _c_ptr]),
     "cgnn_cross_entropy_scratch_bytes": (_c_size, []),
+    "cgnn_cross_entropy_wait_limit": (_c_int, [_c_int]),
     "cgnn_cross_entropy": (_c_int, [_c_int, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr, _c_ptr, _c_ptr,
                                     _c_ptr, _c_ptr, _c_size, _c_ptr]),
     "cgnn_cross_entropy_backward": (_c_int, [_c_int, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr, _c_ptr,

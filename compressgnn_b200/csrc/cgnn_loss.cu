@@ -8,6 +8,7 @@
 // loss, from the copy of the row it holds anyway: the scores are read once a step, not twice.  Losses are added up in
 // fp64 and in a fixed order.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include <cooperative_groups.h>
@@ -59,6 +60,7 @@ struct LossArgs {
     int skip_one;          // backward: `grad` holds the gradient for an incoming one already
     int dense;             // rows lie one behind the other from a 16-byte boundary on, in the scores and the gradient
     int whole_tiles;       // dense and narrow: a tile comes in one copy, unlabelled rows and all
+    int polls;             // after which a copy is given up
 };
 
 // The class of a row, or -1 for a row without one.
@@ -133,7 +135,7 @@ __device__ __forceinline__ void copy16(void *shared, const void *global, int byt
                  "r"(bytes)
                  : "memory");
 }
-// Bulk copies (whole 16-byte vectors) report to a barrier in shared memory, for which threads wait with a limit.
+// Bulk copies (whole 16-byte vectors) report to a barrier in shared memory, for which threads wait with a limit of polls.
 constexpr int WAIT_LIMIT = 1 << 20;
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void barrier_init(uint64_t *barrier, int arrivals) {
@@ -147,8 +149,8 @@ __device__ __forceinline__ void bulk_copy(void *shared, const void *global, uint
                  "l"(global), "r"(bytes), "r"(shared_address(barrier))
                  : "memory");
 }
-__device__ __forceinline__ bool barrier_wait(uint64_t *barrier, uint32_t parity) {
-    for (int i = 0; i < WAIT_LIMIT; ++i) {
+__device__ __forceinline__ bool barrier_wait(uint64_t *barrier, uint32_t parity, int polls) {
+    for (int i = 0; i < polls; ++i) {
         uint32_t done;
         asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
                      : "=r"(done)
@@ -342,16 +344,14 @@ __global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS, COLU
     int t = class_or_none(label_of(blockIdx.x)), round = 0;
     int64_t label_next = label_of(blockIdx.x + gridDim.x);
     if ((int)blockIdx.x < tiles) copy(blockIdx.x, t >= 0, 0, here);
-    for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++round) {
+    int i = blockIdx.x;
+    bool late = false;
+    for (; i < tiles; i += gridDim.x, ++round) {
         // (ordinary accesses to the other tile's place come before the copy into it)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        const uint32_t parity = (uint32_t)(round >> 1) & 1u;
-        const bool late = a.dense && !barrier_wait(&arrived[round & 1], parity);
-        if (__syncthreads_or(late)) {  // the tile is here, and the one before it has left; or a copy did not arrive
-            if (threadIdx.x == 0) atomicOr(&g_loss_status, STATUS_WAIT_EXPIRED);
-            barrier_wait(&arrived[round & 1], parity);
-            return;
-        }
+        late = a.dense && !barrier_wait(&arrived[round & 1], (uint32_t)(round >> 1) & 1u, a.polls);
+        late = __syncthreads_or(late);  // the tile is here, and the one before it has left; or a copy did not arrive
+        if (late) break;
         const int t_next = class_or_none(label_next);
         if (i + (int)gridDim.x < tiles) copy(i + gridDim.x, t_next >= 0, (round & 1) ^ 1, there);
         label_next = label_of(i + 2 * gridDim.x);
@@ -438,6 +438,24 @@ __global__ void __launch_bounds__(LANES *ROWS, TILE_BLOCKS<T, LANES * ROWS, COLU
             }
         }
         t = t_next;
+    }
+    if (late) {
+        // What was not computed is NaN, and the block takes part in the sum like the others, which wait for it.  Its copy
+        // comes to its end before the memory is another block's.
+        if (threadIdx.x == 0) atomicOr(&g_loss_status, STATUS_WAIT_EXPIRED);
+        barrier_wait(&arrived[round & 1], (uint32_t)(round >> 1) & 1u, WAIT_LIMIT);
+        const A none = (A)NAN;
+        total = NAN;
+        for (; i < tiles; i += gridDim.x) {
+            const int64_t r = (int64_t)i * ROWS + team;
+            if (FORWARD && lane == 0 && r < a.rows) {
+                if (a.reduction == CGNN_NONE) a.loss[r] = none;
+                if (a.stats) vec_store<A, 2>(a.stats + 2 * r, Vec<A, 2>{{none, none}});
+            }
+            const int n = i < tiles - 1 ? ROWS * classes : (int)(a.rows - (int64_t)i * ROWS) * classes;
+            if (a.grad)
+                for (int e = threadIdx.x; e < n; e += THREADS) a.grad[(int64_t)i * (ROWS * classes) + e] = narrow<T>(none);
+        }
     }
     if constexpr (FORWARD) {
         if (a.reduction != CGNN_NONE) finish<T, THREADS>(a, total, labelled);
@@ -847,6 +865,8 @@ __global__ void __launch_bounds__(LONG_THREADS, sizeof(T) == 8 ? 1 : 2) loss_lon
 // ---------------------------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------------------------
+static std::atomic<int> wait_limit{WAIT_LIMIT};
+
 // Units of work of a call (tiles or rows) that one cluster does alone, saving the launch that counts: as many rounds of its
 // blocks take no longer than that launch.
 constexpr int64_t CLUSTER_TILES = 4 * CLUSTER, CLUSTER_LONG_ROWS = CLUSTER;
@@ -954,6 +974,7 @@ static LossArgs<T> args_of(int64_t rows, int64_t classes, int64_t stride, const 
     a.ignore_index = ignore_index;
     a.reduction = reduction;
     a.grad = (T *)grad;
+    a.polls = wait_limit.load(std::memory_order_relaxed);
     a.dense = (stride == classes || rows == 1) && (((uintptr_t)logits | (uintptr_t)grad) & 15) == 0;
     // (a row of 96 bytes shares half of the 64-byte pieces it lies in, and small copies cost ten cycles each: 8.6 M x 7 with a
     // copy for every row 298 us)
@@ -977,6 +998,8 @@ using namespace cgnn;
 extern "C" {
 
 size_t cgnn_cross_entropy_scratch_bytes(void) { return sizeof(LossScratch); }
+
+int cgnn_cross_entropy_wait_limit(int polls) { return wait_limit.exchange(polls < 0 ? WAIT_LIMIT : polls); }
 
 int cgnn_cross_entropy(int dtype, int64_t rows, int64_t classes, int64_t stride, const void *logits, const int64_t *target,
                        int64_t ignore_index, int reduction, void *loss, void *stats, void *grad, int64_t *labelled, void *scratch,

@@ -402,8 +402,12 @@ int cgnn_dropout(int dtype, int64_t n, const void *x, const void *residual, doub
  *   labelled    one int64, with CGNN_SUM and CGNN_MEAN: the number of rows with a class (0 with CGNN_SUM)
  *   scratch     cgnn_cross_entropy_scratch_bytes(), 8-byte aligned, with CGNN_SUM and CGNN_MEAN
  * Backward: upstream is one value, or one per row with CGNN_NONE, of the loss' type.  With holds_unit_gradient `grad` is what
- * the forward call wrote: it is left alone when the incoming gradient is one, and computed anew otherwise. */
+ * the forward call wrote: it is left alone when the incoming gradient is one, and computed anew otherwise.
+ * A kernel that waits for a copy gives it up after a number of polls: what it has not computed, and a reduced loss, is NaN then,
+ * and status bit 2 is set.  cgnn_cross_entropy_wait_limit sets that number for the calls that follow (2^20 unless set; a
+ * negative one: 2^20) and returns the one before; with 0 every such wait is given up, which is what a test wants. */
 size_t cgnn_cross_entropy_scratch_bytes(void);
+int cgnn_cross_entropy_wait_limit(int polls);
 int cgnn_cross_entropy(int dtype, int64_t rows, int64_t classes, int64_t stride, const void *logits,
                        const int64_t *target, int64_t ignore_index, int reduction, void *loss, void *stats,
                        void *grad, int64_t *labelled, void *scratch, size_t scratch_bytes, cgnn_stream_t stream);

@@ -562,6 +562,37 @@ def test_loss_of_labels_that_are_no_classes():
         assert rt.device_status() == (1 if (target == IGNORED).any() else 0)
 
 
+def test_a_copy_that_is_given_up():
+    """Every wait of the loss for a copy given up at once: the blocks meet all the same, the call's results are NaN and the
+    status says so; the next call is as ever."""
+    from compressgnn_b200 import _lib
+    for rows, classes in ((40, 7), (500, 47), (4000, 500), (100001, 7), (60000, 47), (9000, 768)):
+        logits, target = loss_case(rows, classes)
+        logits.requires_grad_()
+        up = rand(rows, seed=1)
+
+        def results():
+            out = []
+            for reduction in ("mean", "sum", "none"):
+                loss = rt.cross_entropy(logits, target, reduction=reduction)
+                for factor in (1.0, 2.0):
+                    incoming = up if reduction == "none" else torch.full_like(loss, factor)
+                    out += [loss.detach(), torch.autograd.grad(loss, logits, incoming, retain_graph=True)[0]]
+            return out
+
+        want = results()
+        assert _lib.lib().cgnn_cross_entropy_wait_limit(0) == 2**20
+        try:
+            got = results()
+            torch.cuda.synchronize()
+        finally:
+            assert _lib.lib().cgnn_cross_entropy_wait_limit(-1) == 0
+        assert all(t.isnan().all() for t in got), (rows, classes)
+        assert rt.device_status() == 2 and rt.device_status() == 0
+        assert all(torch.equal(a, b) for a, b in zip(results(), want))
+    assert _lib.lib().cgnn_cross_entropy_wait_limit(-1) == 2**20
+
+
 def test_loss_gradients_against_differences():
     for classes in (5, 48, 1300):
         logits, target = loss_case(6, classes, F64)
