@@ -8,6 +8,14 @@ import torch
 from .. import runtime as _native
 
 
+def dropout_onto(residual, x, p, seed=None):
+    """``residual + dropout(x)`` with whatever may be added to ``x``: in one pass where the two have the same shape, type and
+    device, else broadcast and promoted by torch, as the sum is where nothing is dropped."""
+    if residual.shape == x.shape and residual.dtype == x.dtype and residual.device == x.device:
+        return _native.dropout(x, p, residual, seed)
+    return residual + _native.dropout(x, p, None, seed)
+
+
 class LayerNorm(torch.nn.Module):
     """Layer normalisation over the last dimension, with the ReLU and the dropout that follow it in the same pass."""
 
@@ -37,9 +45,9 @@ class Dropout(torch.nn.Module):
         self.p = p
 
     def forward(self, x, residual=None, seed=None):
-        if self.training and self.p:
-            return _native.dropout(x, self.p, residual, seed)
-        return x if residual is None else x + residual
+        if not (self.training and self.p):
+            return x if residual is None else x + residual
+        return _native.dropout(x, self.p, None, seed) if residual is None else dropout_onto(residual, x, self.p, seed)
 
     def extra_repr(self):
         return f"p={self.p}"

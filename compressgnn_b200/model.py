@@ -11,6 +11,7 @@ from torch import Tensor
 
 from . import runtime as _native
 from .layer import Compressgnn_Cluster, Compressgnn_Reconstruct, KPropagate, LayerNorm
+from .layer.training import dropout_onto
 
 
 class GNNLayer(torch.nn.Module):
@@ -50,7 +51,7 @@ class GNNLayer(torch.nn.Module):
         ``residual``: added to the layer's output, in the pass of the dropout when there is one."""
         if residual is not None:
             out = GNNLayer.forward(self, x, edge_index, edge_weight, vertex_cnt, rule_cnt)
-            return _native.dropout(out, dropout, residual) if dropout else out + residual
+            return dropout_onto(residual, out, dropout) if dropout else out + residual
         x = self.P(x=x, edge_index=edge_index, edge_weight=edge_weight, vertex_cnt=vertex_cnt, rule_cnt=rule_cnt)
         if self.norm is not None:
             return self.norm(self._transform(x, None, 0.0), dropout)

@@ -995,6 +995,38 @@ def test_modules():
     assert torch.equal(drop(h, residual=x), h + x) and LayerNorm(8, bias=False).bias is None
 
 
+@pytest.mark.parametrize("training", [False, True])
+def test_a_residual_of_another_shape_or_type(training):
+    """What may be added outside of training may be added in training, with the same shape and type: the residual is
+    broadcast and promoted as torch does."""
+    from compressgnn_b200.model import GNNLayer
+    data = graph_data()
+    layer = GNNLayer(24, 24, activation="relu", norm="layer").cuda()
+    drop = Dropout(0.4).train(training)
+    x = rand(data.vertex_cnt, 24, seed=1)
+    half = x.half()
+    for value, residual in ((x, rand(1, 24, seed=2)), (x, rand(24, seed=2)), (x, rand(2, *x.shape, seed=2)), (x, rand(*x.shape, dtype=F64, seed=2)),
+                            (half, rand(*x.shape, seed=2)), (x, half)):
+        residual.requires_grad_()
+        leaf = value.clone().requires_grad_()
+        y = drop(leaf, residual=residual, seed=9)
+        dropped = rt.dropout(value, 0.4, seed=9) if training else value
+        want = dropped + residual.detach()
+        assert y.dtype == want.dtype and torch.equal(y.detach(), want)
+        dx, dr = torch.autograd.grad(y, (leaf, residual), torch.ones_like(y))
+        times = y.numel() // value.numel()
+        assert torch.equal(dx, (rt.dropout(torch.ones_like(value), 0.4, seed=9) if training else torch.ones_like(value)) * times)
+        assert dr.shape == residual.shape and (dr == y.numel() // residual.numel()).all()
+        if value is x and residual.dim() < 3:
+            torch.manual_seed(4)
+            out = layer(x, data.edge_index, dropout=0.4 if training else 0.0, residual=residual.detach())
+            torch.manual_seed(4)
+            plain = layer(x, data.edge_index)
+            want = (rt.dropout(plain, 0.4) if training else plain) + residual.detach()
+            # (in one pass the sum is rounded once, from a product that is not: one rounding of the product apart)
+            assert out.dtype == want.dtype and (out - want).abs().max() <= 2.0**-24 * 2 * want.abs().max()
+
+
 def test_a_training_loop_runs():
     """The training loop of the example in the documents runs, and every parameter gets a gradient."""
     data = graph_data()
