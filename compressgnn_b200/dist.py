@@ -106,7 +106,7 @@ class ShardedGNNLayer(torch.nn.Module):
         from .layer import Compressgnn_Cluster, Compressgnn_Reconstruct, KPropagate
         if not layer.use_transformation:
             raise ValueError("ShardedGNNLayer needs a layer built with use_transformation=True")
-        if layer.norm is not None:
+        if getattr(layer, "norm", None) is not None:
             raise ValueError("a normalised layer needs whole rows: it is not sharded by columns")
         self.group, self.shard_output = group, shard_output
         self.rank, self.world = dist.get_rank(group), dist.get_world_size(group)
@@ -157,7 +157,7 @@ class ShardedGCN(torch.nn.Module):
 
     def __init__(self, model, group=None):
         super().__init__()
-        if model.residual:
+        if getattr(model, "residual", False):
             raise ValueError("a model with residual connections is not sharded by columns")
         last = len(model.layers) - 1
         self.group = group

@@ -112,3 +112,37 @@ def test_differentiable_column_gather_on_two_ranks():
     backward sums over ranks when the consumers differ and only slices when they are replicas."""
     world, port = 2, _free_port()
     mp.spawn(_gather_worker, args=(world, port), nprocs=world, join=True)
+
+
+def _foreign_worker(rank, world, port):
+    sys.path.insert(0, str(ROOT))
+    from compressgnn_b200 import dist as cdist
+    from compressgnn_b200.model import GCN
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        class Layer(torch.nn.Module):
+            def __init__(self, like):
+                super().__init__()
+                self.use_transformation, self.activation = like.use_transformation, like.activation
+                self.lin, self.cluster = like.lin, like.cluster
+
+        class Model(torch.nn.Module):
+            def __init__(self, like):
+                super().__init__()
+                self.dropout, self.layers = like.dropout, torch.nn.ModuleList(Layer(layer) for layer in like.layers)
+
+        model = Model(GCN(512, 5, hidden_features=16, param_H=4, use_transformation=True, num_layers=2))
+        assert len(cdist.ShardedGCN(model).layers) == 2
+        assert cdist.ShardedGNNLayer(model.layers[0]).lin is model.layers[0].lin
+        net, sharded = cdist.place_model(model, 512)
+        assert sharded and isinstance(net, cdist.ShardedGCN)
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.timeout(300)
+def test_models_of_the_same_shape_are_sharded():
+    """A model and layers with the attributes that sharding reads, of classes that know neither norm nor residual."""
+    world, port = 2, _free_port()
+    mp.spawn(_foreign_worker, args=(world, port), nprocs=world, join=True)
