@@ -165,6 +165,15 @@ def test_norm_rows(rows, width):
     check_norm(rand(rows, width), rand(width, seed=1, offset=1.0), rand(width, seed=2), p=0.1, what=f"{rows}x{width}")
 
 
+@pytest.mark.parametrize("dtype,rows,width", [(F64, 1500, 601), (F64, 700, 4098), (F32, 1100, 8200), (F32, 1537, 8193), (BF16, 1100, 8193),
+                                              (F16, 1025, 8200)])
+def test_norm_parameters_of_many_long_rows(dtype, rows, width):
+    """Rows that no team holds, more of them than one block of the parameters' sums takes, in shares of unequal size."""
+    for relu, p in ((False, 0.0), (True, 0.3)):
+        check_norm(rand(rows, width, dtype=dtype, offset=0.3), rand(width, dtype=dtype, seed=1, scale=0.3, offset=1.0),
+                   rand(width, dtype=dtype, seed=2, scale=0.3), relu, p, what=f"{dtype} {rows}x{width}")
+
+
 def test_norm_of_rows_far_from_zero():
     """Deviations are squared, not squares subtracted: a mean of a thousand deviations leaves the result exact to its bound."""
     for dtype in (F32, F64):
