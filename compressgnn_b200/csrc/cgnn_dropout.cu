@@ -19,7 +19,7 @@ struct DropArgs {
 // A block takes tiles of whole vectors, UNITS a thread, side by side; the elements behind the last tile and arrays that
 // do not lie on vector boundaries go element by element, a thread per block of four random words.
 // Memory bounds it in fp32: 325,557 x 256 with a residual 144 us for 1.0 GB (two units a thread: 154).
-// In bf16, 64 us for 333 MB (51 us), the random words are near it.
+// In bf16, 63 us for 333 MB (51 us) and 84 us with a residual (76 us).
 template <typename T, int VW, int UNITS, bool ADDED>
 __global__ void __launch_bounds__(256) dropout_kernel(const DropArgs<T> a, int64_t tiles) {
     using A = Acc<T>;
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(const DropArgs<T> a, int64
 
 template <typename T, bool ADDED>
 static int dropout_typed(const DropArgs<T> &a, cudaStream_t stream) {
-        constexpr int VW = sizeof(T) == 2 ? 8 : 4, UNITS = 4, TILE = 256 * VW * UNITS;
+    constexpr int VW = sizeof(T) == 2 ? 8 : 4, UNITS = 4, TILE = 256 * VW * UNITS;
     const bool vectors = (((uintptr_t)a.x | (uintptr_t)a.residual | (uintptr_t)a.out) & (sizeof(T) * VW - 1)) == 0;
     const int64_t tiles = vectors ? a.n / TILE : 0, rest = ceil_div(a.n - tiles * TILE, 1024);
     static const int resident = resident_blocks(dropout_kernel<T, VW, UNITS, ADDED>, 256);

@@ -677,8 +677,8 @@ __device__ __forceinline__ void store_vector(T *out, int first, int classes, boo
 
 // Rows of more classes: a block holds one row in shared memory.  A thread copies, reads and writes the same vectors
 // throughout, so that only the sums over the block need a barrier, and it fetches the next row's vector as soon as it is
-// done with this row's: one row is read while the other is written.  8192 x 50001 in bf16, 0.9 of the rows labelled: 333 us
-// (1.56 GB, 238 us at the copy rate); the special function unit is 56 % busy, issue slots 53 %, DRAM 47 %.
+// done with this row's: one row is read while the other is written.  8192 x 50001 in bf16, 0.9 of the rows labelled: 327 us
+// (1.56 GB, 238 us at the copy rate); the special function unit is 55 % busy, issue slots 53 %, DRAM 46 %.
 template <typename T, int THREADS, bool FORWARD>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_row_kernel(const LossArgs<T> a) {
     using A = Acc<T>;
@@ -782,7 +782,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_row_kernel(const
 }
 
 // Rows that shared memory does not hold: read a second time for the gradient, out of L2.  (8192 x 50001 in bf16, which
-// it holds: 441 us this way, 333 with the row kept.)
+// it holds: 441 us this way, 333 with the row kept, timed in turn.)
 template <typename T, bool FORWARD>
 __global__ void __launch_bounds__(LONG_THREADS, sizeof(T) == 8 ? 1 : 2) loss_long_kernel(const LossArgs<T> a) {
     using A = Acc<T>;

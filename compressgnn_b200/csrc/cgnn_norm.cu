@@ -94,8 +94,8 @@ __device__ __forceinline__ void load_row(const T *row, int width, int lane, Vec<
 }
 
 // Forward.  600,000 x 128 in fp32 with dropout: 96 us for 614 MB, the copy rate.  16384 x 4096 in bf16 with ReLU and dropout:
-// 76 us, and 45.5 without the dropout (268 MB, 41 us): there the random words bound it, 12 multiplications at four
-// cycles each for four elements.
+// 76 us, and 45.5 without the dropout (268 MB, 41 us): the random words double the instructions, and 16 warps a multiprocessor
+// (112 registers) do not hide their latency between a row's two barriers; issue slots 56 % busy, DRAM 35 %.
 template <typename T, int VW, int TEAM, int VPL, bool DROP>
 __global__ void __launch_bounds__(FORWARD_THREADS<TEAM>, 512 / FORWARD_THREADS<TEAM>) norm_kernel(const NormArgs<T> a) {
     using A = Acc<T>;
@@ -425,8 +425,13 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(const Acc<T> *partial, 
 // ---------------------------------------------------------------------------------------------
 // Rows of `vectors` vectors of VW elements: the least team that holds them with at most 16 elements a lane, whose
 // parameters then stay in registers.  (600,000 x 128 in fp32 and 100,000 x 768 in bf16, forward / backward with dropout: 96 / 139 and
-// 104 / 142 us; 8 elements: 111 / 227 and 110 / 162.)  Single elements are held by a warp, whose lanes draw random
-// words together.
+// 104 / 142 us, for 94 / 141 and 47 / 70 us at the copy rate; 8 elements: 111 / 227 and 110 / 162.)  Single elements are held by a
+// warp, whose lanes draw random words together.  Its steps are closer than powers of two because idle columns cost as much as
+// others.  60 M elements, us forward / backward, with dropout forward / backward, by these steps and by powers of two:
+//   fp32  187: 85 149 146 174, 95 149 197 228    319: 81 138 133 174, 97 145 203 283    603: 119 134 190 233, 140 238 278 608
+//         383: 89 130 139 180, 92 133 173 246    761: 117 126 191 221, 136 205 235 534
+//   bf16  187: 60 118 150 184, 75 125 206 244    319: 59 113 140 186, 75 143 212 294    603: 172 143 240 248, 199 250 313 571
+//         383: 68 110 149 199, 69 127 183 255    761: 164 138 223 238, 179 215 270 479
 // f(team, vectors a lane) with both as constants.
 template <int N>
 struct Num {

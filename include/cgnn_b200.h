@@ -11,8 +11,6 @@
  * row stride == width.  Index arrays handed to plan constructors may be 4 or 8 bytes wide;
  * plans keep private 32-bit copies.  The row operators of a training step (cgnn_layer_norm, cgnn_dropout,
  * cgnn_cross_entropy) also take CGNN_BF16 and CGNN_F16.
- * The row operators of a training step (cgnn_layer_norm, cgnn_dropout, cgnn_cross_entropy) also take
- * CGNN_BF16 and CGNN_F16.
  */
 #ifndef CGNN_B200_H
 #define CGNN_B200_H
