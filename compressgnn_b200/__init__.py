@@ -9,6 +9,7 @@ and layer API.
 ``offline``   numpy front end of the host library (compressor, filters, partitions)
 ``sample``    neighbour sampling on the compressed graph (the reference's ``compressgnn_sample``)
 ``dist``      column sharding over several GPUs (ShardedGCN, place_model)
+``optim``     AdamW: one launch for all tensors, moments in 32 or 8 bits
 ``model``     GNNLayer / GCN, the caller used by the end-to-end configurations
 
 Importing the package does not load CUDA; the first native call does, and fails loudly when

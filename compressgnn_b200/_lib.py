@@ -91,6 +91,16 @@ SIGNATURES = {
                                     _c_ptr, _c_ptr, _c_size, _c_ptr]),
     "cgnn_cross_entropy_backward": (_c_int, [_c_int, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr, _c_ptr,
                                              _c_ptr, _c_int, _c_ptr, _c_ptr]),
+    "cgnn_linear_mask_bytes": (_c_size, [_c_i64, _c_i64]),
+    "cgnn_linear_scratch_bytes": (_c_size, [_c_int, _c_i64, _c_i64, _c_i64]),
+    "cgnn_linear": (_c_int, [_c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, ctypes.c_double,
+                             ctypes.c_uint64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr]),
+    "cgnn_linear_backward_scratch_bytes": (_c_size, [_c_int, _c_i64, _c_i64, _c_i64]),
+    "cgnn_linear_backward": (_c_int, [_c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, ctypes.c_double,
+                                      _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr]),
+    "cgnn_linear_wait_limit": (_c_int, [_c_int]),
+    "cgnn_adamw_scratch_bytes": (_c_size, [_c_ptr, _c_i64]),
+    "cgnn_adamw": (_c_int, [_c_ptr, _c_i64] + [ctypes.c_double] * 4 + [ctypes.c_uint64, _c_ptr, _c_ptr, _c_size, _c_ptr]),
 }
 
 _lib = None

@@ -957,6 +957,211 @@ Tensor cross_entropy_autograd(const Tensor &logits, const Tensor &target_in, int
 }
 
 // ---------------------------------------------------------------------------------------------
+// a dense layer as one product
+// ---------------------------------------------------------------------------------------------
+struct LinearBackward : public Node {
+    SavedVariable x_, weight_, mask_;
+    int dtype = 0;
+    bool masked = false;
+    double p = 0.0;
+    at::TensorOptions weight_options;
+    variable_list apply(variable_list &&grads) override {
+        Tensor dx, dw, db, dresidual;
+        {
+            at::NoGradGuard no_grad;
+            const Tensor incoming = materialized(*this, grads[0]);
+            const c10::cuda::OptionalCUDAGuard guard(incoming.device());
+            // both of them, needed or not: one that was modified in place since the forward pass is an error
+            const Tensor x_in = x_.unpack(), weight = weight_.unpack().contiguous();
+            const Tensor mask = masked ? mask_.unpack().contiguous() : Tensor();
+            const int64_t in = weight.size(1), out = weight.size(0);
+            if (task_should_compute_output(0)) dx = at::empty(x_in.sizes(), x_in.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+            if (task_should_compute_output(1)) dw = at::empty({out, in}, weight_options);
+            if (task_should_compute_output(2)) db = at::empty({out}, weight_options);
+            if (dx.defined() || dw.defined() || db.defined()) {
+                const Tensor grad = incoming.contiguous();
+                const Rows x(x_in);
+                const int64_t rows = out ? grad.numel() / out : x.rows;
+                const size_t bytes = cgnn_linear_backward_scratch_bytes(dtype, rows, in, out);
+                const Tensor scratch = at::empty({(int64_t)bytes}, weight_options.dtype(at::kByte));
+                check(cgnn_linear_backward(dtype, rows, in, out, x.stride, data(x.held), data(weight), data(mask), data(grad), p,
+                                           data(dx), data(dw), data(db), data(scratch), bytes, current_stream(grad)));
+            }
+            if (task_should_compute_output(3)) dresidual = incoming;
+        }
+        return first_order({dx, dw, db, dresidual}, grads);
+    }
+    void release_variables() override {
+        for (SavedVariable *v : {&x_, &weight_, &mask_}) v->reset_data();
+    }
+    std::string name() const override { return "CompressgnnLinearBackward"; }
+};
+
+Tensor linear_autograd(const Tensor &x_in, const Tensor &weight, const c10::optional<Tensor> &bias_in, bool relu, double p,
+                       const c10::optional<Tensor> &residual_in, const c10::optional<int64_t> &seed,
+                       const c10::optional<Tensor> &seed_tensor) {
+    const Tensor bias = bias_in.value_or(Tensor()), residual = residual_in.value_or(Tensor());
+    TORCH_CHECK(x_in.is_cuda() && x_in.dim() >= 1, "linear: Expected a CUDA tensor of one dimension or more");
+    const int dtype = row_dtype(x_in, "linear");
+    refuse_dual("the dense layer", {x_in, weight, bias, residual});
+    TORCH_CHECK(weight.dim() == 2 && weight.size(1) == x_in.size(-1) && weight.device() == x_in.device() &&
+                    weight.scalar_type() == x_in.scalar_type(),
+                "linear: the weight is [out, in] for the input's last dimension, of its type and on its device");
+    const int64_t in = weight.size(1), out = weight.size(0);
+    TORCH_CHECK(!bias.defined() || (bias.dim() == 1 && bias.size(0) == out && bias.device() == x_in.device() &&
+                                    bias.scalar_type() == x_in.scalar_type()),
+                "linear: the bias is a vector over the weight's rows, of the input's type and on its device");
+    auto sizes = x_in.sizes().vec();
+    sizes.back() = out;
+    TORCH_CHECK(!residual.defined() || (residual.sizes() == at::IntArrayRef(sizes) && residual.device() == x_in.device() &&
+                                        residual.scalar_type() == x_in.scalar_type()),
+                "linear: the residual has the output's shape, type and device");
+    const c10::cuda::OptionalCUDAGuard guard(x_in.device());
+    const Key key = key_of("linear", p, seed, seed_tensor, x_in);
+    refuse_foreign_leaves("linear", {x_in, weight, bias, residual});
+    const bool differentiated = torch::autograd::compute_requires_grad(x_in, weight, bias, residual);
+    const bool masked = differentiated && (relu || p > 0.0);
+    Tensor y, mask;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const auto plain = x_in.options().requires_grad(false);
+        const Rows x(x_in);
+        y = at::empty(sizes, plain.memory_format(at::MemoryFormat::Contiguous));
+        const int64_t rows = out ? y.numel() / out : 0;
+        if (masked) mask = at::empty({(int64_t)cgnn_linear_mask_bytes(rows, out)}, plain.dtype(at::kByte));
+        const size_t bytes = cgnn_linear_scratch_bytes(dtype, rows, in, out);
+        const Tensor scratch = at::empty({(int64_t)bytes}, plain.dtype(at::kByte));
+        const Tensor w = weight.contiguous(), b = dense(bias), r = dense(residual);
+        check(cgnn_linear(dtype, rows, in, out, x.stride, data(x.held), data(w), data(b), data(r), relu, p, key.seed, key.pointer(),
+                          data(y), data(mask), data(scratch), bytes, current_stream(x_in)));
+    }
+    if (differentiated) {
+        auto node = new_node<LinearBackward>();
+        node->dtype = dtype;
+        node->masked = masked;
+        node->p = p;
+        node->weight_options = weight.options().requires_grad(false);
+        node->x_ = SavedVariable(x_in, false);
+        node->weight_ = SavedVariable(weight, false);
+        node->mask_ = SavedVariable(mask, false);
+        node->set_next_edges(torch::autograd::collect_next_edges(x_in, weight, bias, residual));
+        torch::autograd::set_history(y, node);
+    }
+    return y;
+}
+
+// ---------------------------------------------------------------------------------------------
+// one optimiser step over many tensors
+// ---------------------------------------------------------------------------------------------
+// The places that a step writes: no two of its tensors may share memory.
+struct Places {
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    void add(const Tensor &t) {
+        TORCH_CHECK(!t.is_inference() || c10::InferenceMode::is_enabled(), "adamw_step: an inference tensor is written in inference mode only");
+        if (!t.numel()) return;
+        const uintptr_t first = reinterpret_cast<uintptr_t>(t.data_ptr());
+        spans.push_back({first, first + t.nbytes()});
+    }
+    bool apart() {
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i)
+            if (spans[i].first < spans[i - 1].second) return false;
+        return true;
+    }
+};
+
+c10::optional<Tensor> adamw_step(const std::vector<Tensor> &params, const std::vector<Tensor> &grads, const std::vector<Tensor> &firsts,
+                                 const std::vector<Tensor> &seconds, const std::vector<Tensor> &steps,
+                                 const std::vector<c10::optional<Tensor>> &first_scales,
+                                 const std::vector<c10::optional<Tensor>> &second_scales, const std::vector<double> &rates,
+                                 const std::vector<c10::optional<Tensor>> &rate_tensors, const std::vector<double> &decays, double beta1,
+                                 double beta2, double eps, const c10::optional<double> &max_norm, int64_t seed) {
+    const size_t n = params.size();
+    TORCH_CHECK(grads.size() == n && firsts.size() == n && seconds.size() == n && steps.size() == n && first_scales.size() == n &&
+                    second_scales.size() == n && rates.size() == n && rate_tensors.size() == n && decays.size() == n,
+                "adamw_step: as many gradients, moments, steps, scales and rates as parameters are needed");
+    // (the library's bounds, before anything is looked at: a list without tensors is checked too)
+    TORCH_CHECK(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adamw_step: the betas must lie in [0, 1)");
+    TORCH_CHECK(eps >= 0.0, "adamw_step: eps must not be negative");
+    TORCH_CHECK(!max_norm.has_value() || *max_norm >= 0.0, "adamw_step: max_norm must not be negative");
+    if (n == 0) return c10::nullopt;
+    const auto device = params[0].device();
+    TORCH_CHECK(device.is_cuda(), "compressgnn_b200 runs on CUDA tensors only (no CPU optimiser path)");
+    std::vector<cgnn_adamw_tensor> list(n);
+    Places written;
+    written.spans.reserve(6 * n);
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor &p = params[i], &g = grads[i], &m = firsts[i], &v = seconds[i], &t = steps[i];
+        const int dtype = row_dtype(p, "adamw_step");
+        TORCH_CHECK(p.device() == device && g.device() == device && m.device() == device && v.device() == device && t.device() == device,
+                    "adamw_step: all tensors lie on one device");
+        TORCH_CHECK(p.is_contiguous(), "adamw_step: parameters are contiguous");
+        TORCH_CHECK(g.sizes() == p.sizes() && g.scalar_type() == p.scalar_type() && g.is_contiguous(),
+                    "adamw_step: a gradient is contiguous and has its parameter's shape and type");
+        const bool eight = m.scalar_type() == at::kFloat8_e4m3fn;
+        TORCH_CHECK(m.sizes() == p.sizes() && v.sizes() == p.sizes() && m.is_contiguous() && v.is_contiguous(),
+                    "adamw_step: moments are contiguous and have their parameter's shape");
+        TORCH_CHECK(m.scalar_type() == v.scalar_type() && (eight ? dtype != CGNN_F64 : m.scalar_type() == sum_type(p)),
+                    "adamw_step: moments are float32 (float64 beside float64 parameters) or, with scales, float8_e4m3fn");
+        TORCH_CHECK(t.scalar_type() == at::kLong && t.numel() == 1, "adamw_step: the steps taken are one int64 for each parameter");
+        TORCH_CHECK(eight == (first_scales[i].has_value() && first_scales[i]->defined()) &&
+                        eight == (second_scales[i].has_value() && second_scales[i]->defined()),
+                    "adamw_step: moments of 8 bits come with scales, others without");
+        cgnn_adamw_tensor &e = list[i];
+        e.lr = rates[i];
+        e.weight_decay = decays[i];
+        e.device_lr = nullptr;
+        TORCH_CHECK(e.lr >= 0.0 && e.weight_decay >= 0.0, "adamw_step: lr and weight_decay must not be negative");
+        if (rate_tensors[i].has_value()) {
+            const Tensor &rate = *rate_tensors[i];
+            TORCH_CHECK(rate.device() == device && rate.scalar_type() == at::kFloat && rate.numel() == 1,
+                        "adamw_step: a learning rate in a tensor is one float32 on the parameters' device");
+            e.device_lr = rate.const_data_ptr<float>();
+        }
+        if (eight)
+            for (const Tensor &s : {*first_scales[i], *second_scales[i]})
+                TORCH_CHECK(s.device() == device && s.scalar_type() == at::kFloat && s.is_contiguous() && s.numel() == (p.numel() + 255) / 256,
+                            "adamw_step: a moment has one float32 scale for each block of 256 elements");
+        for (const Tensor *w : {&p, &m, &v, &t}) written.add(*w);
+        e.param = data(p);
+        e.grad = data(g);
+        e.exp_avg = data(m);
+        e.exp_avg_sq = data(v);
+        e.exp_avg_scale = e.exp_avg_sq_scale = nullptr;
+        if (eight) {
+            written.add(*first_scales[i]);
+            written.add(*second_scales[i]);
+            // (of an empty tensor: no scales, which are not looked at, but moments of 8 bits all the same)
+            e.exp_avg_scale = static_cast<float *>(p.numel() ? data(*first_scales[i]) : data(t));
+            e.exp_avg_sq_scale = static_cast<float *>(p.numel() ? data(*second_scales[i]) : data(t));
+        }
+        e.step = t.data_ptr<int64_t>();
+        e.n = p.numel();
+        e.dtype = dtype;
+    }
+    TORCH_CHECK(written.apart(), "adamw_step: parameters, moments, scales and steps must not share memory");
+    const c10::cuda::OptionalCUDAGuard guard(device);
+    at::AutoDispatchBelowADInplaceOrView below;
+    Tensor norm, scratch;
+    size_t bytes = 0;
+    if (max_norm.has_value()) {
+        const auto options = at::TensorOptions().device(device);
+        norm = at::empty({}, options.dtype(at::kFloat));
+        bytes = cgnn_adamw_scratch_bytes(list.data(), (int64_t)n);
+        scratch = at::empty({(int64_t)bytes}, options.dtype(at::kByte));
+    }
+    check(cgnn_adamw(list.data(), (int64_t)n, beta1, beta2, eps, max_norm.value_or(-1.0), (uint64_t)seed,
+                     static_cast<float *>(data(norm)), data(scratch), bytes, current_stream(params[0])));
+    // what was written in place is newer than what autograd may have saved of it
+    for (size_t i = 0; i < n; ++i) {
+        for (const Tensor *w : {&params[i], &firsts[i], &seconds[i], &steps[i]}) w->unsafeGetTensorImpl()->bump_version();
+        if (list[i].exp_avg_scale != nullptr)
+            for (const Tensor &s : {*first_scales[i], *second_scales[i]}) s.unsafeGetTensorImpl()->bump_version();
+    }
+    return norm.defined() ? c10::optional<Tensor>(norm) : c10::nullopt;
+}
+
+// ---------------------------------------------------------------------------------------------
 // assignment
 // ---------------------------------------------------------------------------------------------
 std::tuple<Tensor, Tensor, int64_t, PlanPtr> assign(const Tensor &x, const Tensor &planes, int bits, const Tensor &workspace) {
@@ -1003,6 +1208,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("layer_norm", &layer_norm_autograd, nogil());
     m.def("dropout", &dropout_autograd, nogil());
     m.def("cross_entropy", &cross_entropy_autograd, nogil());
+    m.def("linear", &linear_autograd, nogil());
+    m.def("adamw_step", &adamw_step, nogil());
     m.def("assign", &assign, nogil());
     m.def("matmul_tn", [](const Tensor &a, const Tensor &b) {
         TORCH_CHECK(a.is_cuda() && a.device() == b.device() && a.scalar_type() == b.scalar_type() && a.dim() == 2 &&

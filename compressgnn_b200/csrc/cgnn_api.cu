@@ -107,6 +107,7 @@ cudaError_t pool_alloc(void **ptr, size_t bytes, cudaStream_t stream) {
 namespace cgnn {
 int sample_status(int *out);  // cgnn_sample.cu
 int loss_status(int *out);    // cgnn_loss.cu
+int linear_status(int *out);  // cgnn_linear.cu
 }
 
 extern "C" {
@@ -126,7 +127,9 @@ int cgnn_device_status(int *status_out) {
     if (rc == CGNN_OK) rc = cgnn::sample_status(&d);  // defined in cgnn_sample.cu
     int e = 0;
     if (rc == CGNN_OK) rc = cgnn::loss_status(&e);
-    *status_out = a | b | c | d | e;
+    int f = 0;
+    if (rc == CGNN_OK) rc = cgnn::linear_status(&f);
+    *status_out = a | b | c | d | e | f;
     return rc;
 }
 

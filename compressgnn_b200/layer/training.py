@@ -1,8 +1,8 @@
-"""Modules of a training step that stand between and behind the propagations: normalisation, dropout, loss.
+"""Modules of a training step that stand between and behind the propagations: dense layer, normalisation, dropout, loss.
 
 The reference's model calls ``torch.nn.functional`` for its dropout and leaves the loss to the caller (ref:
-``model/compressgnn/gcn.py:59``); these run on the package's own kernels (``runtime.layer_norm``, ``runtime.dropout``,
-``runtime.cross_entropy``)."""
+``model/compressgnn/gcn.py:59``); these run on the package's own kernels (``runtime.linear``, ``runtime.layer_norm``,
+``runtime.dropout``, ``runtime.cross_entropy``)."""
 import torch
 
 from .. import runtime as _native
@@ -14,6 +14,27 @@ def dropout_onto(residual, x, p, seed=None):
     if residual.shape == x.shape and residual.dtype == x.dtype and residual.device == x.device:
         return _native.dropout(x, p, residual, seed)
     return residual + _native.dropout(x, p, None, seed)
+
+
+class Linear(torch.nn.Linear):
+    """A dense layer with its bias, the ReLU, the dropout and the residual stream that follow it as one product."""
+
+    def __init__(self, in_features, out_features, bias=True, activation=None, device=None, dtype=None):
+        if activation not in (None, "relu"):
+            raise ValueError("Supported activations: None, relu")
+        super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
+        self.activation = activation
+
+    def forward(self, x, dropout=0.0, residual=None, seed=None):
+        """``dropout``: its probability; the caller passes 0 outside of training.  A residual of another shape, type or device
+        than the output is added by torch."""
+        fits = residual is not None and residual.shape == (*x.shape[:-1], self.out_features) and \
+            residual.dtype == x.dtype and residual.device == x.device
+        out = _native.linear(x, self.weight, self.bias, self.activation, dropout, residual if fits else None, seed)
+        return out if fits or residual is None else residual + out
+
+    def extra_repr(self):
+        return f"{super().extra_repr()}, activation={self.activation}"
 
 
 class LayerNorm(torch.nn.Module):

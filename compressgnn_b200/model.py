@@ -10,20 +10,25 @@ import torch.nn.functional as F
 from torch import Tensor
 
 from . import runtime as _native
-from .layer import Compressgnn_Cluster, Compressgnn_Reconstruct, KPropagate, LayerNorm
+from .layer import Compressgnn_Cluster, Compressgnn_Reconstruct, KPropagate, LayerNorm, Linear
 from .layer.training import dropout_onto
 
 
 class GNNLayer(torch.nn.Module):
     def __init__(self, in_features, out_features, param_H=1, use_transformation=False, refresh_interval=1,
-                 process_group=None, activation=None, norm=None):
+                 process_group=None, activation=None, norm=None, linear=None):
         super().__init__()
+        if linear not in (None, "fused"):
+            raise ValueError("linear must be None or 'fused'")
         if norm not in (None, "layer"):
             raise ValueError("norm must be None or 'layer'")
         if activation not in (None, "relu"):
             raise ValueError("activation must be None or 'relu'")
         self.activation = activation  # applied to the layer's output (fused into the reconstruction)
-        self.lin = torch.nn.Linear(in_features=in_features, out_features=out_features, bias=True)
+        if linear:  # one product with what follows it, on the package's kernel
+            self.lin = Linear(in_features, out_features, activation=None if norm else activation)
+        else:
+            self.lin = torch.nn.Linear(in_features=in_features, out_features=out_features, bias=True)
         self.P = KPropagate()
         self.use_transformation = use_transformation
         self.cluster = Compressgnn_Cluster(in_feature=in_features, param_H=param_H, training=True, cache=True,
@@ -49,6 +54,10 @@ class GNNLayer(torch.nn.Module):
         """``dropout``: probability of the dropout the model applies to this layer's (ReLU) output; with the
         transformation path it runs inside the reconstruct kernel, behind a normalisation inside its kernel.
         ``residual``: added to the layer's output, in the pass of the dropout when there is one."""
+        fused = isinstance(self.lin, Linear) and not self.use_transformation and self.norm is None
+        if fused:
+            x = self.P(x=x, edge_index=edge_index, edge_weight=edge_weight, vertex_cnt=vertex_cnt, rule_cnt=rule_cnt)
+            return self.lin(x, dropout, residual)
         if residual is not None:
             out = GNNLayer.forward(self, x, edge_index, edge_weight, vertex_cnt, rule_cnt)
             return dropout_onto(residual, out, dropout) if dropout else out + residual
@@ -81,15 +90,17 @@ class GCN(torch.nn.Module):
     residual = False  # (of a model that was saved whole before there was a choice)
 
     def __init__(self, in_features, out_features, hidden_features=128, param_H=1, dropout=0.3,
-                 use_transformation=False, refresh_interval=1, num_layers=3, norm=None, residual=False):
+                 use_transformation=False, refresh_interval=1, num_layers=3, norm=None, residual=False, linear=None):
         """``norm="layer"`` normalises the hidden layers' outputs in front of their ReLU; ``residual`` adds a hidden layer's
-        input to its output where the two are equally wide (neither is in the reference: deep stacks need them)."""
+        input to its output where the two are equally wide (neither is in the reference: deep stacks need them).
+        ``linear="fused"`` computes the layers' products without the transformation with what follows them in one pass
+        (``runtime.linear``): the same function, but its dropout draws from the package's generator."""
         super().__init__()
         dims = [in_features] + [hidden_features] * (num_layers - 1) + [out_features]
         self.layers = torch.nn.ModuleList(
             GNNLayer(dims[i], dims[i + 1], param_H=param_H, use_transformation=use_transformation,
                      refresh_interval=refresh_interval, activation="relu" if i + 1 < num_layers else None,
-                     norm=norm if i + 1 < num_layers else None)
+                     norm=norm if i + 1 < num_layers else None, linear=linear)
             for i in range(num_layers))
         self.dropout = dropout
         self.residual = residual

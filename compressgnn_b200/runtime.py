@@ -686,6 +686,56 @@ def cross_entropy(logits, target, ignore_index=-100, reduction="mean"):
     return differentiable(ops().cross_entropy, logits, target, int(ignore_index), _REDUCTIONS[reduction])
 
 
+def linear(input, weight, bias=None, activation=None, dropout=0.0, residual=None, seed=None):
+    """``residual + dropout(act(input @ weight.T + bias))`` as one product with everything behind it in its epilogue,
+    differentiable in ``input``, ``weight``, ``bias`` and ``residual``.
+
+    ``input``: float32, float64, bfloat16 or float16, ``[..., in]``; rows of a matrix may lie apart.  ``weight``
+    ``[out, in]``, ``bias`` ``[out]`` or None and ``residual`` (of the output's shape, or None) have its type.  Products are
+    added up in float32 (float64 for float64) and rounded once; float32 is computed to its last digits whatever torch's
+    switches for TF32 say.  ``activation``: None or ``"relu"``.  ``dropout``: the probability of the dropout that
+    follows; its mask is ``runtime.dropout``'s for the same ``seed``.  What the backward pass needs to know of the
+    output is one bit for each element; the output itself is not kept."""
+    _require(activation in (None, "relu"), "Supported activations: None, relu")
+    _require(torch.is_tensor(input) and input.is_cuda, "compressgnn_b200 runs on CUDA tensors only (no CPU product)")
+    _require(torch.is_tensor(weight), "linear: the weight is a tensor")
+    return differentiable(ops().linear, input, weight, bias, activation == "relu", float(dropout), residual,
+                          *_seed_args(seed))
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+               max_norm=None, exp_avg_scales=None, exp_avg_sq_scales=None, seed=0):
+    """One AdamW step over lists of tensors, in place and in one launch (for each type of parameter, and 300 tensors):
+
+    ``t = step + 1``, ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``,
+    ``p = p (1 - lr weight_decay) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)``.
+
+    ``params``, ``grads``: float32, float64, bfloat16 or float16, contiguous.  ``exp_avgs``, ``exp_avg_sqs``: float32
+    (float64 beside float64).  ``steps``: one int64 on the device for each parameter, the steps taken before; it is
+    counted on.  ``lr``: a number, or a CUDA tensor of one float32 that the kernels read when they run.  ``lr`` and
+    ``weight_decay`` may be lists with one for each parameter.
+
+    Moments of 8 bits are ``float8_e4m3fn`` tensors with a float32 scale for each block of 256 elements in
+    ``exp_avg_scales`` and ``exp_avg_sq_scales`` (lists, None for a parameter with the other kind): ``exp_avgs`` then holds
+    ``m`` and ``exp_avg_sqs`` the root of ``v``, both in units of their block's scale, a power of two.  They are rounded
+    stochastically under the key ``seed`` (of 64 bits), the position in the list and the step.
+
+    ``max_norm``: the gradients are taken times ``min(1, max_norm / (norm + 1e-6))`` with the 2-norm of all of them, which is
+    returned (a float32 tensor; None without ``max_norm``); they are not written."""
+    params = list(params)
+    none = [None] * len(params)
+    rates = list(lr) if isinstance(lr, (list, tuple)) else [lr] * len(params)
+    decays = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * len(params)
+    beta1, beta2 = betas
+    seed, _ = _seed_args(int(seed))
+    return ops().adamw_step(params, list(grads), list(exp_avgs), list(exp_avg_sqs), list(steps),
+                            none if exp_avg_scales is None else list(exp_avg_scales),
+                            none if exp_avg_sq_scales is None else list(exp_avg_sq_scales),
+                            [0.0 if torch.is_tensor(r) else float(r) for r in rates],
+                            [r if torch.is_tensor(r) else None for r in rates], [float(d) for d in decays],
+                            float(beta1), float(beta2), float(eps), None if max_norm is None else float(max_norm), seed)
+
+
 def device_status():
     """Read and clear the kernels' status word (synchronises the device)."""
     status = ctypes.c_int(0)

@@ -9,8 +9,8 @@
  * dtype: CGNN_F32 or CGNN_F64 (the reference dispatches both, ref:
  * src/runtime/csrc/sparse/cuda/spmm_gpu.cu:37).  All matrices are dense row-major with
  * row stride == width.  Index arrays handed to plan constructors may be 4 or 8 bytes wide;
- * plans keep private 32-bit copies.  The row operators of a training step (cgnn_layer_norm, cgnn_dropout,
- * cgnn_cross_entropy) also take CGNN_BF16 and CGNN_F16.
+ * plans keep private 32-bit copies.  The operators of a training step (cgnn_layer_norm, cgnn_dropout, cgnn_cross_entropy,
+ * cgnn_linear, cgnn_adamw) also take CGNN_BF16 and CGNN_F16.
  */
 #ifndef CGNN_B200_H
 #define CGNN_B200_H
@@ -413,6 +413,56 @@ int cgnn_cross_entropy_backward(int dtype, int64_t rows, int64_t classes, int64_
                                 const int64_t *target, int64_t ignore_index, int reduction, const void *stats,
                                 const int64_t *labelled, const void *upstream, int holds_unit_gradient, void *grad,
                                 cgnn_stream_t stream);
+
+/* A dense layer as one product: y[r,:] = residual[r,:] + dropout(act(x[r,:] weight^T + bias)), act = ReLU or nothing, the dropout
+ * that of cgnn_dropout on y.  weight: [out, in]; bias ([out]) and residual ([rows, out]) may be null; row r of x begins at
+ * x + r * stride elements; everything else is dense.  All of one type; products are added up in fp32 (fp64 for fp64) and
+ * a result is rounded once.  fp32 products are exact to fp32's last digits (no TF32).
+ *   mask      cgnn_linear_mask_bytes(), 8-byte aligned: a bit for each element of y that the ReLU and the dropout let through, what
+ *             the backward pass reads; may be null; not written where neither is asked for
+ *   scratch   cgnn_linear_scratch_bytes(), 16-byte aligned; its contents do not matter; the same for the backward pass
+ * Backward: grad: dense [rows, out]; mask: as written, or null where there was neither; p: of the forward call.  dx (dense
+ * [rows, in]), dweight, dbias: each may be null.  Sums over rows are added up in a fixed order.
+ * A kernel that waits for its own copies or products gives up after a number of polls; it writes NaN for what it has not
+ * computed and sets status bit 2.  cgnn_linear_wait_limit sets that number as cgnn_cross_entropy_wait_limit does. */
+size_t cgnn_linear_mask_bytes(int64_t rows, int64_t out);
+size_t cgnn_linear_scratch_bytes(int dtype, int64_t rows, int64_t in, int64_t out);
+int cgnn_linear(int dtype, int64_t rows, int64_t in, int64_t out, int64_t stride, const void *x, const void *weight,
+                const void *bias, const void *residual, int relu, double p, uint64_t seed, const int64_t *device_seed,
+                void *y, void *mask, void *scratch, size_t scratch_bytes, cgnn_stream_t stream);
+size_t cgnn_linear_backward_scratch_bytes(int dtype, int64_t rows, int64_t in, int64_t out);
+int cgnn_linear_backward(int dtype, int64_t rows, int64_t in, int64_t out, int64_t stride, const void *x,
+                         const void *weight, const void *mask, const void *grad, double p, void *dx, void *dweight,
+                         void *dbias, void *scratch, size_t scratch_bytes, cgnn_stream_t stream);
+int cgnn_linear_wait_limit(int polls);
+
+/* One AdamW step over many tensors at once:
+ *   t = step + 1, g = grad * clip, m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2,
+ *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps), step = t.
+ * A parameter and its gradient have one of the four types, moments are fp32 (fp64 for fp64).  With scales (not for fp64) the
+ * moments are held in 8 bits: exp_avg holds m and exp_avg_sq holds sqrt(v) as e4m3 numbers, to be multiplied by the
+ * scale of their block of 256 elements (ceil(n / 256) scales, powers of two), rounded stochastically by the Philox words of
+ * the key seed + i * 0x9E3779B97F4A7C15 + step * 0xD1342543DE82EF95 for tensor i of the list: element e of the tensor takes word e,
+ * the lower 16 bits for m, the upper ones for sqrt(v).
+ *   lr          of a tensor; or, when its device_lr is not null, the value found there when the kernel runs
+ *   max_norm    clip = min(1, max_norm / (norm + 1e-6)) with the 2-norm of all gradients; negative: clip = 1
+ *   norm        one float for that norm (written with max_norm >= 0 only); may be null
+ *   scratch     cgnn_adamw_scratch_bytes(), 8-byte aligned, needed with max_norm >= 0; its contents do not matter
+ * The list lies in host memory and is read before the call returns.  No two of its tensors may share memory. */
+typedef struct {
+    void *param;
+    const void *grad;
+    void *exp_avg, *exp_avg_sq;
+    float *exp_avg_scale, *exp_avg_sq_scale; /* null: moments of 32 (64) bits */
+    int64_t *step;                           /* one number on the device: the steps taken before (below 2^31) */
+    int64_t n;
+    double lr, weight_decay;
+    const float *device_lr;
+    int32_t dtype;
+} cgnn_adamw_tensor;
+size_t cgnn_adamw_scratch_bytes(const cgnn_adamw_tensor *tensors, int64_t count);
+int cgnn_adamw(const cgnn_adamw_tensor *tensors, int64_t count, double beta1, double beta2, double eps, double max_norm,
+               uint64_t seed, float *norm, void *scratch, size_t scratch_bytes, cgnn_stream_t stream);
 
 #ifdef __cplusplus
 }
