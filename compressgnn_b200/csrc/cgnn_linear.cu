@@ -137,23 +137,6 @@ __global__ void __launch_bounds__(TILE_THREADS) small_kernel(const Small<T> s) {
     }
 }
 
-// out[i] = scale * the sum over the splits, in their order.
-template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const Acc<T> *parts, int64_t splits, int64_t n, double scale, T *out) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    Acc<T> sum = parts[i];
-    for (int64_t s = 1; s < splits; ++s) sum += parts[s * n + i];
-    out[i] = narrow<T>(sum * (Acc<T>)scale);
-}
-
-template <typename T>
-int join(const Acc<T> *parts, int64_t splits, int64_t n, double scale, T *out, cudaStream_t stream) {
-    join_kernel<T><<<(unsigned)ceil_div(n, 256), 256, 0, stream>>>(parts, splits, n, scale, out);
-    CGNN_LAUNCH_CHECK();
-    return CGNN_OK;
-}
-
 int64_t small_tiles(int64_t M, int64_t N) { return ceil_div(M, TM) * std::max<int64_t>(1, ceil_div(N, TN)); }
 
 // Splits of the rows for a weight gradient: one wave of blocks, and none of fewer than 8 stages.
@@ -235,8 +218,36 @@ int small_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
 }
 
 template <typename T>
+constexpr bool HAS_TILES = sizeof(T) < 8;
+
+// Whether a call goes to the tensor cores: from 3e8 multiplications (fp32) and 8e7 (16 bits) on.  Us by tiles / by single
+// elements: fp32 forward 10,000 x 256 -> 128 25 / 37, 10,000 x 128 -> 64 21 / 14; bf16 10,000 x 128 -> 64 13 / 16, 40,000 x
+// 64 -> 64 19 / 21, 10,000 x 64 -> 64 12 / 11.
+bool by_tiles(int dtype, int64_t rows, int64_t in, int64_t out) {
+    return dtype != CGNN_F64 && in > 0 && (double)rows * (double)in * (double)out >= (dtype == CGNN_F32 ? 3e8 : 8e7);
+}
+
+std::atomic<int> wait_limit{WAIT_LIMIT};
+
+int status_address(int **out) {
+    void *p = nullptr;
+    CGNN_CUDA(cudaGetSymbolAddress(&p, g_linear_status));
+    *out = static_cast<int *>(p);
+    return CGNN_OK;
+}
+
+template <typename F>
+size_t bytes_of_type(int dtype, F &&call) {
+    switch (dtype) {
+        case CGNN_F32: return call(float());
+        case CGNN_BF16: return call(__nv_bfloat16());
+        default: return call(__half());
+    }
+}
+
+template <typename T>
 int forward(const Call &c, const void *weight, const void *bias, const void *residual, int relu, const Drop &drop, void *y, void *mask,
-            cudaStream_t stream) {
+            void *scratch, bool tiles, cudaStream_t stream) {
     Epilogue<T> e{};
     e.bias = static_cast<const T *>(bias);
     e.residual = static_cast<const T *>(residual);
@@ -245,17 +256,31 @@ int forward(const Call &c, const void *weight, const void *bias, const void *res
     e.width = c.out;
     e.relu = relu;
     e.drop = drop;
+    if constexpr (HAS_TILES<T>)
+        if (tiles) {
+            int *status;
+            const int rc = status_address(&status);
+            if (rc != CGNN_OK) return rc;
+            return tiles_forward<T>(c, static_cast<const T *>(weight), e, static_cast<T *>(y), scratch, wait_limit.load(), status, stream);
+        }
     return small_forward<T>(c, static_cast<const T *>(weight), e, static_cast<T *>(y), stream);
 }
 
 template <typename T>
 int backward(const Call &c, const void *weight, const void *mask, const void *grad, double scale, void *dx, void *dweight, void *dbias,
-             void *scratch, cudaStream_t stream) {
+             void *scratch, bool tiles, cudaStream_t stream) {
+    if constexpr (HAS_TILES<T>)
+        if (tiles) {
+            int *status;
+            const int rc = status_address(&status);
+            if (rc != CGNN_OK) return rc;
+            return tiles_backward<T>(c, static_cast<const T *>(weight), static_cast<const T *>(grad), static_cast<const uint8_t *>(mask),
+                                     scale, static_cast<T *>(dx), static_cast<T *>(dweight), static_cast<T *>(dbias), scratch,
+                                     wait_limit.load(), status, stream);
+        }
     return small_backward<T>(c, static_cast<const T *>(weight), static_cast<const T *>(grad), static_cast<const uint8_t *>(mask),
                              scale, static_cast<T *>(dx), static_cast<T *>(dweight), static_cast<T *>(dbias), scratch, stream);
 }
-
-std::atomic<int> wait_limit{WAIT_LIMIT};
 
 int check_call(int dtype, const Call &c, double p) {
     CGNN_REQUIRE(dtype >= CGNN_F32 && dtype <= CGNN_F16, "linear: unknown dtype");
@@ -275,8 +300,9 @@ extern "C" {
 size_t cgnn_linear_mask_bytes(int64_t rows, int64_t out) { return rows <= 0 || out <= 0 ? 0 : (size_t)rows * mask_pitch(out); }
 
 size_t cgnn_linear_scratch_bytes(int dtype, int64_t rows, int64_t in, int64_t out) {
-    (void)dtype, (void)rows, (void)in, (void)out;
-    return 0;
+    if (dtype < CGNN_F32 || dtype > CGNN_F16 || rows <= 0 || in <= 0 || out <= 0 || in >= WIDEST || out >= WIDEST) return 0;
+    if (!by_tiles(dtype, rows, in, out)) return 0;
+    return bytes_of_type(dtype, [&](auto zero) { return tiles_forward_bytes<decltype(zero)>(in, out); });
 }
 
 int cgnn_linear(int dtype, int64_t rows, int64_t in, int64_t out, int64_t stride, const void *x, const void *weight, const void *bias,
@@ -293,16 +319,19 @@ int cgnn_linear(int dtype, int64_t rows, int64_t in, int64_t out, int64_t stride
     CGNN_REQUIRE(need == 0 || (scratch != nullptr && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0),
                  "linear: scratch too small or not on a 16-byte boundary");
     const Drop drop = Drop::of(p, seed, device_seed);
+    const bool tiles = by_tiles(dtype, rows, in, out);
     switch (dtype) {
-        case CGNN_F32: return forward<float>(c, weight, bias, residual, relu, drop, y, mask, stream);
-        case CGNN_F64: return forward<double>(c, weight, bias, residual, relu, drop, y, mask, stream);
-        case CGNN_BF16: return forward<__nv_bfloat16>(c, weight, bias, residual, relu, drop, y, mask, stream);
-        default: return forward<__half>(c, weight, bias, residual, relu, drop, y, mask, stream);
+        case CGNN_F32: return forward<float>(c, weight, bias, residual, relu, drop, y, mask, scratch, tiles, stream);
+        case CGNN_F64: return forward<double>(c, weight, bias, residual, relu, drop, y, mask, scratch, tiles, stream);
+        case CGNN_BF16: return forward<__nv_bfloat16>(c, weight, bias, residual, relu, drop, y, mask, scratch, tiles, stream);
+        default: return forward<__half>(c, weight, bias, residual, relu, drop, y, mask, scratch, tiles, stream);
     }
 }
 
 size_t cgnn_linear_backward_scratch_bytes(int dtype, int64_t rows, int64_t in, int64_t out) {
     if (dtype < CGNN_F32 || dtype > CGNN_F16 || rows <= 0 || in < 0 || out <= 0 || in >= WIDEST || out >= WIDEST) return 0;
+    if (by_tiles(dtype, rows, in, out))
+        return bytes_of_type(dtype, [&](auto zero) { return tiles_backward_bytes<decltype(zero)>(rows, in, out); });
     return small_backward_bytes(dtype == CGNN_F64 ? 8 : 4, rows, in, out);
 }
 
@@ -325,15 +354,16 @@ int cgnn_linear_backward(int dtype, int64_t rows, int64_t in, int64_t out, int64
     CGNN_REQUIRE(dx == nullptr || weight != nullptr, "linear backward: the input's gradient needs the weight");
     CGNN_REQUIRE(dweight == nullptr || x != nullptr, "linear backward: the weight's gradient needs the input");
     CGNN_REQUIRE(((uintptr_t)mask & 7) == 0, "linear backward: the mask lies on an 8-byte boundary");
-    const size_t need = dweight != nullptr || dbias != nullptr ? cgnn_linear_backward_scratch_bytes(dtype, rows, in, out) : 0;
+    const size_t need = dx != nullptr || dweight != nullptr || dbias != nullptr ? cgnn_linear_backward_scratch_bytes(dtype, rows, in, out) : 0;
     CGNN_REQUIRE(need == 0 || (scratch != nullptr && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0),
                  "linear backward: scratch too small or not on a 16-byte boundary");
     const double scale = Drop::of(p, 0, nullptr).scale;
+    const bool tiles = by_tiles(dtype, rows, in, out);
     switch (dtype) {
-        case CGNN_F32: return backward<float>(c, weight, mask, grad, scale, dx, dweight, dbias, scratch, stream);
-        case CGNN_F64: return backward<double>(c, weight, mask, grad, scale, dx, dweight, dbias, scratch, stream);
-        case CGNN_BF16: return backward<__nv_bfloat16>(c, weight, mask, grad, scale, dx, dweight, dbias, scratch, stream);
-        default: return backward<__half>(c, weight, mask, grad, scale, dx, dweight, dbias, scratch, stream);
+        case CGNN_F32: return backward<float>(c, weight, mask, grad, scale, dx, dweight, dbias, scratch, tiles, stream);
+        case CGNN_F64: return backward<double>(c, weight, mask, grad, scale, dx, dweight, dbias, scratch, tiles, stream);
+        case CGNN_BF16: return backward<__nv_bfloat16>(c, weight, mask, grad, scale, dx, dweight, dbias, scratch, tiles, stream);
+        default: return backward<__half>(c, weight, mask, grad, scale, dx, dweight, dbias, scratch, tiles, stream);
     }
 }
 

@@ -52,4 +52,33 @@ struct Epilogue {
     }
 };
 
+// out[i] = scale * the sum over the splits, in their order.
+template <typename T>
+static __global__ void __launch_bounds__(256) join_kernel(const Acc<T> *parts, int64_t splits, int64_t n, double scale, T *out) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    Acc<T> sum = parts[i];
+    for (int64_t s = 1; s < splits; ++s) sum += parts[s * n + i];
+    out[i] = narrow<T>(sum * (Acc<T>)scale);
+}
+
+template <typename T>
+static int join(const Acc<T> *parts, int64_t splits, int64_t n, double scale, T *out, cudaStream_t stream) {
+    join_kernel<T><<<(unsigned)ceil_div(n, 256), 256, 0, stream>>>(parts, splits, n, scale, out);
+    CGNN_LAUNCH_CHECK();
+    return CGNN_OK;
+}
+
+// The products on the tensor cores (fp32, bf16, fp16).
+template <typename T>
+size_t tiles_forward_bytes(int64_t in, int64_t out);
+template <typename T>
+int tiles_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T *y, void *scratch, int polls, int *status,
+                  cudaStream_t stream);
+template <typename T>
+size_t tiles_backward_bytes(int64_t rows, int64_t in, int64_t out);
+template <typename T>
+int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t *mask, double scale, T *dx, T *dweight, T *dbias,
+                   void *scratch, int polls, int *status, cudaStream_t stream);
+
 }  // namespace cgnn
