@@ -22,25 +22,34 @@
 namespace cgnn {
 namespace {
 
-constexpr int BM = 128, BK = 64;  // BK 16-bit elements are a row of 128 bytes, the width of the swizzle
+constexpr int BM = 128;
 constexpr int EPILOGUE_WARPS = 8, PRODUCER_WARPS = 8;
 constexpr int PRODUCERS = PRODUCER_WARPS * 32;
 constexpr int MMA_WARP = EPILOGUE_WARPS + PRODUCER_WARPS, COPY_WARP = MMA_WARP + 1;
-constexpr int THREADS = (COPY_WARP + 1) * 32;
+constexpr int THREADS = (MMA_WARP + 4) * 32;
+// Registers of a thread by warpgroup; a launch brings 96 a thread, and the five groups share that: 2 x 112 + 2 x 112 + 32 = 5 x 96.
+constexpr int EPILOGUE_REGISTERS = 112, PRODUCER_REGISTERS = 112, OTHER_REGISTERS = 32;
 constexpr int SMS = 148;
 constexpr int TMEM_COLUMNS = 512;  // two buffers of 256
+constexpr int PIECE = 16;          // columns that a warp of the epilogue takes through shared memory at once
 
-template <typename T>
+// A stage holds BK of the contraction: rows of BK 16-bit elements (FORWARD, INPUT), or BK rows of panels of 64 (WEIGHT).
+template <typename T, int FORM>
 struct Shape {
     static constexpr bool SPLIT = sizeof(T) == 4;
     static constexpr int PLANES = SPLIT ? 3 : 1;
     static constexpr int BN = SPLIT ? 128 : 256;
-    static constexpr int STAGES = SPLIT ? 2 : 4;
+    static constexpr int BK = SPLIT || FORM == WEIGHT ? 32 : 64;
     static constexpr int A_PLANE = BM * BK * 2, B_PLANE = BN * BK * 2;
     static constexpr int STAGE = PLANES * (A_PLANE + B_PLANE);
-    static constexpr int SEGMENT = SPLIT ? 4 : 1 << 30;  // chunks of BK that an accumulator takes
-    static constexpr int SUMS = 16 * BM * 4;             // shared memory of the column sums
-    static constexpr int SHARED = STAGES * STAGE + SUMS + 1024;
+    static constexpr int STAGES = 192 * 1024 / STAGE;
+    static constexpr int SEGMENT = SPLIT ? 256 / BK : 1 << 30;  // chunks of BK that an accumulator takes
+    static constexpr int A_UNITS = BM * BK / 8 / PRODUCERS, B_UNITS = FORM == WEIGHT ? BN * BK / 8 / PRODUCERS : 0;
+    // Chunks on their way to a producer's registers: 64 KB a multiprocessor in fp32 (HBM wants 35), 48 in 16 bits.
+    static constexpr int DEPTH = SPLIT ? (FORM == WEIGHT ? 2 : 4) : 3;
+    static constexpr int STAGING = EPILOGUE_WARPS * 32 * PIECE * 4;
+    static constexpr int SUMS = FORM == WEIGHT ? 16 * BM * 4 : 0;  // of the columns
+    static constexpr int SHARED = STAGES * STAGE + STAGING + SUMS + 1024;
 };
 
 template <typename T>
@@ -54,8 +63,8 @@ struct Tiles {
     int64_t k_per_item;
     int tiles_m, tiles_n, items;
     int a_whole, b_whole;         // rows lie on vectors of 8 elements
+    int out_whole;                // rows of the output and the residual lie on vectors of 4
     void *out;                    // [M, N] of T, or (WEIGHT of several splits) [splits, M, N] of fp32
-    int64_t out_whole;            // its rows lie on vectors of 8 elements
     int partial;
     float *column_sums;           // WEIGHT: [splits, M]
     float scale;
@@ -100,11 +109,12 @@ __device__ __forceinline__ void bulk_copy(uint32_t to, const void *from, uint32_
 // ---------------------------------------------------------------------------------------------
 // tensor core instructions
 // ---------------------------------------------------------------------------------------------
-// A matrix in shared memory, rows of 128 bytes swizzled in groups of eight.  `leading`: bytes between panels of 64 elements along
-// m or n where those are contiguous; `stride`: bytes between groups of eight rows.
-__device__ __forceinline__ uint64_t matrix_descriptor(uint32_t address, uint32_t leading, uint32_t stride) {
-    return (uint64_t)((address >> 4) & 0x3fff) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | (uint64_t)1 << 46 |
-           (uint64_t)2 << 61;
+// A matrix in shared memory, rows of ROW bytes (128 or 64) swizzled in groups of eight.  `leading`: bytes between panels of 64
+// elements along m or n where those are contiguous.
+template <int ROW>
+__device__ __forceinline__ uint64_t matrix_descriptor(uint32_t address, uint32_t leading) {
+    return (uint64_t)((address >> 4) & 0x3fff) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(8 * ROW >> 4) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)(ROW == 128 ? 2 : 4) << 61;
 }
 // fp32 accumulators; operands bf16 or fp16, contiguous along k or (along_mn) along m and n.
 __host__ __device__ constexpr uint32_t product_descriptor(bool bf16, bool along_mn) {
@@ -148,6 +158,20 @@ __device__ __forceinline__ void tmem_load16(uint32_t address, float (&v)[16]) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
     }
+}
+// Eight columns, with the small products'.
+__device__ __forceinline__ void tmem_load8(uint32_t address, float (&v)[8]) {
+    uint32_t r[8], q[8];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%16];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%17];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=&r"(r[0]), "=&r"(r[1]), "=&r"(r[2]), "=&r"(r[3]), "=&r"(r[4]), "=&r"(r[5]), "=&r"(r[6]), "=&r"(r[7]), "=&r"(q[0]), "=&r"(q[1]),
+          "=&r"(q[2]), "=&r"(q[3]), "=&r"(q[4]), "=&r"(q[5]), "=&r"(q[6]), "=&r"(q[7])
+        : "r"(address), "r"(address + 128)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]) + __uint_as_float(q[i]);
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -236,21 +260,25 @@ struct Unit<__nv_bfloat16> : Unit16<__nv_bfloat16> {};
 template <>
 struct Unit<__half> : Unit16<__half> {};
 
-// Where a unit lies in a plane of shared memory: row r, unit c of its 128 bytes.
-__device__ __forceinline__ uint32_t place(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+// Where a unit lies in a plane of shared memory: row r of ROW bytes, unit c of them.
+template <int ROW>
+__device__ __forceinline__ uint32_t place(int r, int c) {
+    return (uint32_t)(r * ROW + ((ROW == 128 ? c ^ (r & 7) : c ^ (r >> 1 & 3)) << 4));
+}
 
 // ---------------------------------------------------------------------------------------------
-// the weight as images of shared memory: [tile of BN][chunk of BK][plane][BN rows of 128 bytes]
+// the weight as images of shared memory: [tile of BN][chunk of BK][plane][BN rows of BK]
 // ---------------------------------------------------------------------------------------------
 template <typename T, int FORM>
 __global__ void __launch_bounds__(256) pack_kernel(const T *weight, int64_t in, int64_t N, int64_t K, int64_t chunks, uint8_t *packed,
                                                    int whole) {
-    using S = Shape<T>;
+    using S = Shape<T, FORM>;
+    constexpr int UNITS = S::BK / 8;  // of a row
     const int64_t n_rows = (N + S::BN - 1) / S::BN * S::BN;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n_rows * chunks * 8) return;
+    if (i >= n_rows * chunks * UNITS) return;
     // neighbouring threads take neighbouring places in memory: units of a row, or (transposed) columns
-    const int64_t n = FORM == FORWARD ? i / (chunks * 8) : i % n_rows, unit = FORM == FORWARD ? i % (chunks * 8) : i / n_rows;
+    const int64_t n = FORM == FORWARD ? i / (chunks * UNITS) : i % n_rows, unit = FORM == FORWARD ? i % (chunks * UNITS) : i / n_rows;
     const int64_t k = unit * 8;
     Unit<T> u;
     u.clear();
@@ -266,10 +294,10 @@ __global__ void __launch_bounds__(256) pack_kernel(const T *weight, int64_t in, 
     }
     uint4 planes[S::PLANES];
     u.planes(planes);
-    uint8_t *const image = packed + ((n / S::BN) * chunks + unit / 8) * S::PLANES * S::B_PLANE;
+    uint8_t *const image = packed + ((n / S::BN) * chunks + unit / UNITS) * S::PLANES * S::B_PLANE;
 #pragma unroll
     for (int q = 0; q < S::PLANES; ++q)
-        *reinterpret_cast<uint4 *>(image + q * S::B_PLANE + place((int)(n % S::BN), (int)(unit % 8))) = planes[q];
+        *reinterpret_cast<uint4 *>(image + q * S::B_PLANE + place<S::BK * 2>((int)(n % S::BN), (int)(unit % UNITS))) = planes[q];
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -277,7 +305,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const T *weight, int64_t in, 
 // ---------------------------------------------------------------------------------------------
 struct Item {
     int64_t m0, n0, k0, k1;
-    int split, chunks;
+    int split;
 };
 template <typename T, int FORM>
 __device__ __forceinline__ Item item_of(const Tiles<T> &t, int item) {
@@ -286,11 +314,19 @@ __device__ __forceinline__ Item item_of(const Tiles<T> &t, int item) {
     i.split = FORM == WEIGHT ? item / tiles : 0;
     const int tile = FORM == WEIGHT ? item % tiles : item;
     i.m0 = (int64_t)(tile / t.tiles_n) * BM;
-    i.n0 = (int64_t)(tile % t.tiles_n) * Shape<T>::BN;
+    i.n0 = (int64_t)(tile % t.tiles_n) * Shape<T, FORM>::BN;
     i.k0 = i.split * t.k_per_item;
     i.k1 = min(t.K, i.k0 + t.k_per_item);
-    i.chunks = (int)((i.k1 - i.k0 + BK - 1) / BK);
     return i;
+}
+template <typename T, int FORM>
+__device__ __forceinline__ int chunks_of(const Tiles<T> &t, int item) {
+    int64_t k = t.K;
+    if (FORM == WEIGHT) {
+        const int64_t k0 = item / (t.tiles_m * t.tiles_n) * t.k_per_item;
+        k = min(k, k0 + t.k_per_item) - k0;
+    }
+    return (int)((k + Shape<T, FORM>::BK - 1) / Shape<T, FORM>::BK);
 }
 
 // One element by fp32 arithmetic: where an operand is infinite, no number or beyond bf16's range, its parts say nothing.
@@ -307,82 +343,264 @@ __device__ __noinline__ float single_element(const Tiles<T> &t, int64_t m, int64
     return sum;
 }
 
-// Eight neighbouring outputs.
+// Four neighbouring elements of a row.
 template <typename T>
-__device__ __forceinline__ void store8(T *p, const float (&y)[8], int64_t left, bool whole) {
-    if (whole && left >= 8) {
-        if constexpr (sizeof(T) == 4)
-            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]),
-                         "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7])
-                         : "memory");
-        else
-            vec_store<T, 8>(p, narrow_all<T, 8>(y));
+__device__ __forceinline__ void load4(const T *p, float (&y)[4], int left, bool whole) {
+    if (whole && left >= 4) {
+        widen_all<T, 4>(vec_load<T, 4>(p), y);
     } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < 4; ++k) y[k] = k < left ? widen(p[k]) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T *p, const float (&y)[4], int left, bool whole) {
+    if (whole && left >= 4) {
+        vec_store<T, 4>(p, narrow_all<T, 4>(y));
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
             if (k < left) p[k] = narrow<T>(y[k]);
     }
 }
 
-// What follows the product of eight neighbouring elements of a row; the bits of those that ReLU and dropout let through.
+// What follows the product of four neighbouring elements of a row; the bits of those that ReLU and dropout let through.
 template <typename T>
-__device__ __forceinline__ uint32_t follow(const Epilogue<T> &e, float (&y)[8], int64_t m, int64_t n, int64_t left, bool whole,
-                                           const float *bias, Philox &words) {
-    uint32_t passed = 0xff;
-    if (e.bias != nullptr) {
+__device__ __forceinline__ uint32_t follow(const Epilogue<T> &e, float (&y)[4], int64_t at, const float (&bias)[4], const float (&residual)[4],
+                                           float scale, Philox &words) {
+    uint32_t passed = 0xf;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] += bias[k];
-    }
+    for (int k = 0; k < 4; ++k) y[k] += bias[k];
     if (e.relu) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < 4; ++k)
             if (y[k] <= 0.f) {  // (a NaN stays one)
                 y[k] = 0.f;
                 passed &= ~(1u << k);
             }
     }
-    const int64_t at = m * e.width + n;
     if (e.drop.threshold) {
         const uint64_t block = (uint64_t)at >> 2;
         const int ahead = (int)(at & 3);
-        const uint4 q0 = words(block), q1 = words(block + 1);
-        uint32_t w[12] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w, 0, 0, 0, 0};
-        if (ahead) {  // the row does not begin with a block
-            const uint4 q2 = words(block + 2);
-            w[8] = q2.x, w[9] = q2.y, w[10] = q2.z, w[11] = q2.w;
+        const uint4 q = words(block);
+        uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        if (ahead) {  // the rows do not begin with a block of words
+            const uint4 r = words(block + 1);
+            const uint32_t all[8] = {q.x, q.y, q.z, q.w, r.x, r.y, r.z, r.w};
 #pragma unroll
-            for (int k = 0; k < 11; ++k) w[k] = ahead & 1 ? w[k + 1] : w[k];
-#pragma unroll
-            for (int k = 0; k < 9; ++k) w[k] = ahead & 2 ? w[k + 2] : w[k];
+            for (int k = 0; k < 4; ++k) w[k] = ahead == 1 ? all[k + 1] : ahead == 2 ? all[k + 2] : all[k + 3];
         }
-        const float scale = (float)e.drop.scale;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 4; ++k) {
             const bool kept = w[k] >= e.drop.threshold;
             y[k] = kept ? y[k] * scale : 0.f;
             if (!kept) passed &= ~(1u << k);
         }
     }
-    if (e.residual != nullptr) {
-        Unit<T> r;
-        r.load(e.residual + at, left, whole);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] += r.value(k);
-    }
+    for (int k = 0; k < 4; ++k) y[k] += residual[k];
     return passed;
 }
 
+// The epilogue of one warp: 32 rows (a row a lane in the accumulators) by PIECE columns at a time through shared memory, from
+// where four lanes take the columns of a row, eight rows at once, so that whole sectors are read and written.
+template <typename T, int FORM>
+struct Finish {
+    const Tiles<T> &t;
+    float *staging;        // [32][PIECE], units of four swizzled
+    const float *bias;     // of the warp's columns
+    Philox words;
+    int lane;
+
+    // Columns n .. n + PIECE of the rows m0 .. m0 + 32; x: the lane's row, k0 .. k1: the contraction behind it.
+    __device__ __forceinline__ void piece(float (&x)[PIECE], const Item &i, int64_t m0, int64_t n, int bias_at, bool alive) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<float4 *>(staging + lane * PIECE + (c ^ (lane >> 1 & 3)) * 4) =
+                make_float4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+        __syncwarp();
+        const int q = lane & 3;
+        const int64_t first = n + q * 4;
+        const int left = (int)min(t.N - first, (int64_t)4);
+        float b[4] = {0.f, 0.f, 0.f, 0.f};
+        if (FORM == FORWARD && t.epilogue.bias != nullptr) {
+            const float4 v = *reinterpret_cast<const float4 *>(bias + bias_at + q * 4);
+            b[0] = v.x, b[1] = v.y, b[2] = v.z, b[3] = v.w;
+        }
+        const float scale = FORM == FORWARD ? (float)t.epilogue.drop.scale : t.scale;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int row = lane / 4 + j * 8;
+            const int64_t m = m0 + row, at = m * t.N + first;
+            const bool inside = m < t.M && left > 0;
+            uint32_t passed = 0;
+            if (inside) {
+                float added[4] = {0.f, 0.f, 0.f, 0.f};
+                if (FORM == FORWARD && t.epilogue.residual != nullptr) load4<T>(t.epilogue.residual + at, added, left, t.out_whole);
+                const float4 v = *reinterpret_cast<const float4 *>(staging + row * PIECE + (q ^ (row >> 1 & 3)) * 4);
+                float y[4] = {v.x, v.y, v.z, v.w};
+                if constexpr (Shape<T, FORM>::SPLIT) {
+                    const float largest = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
+                    const float none = (y[0] + y[1]) * 0.f + (y[2] + y[3]) * 0.f;  // (fmaxf passes over what is no number)
+                    if (!(largest <= 3.402823466e38f && none == 0.f) && alive) {
+#pragma unroll 1
+                        for (int k = 0; k < left; ++k) {
+                            const float exact = single_element<T, FORM>(t, m, first + k, i.k0, i.k1);
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+                                if (c == k) y[c] = exact;
+                        }
+                    }
+                }
+                if (!alive)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[k] = __uint_as_float(0x7fffffffu);
+                if constexpr (FORM == FORWARD) {
+                    passed = follow<T>(t.epilogue, y, at, b, added, scale, words) & ((1u << left) - 1u);
+                    store4<T>(static_cast<T *>(t.out) + at, y, left, t.out_whole);
+                } else if (FORM == WEIGHT && t.partial) {
+                    store4<float>(static_cast<float *>(t.out) + i.split * t.M * t.N + at, y, left, t.out_whole);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[k] *= scale;
+                    store4<T>(static_cast<T *>(t.out) + at, y, left, t.out_whole);
+                }
+            }
+            if (FORM == FORWARD && t.epilogue.mask != nullptr) {
+                passed <<= 4 * q;
+                passed |= __shfl_xor_sync(0xffffffffu, passed, 1);
+                passed |= __shfl_xor_sync(0xffffffffu, passed, 2);
+                if (q == 0 && m < t.M && n < t.epilogue.mask_pitch * 8)
+                    *reinterpret_cast<uint16_t *>(t.epilogue.mask + m * t.epilogue.mask_pitch + n / 8) = (uint16_t)passed;
+            }
+        }
+        __syncwarp();
+    }
+};
+
+// The units of a producer, DEPTH chunks ahead of the stage that it writes.
+template <typename T, int FORM>
+struct Producer {
+    using S = Shape<T, FORM>;
+    static constexpr int BK = S::BK, ACROSS = BK / 8, DOWN = PRODUCERS / ACROSS;  // FORWARD, INPUT: units of a row, rows of a turn
+    static constexpr int A_ACROSS = BM / 8, A_DOWN = PRODUCERS / A_ACROSS;        // WEIGHT
+    [[maybe_unused]] static constexpr int B_ACROSS = S::BN / 8, B_DOWN = PRODUCERS / B_ACROSS;
+    const Tiles<T> &t;
+    int p;
+    // where the next chunk is read
+    int item, chunk, chunks;
+    const T *a, *b;
+    const uint8_t *mask;
+    int rows;           // of A from this thread's first on (WEIGHT: of A and B)
+    int b_rows;
+    int a_left, b_left; // elements of a row from this thread's first on
+
+    __device__ __forceinline__ Producer(const Tiles<T> &t_, int p_) : t(t_), p(p_), item(blockIdx.x), chunk(0), b(nullptr), mask(nullptr) {
+        begin();
+    }
+    __device__ __forceinline__ static int clamped(int64_t n) { return (int)max((int64_t)0, min(n, (int64_t)1 << 30)); }
+    __device__ __forceinline__ void begin() {
+        if (item >= t.items) return;
+        const Item i = item_of<T, FORM>(t, item);
+        chunk = 0;
+        chunks = chunks_of<T, FORM>(t, item);
+        if constexpr (FORM == WEIGHT) {
+            const int64_t row = i.k0 + p / A_ACROSS, column = i.m0 + p % A_ACROSS * 8;
+            const int64_t b_row = i.k0 + p / B_ACROSS, b_column = i.n0 + p % B_ACROSS * 8;
+            a = t.a + row * t.a_stride + column;
+            b = t.b + b_row * t.b_stride + b_column;
+            if (t.mask != nullptr) mask = t.mask + row * t.mask_pitch + column / 8;
+            rows = clamped(i.k1 - row);
+            b_rows = clamped(i.k1 - b_row);
+            a_left = clamped(t.M - column);
+            b_left = clamped(t.N - b_column);
+        } else {
+            const int64_t row = i.m0 + p / ACROSS, column = p % ACROSS * 8;
+            a = t.a + row * t.a_stride + column;
+            if (FORM == INPUT && t.mask != nullptr) mask = t.mask + row * t.mask_pitch + column / 8;
+            rows = clamped(t.M - row);
+            a_left = clamped(t.K - column);
+        }
+    }
+    __device__ __forceinline__ void load(Unit<T> (&x)[S::A_UNITS + S::B_UNITS], uint32_t (&keep)[S::A_UNITS]) {
+        if (item >= t.items) return;
+        constexpr int STEP = FORM == WEIGHT ? A_DOWN : DOWN;
+#pragma unroll
+        for (int u = 0; u < S::A_UNITS; ++u) {
+            keep[u] = 0xff;
+            if (u * STEP < rows && a_left > 0) {
+                x[u].load(a + u * STEP * t.a_stride, a_left, t.a_whole);
+                if (FORM != FORWARD && t.mask != nullptr) keep[u] = mask[u * STEP * t.mask_pitch];
+            } else {
+                x[u].clear();
+            }
+        }
+        if constexpr (FORM == WEIGHT) {
+#pragma unroll
+            for (int u = 0; u < S::B_UNITS; ++u) {
+                Unit<T> &y = x[S::A_UNITS + u];
+                if (u * B_DOWN < b_rows && b_left > 0) y.load(b + u * B_DOWN * t.b_stride, b_left, t.b_whole);
+                else y.clear();
+            }
+        }
+        if (++chunk == chunks) {
+            item += gridDim.x;
+            begin();
+        } else if constexpr (FORM == WEIGHT) {
+            a += BK * t.a_stride;
+            b += BK * t.b_stride;
+            mask += BK * t.mask_pitch;
+            rows -= BK;
+            b_rows -= BK;
+        } else {
+            a += BK;
+            mask += BK / 8;
+            a_left -= BK;
+        }
+    }
+    __device__ __forceinline__ void store(Unit<T> (&x)[S::A_UNITS + S::B_UNITS], uint32_t (&keep)[S::A_UNITS], uint32_t stage,
+                                          float (&columns)[8]) {
+        float sum[8];
+#pragma unroll
+        for (int u = 0; u < S::A_UNITS; ++u) {
+            if (FORM != FORWARD && t.mask != nullptr) x[u].keep(keep[u]);
+            if constexpr (FORM == WEIGHT)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum[k] = u == 0 ? x[u].value(k) : sum[k] + x[u].value(k);
+            uint4 planes[S::PLANES];
+            x[u].planes(planes);
+            const uint32_t at = FORM == WEIGHT ? p % A_ACROSS / 8 * (BK * 128) + place<128>(p / A_ACROSS + u * A_DOWN, p % 8)
+                                               : place<BK * 2>(p / ACROSS + u * DOWN, p % ACROSS);
+#pragma unroll
+            for (int q = 0; q < S::PLANES; ++q) store_shared(stage + q * S::A_PLANE + at, planes[q]);
+        }
+        if constexpr (FORM == WEIGHT) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) columns[k] += sum[k];
+#pragma unroll
+            for (int u = 0; u < S::B_UNITS; ++u) {
+                uint4 planes[S::PLANES];
+                x[S::A_UNITS + u].planes(planes);
+                const uint32_t at = p % B_ACROSS / 8 * (BK * 128) + place<128>(p / B_ACROSS + u * B_DOWN, p % 8);
+#pragma unroll
+                for (int q = 0; q < S::PLANES; ++q) store_shared(stage + S::PLANES * S::A_PLANE + q * S::B_PLANE + at, planes[q]);
+            }
+        }
+    }
+};
+
 template <typename T, int FORM>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ Tiles<T> t) {
-    using S = Shape<T>;
-    constexpr int BN = S::BN, STAGES = S::STAGES, PLANES = S::PLANES;
+    using S = Shape<T, FORM>;
+    constexpr int BN = S::BN, BK = S::BK, STAGES = S::STAGES, PLANES = S::PLANES;
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t a_full[STAGES], b_full[STAGES], empty[STAGES], sums_full[2], sums_empty[2], drained;
     __shared__ uint32_t tmem_base;
     __shared__ int given_up;
-    __shared__ float bias_of_tile[2][BN];
+    __shared__ __align__(16) float bias_of_tile[2][BN / 2];
     uint8_t *const stages = raw + (1024 - shared_address(raw) % 1024) % 1024;  // groups of eight swizzled rows lie on 1024 bytes
-    float *const column_parts = reinterpret_cast<float *>(stages + STAGES * S::STAGE);
+    float *const staging = reinterpret_cast<float *>(stages + STAGES * S::STAGE);
+    float *const column_parts = staging + S::STAGING / 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -413,209 +631,144 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 
     if (warp < EPILOGUE_WARPS) {
         // ------------------------------------------------------------------ accumulators to results
-        constexpr int COLUMNS = 64, PASSES = BN / (2 * COLUMNS);  // of a warp's half of the tile
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(EPILOGUE_REGISTERS));
+        constexpr int COLUMNS = BN / 2;  // of a warp's half of the tile
         const int quarter = warp & 3, half = warp >> 2;
-        Philox words(FORM == FORWARD ? t.epilogue.drop.key() : 0);
+        Finish<T, FORM> finish{t, staging + warp * 32 * PIECE, bias_of_tile[half], Philox(FORM == FORWARD ? t.epilogue.drop.key() : 0), lane};
         uint32_t segment = 0;
         for (int item = blockIdx.x; item < t.items; item += gridDim.x) {
             const Item i = item_of<T, FORM>(t, item);
-            const int64_t m = i.m0 + quarter * 32 + lane;
-            const bool inside = m < t.M;
-            float *const bias = bias_of_tile[half];
+            const int64_t m0 = i.m0 + quarter * 32, n0 = i.n0 + half * COLUMNS;
             if (FORM == FORWARD && t.epilogue.bias != nullptr) {
                 // the half's columns, by the four warps of the half
                 asm volatile("bar.sync %0, %1;" ::"r"(1 + half), "n"(EPILOGUE_WARPS / 2 * 32) : "memory");
-                for (int c = quarter * 32 + lane; c < BN / 2; c += EPILOGUE_WARPS / 2 * 32) {
-                    const int64_t n = i.n0 + half * (BN / 2) + c;
-                    bias[c] = n < t.N ? widen(t.epilogue.bias[n]) : 0.f;
-                }
+                for (int c = quarter * 32 + lane; c < COLUMNS; c += EPILOGUE_WARPS / 2 * 32)
+                    bias_of_tile[half][c] = n0 + c < t.N ? widen(t.epilogue.bias[n0 + c]) : 0.f;
                 asm volatile("bar.sync %0, %1;" ::"r"(1 + half), "n"(EPILOGUE_WARPS / 2 * 32) : "memory");
             }
-            if (FORM == FORWARD && t.epilogue.residual != nullptr && inside) {  // on its way while the products are formed
-                const int64_t first = i.n0 + half * (BN / 2), last = min(first + BN / 2, t.N);
-                for (int64_t n = first; n < last; n += 128 / (int)sizeof(T))
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(t.epilogue.residual + m * t.N + n));
+            if (FORM == FORWARD && t.epilogue.residual != nullptr && m0 + lane < t.M) {  // on its way while the products are formed
+                const int64_t last = min(n0 + COLUMNS, t.N);
+                for (int64_t n = n0; n < last; n += 128 / (int)sizeof(T))
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(t.epilogue.residual + (m0 + lane) * t.N + n));
             }
-            float sum[COLUMNS];
-            const int segments = S::SPLIT ? (i.chunks + S::SEGMENT - 1) / S::SEGMENT : 1;
-            for (int s = 0; s < segments; ++s, ++segment) {
-                const uint32_t buffer = segment & 1, parity = segment >> 1 & 1;
-                const bool good = barrier_wait(&sums_full[buffer], parity, polls, &given_up);
-                const bool alive = __all_sync(0xffffffffu, good);
-                const float lost = __uint_as_float(0x7fffffffu);
+            const uint32_t rows = tmem + ((uint32_t)(quarter * 32) << 16) + half * COLUMNS;
+            bool alive = true;
+            const auto await = [&] {
+                const uint32_t buffer = segment & 1;
+                alive = __all_sync(0xffffffffu, barrier_wait(&sums_full[buffer], segment >> 1 & 1, polls, &given_up)) && alive;
                 fence_after();
-#pragma unroll
-                for (int pass = 0; pass < PASSES; ++pass) {
-                    const int64_t first = i.n0 + half * (BN / 2) + pass * COLUMNS;
-                    const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + buffer * 256 + half * (BN / 2) + pass * COLUMNS;
-#pragma unroll
-                    for (int c = 0; c < COLUMNS; c += 16) {
-                        float part[16];
-                        if (alive) tmem_load16<S::SPLIT>(at + c, part);
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) sum[c + k] = !alive ? lost : s == 0 ? part[k] : sum[c + k] + part[k];
-                    }
-                    if (pass == PASSES - 1) {
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) barrier_arrive(&sums_empty[buffer]);
-                    }
-                    if (s + 1 < segments || !inside || first >= t.N) continue;
-                    uint32_t bits[2] = {0, 0};
-#pragma unroll
-                    for (int c = 0; c < COLUMNS; c += 8) {
-                        const int64_t n = first + c, left = t.N - n;
-                        if (left <= 0) continue;
-                        float y[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) y[k] = sum[c + k];
-                        if constexpr (S::SPLIT) {
-                            bool finite = true;
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) finite = finite && fabsf(y[k]) <= 3.402823466e38f;
-                            if (!finite && alive) {
+                return buffer;
+            };
+            const auto release = [&](uint32_t buffer) {
+                fence_before();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(&sums_empty[buffer]);
+                ++segment;
+            };
+            int before = 0;  // segments ahead of the last
+            if constexpr (S::SPLIT) before = (chunks_of<T, FORM>(t, item) - 1) / S::SEGMENT;
+            if (before == 0) {
+                const uint32_t buffer = await();
 #pragma unroll 1
-                                for (int k = 0; k < 8 && k < left; ++k) {
-                                    const float exact = single_element<T, FORM>(t, m, n + k, i.k0, i.k1);
+                for (int c = 0; c < COLUMNS; c += PIECE) {
+                    float x[PIECE];
+                    if (alive) tmem_load16<S::SPLIT>(rows + buffer * 256 + c, x);
+                    if (c + PIECE == COLUMNS) release(buffer);
+                    if (n0 + c < t.N && m0 < t.M) finish.piece(x, i, m0, n0 + c, c, alive);
+                }
+            } else if constexpr (S::SPLIT) {
+                float sum[COLUMNS];  // (a path of its own: the other keeps its registers)
 #pragma unroll
-                                    for (int j = 0; j < 8; ++j)
-                                        if (j == k) y[j] = exact;
-                                }
-                            }
-                        }
-                        if constexpr (FORM == FORWARD) {
-                            const uint32_t passed = follow<T>(t.epilogue, y, m, n, left, t.out_whole, bias + pass * COLUMNS + c, words);
-                            bits[c / 32] |= (left >= 8 ? passed : passed & ((1u << left) - 1u)) << (c % 32);
-                            store8<T>(static_cast<T *>(t.out) + m * t.N + n, y, left, t.out_whole);
-                        } else if (FORM == WEIGHT && t.partial) {
-                            store8<float>(static_cast<float *>(t.out) + (i.split * t.M + m) * t.N + n, y, left, t.out_whole);
-                        } else {
+                for (int c = 0; c < COLUMNS; ++c) sum[c] = 0.f;
+                for (; before >= 0; --before) {
+                    const uint32_t buffer = await();
+                    if (alive)
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) y[k] *= t.scale;
-                            store8<T>(static_cast<T *>(t.out) + m * t.N + n, y, left, t.out_whole);
+                        for (int c = 0; c < COLUMNS; c += 8) {
+                            float part[8];
+                            tmem_load8(rows + buffer * 256 + c, part);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) sum[c + k] += part[k];
                         }
-                    }
-                    if (FORM == FORWARD && t.epilogue.mask != nullptr)
-                        *reinterpret_cast<uint2 *>(t.epilogue.mask + m * t.epilogue.mask_pitch + first / 8) = make_uint2(bits[0], bits[1]);
+                    release(buffer);
+                }
+#pragma unroll
+                for (int c = 0; c < COLUMNS; c += PIECE) {
+                    float x[PIECE];
+#pragma unroll
+                    for (int k = 0; k < PIECE; ++k) x[k] = sum[c + k];
+                    if (n0 + c < t.N && m0 < t.M) finish.piece(x, i, m0, n0 + c, c, alive);
                 }
             }
         }
     } else if (warp < MMA_WARP) {
         // ------------------------------------------------------------------ operands to shared memory
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
         const int p = threadIdx.x - EPILOGUE_WARPS * 32;
-        constexpr int A_UNITS = BM * BK / 8 / PRODUCERS, B_UNITS = FORM == WEIGHT ? BN * BK / 8 / PRODUCERS : 1;
-        Unit<T> a[A_UNITS], b[B_UNITS];
-        uint32_t keep[A_UNITS];
-        const bool masked = FORM != FORWARD && t.mask != nullptr;
+        Unit<T> x[S::DEPTH][S::A_UNITS + S::B_UNITS];
+        uint32_t keep[S::DEPTH][S::A_UNITS];
         float columns[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) columns[k] = 0.f;
-
-        const auto load = [&](const Item &i, int chunk) {
-            const int64_t k0 = i.k0 + (int64_t)chunk * BK;
+        Producer<T, FORM> ahead(t, p);
 #pragma unroll
-            for (int u = 0; u < A_UNITS; ++u) {
-                const int64_t row = FORM == WEIGHT ? k0 + p / 16 + u * 16 : i.m0 + p / 8 + u * 32;
-                const int64_t column = FORM == WEIGHT ? i.m0 + p % 16 * 8 : k0 + p % 8 * 8;
-                const int64_t rows = FORM == WEIGHT ? i.k1 : t.M, width = FORM == WEIGHT ? t.M : t.K;
-                keep[u] = 0xff;
-                if (row < rows && column < width) {
-                    a[u].load(t.a + row * t.a_stride + column, width - column, t.a_whole);
-                    if (masked) keep[u] = t.mask[row * t.mask_pitch + column / 8];
-                } else {
-                    a[u].clear();
-                }
-            }
-            if constexpr (FORM == WEIGHT) {
-                constexpr int ACROSS = BN / 8;
-#pragma unroll
-                for (int u = 0; u < B_UNITS; ++u) {
-                    const int64_t row = k0 + p / ACROSS + u * (PRODUCERS / ACROSS), column = i.n0 + p % ACROSS * 8;
-                    if (row < i.k1 && column < t.N) b[u].load(t.b + row * t.b_stride + column, t.N - column, t.b_whole);
-                    else b[u].clear();
-                }
-            }
-        };
-        const auto store = [&](uint32_t stage, bool summed) {
-            float four[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) four[k] = 0.f;
-#pragma unroll
-            for (int u = 0; u < A_UNITS; ++u) {
-                if (masked) a[u].keep(keep[u]);
-                if (FORM == WEIGHT && summed)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) four[k] += a[u].value(k);
-                uint4 planes[PLANES];
-                a[u].planes(planes);
-                const uint32_t at = FORM == WEIGHT ? (p % 16 / 8) * (BK * 128) + place(p / 16 + u * 16, p % 8)
-                                                   : place(p / 8 + u * 32, p % 8);
-#pragma unroll
-                for (int q = 0; q < PLANES; ++q) store_shared(stage + q * S::A_PLANE + at, planes[q]);
-            }
-            if constexpr (FORM == WEIGHT) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) columns[k] += four[k];
-                constexpr int ACROSS = BN / 8;
-#pragma unroll
-                for (int u = 0; u < B_UNITS; ++u) {
-                    uint4 planes[PLANES];
-                    b[u].planes(planes);
-                    const uint32_t at = (p % ACROSS / 8) * (BK * 128) + place(p / ACROSS + u * (PRODUCERS / ACROSS), p % 8);
-#pragma unroll
-                    for (int q = 0; q < PLANES; ++q) store_shared(stage + PLANES * S::A_PLANE + q * S::B_PLANE + at, planes[q]);
-                }
-            }
-        };
-
+        for (int d = 0; d < S::DEPTH; ++d) ahead.load(x[d], keep[d]);
         uint32_t round = 0;
         bool alive = true;
-        int item = blockIdx.x;
-        if (item < t.items) load(item_of<T, FORM>(t, item), 0);
-        for (; item < t.items; item += gridDim.x) {  // (to the end whatever happens: the barriers below want every thread)
-            const Item i = item_of<T, FORM>(t, item);
-            const bool summed = FORM == WEIGHT && t.column_sums != nullptr && i.n0 == 0;
-            for (int chunk = 0; alive && chunk < i.chunks; ++chunk, ++round) {
+        int item = blockIdx.x, chunk = 0;
+        while (item < t.items) {  // (to the end whatever happens: the barriers below want every thread)
+#pragma unroll
+            for (int d = 0; d < S::DEPTH; ++d) {
+                if (item >= t.items) continue;
                 const uint32_t s = round % STAGES, parity = (round / STAGES & 1) ^ 1;
-                alive = __all_sync(0xffffffffu, barrier_wait(&empty[s], parity, polls, &given_up));
-                if (!alive) break;
-                store(shared_address(stages) + s * S::STAGE, summed);
-                fence_to_async();
-                __syncwarp();
-                if (lane == 0) barrier_arrive(&a_full[s]);
-                if (chunk + 1 < i.chunks) load(i, chunk + 1);
-                else if (item + gridDim.x < t.items) load(item_of<T, FORM>(t, item + gridDim.x), 0);
-            }
-            if (FORM == WEIGHT && summed) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    column_parts[(p / 16) * BM + p % 16 * 8 + k] = columns[k];
-                    columns[k] = 0.f;
+                if (alive) alive = __all_sync(0xffffffffu, barrier_wait(&empty[s], parity, polls, &given_up));
+                if (alive) {
+                    ahead.store(x[d], keep[d], shared_address(stages) + s * S::STAGE, columns);
+                    fence_to_async();
+                    __syncwarp();
+                    if (lane == 0) barrier_arrive(&a_full[s]);
+                    ahead.load(x[d], keep[d]);
                 }
-                asm volatile("bar.sync 3, %0;" ::"n"(PRODUCERS) : "memory");
-                if (p < BM && i.m0 + p < t.M) {
-                    float sum = 0.f;
+                ++round;
+                if (++chunk < chunks_of<T, FORM>(t, item)) continue;
+                if (FORM == WEIGHT && t.column_sums != nullptr) {
+                    const Item i = item_of<T, FORM>(t, item);
+                    if (i.n0 == 0) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) sum += column_parts[r * BM + p];
-                    if (*(volatile int *)&given_up) sum = __uint_as_float(0x7fffffffu);
-                    t.column_sums[i.split * t.M + i.m0 + p] = sum;
+                        for (int k = 0; k < 8; ++k) column_parts[(p / 16) * BM + p % 16 * 8 + k] = columns[k];
+                        asm volatile("bar.sync 3, %0;" ::"n"(PRODUCERS) : "memory");
+                        if (p < BM && i.m0 + p < t.M) {
+                            float total = 0.f;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) total += column_parts[r * BM + p];
+                            if (*(volatile int *)&given_up) total = __uint_as_float(0x7fffffffu);
+                            t.column_sums[i.split * t.M + i.m0 + p] = total;
+                        }
+                        asm volatile("bar.sync 3, %0;" ::"n"(PRODUCERS) : "memory");
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) columns[k] = 0.f;
                 }
-                asm volatile("bar.sync 3, %0;" ::"n"(PRODUCERS) : "memory");
+                chunk = 0;
+                item += gridDim.x;
             }
         }
-    } else if (warp == MMA_WARP) {
-        // ------------------------------------------------------------------ products
-        if (lane == 0) {
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGISTERS));
+        if (warp == MMA_WARP && lane == 0) {
+            // -------------------------------------------------------------- products
             constexpr bool ALONG_MN = FORM == WEIGHT;
             constexpr uint32_t base = product_descriptor(sizeof(T) == 4 || __is_same(T, __nv_bfloat16), ALONG_MN);
+            constexpr int ROW = ALONG_MN ? 128 : BK * 2;
             constexpr uint32_t LEADING = ALONG_MN ? BK * 128 : 16, STEP = ALONG_MN ? 16 * 128 : 32;  // STEP: 16 along k
             uint32_t round = 0, segment = 0;
             bool alive = true;
             for (int item = blockIdx.x; alive && item < t.items; item += gridDim.x) {
-                const Item i = item_of<T, FORM>(t, item);
-                const int columns = (int)min((int64_t)BN, (t.N - i.n0 + 15) / 16 * 16);
+                const int64_t n0 = item_of<T, FORM>(t, item).n0;
+                const int chunks = chunks_of<T, FORM>(t, item);
+                const int columns = (int)min((int64_t)BN, (t.N - n0 + 15) / 16 * 16);
                 const uint32_t descriptor = base | (uint32_t)(columns / 8) << 17;
-                for (int chunk = 0; alive && chunk < i.chunks; ++chunk, ++round) {
+                for (int chunk = 0; alive && chunk < chunks; ++chunk, ++round) {
                     const uint32_t buffer = segment & 1, accumulator = tmem + buffer * 256;
                     const bool fresh = chunk % S::SEGMENT == 0;
                     if (fresh) alive = barrier_wait(&sums_empty[buffer], (segment >> 1 & 1) ^ 1, polls, &given_up);
@@ -625,28 +778,24 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     if (!alive) break;
                     fence_after();
                     const uint32_t stage = shared_address(stages) + s * S::STAGE;
-                    uint64_t a[PLANES], b[PLANES];
-#pragma unroll
-                    for (int q = 0; q < PLANES; ++q) {
-                        a[q] = matrix_descriptor(stage + q * S::A_PLANE, LEADING, 1024);
-                        b[q] = matrix_descriptor(stage + PLANES * S::A_PLANE + q * S::B_PLANE, LEADING, 1024);
-                    }
+                    const uint64_t a = matrix_descriptor<ROW>(stage, LEADING), b = matrix_descriptor<ROW>(stage + PLANES * S::A_PLANE, LEADING);
+                    constexpr uint64_t AP = S::A_PLANE >> 4, BP = S::B_PLANE >> 4;
 #pragma unroll
                     for (int k = 0; k < BK / 16; ++k) {
-                        const uint64_t step = (uint64_t)(k * STEP >> 4);
+                        const uint64_t step = (uint64_t)(k * STEP >> 4), ak = a + step, bk = b + step;
                         const bool add = !fresh || k > 0;
-                        multiply(accumulator, a[0] + step, b[0] + step, descriptor, add);
+                        multiply(accumulator, ak, bk, descriptor, add);
                         if constexpr (S::SPLIT) {
                             const uint32_t small = accumulator + 128;
-                            multiply(small, a[0] + step, b[1] + step, descriptor, add);
-                            multiply(small, a[1] + step, b[0] + step, descriptor, true);
-                            multiply(small, a[0] + step, b[2] + step, descriptor, true);
-                            multiply(small, a[2] + step, b[0] + step, descriptor, true);
-                            multiply(small, a[1] + step, b[1] + step, descriptor, true);
+                            multiply(small, ak, bk + BP, descriptor, add);
+                            multiply(small, ak + AP, bk, descriptor, true);
+                            multiply(small, ak, bk + 2 * BP, descriptor, true);
+                            multiply(small, ak + 2 * AP, bk, descriptor, true);
+                            multiply(small, ak + AP, bk + BP, descriptor, true);
                         }
                     }
                     commit(&empty[s]);
-                    if (chunk + 1 == i.chunks || (chunk + 1) % S::SEGMENT == 0) {
+                    if (chunk + 1 == chunks || (chunk + 1) % S::SEGMENT == 0) {
                         commit(&sums_full[buffer]);
                         ++segment;
                     }
@@ -655,29 +804,26 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             for (uint32_t r = round > STAGES ? round - STAGES : 0; alive && r < round; ++r)  // the last reports have come in
                 alive = barrier_wait(&empty[r % STAGES], r / STAGES & 1, polls, &given_up);
             if (!alive) {  // products that are still under way read shared memory and write the accumulators
-                atomicOr(t.status, STATUS_WAIT_EXPIRED);
                 commit(&drained);
                 for (int k = 0; k < WAIT_LIMIT && !barrier_poll(&drained, 0); ++k) {}
             }
-        }
-    } else if (FORM != WEIGHT) {
-        // ------------------------------------------------------------------ the weight's images
-        if (lane == 0) {
+        } else if (FORM != WEIGHT && warp == COPY_WARP && lane == 0) {
+            // -------------------------------------------------------------- the weight's images
             uint32_t round = 0;
             bool alive = true;
-            const int64_t chunks = (t.K + BK - 1) / BK;
+            const int chunks = chunks_of<T, FORM>(t, 0);
             for (int item = blockIdx.x; alive && item < t.items; item += gridDim.x) {
-                const Item i = item_of<T, FORM>(t, item);
-                const uint32_t rows = (uint32_t)min((int64_t)BN, (t.N - i.n0 + 15) / 16 * 16);
-                const uint8_t *image = t.packed + (i.n0 / BN) * chunks * PLANES * S::B_PLANE;
-                for (int chunk = 0; alive && chunk < i.chunks; ++chunk, ++round, image += PLANES * S::B_PLANE) {
+                const int64_t n0 = item_of<T, FORM>(t, item).n0;
+                const uint32_t rows = (uint32_t)min((int64_t)BN, (t.N - n0 + 15) / 16 * 16);
+                const uint8_t *image = t.packed + (n0 / BN) * chunks * PLANES * S::B_PLANE;
+                for (int chunk = 0; alive && chunk < chunks; ++chunk, ++round, image += PLANES * S::B_PLANE) {
                     const uint32_t s = round % STAGES;
                     alive = barrier_wait(&empty[s], (round / STAGES & 1) ^ 1, polls, &given_up);
                     if (!alive) break;
                     const uint32_t to = shared_address(stages) + s * S::STAGE + PLANES * S::A_PLANE;
-                    barrier_expect(&b_full[s], rows * 128 * PLANES);
+                    barrier_expect(&b_full[s], rows * (BK * 2) * PLANES);
 #pragma unroll
-                    for (int q = 0; q < PLANES; ++q) bulk_copy(to + q * S::B_PLANE, image + q * S::B_PLANE, rows * 128, &b_full[s]);
+                    for (int q = 0; q < PLANES; ++q) bulk_copy(to + q * S::B_PLANE, image + q * S::B_PLANE, rows * (BK * 2), &b_full[s]);
                 }
             }
             if (!alive)  // copies that are still under way write shared memory
@@ -695,19 +841,19 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     }
 }
 
-bool whole_rows(const void *p, int64_t stride, size_t item) {
-    return stride % 8 == 0 && (uintptr_t)p % (8 * item) == 0;
+bool whole_rows(const void *p, int64_t stride, size_t item, int vector = 8) {
+    return stride % vector == 0 && (uintptr_t)p % (vector * item) == 0;
 }
 
 template <typename T>
 size_t packed_bytes(int64_t N, int64_t K) {
-    using S = Shape<T>;
-    return (size_t)ceil_div(N, S::BN) * (size_t)ceil_div(K, BK) * S::PLANES * S::B_PLANE;
+    using S = Shape<T, FORWARD>;  // (and INPUT)
+    return (size_t)ceil_div(N, S::BN) * (size_t)ceil_div(K, S::BK) * S::PLANES * S::B_PLANE;
 }
 
 template <typename T, int FORM>
 int launch(Tiles<T> &t, int64_t splits, cudaStream_t stream) {
-    using S = Shape<T>;
+    using S = Shape<T, FORM>;
     const int64_t tiles_m = ceil_div(t.M, BM), tiles_n = ceil_div(t.N, S::BN);
     CGNN_REQUIRE(tiles_m * tiles_n * splits < (1ll << 30), "linear: too many tiles");
     t.tiles_m = (int)tiles_m;
@@ -721,8 +867,8 @@ int launch(Tiles<T> &t, int64_t splits, cudaStream_t stream) {
 
 template <typename T, int FORM>
 int pack(const T *weight, int64_t in, int64_t N, int64_t K, uint8_t *packed, cudaStream_t stream) {
-    using S = Shape<T>;
-    const int64_t chunks = ceil_div(K, BK), units = ceil_div(N, S::BN) * S::BN * chunks * 8;
+    using S = Shape<T, FORM>;
+    const int64_t chunks = ceil_div(K, S::BK), units = ceil_div(N, S::BN) * S::BN * chunks * (S::BK / 8);
     pack_kernel<T, FORM><<<(unsigned)ceil_div(units, 256), 256, 0, stream>>>(weight, in, N, K, chunks, packed,
                                                                               whole_rows(weight, in, sizeof(T)));
     CGNN_LAUNCH_CHECK();
@@ -753,7 +899,7 @@ int tiles_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T
     t.N = c.out;
     t.K = t.k_per_item = c.in;
     t.out = y;
-    t.out_whole = whole_rows(y, c.out, sizeof(T)) && (epilogue.residual == nullptr || whole_rows(epilogue.residual, c.out, sizeof(T)));
+    t.out_whole = whole_rows(y, c.out, sizeof(T), 4) && (epilogue.residual == nullptr || whole_rows(epilogue.residual, c.out, sizeof(T), 4));
     t.epilogue = epilogue;
     t.polls = polls;
     t.status = status;
@@ -763,9 +909,10 @@ int tiles_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T
 // Splits of the rows of a weight gradient: what gives every multiprocessor one item, and none of fewer than four chunks.
 template <typename T>
 static int64_t weight_splits(int64_t rows, int64_t in, int64_t out, int64_t *rows_per_split) {
-    const int64_t tiles = ceil_div(out, BM) * ceil_div(in, Shape<T>::BN);
-    const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>(SMS / tiles, rows / (4 * BK)));
-    *rows_per_split = ceil_div(ceil_div(rows, wanted), BK) * BK;
+    using S = Shape<T, WEIGHT>;
+    const int64_t tiles = ceil_div(out, BM) * ceil_div(in, S::BN);
+    const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>(SMS / tiles, rows / (8 * S::BK)));
+    *rows_per_split = ceil_div(ceil_div(rows, wanted), S::BK) * S::BK;
     return ceil_div(rows, *rows_per_split);
 }
 
@@ -799,7 +946,7 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
         t.N = c.in;
         t.K = t.k_per_item = c.out;
         t.out = dx;
-        t.out_whole = whole_rows(dx, c.in, sizeof(T));
+        t.out_whole = whole_rows(dx, c.in, sizeof(T), 4);
         rc = launch<T, INPUT>(t, 1, stream);
         if (rc != CGNN_OK) return rc;
     }
@@ -818,7 +965,7 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
     t.k_per_item = per_split;
     t.partial = splits > 1 || dweight == nullptr;
     t.out = t.partial ? static_cast<void *>(parts) : dweight;
-    t.out_whole = t.partial ? c.in % 8 == 0 : whole_rows(dweight, c.in, sizeof(T));
+    t.out_whole = whole_rows(t.out, c.in, t.partial ? sizeof(float) : sizeof(T), 4);
     t.column_sums = dbias != nullptr ? sums : nullptr;
     int rc = launch<T, WEIGHT>(t, splits, stream);
     if (rc == CGNN_OK && t.partial && dweight != nullptr) rc = join<T>(parts, splits, c.out * c.in, scale, dweight, stream);
