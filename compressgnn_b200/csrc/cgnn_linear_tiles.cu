@@ -62,7 +62,6 @@ struct Tiles {
     int64_t M, N, K;
     int64_t k_per_item;
     int tiles_m, tiles_n, items;
-    int a_whole, b_whole;         // rows lie on vectors of 8 elements
     int out_whole;                // rows of the output and the residual lie on vectors of 4
     void *out;                    // [M, N] of T, or (WEIGHT of several splits) [splits, M, N] of fp32
     int partial;
@@ -109,21 +108,30 @@ __device__ __forceinline__ void bulk_copy(uint32_t to, const void *from, uint32_
 // ---------------------------------------------------------------------------------------------
 // tensor core instructions
 // ---------------------------------------------------------------------------------------------
-// A matrix in shared memory, rows of ROW bytes (128 or 64) swizzled in groups of eight.  `leading`: bytes between panels of 64
-// elements along m or n where those are contiguous.
-template <int ROW>
-__device__ __forceinline__ uint64_t matrix_descriptor(uint32_t address, uint32_t leading) {
-    return (uint64_t)((address >> 4) & 0x3fff) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(8 * ROW >> 4) << 32 | (uint64_t)1 << 46 |
-           (uint64_t)(ROW == 128 ? 2 : 4) << 61;
+// A matrix in shared memory, rows of ROW bytes (128 or 64) swizzled in groups of eight.  The lower word of its descriptor: its
+// address, and the bytes between panels of 64 elements along m or n where those are contiguous.  The upper word is the same for all.
+__device__ __forceinline__ uint32_t matrix_descriptor(uint32_t address, uint32_t leading) {
+    return (address >> 4 & 0x3fff) | leading >> 4 << 16;
 }
+template <int ROW>
+constexpr uint32_t MATRIX_UPPER = 8 * ROW >> 4 | 1u << 14 | (ROW == 128 ? 2u : 4u) << 29;
 // fp32 accumulators; operands bf16 or fp16, contiguous along k or (along_mn) along m and n.
 __host__ __device__ constexpr uint32_t product_descriptor(bool bf16, bool along_mn) {
     return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (along_mn ? 1u << 15 | 1u << 16 : 0u) | (uint32_t)(BM / 16) << 24;
 }
-__device__ __forceinline__ void multiply(uint32_t accumulator, uint64_t a, uint64_t b, uint32_t descriptor, bool add) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(accumulator),
-                 "l"(a), "l"(b), "r"(descriptor), "r"((uint32_t)add)
-                 : "memory");
+template <uint32_t UPPER>
+__device__ __forceinline__ void multiply(uint32_t accumulator, uint32_t a, uint32_t b, uint32_t descriptor, bool add) {
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 a, b;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}" ::"r"(accumulator),
+        "r"(a), "r"(b), "r"(descriptor), "r"((uint32_t)add), "n"(UPPER)
+        : "memory");
+}
+// True for one lane of the warp, the same every time.
+__device__ __forceinline__ bool leader_of_warp() {
+    uint32_t leads;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(leads));
+    return leads != 0;
 }
 // The barrier is told when the products issued by this thread up to here are done.
 __device__ __forceinline__ void commit(uint64_t *barrier) {
@@ -192,15 +200,19 @@ struct Unit<float> {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = 0.f;
     }
-    __device__ __forceinline__ void load(const float *p, int64_t left, bool whole) {
-        if (whole && left >= 8) {
-            asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                         : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
-                         : "l"(p));
-        } else {
+    // The first `left` elements, zeros behind them.
+    __device__ __forceinline__ void load(const float *p, int left) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = k < left ? p[k] : 0.f;
-        }
+        for (int k = 0; k < 8; ++k) v[k] = k < left ? p[k] : 0.f;
+    }
+    // All of them (on a boundary of 32 bytes), or zeros; without a branch.
+    __device__ __forceinline__ void load_whole(const float *p, bool there) {
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.u32 p, %9, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n"
+            " mov.b32 %4, 0;\n mov.b32 %5, 0;\n mov.b32 %6, 0;\n mov.b32 %7, 0;\n"
+            " @p ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n}"
+            : "=&f"(v[0]), "=&f"(v[1]), "=&f"(v[2]), "=&f"(v[3]), "=&f"(v[4]), "=&f"(v[5]), "=&f"(v[6]), "=&f"(v[7])
+            : "l"(p), "r"((uint32_t)there));
     }
     __device__ __forceinline__ void keep(uint32_t bits) {
 #pragma unroll
@@ -232,16 +244,19 @@ template <typename T>
 struct Unit16 {
     uint4 v;
     __device__ __forceinline__ void clear() { v = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void load(const T *p, int64_t left, bool whole) {
-        if (whole && left >= 8) {
-            v = *reinterpret_cast<const uint4 *>(p);
-        } else {
-            const uint16_t *const q = reinterpret_cast<const uint16_t *>(p);
-            uint32_t *const w = &v.x;
+    __device__ __forceinline__ void load(const T *p, int left) {
+        const uint16_t *const q = reinterpret_cast<const uint16_t *>(p);
+        uint32_t *const w = &v.x;
 #pragma unroll
-            for (int k = 0; k < 8; k += 2)
-                w[k / 2] = (k < left ? (uint32_t)q[k] : 0u) | (k + 1 < left ? (uint32_t)q[k + 1] : 0u) << 16;
-        }
+        for (int k = 0; k < 8; k += 2)
+            w[k / 2] = (k < left ? (uint32_t)q[k] : 0u) | (k + 1 < left ? (uint32_t)q[k + 1] : 0u) << 16;
+    }
+    __device__ __forceinline__ void load_whole(const T *p, bool there) {
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.u32 p, %5, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n"
+            " @p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n}"
+            : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+            : "l"(p), "r"((uint32_t)there));
     }
     __device__ __forceinline__ void keep(uint32_t bits) {
         uint32_t *const w = &v.x;
@@ -284,12 +299,13 @@ __global__ void __launch_bounds__(256) pack_kernel(const T *weight, int64_t in, 
     u.clear();
     if (n < N && k < K) {
         if (FORM == FORWARD) {
-            u.load(weight + n * in + k, K - k, whole);
+            if (whole && k + 8 <= K) u.load_whole(weight + n * in + k, true);
+            else u.load(weight + n * in + k, (int)min(K - k, (int64_t)8));
         } else {
             T v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = k + j < K ? weight[(k + j) * in + n] : narrow<T>(0.f);
-            u.load(v, 8, false);
+            u.load(v, 8);
         }
     }
     uint4 planes[S::PLANES];
@@ -343,159 +359,194 @@ __device__ __noinline__ float single_element(const Tiles<T> &t, int64_t m, int64
     return sum;
 }
 
-// Four neighbouring elements of a row.
-template <typename T>
-__device__ __forceinline__ void load4(const T *p, float (&y)[4], int left, bool whole) {
-    if (whole && left >= 4) {
-        widen_all<T, 4>(vec_load<T, 4>(p), y);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) y[k] = k < left ? widen(p[k]) : 0.f;
-    }
-}
-template <typename T>
-__device__ __forceinline__ void store4(T *p, const float (&y)[4], int left, bool whole) {
-    if (whole && left >= 4) {
-        vec_store<T, 4>(p, narrow_all<T, 4>(y));
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k < left) p[k] = narrow<T>(y[k]);
-    }
-}
-
-// What follows the product of four neighbouring elements of a row; the bits of those that ReLU and dropout let through.
-template <typename T>
-__device__ __forceinline__ uint32_t follow(const Epilogue<T> &e, float (&y)[4], int64_t at, const float (&bias)[4], const float (&residual)[4],
-                                           float scale, Philox &words) {
-    uint32_t passed = 0xf;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) y[k] += bias[k];
-    if (e.relu) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (y[k] <= 0.f) {  // (a NaN stays one)
-                y[k] = 0.f;
-                passed &= ~(1u << k);
-            }
-    }
-    if (e.drop.threshold) {
-        const uint64_t block = (uint64_t)at >> 2;
-        const int ahead = (int)(at & 3);
-        const uint4 q = words(block);
-        uint32_t w[4] = {q.x, q.y, q.z, q.w};
-        if (ahead) {  // the rows do not begin with a block of words
-            const uint4 r = words(block + 1);
-            const uint32_t all[8] = {q.x, q.y, q.z, q.w, r.x, r.y, r.z, r.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = ahead == 1 ? all[k + 1] : ahead == 2 ? all[k + 2] : all[k + 3];
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const bool kept = w[k] >= e.drop.threshold;
-            y[k] = kept ? y[k] * scale : 0.f;
-            if (!kept) passed &= ~(1u << k);
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) y[k] += residual[k];
-    return passed;
-}
-
 // The epilogue of one warp: 32 rows (a row a lane in the accumulators) by PIECE columns at a time through shared memory, from
-// where four lanes take the columns of a row, eight rows at once, so that whole sectors are read and written.
+// where four lanes take the columns of a row, eight rows at once, so that whole sectors are read and written.  A lane
+// has four rows, eight apart, and four columns of them.
 template <typename T, int FORM>
 struct Finish {
     const Tiles<T> &t;
-    float *staging;        // [32][PIECE], units of four swizzled
-    const float *bias;     // of the warp's columns
+    float *const staging;  // [32][PIECE], units of four swizzled
+    const float *const bias;
+    const int lane;
+    const bool has_bias, relu, vectors, partial;
+    const uint32_t threshold;
+    const float scale;
     Philox words;
-    int lane;
+    // of the present item
+    int64_t first;         // the element of the output that the lane's first row and column is
+    int rows, columns;     // from there on
+    const T *residual;
+    uint8_t *mask;
 
-    // Columns n .. n + PIECE of the rows m0 .. m0 + 32; x: the lane's row, k0 .. k1: the contraction behind it.
-    __device__ __forceinline__ void piece(float (&x)[PIECE], const Item &i, int64_t m0, int64_t n, int bias_at, bool alive) {
+    __device__ __forceinline__ Finish(const Tiles<T> &t_, float *staging_, const float *bias_, int lane_)
+        : t(t_), staging(staging_), bias(bias_), lane(lane_), has_bias(FORM == FORWARD && t_.epilogue.bias != nullptr),
+          relu(FORM == FORWARD && t_.epilogue.relu), vectors(t_.out_whole), partial(FORM == WEIGHT && t_.partial),
+          threshold(FORM == FORWARD ? t_.epilogue.drop.threshold : 0), scale(FORM == FORWARD ? (float)t_.epilogue.drop.scale : t_.scale),
+          words(FORM == FORWARD && threshold ? t_.epilogue.drop.key() : 0) {}
+
+    __device__ __forceinline__ void begin(int64_t m0, int64_t n0) {
+        const int64_t m = m0 + lane / 4, n = n0 + lane % 4 * 4;
+        first = m * t.N + n;
+        rows = (int)max((int64_t)0, min(t.M - m, (int64_t)32));
+        columns = (int)max((int64_t)-PIECE, min(t.N - n, (int64_t)1024));
+        residual = FORM == FORWARD && t.epilogue.residual != nullptr ? t.epilogue.residual + first : nullptr;
+        mask = FORM == FORWARD && t.epilogue.mask != nullptr ? t.epilogue.mask + m * t.epilogue.mask_pitch + n0 / 8 : nullptr;
+    }
+
+    // Columns c .. c + PIECE of the item; x: the lane's row of the accumulators.
+    __device__ __forceinline__ void piece(float (&x)[PIECE], const Item &i, int64_t m0, int64_t n0, int c, bool alive) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<float4 *>(staging + lane * PIECE + (c ^ (lane >> 1 & 3)) * 4) =
-                make_float4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
-        __syncwarp();
-        const int q = lane & 3;
-        const int64_t first = n + q * 4;
-        const int left = (int)min(t.N - first, (int64_t)4);
-        float b[4] = {0.f, 0.f, 0.f, 0.f};
-        if (FORM == FORWARD && t.epilogue.bias != nullptr) {
-            const float4 v = *reinterpret_cast<const float4 *>(bias + bias_at + q * 4);
-            b[0] = v.x, b[1] = v.y, b[2] = v.z, b[3] = v.w;
+        for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<float4 *>(staging + lane * PIECE + (k ^ (lane >> 1 & 3)) * 4) =
+                make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+        const int q = lane & 3, left = columns - c;
+        const bool vector = vectors && left >= 4;
+        const int64_t down = 8 * t.N;
+        float y[4][4], added[4][4];
+        if (FORM == FORWARD && residual != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const T *const r = residual + c + j * down;
+                if (vector && 8 * j < rows) {
+                    widen_all<T, 4>(vec_load<T, 4>(r), added[j]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) added[j][k] = 8 * j < rows && k < left ? widen(r[k]) : 0.f;
+                }
+            }
         }
-        const float scale = FORM == FORWARD ? (float)t.epilogue.drop.scale : t.scale;
+        __syncwarp();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int row = lane / 4 + j * 8;
-            const int64_t m = m0 + row, at = m * t.N + first;
-            const bool inside = m < t.M && left > 0;
-            uint32_t passed = 0;
-            if (inside) {
-                float added[4] = {0.f, 0.f, 0.f, 0.f};
-                if (FORM == FORWARD && t.epilogue.residual != nullptr) load4<T>(t.epilogue.residual + at, added, left, t.out_whole);
-                const float4 v = *reinterpret_cast<const float4 *>(staging + row * PIECE + (q ^ (row >> 1 & 3)) * 4);
-                float y[4] = {v.x, v.y, v.z, v.w};
-                if constexpr (Shape<T, FORM>::SPLIT) {
-                    const float largest = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
-                    const float none = (y[0] + y[1]) * 0.f + (y[2] + y[3]) * 0.f;  // (fmaxf passes over what is no number)
-                    if (!(largest <= 3.402823466e38f && none == 0.f) && alive) {
-#pragma unroll 1
-                        for (int k = 0; k < left; ++k) {
-                            const float exact = single_element<T, FORM>(t, m, first + k, i.k0, i.k1);
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                if (c == k) y[c] = exact;
-                        }
-                    }
-                }
-                if (!alive)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) y[k] = __uint_as_float(0x7fffffffu);
-                if constexpr (FORM == FORWARD) {
-                    passed = follow<T>(t.epilogue, y, at, b, added, scale, words) & ((1u << left) - 1u);
-                    store4<T>(static_cast<T *>(t.out) + at, y, left, t.out_whole);
-                } else if (FORM == WEIGHT && t.partial) {
-                    store4<float>(static_cast<float *>(t.out) + i.split * t.M * t.N + at, y, left, t.out_whole);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) y[k] *= scale;
-                    store4<T>(static_cast<T *>(t.out) + at, y, left, t.out_whole);
-                }
-            }
-            if (FORM == FORWARD && t.epilogue.mask != nullptr) {
-                passed <<= 4 * q;
-                passed |= __shfl_xor_sync(0xffffffffu, passed, 1);
-                passed |= __shfl_xor_sync(0xffffffffu, passed, 2);
-                if (q == 0 && m < t.M && n < t.epilogue.mask_pitch * 8)
-                    *reinterpret_cast<uint16_t *>(t.epilogue.mask + m * t.epilogue.mask_pitch + n / 8) = (uint16_t)passed;
-            }
+            const float4 v = *reinterpret_cast<const float4 *>(staging + row * PIECE + (q ^ (row >> 1 & 3)) * 4);
+            y[j][0] = v.x, y[j][1] = v.y, y[j][2] = v.z, y[j][3] = v.w;
         }
         __syncwarp();
+        if constexpr (Shape<T, FORM>::SPLIT) {
+            float none = 0.f;  // zero unless one of them is no finite number
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) none = fmaf(y[j][k], 0.f, none);
+            if (none != 0.f && alive) {
+                uint32_t which = 0;
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!(fabsf(y[e / 4][e % 4]) <= 3.402823466e38f)) which |= 1u << e;
+#pragma unroll 1
+                for (int e = 0; e < 16; ++e) {
+                    const int j = e / 4, k = e % 4;
+                    if (8 * j >= rows || k >= left || !(which >> e & 1)) continue;
+                    const float exact = single_element<T, FORM>(t, m0 + lane / 4 + 8 * j, n0 + q * 4 + c + k, i.k0, i.k1);
+#pragma unroll
+                    for (int f = 0; f < 16; ++f)
+                        if (f == e) y[f / 4][f % 4] = exact;
+                }
+            }
+        }
+        if (!alive) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e / 4][e % 4] = __uint_as_float(0x7fffffffu);
+        }
+        if constexpr (FORM == FORWARD) {
+            uint32_t passed = 0xffff;  // a bit for each, four a row
+            if (has_bias) {
+                const float4 v = *reinterpret_cast<const float4 *>(bias + c + q * 4);
+                const float b[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < 16; ++e) y[e / 4][e % 4] += b[e % 4];
+            }
+            if (relu) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (y[e / 4][e % 4] <= 0.f) {  // (a NaN stays one)
+                        y[e / 4][e % 4] = 0.f;
+                        passed &= ~(1u << e);
+                    }
+            }
+            if (threshold) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int64_t at = first + c + j * down;
+                    const int ahead = (int)(at & 3);
+                    const uint4 w4 = words((uint64_t)at >> 2);
+                    uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                    if (ahead) {  // the rows do not begin with a block of words
+                        const uint4 r = words(((uint64_t)at >> 2) + 1);
+                        const uint32_t all[8] = {w[0], w[1], w[2], w[3], r.x, r.y, r.z, r.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) w[k] = ahead == 1 ? all[k + 1] : ahead == 2 ? all[k + 2] : all[k + 3];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const bool kept = w[k] >= threshold;
+                        y[j][k] = kept ? y[j][k] * scale : 0.f;
+                        if (!kept) passed &= ~(1u << (4 * j + k));
+                    }
+                }
+            }
+            if (residual != nullptr) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) y[e / 4][e % 4] += added[e / 4][e % 4];
+            }
+            if (mask != nullptr) {
+                const uint32_t inside = left >= 4 ? 0xfu : left > 0 ? (1u << left) - 1u : 0u;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t bits = (passed >> (4 * j) & inside) << (4 * q);
+                    bits |= __shfl_xor_sync(0xffffffffu, bits, 1);
+                    bits |= __shfl_xor_sync(0xffffffffu, bits, 2);
+                    if (q == 0 && 8 * j < rows)
+                        *reinterpret_cast<uint16_t *>(mask + c / 8 + 8 * j * t.epilogue.mask_pitch) = (uint16_t)bits;
+                }
+            }
+        } else if (!partial) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e / 4][e % 4] *= scale;
+        }
+        if (FORM == WEIGHT && partial) write(static_cast<float *>(t.out) + i.split * t.M * t.N + first + c, y, left, vector, down);
+        else write(static_cast<T *>(t.out) + first + c, y, left, vector, down);
+    }
+    template <typename O>
+    __device__ __forceinline__ void write(O *out, const float (&y)[4][4], int left, bool vector, int64_t down) {
+        if (vector) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (8 * j < rows) vec_store<O, 4>(out + j * down, narrow_all<O, 4>(y[j]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (8 * j < rows && k < left) out[j * down + k] = narrow<O>(y[j][k]);
+        }
     }
 };
 
-// The units of a producer, DEPTH chunks ahead of the stage that it writes.
-template <typename T, int FORM>
+// The units of a producer, DEPTH chunks ahead of the stage that it writes.  WHOLE: rows lie on vectors of 8 elements and are whole
+// vectors long, so that a unit is there or not.
+template <typename T, int FORM, bool WHOLE>
 struct Producer {
     using S = Shape<T, FORM>;
-    static constexpr int BK = S::BK, ACROSS = BK / 8, DOWN = PRODUCERS / ACROSS;  // FORWARD, INPUT: units of a row, rows of a turn
-    static constexpr int A_ACROSS = BM / 8, A_DOWN = PRODUCERS / A_ACROSS;        // WEIGHT
+    static constexpr int BK = S::BK, UNITS = BK / 8;
+    // Units across a row of A and B, and rows of a turn of all producers.
+    static constexpr int A_ACROSS = FORM == WEIGHT ? BM / 8 : UNITS, A_DOWN = PRODUCERS / A_ACROSS;
     [[maybe_unused]] static constexpr int B_ACROSS = S::BN / 8, B_DOWN = PRODUCERS / B_ACROSS;
     const Tiles<T> &t;
-    int p;
+    const int p;
+    const bool masked;
+    const int64_t a_step, b_step, mask_step;  // elements (bytes of the mask) between the rows of two units
     // where the next chunk is read
     int item, chunk, chunks;
     const T *a, *b;
     const uint8_t *mask;
-    int rows;           // of A from this thread's first on (WEIGHT: of A and B)
-    int b_rows;
+    int rows, b_rows;   // from this thread's first on
     int a_left, b_left; // elements of a row from this thread's first on
 
-    __device__ __forceinline__ Producer(const Tiles<T> &t_, int p_) : t(t_), p(p_), item(blockIdx.x), chunk(0), b(nullptr), mask(nullptr) {
+    __device__ __forceinline__ Producer(const Tiles<T> &t_, int p_)
+        : t(t_), p(p_), masked(FORM != FORWARD && t_.mask != nullptr), a_step(A_DOWN * t_.a_stride), b_step(B_DOWN * t_.b_stride),
+          mask_step(A_DOWN * t_.mask_pitch), item(blockIdx.x), chunk(0), b(nullptr), mask(nullptr) {
         begin();
     }
     __device__ __forceinline__ static int clamped(int64_t n) { return (int)max((int64_t)0, min(n, (int64_t)1 << 30)); }
@@ -509,47 +560,49 @@ struct Producer {
             const int64_t b_row = i.k0 + p / B_ACROSS, b_column = i.n0 + p % B_ACROSS * 8;
             a = t.a + row * t.a_stride + column;
             b = t.b + b_row * t.b_stride + b_column;
-            if (t.mask != nullptr) mask = t.mask + row * t.mask_pitch + column / 8;
+            mask = t.mask + row * t.mask_pitch + column / 8;
             rows = clamped(i.k1 - row);
             b_rows = clamped(i.k1 - b_row);
             a_left = clamped(t.M - column);
             b_left = clamped(t.N - b_column);
         } else {
-            const int64_t row = i.m0 + p / ACROSS, column = p % ACROSS * 8;
+            const int64_t row = i.m0 + p / A_ACROSS, column = p % A_ACROSS * 8;
             a = t.a + row * t.a_stride + column;
-            if (FORM == INPUT && t.mask != nullptr) mask = t.mask + row * t.mask_pitch + column / 8;
+            mask = t.mask + row * t.mask_pitch + column / 8;
             rows = clamped(t.M - row);
             a_left = clamped(t.K - column);
         }
     }
     __device__ __forceinline__ void load(Unit<T> (&x)[S::A_UNITS + S::B_UNITS], uint32_t (&keep)[S::A_UNITS]) {
         if (item >= t.items) return;
-        constexpr int STEP = FORM == WEIGHT ? A_DOWN : DOWN;
 #pragma unroll
         for (int u = 0; u < S::A_UNITS; ++u) {
-            keep[u] = 0xff;
-            if (u * STEP < rows && a_left > 0) {
-                x[u].load(a + u * STEP * t.a_stride, a_left, t.a_whole);
-                if (FORM != FORWARD && t.mask != nullptr) keep[u] = mask[u * STEP * t.mask_pitch];
-            } else {
-                x[u].clear();
-            }
+            const bool there = u * A_DOWN < rows && a_left > 0;
+            if constexpr (WHOLE) x[u].load_whole(a + u * a_step, there);
+            else x[u].load(a + u * a_step, there ? a_left : 0);
         }
+        if constexpr (FORM != FORWARD)
+            if (masked)
+#pragma unroll
+                for (int u = 0; u < S::A_UNITS; ++u)
+                    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %2, 0;\n mov.b32 %0, 0;\n @p ld.global.u8 %0, [%1];\n}"
+                                 : "=&r"(keep[u])
+                                 : "l"(mask + u * mask_step), "r"((uint32_t)(u * A_DOWN < rows && a_left > 0)));
         if constexpr (FORM == WEIGHT) {
 #pragma unroll
             for (int u = 0; u < S::B_UNITS; ++u) {
-                Unit<T> &y = x[S::A_UNITS + u];
-                if (u * B_DOWN < b_rows && b_left > 0) y.load(b + u * B_DOWN * t.b_stride, b_left, t.b_whole);
-                else y.clear();
+                const bool there = u * B_DOWN < b_rows && b_left > 0;
+                if constexpr (WHOLE) x[S::A_UNITS + u].load_whole(b + u * b_step, there);
+                else x[S::A_UNITS + u].load(b + u * b_step, there ? b_left : 0);
             }
         }
         if (++chunk == chunks) {
             item += gridDim.x;
             begin();
         } else if constexpr (FORM == WEIGHT) {
-            a += BK * t.a_stride;
-            b += BK * t.b_stride;
-            mask += BK * t.mask_pitch;
+            a += (BK / A_DOWN) * a_step;
+            b += (BK / B_DOWN) * b_step;
+            mask += (BK / A_DOWN) * mask_step;
             rows -= BK;
             b_rows -= BK;
         } else {
@@ -560,36 +613,41 @@ struct Producer {
     }
     __device__ __forceinline__ void store(Unit<T> (&x)[S::A_UNITS + S::B_UNITS], uint32_t (&keep)[S::A_UNITS], uint32_t stage,
                                           float (&columns)[8]) {
-        float sum[8];
+        if constexpr (FORM != FORWARD)
+            if (masked)
+#pragma unroll
+                for (int u = 0; u < S::A_UNITS; ++u) x[u].keep(keep[u]);
+        if constexpr (FORM == WEIGHT)
+            if (t.column_sums != nullptr) {
+                float sum[8];
+#pragma unroll
+                for (int u = 0; u < S::A_UNITS; ++u)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) sum[k] = u == 0 ? x[u].value(k) : sum[k] + x[u].value(k);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) columns[k] += sum[k];
+            }
 #pragma unroll
         for (int u = 0; u < S::A_UNITS; ++u) {
-            if (FORM != FORWARD && t.mask != nullptr) x[u].keep(keep[u]);
-            if constexpr (FORM == WEIGHT)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) sum[k] = u == 0 ? x[u].value(k) : sum[k] + x[u].value(k);
             uint4 planes[S::PLANES];
             x[u].planes(planes);
             const uint32_t at = FORM == WEIGHT ? p % A_ACROSS / 8 * (BK * 128) + place<128>(p / A_ACROSS + u * A_DOWN, p % 8)
-                                               : place<BK * 2>(p / ACROSS + u * DOWN, p % ACROSS);
+                                               : place<BK * 2>(p / A_ACROSS + u * A_DOWN, p % A_ACROSS);
 #pragma unroll
             for (int q = 0; q < S::PLANES; ++q) store_shared(stage + q * S::A_PLANE + at, planes[q]);
         }
-        if constexpr (FORM == WEIGHT) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) columns[k] += sum[k];
+        for (int u = 0; u < S::B_UNITS; ++u) {
+            uint4 planes[S::PLANES];
+            x[S::A_UNITS + u].planes(planes);
+            const uint32_t at = p % B_ACROSS / 8 * (BK * 128) + place<128>(p / B_ACROSS + u * B_DOWN, p % 8);
 #pragma unroll
-            for (int u = 0; u < S::B_UNITS; ++u) {
-                uint4 planes[S::PLANES];
-                x[S::A_UNITS + u].planes(planes);
-                const uint32_t at = p % B_ACROSS / 8 * (BK * 128) + place<128>(p / B_ACROSS + u * B_DOWN, p % 8);
-#pragma unroll
-                for (int q = 0; q < S::PLANES; ++q) store_shared(stage + S::PLANES * S::A_PLANE + q * S::B_PLANE + at, planes[q]);
-            }
+            for (int q = 0; q < S::PLANES; ++q) store_shared(stage + S::PLANES * S::A_PLANE + q * S::B_PLANE + at, planes[q]);
         }
     }
 };
 
-template <typename T, int FORM>
+template <typename T, int FORM, bool WHOLE>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ Tiles<T> t) {
     using S = Shape<T, FORM>;
     constexpr int BN = S::BN, BK = S::BK, STAGES = S::STAGES, PLANES = S::PLANES;
@@ -634,7 +692,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(EPILOGUE_REGISTERS));
         constexpr int COLUMNS = BN / 2;  // of a warp's half of the tile
         const int quarter = warp & 3, half = warp >> 2;
-        Finish<T, FORM> finish{t, staging + warp * 32 * PIECE, bias_of_tile[half], Philox(FORM == FORWARD ? t.epilogue.drop.key() : 0), lane};
+        Finish<T, FORM> finish(t, staging + warp * 32 * PIECE, bias_of_tile[half], lane);
         uint32_t segment = 0;
         for (int item = blockIdx.x; item < t.items; item += gridDim.x) {
             const Item i = item_of<T, FORM>(t, item);
@@ -652,6 +710,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(t.epilogue.residual + (m0 + lane) * t.N + n));
             }
             const uint32_t rows = tmem + ((uint32_t)(quarter * 32) << 16) + half * COLUMNS;
+            const int pieces_end = m0 < t.M ? (int)min((int64_t)COLUMNS, t.N - n0) : 0;
+            finish.begin(m0, n0);
             bool alive = true;
             const auto await = [&] {
                 const uint32_t buffer = segment & 1;
@@ -674,7 +734,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     float x[PIECE];
                     if (alive) tmem_load16<S::SPLIT>(rows + buffer * 256 + c, x);
                     if (c + PIECE == COLUMNS) release(buffer);
-                    if (n0 + c < t.N && m0 < t.M) finish.piece(x, i, m0, n0 + c, c, alive);
+                    if (c < pieces_end) finish.piece(x, i, m0, n0, c, alive);
                 }
             } else if constexpr (S::SPLIT) {
                 float sum[COLUMNS];  // (a path of its own: the other keeps its registers)
@@ -692,12 +752,14 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                         }
                     release(buffer);
                 }
-#pragma unroll
-                for (int c = 0; c < COLUMNS; c += PIECE) {
+#pragma unroll 1
+                for (int c = 0; c < COLUMNS; c += PIECE) {  // (the sums move up, so that one copy of what follows is enough)
                     float x[PIECE];
 #pragma unroll
-                    for (int k = 0; k < PIECE; ++k) x[k] = sum[c + k];
-                    if (n0 + c < t.N && m0 < t.M) finish.piece(x, i, m0, n0 + c, c, alive);
+                    for (int k = 0; k < PIECE; ++k) x[k] = sum[k];
+#pragma unroll
+                    for (int k = 0; k < COLUMNS - PIECE; ++k) sum[k] = sum[k + PIECE];
+                    if (c < pieces_end) finish.piece(x, i, m0, n0, c, alive);
                 }
             }
         }
@@ -710,17 +772,16 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         float columns[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) columns[k] = 0.f;
-        Producer<T, FORM> ahead(t, p);
+        Producer<T, FORM, WHOLE> ahead(t, p);
 #pragma unroll
         for (int d = 0; d < S::DEPTH; ++d) ahead.load(x[d], keep[d]);
-        uint32_t round = 0;
+        uint32_t s = 0, parity = 1;
         bool alive = true;
-        int item = blockIdx.x, chunk = 0;
+        int item = blockIdx.x, chunk = 0, chunks = chunks_of<T, FORM>(t, item);
         while (item < t.items) {  // (to the end whatever happens: the barriers below want every thread)
 #pragma unroll
             for (int d = 0; d < S::DEPTH; ++d) {
                 if (item >= t.items) continue;
-                const uint32_t s = round % STAGES, parity = (round / STAGES & 1) ^ 1;
                 if (alive) alive = __all_sync(0xffffffffu, barrier_wait(&empty[s], parity, polls, &given_up));
                 if (alive) {
                     ahead.store(x[d], keep[d], shared_address(stages) + s * S::STAGE, columns);
@@ -729,8 +790,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     if (lane == 0) barrier_arrive(&a_full[s]);
                     ahead.load(x[d], keep[d]);
                 }
-                ++round;
-                if (++chunk < chunks_of<T, FORM>(t, item)) continue;
+                if (++s == STAGES) s = 0, parity ^= 1;
+                if (++chunk < chunks) continue;
                 if (FORM == WEIGHT && t.column_sums != nullptr) {
                     const Item i = item_of<T, FORM>(t, item);
                     if (i.n0 == 0) {
@@ -751,59 +812,74 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 }
                 chunk = 0;
                 item += gridDim.x;
+                if (FORM == WEIGHT && item < t.items) chunks = chunks_of<T, FORM>(t, item);
             }
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGISTERS));
-        if (warp == MMA_WARP && lane == 0) {
+        if (warp == MMA_WARP) {
             // -------------------------------------------------------------- products
+            // (the whole warp walks, so that what an instruction takes lies in the registers that a warp shares; one lane issues)
             constexpr bool ALONG_MN = FORM == WEIGHT;
             constexpr uint32_t base = product_descriptor(sizeof(T) == 4 || __is_same(T, __nv_bfloat16), ALONG_MN);
-            constexpr int ROW = ALONG_MN ? 128 : BK * 2;
-            constexpr uint32_t LEADING = ALONG_MN ? BK * 128 : 16, STEP = ALONG_MN ? 16 * 128 : 32;  // STEP: 16 along k
-            uint32_t round = 0, segment = 0;
+            constexpr uint32_t UPPER = MATRIX_UPPER<ALONG_MN ? 128 : BK * 2>;
+            constexpr uint32_t LEADING = ALONG_MN ? BK * 128 : 16, STEP = (ALONG_MN ? 16 * 128 : 32) >> 4;  // STEP: 16 along k
+            constexpr uint32_t AP = S::A_PLANE >> 4, BP = S::B_PLANE >> 4;
+            const uint32_t a_first = matrix_descriptor(shared_address(stages), LEADING);
+            const uint32_t b_first = matrix_descriptor(shared_address(stages) + PLANES * S::A_PLANE, LEADING);
+            const bool leads = leader_of_warp();
+            uint32_t s = 0, parity = 0, buffer = 0, buffer_parity = 1, issued = 0;
             bool alive = true;
+            int chunks = chunks_of<T, FORM>(t, blockIdx.x);
             for (int item = blockIdx.x; alive && item < t.items; item += gridDim.x) {
                 const int64_t n0 = item_of<T, FORM>(t, item).n0;
-                const int chunks = chunks_of<T, FORM>(t, item);
+                if (FORM == WEIGHT) chunks = chunks_of<T, FORM>(t, item);
                 const int columns = (int)min((int64_t)BN, (t.N - n0 + 15) / 16 * 16);
                 const uint32_t descriptor = base | (uint32_t)(columns / 8) << 17;
-                for (int chunk = 0; alive && chunk < chunks; ++chunk, ++round) {
-                    const uint32_t buffer = segment & 1, accumulator = tmem + buffer * 256;
-                    const bool fresh = chunk % S::SEGMENT == 0;
-                    if (fresh) alive = barrier_wait(&sums_empty[buffer], (segment >> 1 & 1) ^ 1, polls, &given_up);
-                    const uint32_t s = round % STAGES, parity = round / STAGES & 1;
-                    alive = alive && barrier_wait(&a_full[s], parity, polls, &given_up);
-                    if (FORM != WEIGHT) alive = alive && barrier_wait(&b_full[s], parity, polls, &given_up);
+                int of_segment = 0;
+                for (int chunk = 0; alive && chunk < chunks; ++chunk) {
+                    const uint32_t accumulator = tmem + buffer * 256, small = accumulator + 128;
+                    const bool fresh = of_segment == 0, last = ++of_segment == S::SEGMENT || chunk + 1 == chunks;
+                    bool good = !fresh || barrier_wait(&sums_empty[buffer], buffer_parity, polls, &given_up);
+                    good = good && barrier_wait(&a_full[s], parity, polls, &given_up);
+                    if (FORM != WEIGHT) good = good && barrier_wait(&b_full[s], parity, polls, &given_up);
+                    alive = __all_sync(0xffffffffu, good);
                     if (!alive) break;
                     fence_after();
-                    const uint32_t stage = shared_address(stages) + s * S::STAGE;
-                    const uint64_t a = matrix_descriptor<ROW>(stage, LEADING), b = matrix_descriptor<ROW>(stage + PLANES * S::A_PLANE, LEADING);
-                    constexpr uint64_t AP = S::A_PLANE >> 4, BP = S::B_PLANE >> 4;
+                    const uint32_t a = a_first + s * (S::STAGE >> 4), b = b_first + s * (S::STAGE >> 4);
+                    if (leads) {
 #pragma unroll
-                    for (int k = 0; k < BK / 16; ++k) {
-                        const uint64_t step = (uint64_t)(k * STEP >> 4), ak = a + step, bk = b + step;
-                        const bool add = !fresh || k > 0;
-                        multiply(accumulator, ak, bk, descriptor, add);
-                        if constexpr (S::SPLIT) {
-                            const uint32_t small = accumulator + 128;
-                            multiply(small, ak, bk + BP, descriptor, add);
-                            multiply(small, ak + AP, bk, descriptor, true);
-                            multiply(small, ak, bk + 2 * BP, descriptor, true);
-                            multiply(small, ak + 2 * AP, bk, descriptor, true);
-                            multiply(small, ak + AP, bk + BP, descriptor, true);
+                        for (int k = 0; k < BK / 16; ++k) {
+                            const uint32_t ak = a + k * STEP, bk = b + k * STEP;
+                            const bool add = !fresh || k > 0;
+                            multiply<UPPER>(accumulator, ak, bk, descriptor, add);
+                            if constexpr (S::SPLIT) {
+                                multiply<UPPER>(small, ak, bk + BP, descriptor, add);
+                                multiply<UPPER>(small, ak + AP, bk, descriptor, true);
+                                multiply<UPPER>(small, ak, bk + 2 * BP, descriptor, true);
+                                multiply<UPPER>(small, ak + 2 * AP, bk, descriptor, true);
+                                multiply<UPPER>(small, ak + AP, bk + BP, descriptor, true);
+                            }
                         }
+                        commit(&empty[s]);
+                        if (last) commit(&sums_full[buffer]);
                     }
-                    commit(&empty[s]);
-                    if (chunk + 1 == chunks || (chunk + 1) % S::SEGMENT == 0) {
-                        commit(&sums_full[buffer]);
-                        ++segment;
+                    __syncwarp();
+                    if (last) {
+                        of_segment = 0;
+                        buffer ^= 1;
+                        if (buffer == 0) buffer_parity ^= 1;
                     }
+                    if (++s == STAGES) s = 0, parity ^= 1;
+                    if (issued < STAGES) ++issued;
                 }
             }
-            for (uint32_t r = round > STAGES ? round - STAGES : 0; alive && r < round; ++r)  // the last reports have come in
-                alive = barrier_wait(&empty[r % STAGES], r / STAGES & 1, polls, &given_up);
-            if (!alive) {  // products that are still under way read shared memory and write the accumulators
+            for (; alive && issued > 0; --issued) {  // the last reports have come in
+                if (s == 0) s = STAGES, parity ^= 1;
+                --s;
+                alive = __all_sync(0xffffffffu, barrier_wait(&empty[s], parity, polls, &given_up));
+            }
+            if (!alive && leads) {  // products that are still under way read shared memory and write the accumulators
                 commit(&drained);
                 for (int k = 0; k < WAIT_LIMIT && !barrier_poll(&drained, 0); ++k) {}
             }
@@ -851,18 +927,25 @@ size_t packed_bytes(int64_t N, int64_t K) {
     return (size_t)ceil_div(N, S::BN) * (size_t)ceil_div(K, S::BK) * S::PLANES * S::B_PLANE;
 }
 
+template <typename T, int FORM, bool WHOLE>
+int launch_as(const Tiles<T> &t, cudaStream_t stream) {
+    using S = Shape<T, FORM>;
+    CGNN_CUDA(cudaFuncSetAttribute(tile_kernel<T, FORM, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SHARED));
+    tile_kernel<T, FORM, WHOLE><<<(unsigned)std::min(t.items, SMS), THREADS, S::SHARED, stream>>>(t);
+    CGNN_LAUNCH_CHECK();
+    return CGNN_OK;
+}
+
 template <typename T, int FORM>
 int launch(Tiles<T> &t, int64_t splits, cudaStream_t stream) {
-    using S = Shape<T, FORM>;
-    const int64_t tiles_m = ceil_div(t.M, BM), tiles_n = ceil_div(t.N, S::BN);
+    const int64_t tiles_m = ceil_div(t.M, BM), tiles_n = ceil_div(t.N, Shape<T, FORM>::BN);
     CGNN_REQUIRE(tiles_m * tiles_n * splits < (1ll << 30), "linear: too many tiles");
     t.tiles_m = (int)tiles_m;
     t.tiles_n = (int)tiles_n;
     t.items = (int)(tiles_m * tiles_n * splits);
-    CGNN_CUDA(cudaFuncSetAttribute(tile_kernel<T, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SHARED));
-    tile_kernel<T, FORM><<<(unsigned)std::min(t.items, SMS), THREADS, S::SHARED, stream>>>(t);
-    CGNN_LAUNCH_CHECK();
-    return CGNN_OK;
+    bool whole = whole_rows(t.a, t.a_stride, sizeof(T)) && (FORM == WEIGHT ? t.M : t.K) % 8 == 0;
+    if (FORM == WEIGHT) whole = whole && whole_rows(t.b, t.b_stride, sizeof(T)) && t.N % 8 == 0;
+    return whole ? launch_as<T, FORM, true>(t, stream) : launch_as<T, FORM, false>(t, stream);
 }
 
 template <typename T, int FORM>
@@ -891,7 +974,6 @@ int tiles_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T
     Tiles<T> t{};
     t.a = static_cast<const T *>(c.x);
     t.a_stride = c.stride;
-    t.a_whole = whole_rows(c.x, c.stride, sizeof(T));
     t.b = weight;
     t.b_stride = c.in;
     t.packed = packed;
@@ -930,7 +1012,6 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
     Tiles<T> t{};
     t.a = grad;
     t.a_stride = c.out;
-    t.a_whole = whole_rows(grad, c.out, sizeof(T));
     t.mask = mask;
     t.mask_pitch = mask_pitch(c.out);
     t.scale = (float)scale;
@@ -957,7 +1038,6 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
     float *const sums = parts + splits * c.out * c.in;
     t.b = static_cast<const T *>(c.x);
     t.b_stride = c.stride;
-    t.b_whole = whole_rows(c.x, c.stride, sizeof(T));
     t.packed = nullptr;
     t.M = c.out;
     t.N = c.in;
