@@ -47,7 +47,7 @@ struct Shape {
     static constexpr int A_UNITS = BM * BK / 8 / PRODUCERS, B_UNITS = FORM == WEIGHT ? BN * BK / 8 / PRODUCERS : 0;
     // Chunks on their way to a producer's registers: 64 KB a multiprocessor in fp32 (HBM wants 35), 48 in 16 bits.
     static constexpr int DEPTH = SPLIT ? (FORM == WEIGHT ? 2 : 4) : 3;
-    static constexpr int STAGING = EPILOGUE_WARPS * 32 * PIECE * 4;
+    static constexpr int STAGING = EPILOGUE_WARPS * 32 * (PIECE + 1) * 4;
     static constexpr int SUMS = FORM == WEIGHT ? 16 * BM * 4 : 0;  // of the columns
     static constexpr int SHARED = STAGES * STAGE + STAGING + SUMS + 1024;
 };
@@ -62,7 +62,7 @@ struct Tiles {
     int64_t M, N, K;
     int64_t k_per_item;
     int tiles_m, tiles_n, items;
-    int out_whole;                // rows of the output and the residual lie on vectors of 4
+    int out_whole, out_wide;      // rows of the output and the residual lie on vectors of 8 elements, of 32 bytes
     void *out;                    // [M, N] of T, or (WEIGHT of several splits) [splits, M, N] of fp32
     int partial;
     float *column_sums;           // WEIGHT: [splits, M]
@@ -232,10 +232,9 @@ struct Unit<float> {
                 const __nv_bfloat162 two = __floats2bfloat162_rn(rest.x, rest.y);
                 const uint32_t bits = *reinterpret_cast<const uint32_t *>(&two);
                 part[q][k / 2] = bits;
-                if (q < 2) {
-                    rest.x -= __uint_as_float(bits << 16);
-                    rest.y -= __uint_as_float(bits & 0xffff0000u);
-                }
+                if (q < 2)  // (exact: what is left has the lower bits only)
+                    rest = __ffma2_rn(make_float2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xffff0000u)), make_float2(-1.f, -1.f),
+                                      rest);
             }
         }
     }
@@ -359,167 +358,201 @@ __device__ __noinline__ float single_element(const Tiles<T> &t, int64_t m, int64
     return sum;
 }
 
-// The epilogue of one warp: 32 rows (a row a lane in the accumulators) by PIECE columns at a time through shared memory, from
-// where four lanes take the columns of a row, eight rows at once, so that whole sectors are read and written.  A lane
-// has four rows, eight apart, and four columns of them.
+// Sixteen neighbouring elements of a row, on a boundary of 32 bytes (fp32, wide) or 16.
+__device__ __forceinline__ void load16(const float *p, int left, bool, float (&y)[16]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.u32 p, %9, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n"
+            " mov.b32 %4, 0;\n mov.b32 %5, 0;\n mov.b32 %6, 0;\n mov.b32 %7, 0;\n"
+            " @p ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n}"
+            : "=&f"(y[8 * h]), "=&f"(y[8 * h + 1]), "=&f"(y[8 * h + 2]), "=&f"(y[8 * h + 3]), "=&f"(y[8 * h + 4]), "=&f"(y[8 * h + 5]),
+              "=&f"(y[8 * h + 6]), "=&f"(y[8 * h + 7])
+            : "l"(p + 8 * h), "r"((uint32_t)(left > 8 * h)));
+}
+template <typename T>
+__device__ __forceinline__ void load16(const T *p, int left, bool, float (&y)[16]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        Vec<T, 8> v = vec_zero<T, 8>();
+        if (left > 8 * h) v = vec_load<T, 8>(p + 8 * h);
+        float part[8];
+        widen_all<T, 8>(v, part);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[8 * h + k] = part[k];
+    }
+}
+__device__ __forceinline__ void store16(float *p, int left, bool, const float (&y)[16]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (left > 8 * h)
+            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p + 8 * h), "f"(y[8 * h]), "f"(y[8 * h + 1]),
+                         "f"(y[8 * h + 2]), "f"(y[8 * h + 3]), "f"(y[8 * h + 4]), "f"(y[8 * h + 5]), "f"(y[8 * h + 6]), "f"(y[8 * h + 7])
+                         : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void store16(T *p, int left, bool wide, const float (&y)[16]) {
+    const Vec<T, 16> v = narrow_all<T, 16>(y);
+    const uint32_t *const w = reinterpret_cast<const uint32_t *>(&v);
+    if (wide) {  // a whole sector at once
+        if (left > 0)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                         "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (left > 8 * h) *reinterpret_cast<uint4 *>(p + 8 * h) = make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
+    }
+}
+
+// The epilogue of one warp: 32 rows, a row a lane as they lie in the accumulators, PIECE columns at a time.  Rows of whole vectors are
+// read and written by their lane, a sector or two at once; of others the results go through shared memory, from where
+// neighbouring lanes take neighbouring columns.
 template <typename T, int FORM>
 struct Finish {
     const Tiles<T> &t;
-    float *const staging;  // [32][PIECE], units of four swizzled
+    float *const staging;  // [32][PIECE + 1]
     const float *const bias;
     const int lane;
-    const bool has_bias, relu, vectors, partial;
-    const uint32_t threshold;
-    const float scale;
     Philox words;
     // of the present item
-    int64_t first;         // the element of the output that the lane's first row and column is
-    int rows, columns;     // from there on
-    const T *residual;
-    uint8_t *mask;
+    int64_t m, n0, first;  // the lane's row, the first column, and the output's element that they are
+    int columns;           // from there on, none for a row that is not there
+    uint64_t passed;       // a bit for each column, 64 a turn
 
     __device__ __forceinline__ Finish(const Tiles<T> &t_, float *staging_, const float *bias_, int lane_)
-        : t(t_), staging(staging_), bias(bias_), lane(lane_), has_bias(FORM == FORWARD && t_.epilogue.bias != nullptr),
-          relu(FORM == FORWARD && t_.epilogue.relu), vectors(t_.out_whole), partial(FORM == WEIGHT && t_.partial),
-          threshold(FORM == FORWARD ? t_.epilogue.drop.threshold : 0), scale(FORM == FORWARD ? (float)t_.epilogue.drop.scale : t_.scale),
-          words(FORM == FORWARD && threshold ? t_.epilogue.drop.key() : 0) {}
+        : t(t_), staging(staging_), bias(bias_), lane(lane_),
+          words(FORM == FORWARD && t_.epilogue.drop.threshold ? t_.epilogue.drop.key() : 0) {}
 
-    __device__ __forceinline__ void begin(int64_t m0, int64_t n0) {
-        const int64_t m = m0 + lane / 4, n = n0 + lane % 4 * 4;
-        first = m * t.N + n;
-        rows = (int)max((int64_t)0, min(t.M - m, (int64_t)32));
-        columns = (int)max((int64_t)-PIECE, min(t.N - n, (int64_t)1024));
-        residual = FORM == FORWARD && t.epilogue.residual != nullptr ? t.epilogue.residual + first : nullptr;
-        mask = FORM == FORWARD && t.epilogue.mask != nullptr ? t.epilogue.mask + m * t.epilogue.mask_pitch + n0 / 8 : nullptr;
+    __device__ __forceinline__ void begin(int64_t m0, int64_t n0_) {
+        m = m0 + lane;
+        n0 = n0_;
+        first = m * t.N + n0;
+        columns = m < t.M ? (int)max((int64_t)0, min(t.N - n0, (int64_t)1024)) : 0;
+        passed = 0;
     }
 
-    // Columns c .. c + PIECE of the item; x: the lane's row of the accumulators.
-    __device__ __forceinline__ void piece(float (&x)[PIECE], const Item &i, int64_t m0, int64_t n0, int c, bool alive) {
+    // What the rest of the forward pass adds, on its way while the accumulators are read.
+    __device__ __forceinline__ void fetch(int c, float (&added)[PIECE]) {
+        if (FORM == FORWARD && t.epilogue.residual != nullptr) {
+            const T *const r = t.epilogue.residual + first + c;
+            const int left = columns - c;
+            if (t.out_whole) {
+                load16(r, left, t.out_wide, added);
+            } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<float4 *>(staging + lane * PIECE + (k ^ (lane >> 1 & 3)) * 4) =
-                make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
-        const int q = lane & 3, left = columns - c;
-        const bool vector = vectors && left >= 4;
-        const int64_t down = 8 * t.N;
-        float y[4][4], added[4][4];
-        if (FORM == FORWARD && residual != nullptr) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const T *const r = residual + c + j * down;
-                if (vector && 8 * j < rows) {
-                    widen_all<T, 4>(vec_load<T, 4>(r), added[j]);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) added[j][k] = 8 * j < rows && k < left ? widen(r[k]) : 0.f;
-                }
+                for (int k = 0; k < PIECE; ++k) added[k] = k < left ? widen(r[k]) : 0.f;
             }
         }
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int row = lane / 4 + j * 8;
-            const float4 v = *reinterpret_cast<const float4 *>(staging + row * PIECE + (q ^ (row >> 1 & 3)) * 4);
-            y[j][0] = v.x, y[j][1] = v.y, y[j][2] = v.z, y[j][3] = v.w;
-        }
-        __syncwarp();
+    }
+
+    // Columns c .. c + PIECE of the item.
+    __device__ __forceinline__ void piece(float (&y)[PIECE], const float (&added)[PIECE], const Item &i, int c, bool alive) {
+        const int left = columns - c;
         if constexpr (Shape<T, FORM>::SPLIT) {
             float none = 0.f;  // zero unless one of them is no finite number
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) none = fmaf(y[j][k], 0.f, none);
+            for (int k = 0; k < PIECE; ++k) none = fmaf(y[k], 0.f, none);
             if (none != 0.f && alive) {
                 uint32_t which = 0;
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (!(fabsf(y[e / 4][e % 4]) <= 3.402823466e38f)) which |= 1u << e;
+                for (int k = 0; k < PIECE; ++k)
+                    if (!(fabsf(y[k]) <= 3.402823466e38f)) which |= 1u << k;
 #pragma unroll 1
-                for (int e = 0; e < 16; ++e) {
-                    const int j = e / 4, k = e % 4;
-                    if (8 * j >= rows || k >= left || !(which >> e & 1)) continue;
-                    const float exact = single_element<T, FORM>(t, m0 + lane / 4 + 8 * j, n0 + q * 4 + c + k, i.k0, i.k1);
+                for (int k = 0; k < PIECE && k < left; ++k) {
+                    if (!(which >> k & 1)) continue;
+                    const float exact = single_element<T, FORM>(t, m, n0 + c + k, i.k0, i.k1);
 #pragma unroll
-                    for (int f = 0; f < 16; ++f)
-                        if (f == e) y[f / 4][f % 4] = exact;
+                    for (int f = 0; f < PIECE; ++f)
+                        if (f == k) y[f] = exact;
                 }
             }
         }
         if (!alive) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) y[e / 4][e % 4] = __uint_as_float(0x7fffffffu);
+            for (int k = 0; k < PIECE; ++k) y[k] = __uint_as_float(0x7fffffffu);
         }
         if constexpr (FORM == FORWARD) {
-            uint32_t passed = 0xffff;  // a bit for each, four a row
-            if (has_bias) {
-                const float4 v = *reinterpret_cast<const float4 *>(bias + c + q * 4);
-                const float b[4] = {v.x, v.y, v.z, v.w};
+            uint32_t through = 0xffff;
+            if (t.epilogue.bias != nullptr) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) y[e / 4][e % 4] += b[e % 4];
+                for (int k = 0; k < PIECE; k += 4) {
+                    const float4 b = *reinterpret_cast<const float4 *>(bias + c + k);
+                    y[k] += b.x, y[k + 1] += b.y, y[k + 2] += b.z, y[k + 3] += b.w;
+                }
             }
-            if (relu) {
+            if (t.epilogue.relu) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (y[e / 4][e % 4] <= 0.f) {  // (a NaN stays one)
-                        y[e / 4][e % 4] = 0.f;
-                        passed &= ~(1u << e);
+                for (int k = 0; k < PIECE; ++k)
+                    if (y[k] <= 0.f) {  // (a NaN stays one)
+                        y[k] = 0.f;
+                        through &= ~(1u << k);
                     }
             }
+            const uint32_t threshold = t.epilogue.drop.threshold;
             if (threshold) {
+                const float scale = (float)t.epilogue.drop.scale;
+                const uint64_t block = (uint64_t)(first + c) >> 2;
+                const int ahead = (int)((first + c) & 3);  // not zero: the rows do not begin with a block of words
+                uint4 q = words(block);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int64_t at = first + c + j * down;
-                    const int ahead = (int)(at & 3);
-                    const uint4 w4 = words((uint64_t)at >> 2);
-                    uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-                    if (ahead) {  // the rows do not begin with a block of words
-                        const uint4 r = words(((uint64_t)at >> 2) + 1);
+                for (int b = 0; b < PIECE / 4; ++b) {
+                    uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                    if (ahead || b + 1 < PIECE / 4) {
+                        const uint4 r = words(block + b + 1);
                         const uint32_t all[8] = {w[0], w[1], w[2], w[3], r.x, r.y, r.z, r.w};
+                        if (ahead)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) w[k] = ahead == 1 ? all[k + 1] : ahead == 2 ? all[k + 2] : all[k + 3];
+                            for (int k = 0; k < 4; ++k) w[k] = ahead == 1 ? all[k + 1] : ahead == 2 ? all[k + 2] : all[k + 3];
+                        q = r;
                     }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const bool kept = w[k] >= threshold;
-                        y[j][k] = kept ? y[j][k] * scale : 0.f;
-                        if (!kept) passed &= ~(1u << (4 * j + k));
+                        y[4 * b + k] = kept ? y[4 * b + k] * scale : 0.f;
+                        if (!kept) through &= ~(1u << (4 * b + k));
                     }
                 }
             }
-            if (residual != nullptr) {
+            if (t.epilogue.residual != nullptr) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) y[e / 4][e % 4] += added[e / 4][e % 4];
+                for (int k = 0; k < PIECE; ++k) y[k] += added[k];
             }
-            if (mask != nullptr) {
-                const uint32_t inside = left >= 4 ? 0xfu : left > 0 ? (1u << left) - 1u : 0u;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t bits = (passed >> (4 * j) & inside) << (4 * q);
-                    bits |= __shfl_xor_sync(0xffffffffu, bits, 1);
-                    bits |= __shfl_xor_sync(0xffffffffu, bits, 2);
-                    if (q == 0 && 8 * j < rows)
-                        *reinterpret_cast<uint16_t *>(mask + c / 8 + 8 * j * t.epilogue.mask_pitch) = (uint16_t)bits;
+            if (t.epilogue.mask != nullptr) {
+                if (left < PIECE) through &= left > 0 ? (1u << left) - 1u : 0u;
+                passed |= (uint64_t)through << (c % 64);
+                if (c % 64 + PIECE == 64 || c + PIECE >= columns) {  // (words of 64 columns, the last one whatever is left)
+                    if (left > 0)
+                        *reinterpret_cast<uint64_t *>(t.epilogue.mask + m * t.epilogue.mask_pitch + (n0 + c / 64 * 64) / 8) = passed;
+                    passed = 0;
                 }
             }
-        } else if (!partial) {
+        } else if (!(FORM == WEIGHT && t.partial)) {
+            const float scale = t.scale;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) y[e / 4][e % 4] *= scale;
+            for (int k = 0; k < PIECE; ++k) y[k] *= scale;
         }
-        if (FORM == WEIGHT && partial) write(static_cast<float *>(t.out) + i.split * t.M * t.N + first + c, y, left, vector, down);
-        else write(static_cast<T *>(t.out) + first + c, y, left, vector, down);
+        if (FORM == WEIGHT && t.partial) write(static_cast<float *>(t.out) + i.split * t.M * t.N, c, left, y);
+        else write(static_cast<T *>(t.out), c, left, y);
     }
     template <typename O>
-    __device__ __forceinline__ void write(O *out, const float (&y)[4][4], int left, bool vector, int64_t down) {
-        if (vector) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (8 * j < rows) vec_store<O, 4>(out + j * down, narrow_all<O, 4>(y[j]));
+    __device__ __forceinline__ void write(O *out, int c, int left, const float (&y)[PIECE]) {
+        if (t.out_whole) {
+            store16(out + first + c, left, t.out_wide, y);
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (8 * j < rows && k < left) out[j * down + k] = narrow<O>(y[j][k]);
+            for (int k = 0; k < PIECE; ++k) staging[lane * (PIECE + 1) + k] = y[k];
+            __syncwarp();
+            const int k = lane % PIECE;
+            const int64_t m0 = m - lane, n = n0 + c + k;
+            O *to = out + (m0 + lane / PIECE) * t.N + n;
+            const int rows = (int)min(t.M - m0 - lane / PIECE, (int64_t)32);
+            if (n < t.N)
+#pragma unroll 4
+                for (int j = 0; j < PIECE; ++j, to += 2 * t.N)
+                    if (2 * j < rows) *to = narrow<O>(staging[(lane / PIECE + 2 * j) * (PIECE + 1) + k]);
+            __syncwarp();
         }
     }
 };
@@ -647,7 +680,8 @@ struct Producer {
     }
 };
 
-template <typename T, int FORM, bool WHOLE>
+// MANY: fp32 contractions of more than one segment, whose sums take registers that the others keep.
+template <typename T, int FORM, bool WHOLE, bool MANY>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ Tiles<T> t) {
     using S = Shape<T, FORM>;
     constexpr int BN = S::BN, BK = S::BK, STAGES = S::STAGES, PLANES = S::PLANES;
@@ -692,7 +726,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(EPILOGUE_REGISTERS));
         constexpr int COLUMNS = BN / 2;  // of a warp's half of the tile
         const int quarter = warp & 3, half = warp >> 2;
-        Finish<T, FORM> finish(t, staging + warp * 32 * PIECE, bias_of_tile[half], lane);
+        Finish<T, FORM> finish(t, staging + warp * 32 * (PIECE + 1), bias_of_tile[half], lane);
         uint32_t segment = 0;
         for (int item = blockIdx.x; item < t.items; item += gridDim.x) {
             const Item i = item_of<T, FORM>(t, item);
@@ -710,7 +744,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(t.epilogue.residual + (m0 + lane) * t.N + n));
             }
             const uint32_t rows = tmem + ((uint32_t)(quarter * 32) << 16) + half * COLUMNS;
-            const int pieces_end = m0 < t.M ? (int)min((int64_t)COLUMNS, t.N - n0) : 0;
+            const int pieces_end = m0 < t.M ? (int)min((int64_t)COLUMNS, t.N - n0) : 0;  // (the same for the warp)
             finish.begin(m0, n0);
             bool alive = true;
             const auto await = [&] {
@@ -726,18 +760,19 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 ++segment;
             };
             int before = 0;  // segments ahead of the last
-            if constexpr (S::SPLIT) before = (chunks_of<T, FORM>(t, item) - 1) / S::SEGMENT;
+            if constexpr (MANY) before = (chunks_of<T, FORM>(t, item) - 1) / S::SEGMENT;
             if (before == 0) {
                 const uint32_t buffer = await();
 #pragma unroll 1
                 for (int c = 0; c < COLUMNS; c += PIECE) {
-                    float x[PIECE];
+                    float x[PIECE], added[PIECE];
+                    if (c < pieces_end) finish.fetch(c, added);
                     if (alive) tmem_load16<S::SPLIT>(rows + buffer * 256 + c, x);
                     if (c + PIECE == COLUMNS) release(buffer);
-                    if (c < pieces_end) finish.piece(x, i, m0, n0, c, alive);
+                    if (c < pieces_end) finish.piece(x, added, i, c, alive);
                 }
-            } else if constexpr (S::SPLIT) {
-                float sum[COLUMNS];  // (a path of its own: the other keeps its registers)
+            } else if constexpr (MANY) {
+                float sum[COLUMNS];
 #pragma unroll
                 for (int c = 0; c < COLUMNS; ++c) sum[c] = 0.f;
                 for (; before >= 0; --before) {
@@ -754,12 +789,13 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 }
 #pragma unroll 1
                 for (int c = 0; c < COLUMNS; c += PIECE) {  // (the sums move up, so that one copy of what follows is enough)
-                    float x[PIECE];
+                    float x[PIECE], added[PIECE];
+                    if (c < pieces_end) finish.fetch(c, added);
 #pragma unroll
                     for (int k = 0; k < PIECE; ++k) x[k] = sum[k];
 #pragma unroll
                     for (int k = 0; k < COLUMNS - PIECE; ++k) sum[k] = sum[k + PIECE];
-                    if (c < pieces_end) finish.piece(x, i, m0, n0, c, alive);
+                    if (c < pieces_end) finish.piece(x, added, i, c, alive);
                 }
             }
         }
@@ -922,16 +958,23 @@ bool whole_rows(const void *p, int64_t stride, size_t item, int vector = 8) {
 }
 
 template <typename T>
+void set_out(Tiles<T> &t, void *out, int64_t width, size_t item) {
+    t.out = out;
+    t.out_whole = whole_rows(out, width, item);
+    t.out_wide = whole_rows(out, width, item, (int)(32 / item));
+}
+
+template <typename T>
 size_t packed_bytes(int64_t N, int64_t K) {
     using S = Shape<T, FORWARD>;  // (and INPUT)
     return (size_t)ceil_div(N, S::BN) * (size_t)ceil_div(K, S::BK) * S::PLANES * S::B_PLANE;
 }
 
-template <typename T, int FORM, bool WHOLE>
+template <typename T, int FORM, bool WHOLE, bool MANY>
 int launch_as(const Tiles<T> &t, cudaStream_t stream) {
     using S = Shape<T, FORM>;
-    CGNN_CUDA(cudaFuncSetAttribute(tile_kernel<T, FORM, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SHARED));
-    tile_kernel<T, FORM, WHOLE><<<(unsigned)std::min(t.items, SMS), THREADS, S::SHARED, stream>>>(t);
+    CGNN_CUDA(cudaFuncSetAttribute(tile_kernel<T, FORM, WHOLE, MANY>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SHARED));
+    tile_kernel<T, FORM, WHOLE, MANY><<<(unsigned)std::min(t.items, SMS), THREADS, S::SHARED, stream>>>(t);
     CGNN_LAUNCH_CHECK();
     return CGNN_OK;
 }
@@ -945,7 +988,10 @@ int launch(Tiles<T> &t, int64_t splits, cudaStream_t stream) {
     t.items = (int)(tiles_m * tiles_n * splits);
     bool whole = whole_rows(t.a, t.a_stride, sizeof(T)) && (FORM == WEIGHT ? t.M : t.K) % 8 == 0;
     if (FORM == WEIGHT) whole = whole && whole_rows(t.b, t.b_stride, sizeof(T)) && t.N % 8 == 0;
-    return whole ? launch_as<T, FORM, true>(t, stream) : launch_as<T, FORM, false>(t, stream);
+    if constexpr (Shape<T, FORM>::SPLIT)
+        if (t.k_per_item > Shape<T, FORM>::SEGMENT * Shape<T, FORM>::BK)
+            return whole ? launch_as<T, FORM, true, true>(t, stream) : launch_as<T, FORM, false, true>(t, stream);
+    return whole ? launch_as<T, FORM, true, false>(t, stream) : launch_as<T, FORM, false, false>(t, stream);
 }
 
 template <typename T, int FORM>
@@ -980,8 +1026,8 @@ int tiles_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T
     t.M = c.rows;
     t.N = c.out;
     t.K = t.k_per_item = c.in;
-    t.out = y;
-    t.out_whole = whole_rows(y, c.out, sizeof(T), 4) && (epilogue.residual == nullptr || whole_rows(epilogue.residual, c.out, sizeof(T), 4));
+    set_out(t, y, c.out, sizeof(T));
+    if (epilogue.residual != nullptr) t.out_whole = t.out_whole && whole_rows(epilogue.residual, c.out, sizeof(T));
     t.epilogue = epilogue;
     t.polls = polls;
     t.status = status;
@@ -1026,8 +1072,7 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
         t.M = c.rows;
         t.N = c.in;
         t.K = t.k_per_item = c.out;
-        t.out = dx;
-        t.out_whole = whole_rows(dx, c.in, sizeof(T), 4);
+        set_out(t, dx, c.in, sizeof(T));
         rc = launch<T, INPUT>(t, 1, stream);
         if (rc != CGNN_OK) return rc;
     }
@@ -1044,8 +1089,7 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
     t.K = c.rows;
     t.k_per_item = per_split;
     t.partial = splits > 1 || dweight == nullptr;
-    t.out = t.partial ? static_cast<void *>(parts) : dweight;
-    t.out_whole = whole_rows(t.out, c.in, t.partial ? sizeof(float) : sizeof(T), 4);
+    set_out(t, t.partial ? static_cast<void *>(parts) : dweight, c.in, t.partial ? sizeof(float) : sizeof(T));
     t.column_sums = dbias != nullptr ? sums : nullptr;
     int rc = launch<T, WEIGHT>(t, splits, stream);
     if (rc == CGNN_OK && t.partial && dweight != nullptr) rc = join<T>(parts, splits, c.out * c.in, scale, dweight, stream);
