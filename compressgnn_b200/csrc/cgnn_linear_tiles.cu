@@ -12,9 +12,9 @@
 // small ones share another, and after 256 terms both are added to fp32 registers and begin anew.  Six products at
 // the bf16 rate are 275 TFLOP/s of fp32, where the fp32 pipes have 72.
 //
-// The streamed operand goes through registers (loads of 32 bytes a lane, a chunk ahead), because it has to be masked and split; it is
-// written to shared memory in the swizzled layout that the tensor core reads.  The weight is laid out and split once a
-// call by a kernel of its own, as the images of shared memory that bulk copies fetch.
+// Operands lie in shared memory in the swizzled layout that the tensor core reads.  The streamed ones are masked and split on
+// their way there.  The weight is laid out and split once a call by a kernel of its own, as the images of shared memory
+// that bulk copies fetch.
 #include <algorithm>
 
 #include "cgnn_linear.cuh"
@@ -27,13 +27,18 @@ constexpr int EPILOGUE_WARPS = 8, PRODUCER_WARPS = 8;
 constexpr int PRODUCERS = PRODUCER_WARPS * 32;
 constexpr int MMA_WARP = EPILOGUE_WARPS + PRODUCER_WARPS, COPY_WARP = MMA_WARP + 1;
 constexpr int THREADS = (MMA_WARP + 4) * 32;
-// Registers of a thread by warpgroup; a launch brings 96 a thread, and the five groups share that: 2 x 112 + 2 x 112 + 32 = 5 x 96.
-constexpr int EPILOGUE_REGISTERS = 112, PRODUCER_REGISTERS = 112, OTHER_REGISTERS = 32;
+// Registers of a thread by warpgroup; a launch brings 96 a thread, and the five groups share that: 2 x 128 + 2 x 96 + 32 = 5 x 96.
+constexpr int EPILOGUE_REGISTERS = 128, OTHER_REGISTERS = 32;
 constexpr int SMS = 148;
 constexpr int TMEM_COLUMNS = 512;  // two buffers of 256
 constexpr int PIECE = 16;          // columns that a warp of the epilogue takes through shared memory at once
 
 // A stage holds BK of the contraction: rows of BK 16-bit elements (FORWARD, INPUT), or BK rows of panels of 64 (WEIGHT).
+//
+// HBM wants 35 KB on their way to each multiprocessor.  Loads to registers do not get there: a wait for one of them is a wait for
+// the latest (48 and 16 KB ahead took the same time).  Asynchronous copies do; 16-bit operands are copied to where the
+// tensor core reads them, AHEAD stages early, fp32 ones to a ring of AHEAD chunks from which the thread that copied them
+// takes them to be split.
 template <typename T, int FORM>
 struct Shape {
     static constexpr bool SPLIT = sizeof(T) == 4;
@@ -42,14 +47,18 @@ struct Shape {
     static constexpr int BK = SPLIT || FORM == WEIGHT ? 32 : 64;
     static constexpr int A_PLANE = BM * BK * 2, B_PLANE = BN * BK * 2;
     static constexpr int STAGE = PLANES * (A_PLANE + B_PLANE);
-    static constexpr int STAGES = 192 * 1024 / STAGE;
+    static constexpr int STAGES = SPLIT ? (FORM == WEIGHT ? 2 : 3) : FORM == WEIGHT ? 7 : 4;
+    static constexpr int AHEAD = SPLIT || FORM != WEIGHT ? 3 : 5;
     static constexpr int SEGMENT = SPLIT ? 256 / BK : 1 << 30;  // chunks of BK that an accumulator takes
     static constexpr int A_UNITS = BM * BK / 8 / PRODUCERS, B_UNITS = FORM == WEIGHT ? BN * BK / 8 / PRODUCERS : 0;
-    // Chunks on their way to a producer's registers: 64 KB a multiprocessor in fp32 (HBM wants 35), 48 in 16 bits.
-    static constexpr int DEPTH = SPLIT ? (FORM == WEIGHT ? 2 : 4) : 3;
+    static constexpr int SLOT = SPLIT ? (A_UNITS + B_UNITS) * PRODUCERS * 32 : 0;  // of the ring
+    static constexpr int RING = AHEAD * SLOT;
+    static constexpr int MASK_SLOT = FORM == FORWARD ? 0 : A_UNITS * PRODUCERS * 4;  // a word of the mask for each unit
+    static constexpr int MASKS = (SPLIT ? AHEAD : STAGES) * MASK_SLOT;
     static constexpr int STAGING = EPILOGUE_WARPS * 32 * (PIECE + 1) * 4;
     static constexpr int SUMS = FORM == WEIGHT ? 16 * BM * 4 : 0;  // of the columns
-    static constexpr int SHARED = STAGES * STAGE + STAGING + SUMS + 1024;
+    static constexpr int SHARED = STAGES * STAGE + RING + MASKS + STAGING + SUMS + 1024;
+    static_assert(SHARED + (FORM == FORWARD ? 2048 : 512) <= 232448 && (SPLIT || AHEAD < STAGES), "a block has 227 KB");
 };
 
 template <typename T>
@@ -184,6 +193,18 @@ __device__ __forceinline__ void tmem_load8(uint32_t address, float (&v)[8]) {
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// 16 bytes, of which the first `there` are copied and the others zeros.
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, int there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void *from, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
 __device__ __forceinline__ void store_shared(uint32_t address, const uint4 &v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(address), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -205,14 +226,9 @@ struct Unit<float> {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = k < left ? p[k] : 0.f;
     }
-    // All of them (on a boundary of 32 bytes), or zeros; without a branch.
-    __device__ __forceinline__ void load_whole(const float *p, bool there) {
-        asm volatile(
-            "{\n .reg .pred p;\n setp.ne.u32 p, %9, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n"
-            " mov.b32 %4, 0;\n mov.b32 %5, 0;\n mov.b32 %6, 0;\n mov.b32 %7, 0;\n"
-            " @p ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n}"
-            : "=&f"(v[0]), "=&f"(v[1]), "=&f"(v[2]), "=&f"(v[3]), "=&f"(v[4]), "=&f"(v[5]), "=&f"(v[6]), "=&f"(v[7])
-            : "l"(p), "r"((uint32_t)there));
+    __device__ __forceinline__ void load_whole(const float *p) {
+        const float4 x = *reinterpret_cast<const float4 *>(p), y = *reinterpret_cast<const float4 *>(p + 4);
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
     }
     __device__ __forceinline__ void keep(uint32_t bits) {
 #pragma unroll
@@ -250,13 +266,7 @@ struct Unit16 {
         for (int k = 0; k < 8; k += 2)
             w[k / 2] = (k < left ? (uint32_t)q[k] : 0u) | (k + 1 < left ? (uint32_t)q[k + 1] : 0u) << 16;
     }
-    __device__ __forceinline__ void load_whole(const T *p, bool there) {
-        asm volatile(
-            "{\n .reg .pred p;\n setp.ne.u32 p, %5, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n"
-            " @p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n}"
-            : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
-            : "l"(p), "r"((uint32_t)there));
-    }
+    __device__ __forceinline__ void load_whole(const T *p) { v = *reinterpret_cast<const uint4 *>(p); }
     __device__ __forceinline__ void keep(uint32_t bits) {
         uint32_t *const w = &v.x;
 #pragma unroll
@@ -298,7 +308,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const T *weight, int64_t in, 
     u.clear();
     if (n < N && k < K) {
         if (FORM == FORWARD) {
-            if (whole && k + 8 <= K) u.load_whole(weight + n * in + k, true);
+            if (whole && k + 8 <= K) u.load_whole(weight + n * in + k);
             else u.load(weight + n * in + k, (int)min(K - k, (int64_t)8));
         } else {
             T v[8];
@@ -557,14 +567,14 @@ struct Finish {
     }
 };
 
-// The units of a producer, DEPTH chunks ahead of the stage that it writes.  WHOLE: rows lie on vectors of 8 elements and are whole
-// vectors long, so that a unit is there or not.
+// The units of a producer: a thread has the same place in every chunk.  WHOLE: rows begin on 16 bytes, and units are copied
+// asynchronously; of other rows they are loaded an element at a time.
 template <typename T, int FORM, bool WHOLE>
 struct Producer {
     using S = Shape<T, FORM>;
-    static constexpr int BK = S::BK, UNITS = BK / 8;
+    static constexpr int BK = S::BK;
     // Units across a row of A and B, and rows of a turn of all producers.
-    static constexpr int A_ACROSS = FORM == WEIGHT ? BM / 8 : UNITS, A_DOWN = PRODUCERS / A_ACROSS;
+    static constexpr int A_ACROSS = FORM == WEIGHT ? BM / 8 : BK / 8, A_DOWN = PRODUCERS / A_ACROSS;
     [[maybe_unused]] static constexpr int B_ACROSS = S::BN / 8, B_DOWN = PRODUCERS / B_ACROSS;
     const Tiles<T> &t;
     const int p;
@@ -582,7 +592,8 @@ struct Producer {
           mask_step(A_DOWN * t_.mask_pitch), item(blockIdx.x), chunk(0), b(nullptr), mask(nullptr) {
         begin();
     }
-    __device__ __forceinline__ static int clamped(int64_t n) { return (int)max((int64_t)0, min(n, (int64_t)1 << 30)); }
+    __device__ __forceinline__ static int clamped(int64_t n) { return (int)max((int64_t)0, min(n, (int64_t)1 << 28)); }
+    __device__ __forceinline__ bool more() const { return item < t.items; }
     __device__ __forceinline__ void begin() {
         if (item >= t.items) return;
         const Item i = item_of<T, FORM>(t, item);
@@ -593,7 +604,7 @@ struct Producer {
             const int64_t b_row = i.k0 + p / B_ACROSS, b_column = i.n0 + p % B_ACROSS * 8;
             a = t.a + row * t.a_stride + column;
             b = t.b + b_row * t.b_stride + b_column;
-            mask = t.mask + row * t.mask_pitch + column / 8;
+            mask = t.mask + row * t.mask_pitch + column / 32 * 4;
             rows = clamped(i.k1 - row);
             b_rows = clamped(i.k1 - b_row);
             a_left = clamped(t.M - column);
@@ -601,34 +612,12 @@ struct Producer {
         } else {
             const int64_t row = i.m0 + p / A_ACROSS, column = p % A_ACROSS * 8;
             a = t.a + row * t.a_stride + column;
-            mask = t.mask + row * t.mask_pitch + column / 8;
+            mask = t.mask + row * t.mask_pitch + column / 32 * 4;
             rows = clamped(t.M - row);
             a_left = clamped(t.K - column);
         }
     }
-    __device__ __forceinline__ void load(Unit<T> (&x)[S::A_UNITS + S::B_UNITS], uint32_t (&keep)[S::A_UNITS]) {
-        if (item >= t.items) return;
-#pragma unroll
-        for (int u = 0; u < S::A_UNITS; ++u) {
-            const bool there = u * A_DOWN < rows && a_left > 0;
-            if constexpr (WHOLE) x[u].load_whole(a + u * a_step, there);
-            else x[u].load(a + u * a_step, there ? a_left : 0);
-        }
-        if constexpr (FORM != FORWARD)
-            if (masked)
-#pragma unroll
-                for (int u = 0; u < S::A_UNITS; ++u)
-                    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %2, 0;\n mov.b32 %0, 0;\n @p ld.global.u8 %0, [%1];\n}"
-                                 : "=&r"(keep[u])
-                                 : "l"(mask + u * mask_step), "r"((uint32_t)(u * A_DOWN < rows && a_left > 0)));
-        if constexpr (FORM == WEIGHT) {
-#pragma unroll
-            for (int u = 0; u < S::B_UNITS; ++u) {
-                const bool there = u * B_DOWN < b_rows && b_left > 0;
-                if constexpr (WHOLE) x[S::A_UNITS + u].load_whole(b + u * b_step, there);
-                else x[S::A_UNITS + u].load(b + u * b_step, there ? b_left : 0);
-            }
-        }
+    __device__ __forceinline__ void next() {
         if (++chunk == chunks) {
             item += gridDim.x;
             begin();
@@ -644,38 +633,119 @@ struct Producer {
             a_left -= BK;
         }
     }
-    __device__ __forceinline__ void store(Unit<T> (&x)[S::A_UNITS + S::B_UNITS], uint32_t (&keep)[S::A_UNITS], uint32_t stage,
-                                          float (&columns)[8]) {
+    // Where a unit of A or B lies in a plane.
+    __device__ __forceinline__ uint32_t a_place(int u) const {
+        return FORM == WEIGHT ? p % A_ACROSS / 8 * (BK * 128) + place<128>(p / A_ACROSS + u * A_DOWN, p % 8)
+                              : place<BK * 2>(p / A_ACROSS + u * A_DOWN, p % A_ACROSS);
+    }
+    __device__ __forceinline__ uint32_t b_place(int u) const {
+        return p % B_ACROSS / 8 * (BK * 128) + place<128>(p / B_ACROSS + u * B_DOWN, p % 8);
+    }
+    // The bits of a unit of A in its word of the mask (a unit's column is a multiple of 8).
+    __device__ __forceinline__ uint32_t bits_of(uint32_t word) const { return word >> (p % 4 * 8); }
+
+    // One unit on its way: 16-bit ones to `to`, fp32 ones to `to` and a turn of all producers behind it.
+    __device__ __forceinline__ static void copy_unit(uint32_t to, const T *from, int left) {
+        const int bytes = max(0, left) * (int)sizeof(T);
+        copy16(to, from, min(bytes, 16));
+        if constexpr (S::SPLIT) copy16(to + PRODUCERS * 16, from + 4, max(0, min(bytes - 16, 16)));
+    }
+    // The next chunk on its way: to a slot of the ring (fp32) or its stage (16 bits), the mask's words to theirs.
+    __device__ __forceinline__ void issue(uint32_t to, uint32_t masks) {
+#pragma unroll
+        for (int u = 0; u < S::A_UNITS; ++u) {
+            const int left = u * A_DOWN < rows ? a_left : 0;
+            copy_unit(S::SPLIT ? to + u * (PRODUCERS * 32) + p * 16 : to + a_place(u), left > 0 ? a + u * a_step : t.a, left);
+            if constexpr (FORM != FORWARD)
+                if (masked) copy4(masks + (u * PRODUCERS + p) * 4, left > 0 ? mask + u * mask_step : t.mask, left > 0);
+        }
+#pragma unroll
+        for (int u = 0; u < S::B_UNITS; ++u) {
+            const int left = u * B_DOWN < b_rows ? b_left : 0;
+            copy_unit(S::SPLIT ? to + (S::A_UNITS + u) * (PRODUCERS * 32) + p * 16 : to + S::A_PLANE + b_place(u),
+                      left > 0 ? b + u * b_step : t.b, left);
+        }
+        next();
+    }
+    // The next chunk by loads.
+    __device__ __forceinline__ void load(Unit<T> (&x)[S::A_UNITS + S::B_UNITS], uint32_t (&keep)[S::A_UNITS]) {
+#pragma unroll
+        for (int u = 0; u < S::A_UNITS; ++u) {
+            const int left = u * A_DOWN < rows ? a_left : 0;
+            x[u].load(a + u * a_step, left);
+            keep[u] = 0;
+            if (FORM != FORWARD && masked && left > 0) keep[u] = bits_of(*reinterpret_cast<const uint32_t *>(mask + u * mask_step));
+        }
+#pragma unroll
+        for (int u = 0; u < S::B_UNITS; ++u) x[S::A_UNITS + u].load(b + u * b_step, u * B_DOWN < b_rows ? b_left : 0);
+        next();
+    }
+    // What this thread copied to a slot of the ring.
+    __device__ __forceinline__ void take(const uint8_t *slot, const uint8_t *masks, Unit<T> (&x)[S::A_UNITS + S::B_UNITS],
+                                         uint32_t (&keep)[S::A_UNITS]) const {
+#pragma unroll
+        for (int u = 0; u < S::A_UNITS + S::B_UNITS; ++u) {
+            const uint8_t *const from = slot + u * (PRODUCERS * 32) + p * 16;
+            const float4 lower = *reinterpret_cast<const float4 *>(from), upper = *reinterpret_cast<const float4 *>(from + PRODUCERS * 16);
+            const float v[8] = {lower.x, lower.y, lower.z, lower.w, upper.x, upper.y, upper.z, upper.w};
+            x[u].load_whole(v);
+        }
+        if constexpr (FORM != FORWARD)
+            if (masked)
+#pragma unroll
+                for (int u = 0; u < S::A_UNITS; ++u) keep[u] = bits_of(*reinterpret_cast<const uint32_t *>(masks + (u * PRODUCERS + p) * 4));
+    }
+    __device__ __forceinline__ void add_columns(const Unit<T> (&x)[S::A_UNITS + S::B_UNITS], float (&columns)[8]) const {
+        float sum[8];
+#pragma unroll
+        for (int u = 0; u < S::A_UNITS; ++u)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum[k] = u == 0 ? x[u].value(k) : sum[k] + x[u].value(k);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) columns[k] += sum[k];
+    }
+    // Units to their planes in a stage.
+    __device__ __forceinline__ void store(Unit<T> (&x)[S::A_UNITS + S::B_UNITS], const uint32_t (&keep)[S::A_UNITS], uint32_t stage,
+                                          float (&columns)[8]) const {
         if constexpr (FORM != FORWARD)
             if (masked)
 #pragma unroll
                 for (int u = 0; u < S::A_UNITS; ++u) x[u].keep(keep[u]);
         if constexpr (FORM == WEIGHT)
-            if (t.column_sums != nullptr) {
-                float sum[8];
-#pragma unroll
-                for (int u = 0; u < S::A_UNITS; ++u)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) sum[k] = u == 0 ? x[u].value(k) : sum[k] + x[u].value(k);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) columns[k] += sum[k];
-            }
+            if (t.column_sums != nullptr) add_columns(x, columns);
 #pragma unroll
         for (int u = 0; u < S::A_UNITS; ++u) {
             uint4 planes[S::PLANES];
             x[u].planes(planes);
-            const uint32_t at = FORM == WEIGHT ? p % A_ACROSS / 8 * (BK * 128) + place<128>(p / A_ACROSS + u * A_DOWN, p % 8)
-                                               : place<BK * 2>(p / A_ACROSS + u * A_DOWN, p % A_ACROSS);
 #pragma unroll
-            for (int q = 0; q < S::PLANES; ++q) store_shared(stage + q * S::A_PLANE + at, planes[q]);
+            for (int q = 0; q < S::PLANES; ++q) store_shared(stage + q * S::A_PLANE + a_place(u), planes[q]);
         }
 #pragma unroll
         for (int u = 0; u < S::B_UNITS; ++u) {
             uint4 planes[S::PLANES];
             x[S::A_UNITS + u].planes(planes);
-            const uint32_t at = p % B_ACROSS / 8 * (BK * 128) + place<128>(p / B_ACROSS + u * B_DOWN, p % 8);
 #pragma unroll
-            for (int q = 0; q < S::PLANES; ++q) store_shared(stage + S::PLANES * S::A_PLANE + q * S::B_PLANE + at, planes[q]);
+            for (int q = 0; q < S::PLANES; ++q) store_shared(stage + S::PLANES * S::A_PLANE + q * S::B_PLANE + b_place(u), planes[q]);
+        }
+    }
+    // 16-bit units of A that have arrived in their stage: those of the mask go, and the others are added up.
+    __device__ __forceinline__ void mend(uint8_t *stage, const uint8_t *masks, float (&columns)[8]) const {
+        if constexpr (FORM != FORWARD) {
+            const bool summed = FORM == WEIGHT && t.column_sums != nullptr;
+            if (!masked && !summed) return;
+            Unit<T> x[S::A_UNITS + S::B_UNITS];
+#pragma unroll
+            for (int u = 0; u < S::A_UNITS; ++u) {
+                T *const at = reinterpret_cast<T *>(stage + a_place(u));
+                x[u].load_whole(at);
+                if (masked) {
+                    x[u].keep(bits_of(*reinterpret_cast<const uint32_t *>(masks + (u * PRODUCERS + p) * 4)));
+                    uint4 planes[S::PLANES];
+                    x[u].planes(planes);
+                    store_shared(shared_address(at), planes[0]);
+                }
+            }
+            if (summed) add_columns(x, columns);
         }
     }
 };
@@ -691,8 +761,10 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     __shared__ int given_up;
     __shared__ __align__(16) float bias_of_tile[2][BN / 2];
     uint8_t *const stages = raw + (1024 - shared_address(raw) % 1024) % 1024;  // groups of eight swizzled rows lie on 1024 bytes
-    float *const staging = reinterpret_cast<float *>(stages + STAGES * S::STAGE);
-    float *const column_parts = staging + S::STAGING / 4;
+    [[maybe_unused]] uint8_t *const ring = stages + STAGES * S::STAGE;
+    [[maybe_unused]] uint8_t *const masks = ring + S::RING;
+    float *const staging = reinterpret_cast<float *>(masks + S::MASKS);
+    [[maybe_unused]] float *const column_parts = staging + S::STAGING / 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -801,56 +873,109 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         }
     } else if (warp < MMA_WARP) {
         // ------------------------------------------------------------------ operands to shared memory
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
-        const int p = threadIdx.x - EPILOGUE_WARPS * 32;
-        Unit<T> x[S::DEPTH][S::A_UNITS + S::B_UNITS];
-        uint32_t keep[S::DEPTH][S::A_UNITS];
+const int p = threadIdx.x - EPILOGUE_WARPS * 32;
         float columns[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) columns[k] = 0.f;
         Producer<T, FORM, WHOLE> ahead(t, p);
-#pragma unroll
-        for (int d = 0; d < S::DEPTH; ++d) ahead.load(x[d], keep[d]);
-        uint32_t s = 0, parity = 1;
+        uint32_t s = 0, parity = 1;  // of the stage that is filled next
         bool alive = true;
         int item = blockIdx.x, chunk = 0, chunks = chunks_of<T, FORM>(t, item);
-        while (item < t.items) {  // (to the end whatever happens: the barriers below want every thread)
+        const auto await = [&] {
+            if (alive) alive = __all_sync(0xffffffffu, barrier_wait(&empty[s], parity, polls, &given_up));
+        };
+        const auto filled = [&](uint32_t stage) {
+            fence_to_async();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(&a_full[stage]);
+        };
+        const auto step = [&] {
+            if (++s == STAGES) s = 0, parity ^= 1;
+        };
+        // A chunk of the present item is done.  (To the end of all items whatever happens: the barriers here want every thread.)
+        const auto done = [&] {
+            if (++chunk < chunks) return;
+            if (FORM == WEIGHT && t.column_sums != nullptr) {
+                const Item i = item_of<T, FORM>(t, item);
+                if (i.n0 == 0) {
 #pragma unroll
-            for (int d = 0; d < S::DEPTH; ++d) {
-                if (item >= t.items) continue;
-                if (alive) alive = __all_sync(0xffffffffu, barrier_wait(&empty[s], parity, polls, &given_up));
-                if (alive) {
-                    ahead.store(x[d], keep[d], shared_address(stages) + s * S::STAGE, columns);
-                    fence_to_async();
-                    __syncwarp();
-                    if (lane == 0) barrier_arrive(&a_full[s]);
-                    ahead.load(x[d], keep[d]);
-                }
-                if (++s == STAGES) s = 0, parity ^= 1;
-                if (++chunk < chunks) continue;
-                if (FORM == WEIGHT && t.column_sums != nullptr) {
-                    const Item i = item_of<T, FORM>(t, item);
-                    if (i.n0 == 0) {
+                    for (int k = 0; k < 8; ++k) column_parts[(p / 16) * BM + p % 16 * 8 + k] = columns[k];
+                    asm volatile("bar.sync 3, %0;" ::"n"(PRODUCERS) : "memory");
+                    if (p < BM && i.m0 + p < t.M) {
+                        float total = 0.f;
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) column_parts[(p / 16) * BM + p % 16 * 8 + k] = columns[k];
-                        asm volatile("bar.sync 3, %0;" ::"n"(PRODUCERS) : "memory");
-                        if (p < BM && i.m0 + p < t.M) {
-                            float total = 0.f;
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) total += column_parts[r * BM + p];
-                            if (*(volatile int *)&given_up) total = __uint_as_float(0x7fffffffu);
-                            t.column_sums[i.split * t.M + i.m0 + p] = total;
-                        }
-                        asm volatile("bar.sync 3, %0;" ::"n"(PRODUCERS) : "memory");
+                        for (int r = 0; r < 16; ++r) total += column_parts[r * BM + p];
+                        if (*(volatile int *)&given_up) total = __uint_as_float(0x7fffffffu);
+                        t.column_sums[i.split * t.M + i.m0 + p] = total;
                     }
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) columns[k] = 0.f;
+                    asm volatile("bar.sync 3, %0;" ::"n"(PRODUCERS) : "memory");
                 }
-                chunk = 0;
-                item += gridDim.x;
-                if (FORM == WEIGHT && item < t.items) chunks = chunks_of<T, FORM>(t, item);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) columns[k] = 0.f;
+            }
+            chunk = 0;
+            item += gridDim.x;
+            if (FORM == WEIGHT && item < t.items) chunks = chunks_of<T, FORM>(t, item);
+        };
+        if constexpr (WHOLE && S::SPLIT) {
+            const uint32_t slots = shared_address(ring), words = shared_address(masks);
+#pragma unroll
+            for (int d = 0; d < S::AHEAD; ++d) {
+                if (ahead.more()) ahead.issue(slots + d * S::SLOT, words + d * S::MASK_SLOT);
+                copies_end();
+            }
+            int d = 0;
+            while (item < t.items) {
+                copies_wait<S::AHEAD - 1>();
+                await();
+                if (alive) {
+                    Unit<T> x[S::A_UNITS + S::B_UNITS];
+                    uint32_t keep[S::A_UNITS];
+                    ahead.take(ring + d * S::SLOT, masks + d * S::MASK_SLOT, x, keep);
+                    ahead.store(x, keep, shared_address(stages) + s * S::STAGE, columns);
+                    filled(s);
+                    if (ahead.more()) ahead.issue(slots + d * S::SLOT, words + d * S::MASK_SLOT);
+                }
+                copies_end();
+                if (++d == S::AHEAD) d = 0;
+                step();
+                done();
+            }
+        } else if constexpr (WHOLE) {
+            int begun = 0;        // chunks on their way
+            uint32_t arrived = 0; // the stage of the first of them
+            while (item < t.items) {
+                if (ahead.more() && alive) {
+                    await();
+                    if (alive) ahead.issue(shared_address(stages) + s * S::STAGE, shared_address(masks) + s * S::MASK_SLOT);
+                    step();
+                }
+                copies_end();
+                if (++begun <= S::AHEAD) continue;
+                copies_wait<S::AHEAD>();
+                if (alive) {
+                    ahead.mend(stages + arrived * S::STAGE, masks + arrived * S::MASK_SLOT, columns);
+                    filled(arrived);
+                }
+                if (++arrived == STAGES) arrived = 0;
+                done();
+            }
+        } else {
+            Unit<T> x[S::A_UNITS + S::B_UNITS];
+            uint32_t keep[S::A_UNITS];
+            if (ahead.more()) ahead.load(x, keep);
+            while (item < t.items) {
+                await();
+                if (alive) {
+                    ahead.store(x, keep, shared_address(stages) + s * S::STAGE, columns);
+                    filled(s);
+                    if (ahead.more()) ahead.load(x, keep);
+                }
+                step();
+                done();
             }
         }
+        copies_wait<0>();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGISTERS));
         if (warp == MMA_WARP) {
@@ -986,8 +1111,8 @@ int launch(Tiles<T> &t, int64_t splits, cudaStream_t stream) {
     t.tiles_m = (int)tiles_m;
     t.tiles_n = (int)tiles_n;
     t.items = (int)(tiles_m * tiles_n * splits);
-    bool whole = whole_rows(t.a, t.a_stride, sizeof(T)) && (FORM == WEIGHT ? t.M : t.K) % 8 == 0;
-    if (FORM == WEIGHT) whole = whole && whole_rows(t.b, t.b_stride, sizeof(T)) && t.N % 8 == 0;
+    constexpr int VECTOR = 16 / sizeof(T);
+    const bool whole = whole_rows(t.a, t.a_stride, sizeof(T), VECTOR) && (FORM != WEIGHT || whole_rows(t.b, t.b_stride, sizeof(T), VECTOR));
     if constexpr (Shape<T, FORM>::SPLIT)
         if (t.k_per_item > Shape<T, FORM>::SEGMENT * Shape<T, FORM>::BK)
             return whole ? launch_as<T, FORM, true, true>(t, stream) : launch_as<T, FORM, false, true>(t, stream);
