@@ -27,39 +27,41 @@ constexpr int EPILOGUE_WARPS = 8, PRODUCER_WARPS = 8;
 constexpr int PRODUCERS = PRODUCER_WARPS * 32;
 constexpr int MMA_WARP = EPILOGUE_WARPS + PRODUCER_WARPS, COPY_WARP = MMA_WARP + 1;
 constexpr int THREADS = (MMA_WARP + 4) * 32;
-// Registers of a thread by warpgroup; a launch brings 96 a thread, and the five groups share that: 2 x 128 + 2 x 96 + 32 = 5 x 96.
-constexpr int EPILOGUE_REGISTERS = 128, OTHER_REGISTERS = 32;
+// Registers of a thread by warpgroup; a launch brings 96 a thread, and the five groups share that: 2 x 112 + 2 x 112 + 32 = 5 x 96.
+constexpr int EPILOGUE_REGISTERS = 112, PRODUCER_REGISTERS = 112, OTHER_REGISTERS = 32;
 constexpr int SMS = 148;
 constexpr int TMEM_COLUMNS = 512;  // two buffers of 256
 constexpr int PIECE = 16;          // columns that a warp of the epilogue takes through shared memory at once
 
 // A stage holds BK of the contraction: rows of BK 16-bit elements (FORWARD, INPUT), or BK rows of panels of 64 (WEIGHT).
 //
-// HBM wants 35 KB on their way to each multiprocessor.  Loads to registers do not get there: a wait for one of them is a wait for
-// the latest (48 and 16 KB ahead took the same time).  Asynchronous copies do; 16-bit operands are copied to where the
-// tensor core reads them, AHEAD stages early, fp32 ones to a ring of AHEAD chunks from which the thread that copied them
-// takes them to be split.
-template <typename T, int FORM>
+// HBM wants 35 KB on their way to each multiprocessor.  16-bit operands are copied asynchronously to where the tensor core
+// reads them, as many stages early as there are, or AHEAD where somebody looks at them on their way.  fp32 ones go through
+// registers, by two groups of producers that take every other chunk: a warp's wait for one load is a wait for its latest, so that
+// loads further ahead by the same warps did not help (4 chunks ahead 180 us, 1 chunk 178; two groups TWO_GROUPS_US).
+template <typename T, int FORM, bool WHOLE>
 struct Shape {
     static constexpr bool SPLIT = sizeof(T) == 4;
+    static constexpr bool ASYNC = WHOLE && !SPLIT;
     static constexpr int PLANES = SPLIT ? 3 : 1;
     static constexpr int BN = SPLIT ? 128 : 256;
     static constexpr int BK = SPLIT || FORM == WEIGHT ? 32 : 64;
     static constexpr int A_PLANE = BM * BK * 2, B_PLANE = BN * BK * 2;
     static constexpr int STAGE = PLANES * (A_PLANE + B_PLANE);
-    static constexpr int STAGES = SPLIT ? (FORM == WEIGHT ? 2 : 3) : FORM == WEIGHT ? 7 : 4;
-    static constexpr int AHEAD = SPLIT || FORM != WEIGHT ? 3 : 5;
+    static constexpr int STAGES = !SPLIT && FORM == WEIGHT ? 7 : 4;
+    static constexpr int AHEAD = FORM == WEIGHT ? 5 : 2;
     static constexpr int SEGMENT = SPLIT ? 256 / BK : 1 << 30;  // chunks of BK that an accumulator takes
-    static constexpr int A_UNITS = BM * BK / 8 / PRODUCERS, B_UNITS = FORM == WEIGHT ? BN * BK / 8 / PRODUCERS : 0;
-    static constexpr int SLOT = SPLIT ? (A_UNITS + B_UNITS) * PRODUCERS * 32 : 0;  // of the ring
-    static constexpr int RING = AHEAD * SLOT;
-    static constexpr int MASK_SLOT = FORM == FORWARD ? 0 : A_UNITS * PRODUCERS * 4;  // a word of the mask for each unit
-    static constexpr int MASKS = (SPLIT ? AHEAD : STAGES) * MASK_SLOT;
+    static constexpr int GROUPS = ASYNC ? 1 : 2, MEMBERS = PRODUCERS / GROUPS;  // producers that fill a stage
+    static constexpr int A_UNITS = BM * BK / 8 / MEMBERS, B_UNITS = FORM == WEIGHT ? BN * BK / 8 / MEMBERS : 0;
+    static constexpr int MASK_SLOT = ASYNC && FORM != FORWARD ? A_UNITS * MEMBERS * 4 : 0;  // a word of the mask for each unit
     static constexpr int STAGING = EPILOGUE_WARPS * 32 * (PIECE + 1) * 4;
     static constexpr int SUMS = FORM == WEIGHT ? 16 * BM * 4 : 0;  // of the columns
-    static constexpr int SHARED = STAGES * STAGE + RING + MASKS + STAGING + SUMS + 1024;
-    static_assert(SHARED + (FORM == FORWARD ? 2048 : 512) <= 232448 && (SPLIT || AHEAD < STAGES), "a block has 227 KB");
+    static constexpr int SHARED = STAGES * (STAGE + MASK_SLOT) + STAGING + SUMS + 1024;
+    static_assert(SHARED + (FORM == FORWARD ? 2048 : 512) <= 232448 && (SPLIT || AHEAD + 1 < STAGES), "a block has 227 KB");
 };
+// What does not depend on the way of the operands.
+template <typename T, int FORM>
+using Tile = Shape<T, FORM, true>;
 
 template <typename T>
 struct Tiles {
@@ -200,6 +202,10 @@ __device__ __forceinline__ void copy16(uint32_t to, const void *from, int there)
 __device__ __forceinline__ void copy4(uint32_t to, const void *from, bool there) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
 }
+// The barrier is told when this thread's copies up to here have arrived.
+__device__ __forceinline__ void copies_report(uint64_t *barrier) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(shared_address(barrier)) : "memory");
+}
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>
 __device__ __forceinline__ void copies_wait() {
@@ -229,6 +235,15 @@ struct Unit<float> {
     __device__ __forceinline__ void load_whole(const float *p) {
         const float4 x = *reinterpret_cast<const float4 *>(p), y = *reinterpret_cast<const float4 *>(p + 4);
         v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+    }
+    // All of them (on a boundary of 32 bytes), or zeros; without a branch.
+    __device__ __forceinline__ void load_or_clear(const float *p, bool there) {
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.u32 p, %9, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n"
+            " mov.b32 %4, 0;\n mov.b32 %5, 0;\n mov.b32 %6, 0;\n mov.b32 %7, 0;\n"
+            " @p ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n}"
+            : "=&f"(v[0]), "=&f"(v[1]), "=&f"(v[2]), "=&f"(v[3]), "=&f"(v[4]), "=&f"(v[5]), "=&f"(v[6]), "=&f"(v[7])
+            : "l"(p), "r"((uint32_t)there));
     }
     __device__ __forceinline__ void keep(uint32_t bits) {
 #pragma unroll
@@ -296,7 +311,7 @@ __device__ __forceinline__ uint32_t place(int r, int c) {
 template <typename T, int FORM>
 __global__ void __launch_bounds__(256) pack_kernel(const T *weight, int64_t in, int64_t N, int64_t K, int64_t chunks, uint8_t *packed,
                                                    int whole) {
-    using S = Shape<T, FORM>;
+    using S = Tile<T, FORM>;
     constexpr int UNITS = S::BK / 8;  // of a row
     const int64_t n_rows = (N + S::BN - 1) / S::BN * S::BN;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -339,7 +354,7 @@ __device__ __forceinline__ Item item_of(const Tiles<T> &t, int item) {
     i.split = FORM == WEIGHT ? item / tiles : 0;
     const int tile = FORM == WEIGHT ? item % tiles : item;
     i.m0 = (int64_t)(tile / t.tiles_n) * BM;
-    i.n0 = (int64_t)(tile % t.tiles_n) * Shape<T, FORM>::BN;
+    i.n0 = (int64_t)(tile % t.tiles_n) * Tile<T, FORM>::BN;
     i.k0 = i.split * t.k_per_item;
     i.k1 = min(t.K, i.k0 + t.k_per_item);
     return i;
@@ -351,7 +366,7 @@ __device__ __forceinline__ int chunks_of(const Tiles<T> &t, int item) {
         const int64_t k0 = item / (t.tiles_m * t.tiles_n) * t.k_per_item;
         k = min(k, k0 + t.k_per_item) - k0;
     }
-    return (int)((k + Shape<T, FORM>::BK - 1) / Shape<T, FORM>::BK);
+    return (int)((k + Tile<T, FORM>::BK - 1) / Tile<T, FORM>::BK);
 }
 
 // One element by fp32 arithmetic: where an operand is infinite, no number or beyond bf16's range, its parts say nothing.
@@ -460,7 +475,7 @@ struct Finish {
     // Columns c .. c + PIECE of the item.
     __device__ __forceinline__ void piece(float (&y)[PIECE], const float (&added)[PIECE], const Item &i, int c, bool alive) {
         const int left = columns - c;
-        if constexpr (Shape<T, FORM>::SPLIT) {
+        if constexpr (Tile<T, FORM>::SPLIT) {
             float none = 0.f;  // zero unless one of them is no finite number
 #pragma unroll
             for (int k = 0; k < PIECE; ++k) none = fmaf(y[k], 0.f, none);
@@ -567,15 +582,15 @@ struct Finish {
     }
 };
 
-// The units of a producer: a thread has the same place in every chunk.  WHOLE: rows begin on 16 bytes, and units are copied
-// asynchronously; of other rows they are loaded an element at a time.
+// The units of a producer: a thread has the same place in every chunk of its group.  WHOLE: rows lie on vectors of 8 elements;
+// units of other rows are loaded an element at a time.
 template <typename T, int FORM, bool WHOLE>
 struct Producer {
-    using S = Shape<T, FORM>;
-    static constexpr int BK = S::BK;
-    // Units across a row of A and B, and rows of a turn of all producers.
-    static constexpr int A_ACROSS = FORM == WEIGHT ? BM / 8 : BK / 8, A_DOWN = PRODUCERS / A_ACROSS;
-    [[maybe_unused]] static constexpr int B_ACROSS = S::BN / 8, B_DOWN = PRODUCERS / B_ACROSS;
+    using S = Shape<T, FORM, WHOLE>;
+    static constexpr int BK = S::BK, MEMBERS = S::MEMBERS;
+    // Units across a row of A and B, and rows of a turn of the group.
+    static constexpr int A_ACROSS = FORM == WEIGHT ? BM / 8 : BK / 8, A_DOWN = MEMBERS / A_ACROSS;
+    [[maybe_unused]] static constexpr int B_ACROSS = S::BN / 8, B_DOWN = MEMBERS / B_ACROSS;
     const Tiles<T> &t;
     const int p;
     const bool masked;
@@ -644,56 +659,47 @@ struct Producer {
     // The bits of a unit of A in its word of the mask (a unit's column is a multiple of 8).
     __device__ __forceinline__ uint32_t bits_of(uint32_t word) const { return word >> (p % 4 * 8); }
 
-    // One unit on its way: 16-bit ones to `to`, fp32 ones to `to` and a turn of all producers behind it.
-    __device__ __forceinline__ static void copy_unit(uint32_t to, const T *from, int left) {
-        const int bytes = max(0, left) * (int)sizeof(T);
-        copy16(to, from, min(bytes, 16));
-        if constexpr (S::SPLIT) copy16(to + PRODUCERS * 16, from + 4, max(0, min(bytes - 16, 16)));
+    // The next chunk on its way to its stage (16 bits), the mask's words to theirs.
+    __device__ __forceinline__ void issue(uint32_t stage, uint32_t masks) {
+#pragma unroll
+        for (int u = 0; u < S::A_UNITS; ++u) {
+            const int left = u * A_DOWN < rows ? max(0, a_left) : 0;
+            copy16(stage + a_place(u), left > 0 ? a + u * a_step : t.a, min(left * (int)sizeof(T), 16));
+            if constexpr (FORM != FORWARD)
+                if (masked) copy4(masks + (u * MEMBERS + p) * 4, left > 0 ? mask + u * mask_step : t.mask, left > 0);
+        }
+#pragma unroll
+        for (int u = 0; u < S::B_UNITS; ++u) {
+            const int left = u * B_DOWN < b_rows ? max(0, b_left) : 0;
+            copy16(stage + S::A_PLANE + b_place(u), left > 0 ? b + u * b_step : t.b, min(left * (int)sizeof(T), 16));
+        }
+        next();
     }
-    // The next chunk on its way: to a slot of the ring (fp32) or its stage (16 bits), the mask's words to theirs.
-    __device__ __forceinline__ void issue(uint32_t to, uint32_t masks) {
+    // The next chunk of the group by loads.
+    __device__ __forceinline__ void load(Unit<T> (&x)[S::A_UNITS + S::B_UNITS], uint32_t (&keep)[S::A_UNITS]) {
+        if (!more()) return;
 #pragma unroll
         for (int u = 0; u < S::A_UNITS; ++u) {
             const int left = u * A_DOWN < rows ? a_left : 0;
-            copy_unit(S::SPLIT ? to + u * (PRODUCERS * 32) + p * 16 : to + a_place(u), left > 0 ? a + u * a_step : t.a, left);
-            if constexpr (FORM != FORWARD)
-                if (masked) copy4(masks + (u * PRODUCERS + p) * 4, left > 0 ? mask + u * mask_step : t.mask, left > 0);
+            if constexpr (WHOLE && S::SPLIT) x[u].load_or_clear(a + u * a_step, left > 0);
+            else x[u].load(a + u * a_step, left);
+        }
+        if constexpr (FORM != FORWARD) {
+            if (masked)
+#pragma unroll
+                for (int u = 0; u < S::A_UNITS; ++u)
+                    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %2, 0;\n mov.b32 %0, 0;\n @p ld.global.b32 %0, [%1];\n}"
+                                 : "=&r"(keep[u])
+                                 : "l"(mask + u * mask_step), "r"((uint32_t)(u * A_DOWN < rows && a_left > 0)));
         }
 #pragma unroll
         for (int u = 0; u < S::B_UNITS; ++u) {
             const int left = u * B_DOWN < b_rows ? b_left : 0;
-            copy_unit(S::SPLIT ? to + (S::A_UNITS + u) * (PRODUCERS * 32) + p * 16 : to + S::A_PLANE + b_place(u),
-                      left > 0 ? b + u * b_step : t.b, left);
+            if constexpr (WHOLE && S::SPLIT) x[S::A_UNITS + u].load_or_clear(b + u * b_step, left > 0);
+            else x[S::A_UNITS + u].load(b + u * b_step, left);
         }
         next();
-    }
-    // The next chunk by loads.
-    __device__ __forceinline__ void load(Unit<T> (&x)[S::A_UNITS + S::B_UNITS], uint32_t (&keep)[S::A_UNITS]) {
-#pragma unroll
-        for (int u = 0; u < S::A_UNITS; ++u) {
-            const int left = u * A_DOWN < rows ? a_left : 0;
-            x[u].load(a + u * a_step, left);
-            keep[u] = 0;
-            if (FORM != FORWARD && masked && left > 0) keep[u] = bits_of(*reinterpret_cast<const uint32_t *>(mask + u * mask_step));
-        }
-#pragma unroll
-        for (int u = 0; u < S::B_UNITS; ++u) x[S::A_UNITS + u].load(b + u * b_step, u * B_DOWN < b_rows ? b_left : 0);
-        next();
-    }
-    // What this thread copied to a slot of the ring.
-    __device__ __forceinline__ void take(const uint8_t *slot, const uint8_t *masks, Unit<T> (&x)[S::A_UNITS + S::B_UNITS],
-                                         uint32_t (&keep)[S::A_UNITS]) const {
-#pragma unroll
-        for (int u = 0; u < S::A_UNITS + S::B_UNITS; ++u) {
-            const uint8_t *const from = slot + u * (PRODUCERS * 32) + p * 16;
-            const float4 lower = *reinterpret_cast<const float4 *>(from), upper = *reinterpret_cast<const float4 *>(from + PRODUCERS * 16);
-            const float v[8] = {lower.x, lower.y, lower.z, lower.w, upper.x, upper.y, upper.z, upper.w};
-            x[u].load_whole(v);
-        }
-        if constexpr (FORM != FORWARD)
-            if (masked)
-#pragma unroll
-                for (int u = 0; u < S::A_UNITS; ++u) keep[u] = bits_of(*reinterpret_cast<const uint32_t *>(masks + (u * PRODUCERS + p) * 4));
+        if (S::GROUPS == 2 && more()) next();
     }
     __device__ __forceinline__ void add_columns(const Unit<T> (&x)[S::A_UNITS + S::B_UNITS], float (&columns)[8]) const {
         float sum[8];
@@ -707,12 +713,14 @@ struct Producer {
     // Units to their planes in a stage.
     __device__ __forceinline__ void store(Unit<T> (&x)[S::A_UNITS + S::B_UNITS], const uint32_t (&keep)[S::A_UNITS], uint32_t stage,
                                           float (&columns)[8]) const {
-        if constexpr (FORM != FORWARD)
+        if constexpr (FORM != FORWARD) {
             if (masked)
 #pragma unroll
-                for (int u = 0; u < S::A_UNITS; ++u) x[u].keep(keep[u]);
-        if constexpr (FORM == WEIGHT)
+                for (int u = 0; u < S::A_UNITS; ++u) x[u].keep(bits_of(keep[u]));
+        }
+        if constexpr (FORM == WEIGHT) {
             if (t.column_sums != nullptr) add_columns(x, columns);
+        }
 #pragma unroll
         for (int u = 0; u < S::A_UNITS; ++u) {
             uint4 planes[S::PLANES];
@@ -739,7 +747,7 @@ struct Producer {
                 T *const at = reinterpret_cast<T *>(stage + a_place(u));
                 x[u].load_whole(at);
                 if (masked) {
-                    x[u].keep(bits_of(*reinterpret_cast<const uint32_t *>(masks + (u * PRODUCERS + p) * 4)));
+                    x[u].keep(bits_of(*reinterpret_cast<const uint32_t *>(masks + (u * MEMBERS + p) * 4)));
                     uint4 planes[S::PLANES];
                     x[u].planes(planes);
                     store_shared(shared_address(at), planes[0]);
@@ -753,24 +761,25 @@ struct Producer {
 // MANY: fp32 contractions of more than one segment, whose sums take registers that the others keep.
 template <typename T, int FORM, bool WHOLE, bool MANY>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ Tiles<T> t) {
-    using S = Shape<T, FORM>;
+    using S = Shape<T, FORM, WHOLE>;
     constexpr int BN = S::BN, BK = S::BK, STAGES = S::STAGES, PLANES = S::PLANES;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t a_full[STAGES], b_full[STAGES], empty[STAGES], sums_full[2], sums_empty[2], drained;
+    __shared__ uint64_t full[STAGES], empty[STAGES], sums_full[2], sums_empty[2], drained;
     __shared__ uint32_t tmem_base;
     __shared__ int given_up;
     __shared__ __align__(16) float bias_of_tile[2][BN / 2];
     uint8_t *const stages = raw + (1024 - shared_address(raw) % 1024) % 1024;  // groups of eight swizzled rows lie on 1024 bytes
-    [[maybe_unused]] uint8_t *const ring = stages + STAGES * S::STAGE;
-    [[maybe_unused]] uint8_t *const masks = ring + S::RING;
-    float *const staging = reinterpret_cast<float *>(masks + S::MASKS);
+    [[maybe_unused]] uint8_t *const masks = stages + STAGES * S::STAGE;
+    float *const staging = reinterpret_cast<float *>(masks + STAGES * S::MASK_SLOT);
     [[maybe_unused]] float *const column_parts = staging + S::STAGING / 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // 16-bit operands that nobody looks at on their way: their copies report to the barriers themselves, each thread's.
+    const bool direct = S::ASYNC && (FORM == FORWARD || t.mask == nullptr) && (FORM != WEIGHT || t.column_sums == nullptr);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            barrier_init(&a_full[s], PRODUCER_WARPS);
-            barrier_init(&b_full[s], 1);
+            // (the copies of the weight's images report to the same barrier as whatever fills the rest of the stage)
+            barrier_init(&full[s], (direct ? PRODUCERS : S::MEMBERS / 32) + (FORM == WEIGHT ? 0 : 1));
             barrier_init(&empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -873,7 +882,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         }
     } else if (warp < MMA_WARP) {
         // ------------------------------------------------------------------ operands to shared memory
-const int p = threadIdx.x - EPILOGUE_WARPS * 32;
+asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
+        const int group = (threadIdx.x - EPILOGUE_WARPS * 32) / S::MEMBERS, p = (threadIdx.x - EPILOGUE_WARPS * 32) % S::MEMBERS;
         float columns[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) columns[k] = 0.f;
@@ -887,7 +897,7 @@ const int p = threadIdx.x - EPILOGUE_WARPS * 32;
         const auto filled = [&](uint32_t stage) {
             fence_to_async();
             __syncwarp();
-            if (lane == 0) barrier_arrive(&a_full[stage]);
+            if (lane == 0) barrier_arrive(&full[stage]);
         };
         const auto step = [&] {
             if (++s == STAGES) s = 0, parity ^= 1;
@@ -899,9 +909,9 @@ const int p = threadIdx.x - EPILOGUE_WARPS * 32;
                 const Item i = item_of<T, FORM>(t, item);
                 if (i.n0 == 0) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) column_parts[(p / 16) * BM + p % 16 * 8 + k] = columns[k];
+                    for (int k = 0; k < 8; ++k) column_parts[(group * (S::MEMBERS / 16) + p / 16) * BM + p % 16 * 8 + k] = columns[k];
                     asm volatile("bar.sync 3, %0;" ::"n"(PRODUCERS) : "memory");
-                    if (p < BM && i.m0 + p < t.M) {
+                    if (group == 0 && p < BM && i.m0 + p < t.M) {
                         float total = 0.f;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) total += column_parts[r * BM + p];
@@ -917,65 +927,57 @@ const int p = threadIdx.x - EPILOGUE_WARPS * 32;
             item += gridDim.x;
             if (FORM == WEIGHT && item < t.items) chunks = chunks_of<T, FORM>(t, item);
         };
-        if constexpr (WHOLE && S::SPLIT) {
-            const uint32_t slots = shared_address(ring), words = shared_address(masks);
-#pragma unroll
-            for (int d = 0; d < S::AHEAD; ++d) {
-                if (ahead.more()) ahead.issue(slots + d * S::SLOT, words + d * S::MASK_SLOT);
-                copies_end();
-            }
-            int d = 0;
-            while (item < t.items) {
-                copies_wait<S::AHEAD - 1>();
-                await();
-                if (alive) {
-                    Unit<T> x[S::A_UNITS + S::B_UNITS];
-                    uint32_t keep[S::A_UNITS];
-                    ahead.take(ring + d * S::SLOT, masks + d * S::MASK_SLOT, x, keep);
-                    ahead.store(x, keep, shared_address(stages) + s * S::STAGE, columns);
-                    filled(s);
-                    if (ahead.more()) ahead.issue(slots + d * S::SLOT, words + d * S::MASK_SLOT);
-                }
-                copies_end();
-                if (++d == S::AHEAD) d = 0;
-                step();
-                done();
-            }
-        } else if constexpr (WHOLE) {
-            int begun = 0;        // chunks on their way
-            uint32_t arrived = 0; // the stage of the first of them
-            while (item < t.items) {
-                if (ahead.more() && alive) {
+        if constexpr (S::ASYNC) {
+            if (direct) {
+                while (ahead.more() && alive) {
                     await();
-                    if (alive) ahead.issue(shared_address(stages) + s * S::STAGE, shared_address(masks) + s * S::MASK_SLOT);
+                    if (alive) {
+                        ahead.issue(shared_address(stages) + s * S::STAGE, shared_address(masks) + s * S::MASK_SLOT);
+                        copies_report(&full[s]);
+                    }
                     step();
                 }
-                copies_end();
-                if (++begun <= S::AHEAD) continue;
-                copies_wait<S::AHEAD>();
-                if (alive) {
-                    ahead.mend(stages + arrived * S::STAGE, masks + arrived * S::MASK_SLOT, columns);
-                    filled(arrived);
+            } else {
+                int begun = 0;        // chunks on their way
+                uint32_t arrived = 0; // the stage of the first of them
+                while (item < t.items) {
+                    if (ahead.more() && alive) {
+                        await();
+                        if (alive) ahead.issue(shared_address(stages) + s * S::STAGE, shared_address(masks) + s * S::MASK_SLOT);
+                        step();
+                    }
+                    copies_end();
+                    if (++begun <= S::AHEAD) continue;
+                    copies_wait<S::AHEAD>();
+                    if (alive) {
+                        ahead.mend(stages + arrived * S::STAGE, masks + arrived * S::MASK_SLOT, columns);
+                        filled(arrived);
+                    }
+                    if (++arrived == STAGES) arrived = 0;
+                    done();
                 }
-                if (++arrived == STAGES) arrived = 0;
-                done();
             }
+            copies_wait<0>();
         } else {
             Unit<T> x[S::A_UNITS + S::B_UNITS];
             uint32_t keep[S::A_UNITS];
-            if (ahead.more()) ahead.load(x, keep);
+            if (group == 1 && ahead.more()) ahead.next();
+            ahead.load(x, keep);
+            int turn = 0;  // of the group whose chunk it is
             while (item < t.items) {
-                await();
-                if (alive) {
-                    ahead.store(x, keep, shared_address(stages) + s * S::STAGE, columns);
-                    filled(s);
-                    if (ahead.more()) ahead.load(x, keep);
+                if (turn == group) {
+                    await();
+                    if (alive) {
+                        ahead.store(x, keep, shared_address(stages) + s * S::STAGE, columns);
+                        filled(s);
+                        ahead.load(x, keep);
+                    }
                 }
+                turn ^= 1;
                 step();
                 done();
             }
         }
-        copies_wait<0>();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGISTERS));
         if (warp == MMA_WARP) {
@@ -1002,11 +1004,11 @@ const int p = threadIdx.x - EPILOGUE_WARPS * 32;
                     const uint32_t accumulator = tmem + buffer * 256, small = accumulator + 128;
                     const bool fresh = of_segment == 0, last = ++of_segment == S::SEGMENT || chunk + 1 == chunks;
                     bool good = !fresh || barrier_wait(&sums_empty[buffer], buffer_parity, polls, &given_up);
-                    good = good && barrier_wait(&a_full[s], parity, polls, &given_up);
-                    if (FORM != WEIGHT) good = good && barrier_wait(&b_full[s], parity, polls, &given_up);
+                    good = good && barrier_wait(&full[s], parity, polls, &given_up);
                     alive = __all_sync(0xffffffffu, good);
                     if (!alive) break;
                     fence_after();
+                    if (direct) fence_to_async();  // (what was written by others is for the tensor core from here on)
                     const uint32_t a = a_first + s * (S::STAGE >> 4), b = b_first + s * (S::STAGE >> 4);
                     if (leads) {
 #pragma unroll
@@ -1058,14 +1060,16 @@ const int p = threadIdx.x - EPILOGUE_WARPS * 32;
                     alive = barrier_wait(&empty[s], (round / STAGES & 1) ^ 1, polls, &given_up);
                     if (!alive) break;
                     const uint32_t to = shared_address(stages) + s * S::STAGE + PLANES * S::A_PLANE;
-                    barrier_expect(&b_full[s], rows * (BK * 2) * PLANES);
+                    barrier_expect(&full[s], rows * (BK * 2) * PLANES);
 #pragma unroll
-                    for (int q = 0; q < PLANES; ++q) bulk_copy(to + q * S::B_PLANE, image + q * S::B_PLANE, rows * (BK * 2), &b_full[s]);
+                    for (int q = 0; q < PLANES; ++q) bulk_copy(to + q * S::B_PLANE, image + q * S::B_PLANE, rows * (BK * 2), &full[s]);
                 }
             }
-            if (!alive)  // copies that are still under way write shared memory
+            // Copies that are still under way write shared memory.  (The producers may not come as far as to complete these phases;
+            // the copies take microseconds, and this many polls a hundred times as long.)
+            if (!alive)
                 for (uint32_t r = round > STAGES ? round - STAGES : 0; r < round; ++r)
-                    for (int k = 0; k < WAIT_LIMIT && !barrier_poll(&b_full[r % STAGES], r / STAGES & 1); ++k) {}
+                    for (int k = 0; k < 1 << 14 && !barrier_poll(&full[r % STAGES], r / STAGES & 1); ++k) {}
         }
     }
     __syncwarp();
@@ -1091,13 +1095,13 @@ void set_out(Tiles<T> &t, void *out, int64_t width, size_t item) {
 
 template <typename T>
 size_t packed_bytes(int64_t N, int64_t K) {
-    using S = Shape<T, FORWARD>;  // (and INPUT)
+    using S = Tile<T, FORWARD>;  // (and INPUT)
     return (size_t)ceil_div(N, S::BN) * (size_t)ceil_div(K, S::BK) * S::PLANES * S::B_PLANE;
 }
 
 template <typename T, int FORM, bool WHOLE, bool MANY>
 int launch_as(const Tiles<T> &t, cudaStream_t stream) {
-    using S = Shape<T, FORM>;
+    using S = Shape<T, FORM, WHOLE>;
     CGNN_CUDA(cudaFuncSetAttribute(tile_kernel<T, FORM, WHOLE, MANY>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SHARED));
     tile_kernel<T, FORM, WHOLE, MANY><<<(unsigned)std::min(t.items, SMS), THREADS, S::SHARED, stream>>>(t);
     CGNN_LAUNCH_CHECK();
@@ -1106,22 +1110,23 @@ int launch_as(const Tiles<T> &t, cudaStream_t stream) {
 
 template <typename T, int FORM>
 int launch(Tiles<T> &t, int64_t splits, cudaStream_t stream) {
-    const int64_t tiles_m = ceil_div(t.M, BM), tiles_n = ceil_div(t.N, Shape<T, FORM>::BN);
+    const int64_t tiles_m = ceil_div(t.M, BM), tiles_n = ceil_div(t.N, Tile<T, FORM>::BN);
     CGNN_REQUIRE(tiles_m * tiles_n * splits < (1ll << 30), "linear: too many tiles");
     t.tiles_m = (int)tiles_m;
     t.tiles_n = (int)tiles_n;
     t.items = (int)(tiles_m * tiles_n * splits);
-    constexpr int VECTOR = 16 / sizeof(T);
-    const bool whole = whole_rows(t.a, t.a_stride, sizeof(T), VECTOR) && (FORM != WEIGHT || whole_rows(t.b, t.b_stride, sizeof(T), VECTOR));
-    if constexpr (Shape<T, FORM>::SPLIT)
-        if (t.k_per_item > Shape<T, FORM>::SEGMENT * Shape<T, FORM>::BK)
+    // (fp32 units are loaded at once, and are there or not)
+    const bool whole = whole_rows(t.a, t.a_stride, sizeof(T)) && (FORM != WEIGHT || whole_rows(t.b, t.b_stride, sizeof(T))) &&
+                       (!Tile<T, FORM>::SPLIT || ((FORM == WEIGHT ? t.M : t.K) % 8 == 0 && (FORM != WEIGHT || t.N % 8 == 0)));
+    if constexpr (Tile<T, FORM>::SPLIT)
+        if (t.k_per_item > Tile<T, FORM>::SEGMENT * Tile<T, FORM>::BK)
             return whole ? launch_as<T, FORM, true, true>(t, stream) : launch_as<T, FORM, false, true>(t, stream);
     return whole ? launch_as<T, FORM, true, false>(t, stream) : launch_as<T, FORM, false, false>(t, stream);
 }
 
 template <typename T, int FORM>
 int pack(const T *weight, int64_t in, int64_t N, int64_t K, uint8_t *packed, cudaStream_t stream) {
-    using S = Shape<T, FORM>;
+    using S = Tile<T, FORM>;
     const int64_t chunks = ceil_div(K, S::BK), units = ceil_div(N, S::BN) * S::BN * chunks * (S::BK / 8);
     pack_kernel<T, FORM><<<(unsigned)ceil_div(units, 256), 256, 0, stream>>>(weight, in, N, K, chunks, packed,
                                                                               whole_rows(weight, in, sizeof(T)));
@@ -1162,7 +1167,7 @@ int tiles_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T
 // Splits of the rows of a weight gradient: what gives every multiprocessor one item, and none of fewer than four chunks.
 template <typename T>
 static int64_t weight_splits(int64_t rows, int64_t in, int64_t out, int64_t *rows_per_split) {
-    using S = Shape<T, WEIGHT>;
+    using S = Tile<T, WEIGHT>;
     const int64_t tiles = ceil_div(out, BM) * ceil_div(in, S::BN);
     const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>(SMS / tiles, rows / (8 * S::BK)));
     *rows_per_split = ceil_div(ceil_div(rows, wanted), S::BK) * S::BK;
