@@ -49,15 +49,15 @@ struct Shape {
     static constexpr int A_PLANE = BM * BK * 2, B_PLANE = BN * BK * 2;
     static constexpr int STAGE = PLANES * (A_PLANE + B_PLANE);
     static constexpr int STAGES = !SPLIT && FORM == WEIGHT ? 7 : 4;
-    static constexpr int AHEAD = FORM == WEIGHT ? 5 : 2;
+    static constexpr int AHEAD = FORM == WEIGHT ? 2 : 1;  // of a group's own chunks
     static constexpr int SEGMENT = SPLIT ? 256 / BK : 1 << 30;  // chunks of BK that an accumulator takes
-    static constexpr int GROUPS = ASYNC ? 1 : 2, MEMBERS = PRODUCERS / GROUPS;  // producers that fill a stage
+    static constexpr int GROUPS = SPLIT && FORM == WEIGHT ? 1 : 2, MEMBERS = PRODUCERS / GROUPS;  // producers that fill a stage
     static constexpr int A_UNITS = BM * BK / 8 / MEMBERS, B_UNITS = FORM == WEIGHT ? BN * BK / 8 / MEMBERS : 0;
     static constexpr int MASK_SLOT = ASYNC && FORM != FORWARD ? A_UNITS * MEMBERS * 4 : 0;  // a word of the mask for each unit
     static constexpr int STAGING = EPILOGUE_WARPS * 32 * (PIECE + 1) * 4;
     static constexpr int SUMS = FORM == WEIGHT ? 16 * BM * 4 : 0;  // of the columns
     static constexpr int SHARED = STAGES * (STAGE + MASK_SLOT) + STAGING + SUMS + 1024;
-    static_assert(SHARED + (FORM == FORWARD ? 2048 : 512) <= 232448 && (SPLIT || AHEAD + 1 < STAGES), "a block has 227 KB");
+    static_assert(SHARED + (FORM == FORWARD ? 2048 : 512) <= 232448 && (SPLIT || 2 * (AHEAD + 1) <= STAGES), "a block has 227 KB");
 };
 // What does not depend on the way of the operands.
 template <typename T, int FORM>
@@ -648,6 +648,11 @@ struct Producer {
             a_left -= BK;
         }
     }
+    // The group's next chunk.
+    __device__ __forceinline__ void next_own() {
+        next();
+        if (S::GROUPS == 2 && more()) next();
+    }
     // Where a unit of A or B lies in a plane.
     __device__ __forceinline__ uint32_t a_place(int u) const {
         return FORM == WEIGHT ? p % A_ACROSS / 8 * (BK * 128) + place<128>(p / A_ACROSS + u * A_DOWN, p % 8)
@@ -673,7 +678,7 @@ struct Producer {
             const int left = u * B_DOWN < b_rows ? max(0, b_left) : 0;
             copy16(stage + S::A_PLANE + b_place(u), left > 0 ? b + u * b_step : t.b, min(left * (int)sizeof(T), 16));
         }
-        next();
+        next_own();
     }
     // The next chunk of the group by loads.
     __device__ __forceinline__ void load(Unit<T> (&x)[S::A_UNITS + S::B_UNITS], uint32_t (&keep)[S::A_UNITS]) {
@@ -698,8 +703,7 @@ struct Producer {
             if constexpr (WHOLE && S::SPLIT) x[S::A_UNITS + u].load_or_clear(b + u * b_step, left > 0);
             else x[S::A_UNITS + u].load(b + u * b_step, left);
         }
-        next();
-        if (S::GROUPS == 2 && more()) next();
+        next_own();
     }
     __device__ __forceinline__ void add_columns(const Unit<T> (&x)[S::A_UNITS + S::B_UNITS], float (&columns)[8]) const {
         float sum[8];
@@ -779,7 +783,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             // (the copies of the weight's images report to the same barrier as whatever fills the rest of the stage)
-            barrier_init(&full[s], (direct ? PRODUCERS : S::MEMBERS / 32) + (FORM == WEIGHT ? 0 : 1));
+            barrier_init(&full[s], (direct ? S::MEMBERS : S::MEMBERS / 32) + (FORM == WEIGHT ? 0 : 1));
             barrier_init(&empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -888,7 +892,8 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
 #pragma unroll
         for (int k = 0; k < 8; ++k) columns[k] = 0.f;
         Producer<T, FORM, WHOLE> ahead(t, p);
-        uint32_t s = 0, parity = 1;  // of the stage that is filled next
+        if (group == 1 && ahead.more()) ahead.next();
+        uint32_t s = group, parity = 1;  // of the stage that the group fills next
         bool alive = true;
         int item = blockIdx.x, chunk = 0, chunks = chunks_of<T, FORM>(t, item);
         const auto await = [&] {
@@ -900,7 +905,8 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
             if (lane == 0) barrier_arrive(&full[stage]);
         };
         const auto step = [&] {
-            if (++s == STAGES) s = 0, parity ^= 1;
+            s += S::GROUPS;
+            if (s >= STAGES) s -= STAGES, parity ^= 1;
         };
         // A chunk of the present item is done.  (To the end of all items whatever happens: the barriers here want every thread.)
         const auto done = [&] {
@@ -938,22 +944,30 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
                     step();
                 }
             } else {
-                int begun = 0;        // chunks on their way
-                uint32_t arrived = 0; // the stage of the first of them
-                while (item < t.items) {
+                const auto issue = [&] {
                     if (ahead.more() && alive) {
                         await();
                         if (alive) ahead.issue(shared_address(stages) + s * S::STAGE, shared_address(masks) + s * S::MASK_SLOT);
                         step();
                     }
                     copies_end();
-                    if (++begun <= S::AHEAD) continue;
-                    copies_wait<S::AHEAD>();
-                    if (alive) {
-                        ahead.mend(stages + arrived * S::STAGE, masks + arrived * S::MASK_SLOT, columns);
-                        filled(arrived);
+                };
+#pragma unroll
+                for (int d = 0; d < S::AHEAD; ++d) issue();
+                uint32_t arrived = group;  // the stage of the first chunk on its way
+                int turn = 0;              // of the group whose chunk it is
+                while (item < t.items) {
+                    if (turn == group) {
+                        issue();
+                        copies_wait<S::AHEAD>();
+                        if (alive) {
+                            ahead.mend(stages + arrived * S::STAGE, masks + arrived * S::MASK_SLOT, columns);
+                            filled(arrived);
+                        }
+                        arrived += S::GROUPS;
+                        if (arrived >= STAGES) arrived -= STAGES;
                     }
-                    if (++arrived == STAGES) arrived = 0;
+                    turn ^= 1;
                     done();
                 }
             }
@@ -961,9 +975,8 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
         } else {
             Unit<T> x[S::A_UNITS + S::B_UNITS];
             uint32_t keep[S::A_UNITS];
-            if (group == 1 && ahead.more()) ahead.next();
             ahead.load(x, keep);
-            int turn = 0;  // of the group whose chunk it is
+            int turn = 0;
             while (item < t.items) {
                 if (turn == group) {
                     await();
@@ -972,9 +985,9 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
                         filled(s);
                         ahead.load(x, keep);
                     }
+                    step();
                 }
-                turn ^= 1;
-                step();
+                if (S::GROUPS == 2) turn ^= 1;
                 done();
             }
         }
