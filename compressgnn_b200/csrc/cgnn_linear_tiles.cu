@@ -666,17 +666,44 @@ struct Producer {
 
     // The next chunk on its way to its stage (16 bits), the mask's words to theirs.
     __device__ __forceinline__ void issue(uint32_t stage, uint32_t masks) {
+        // (Instructions bound this: chunks whose rows are all there, nearly all, go without a look at each unit.)
+        constexpr int WHOLE_ROWS = FORM == WEIGHT ? BK : BM;
+        const int bytes = min(max(0, a_left) * (int)sizeof(T), 16);
+        if (rows >= WHOLE_ROWS) {
+            const T *from = bytes ? a : t.a;
+            const int64_t down = bytes ? a_step : 0;
 #pragma unroll
-        for (int u = 0; u < S::A_UNITS; ++u) {
-            const int left = u * A_DOWN < rows ? max(0, a_left) : 0;
-            copy16(stage + a_place(u), left > 0 ? a + u * a_step : t.a, min(left * (int)sizeof(T), 16));
-            if constexpr (FORM != FORWARD)
-                if (masked) copy4(masks + (u * MEMBERS + p) * 4, left > 0 ? mask + u * mask_step : t.mask, left > 0);
+            for (int u = 0; u < S::A_UNITS; ++u, from += down) copy16(stage + a_place(u), from, bytes);
+            if constexpr (FORM != FORWARD) {
+                const uint8_t *word = bytes ? mask : t.mask;
+                const int64_t word_down = bytes ? mask_step : 0;
+                if (masked)
+#pragma unroll
+                    for (int u = 0; u < S::A_UNITS; ++u, word += word_down) copy4(masks + (u * MEMBERS + p) * 4, word, bytes != 0);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < S::A_UNITS; ++u) {
+                const int there = u * A_DOWN < rows ? bytes : 0;
+                copy16(stage + a_place(u), there ? a + u * a_step : t.a, there);
+                if constexpr (FORM != FORWARD)
+                    if (masked) copy4(masks + (u * MEMBERS + p) * 4, there ? mask + u * mask_step : t.mask, there != 0);
+            }
         }
+        if constexpr (FORM == WEIGHT) {
+            const int b_bytes = min(max(0, b_left) * (int)sizeof(T), 16);
+            if (b_rows >= WHOLE_ROWS) {
+                const T *from = b_bytes ? b : t.b;
+                const int64_t down = b_bytes ? b_step : 0;
 #pragma unroll
-        for (int u = 0; u < S::B_UNITS; ++u) {
-            const int left = u * B_DOWN < b_rows ? max(0, b_left) : 0;
-            copy16(stage + S::A_PLANE + b_place(u), left > 0 ? b + u * b_step : t.b, min(left * (int)sizeof(T), 16));
+                for (int u = 0; u < S::B_UNITS; ++u, from += down) copy16(stage + S::A_PLANE + b_place(u), from, b_bytes);
+            } else {
+#pragma unroll
+                for (int u = 0; u < S::B_UNITS; ++u) {
+                    const int there = u * B_DOWN < b_rows ? b_bytes : 0;
+                    copy16(stage + S::A_PLANE + b_place(u), there ? b + u * b_step : t.b, there);
+                }
+            }
         }
         next_own();
     }
@@ -813,11 +840,13 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         const int quarter = warp & 3, half = warp >> 2;
         Finish<T, FORM> finish(t, staging + warp * 32 * (PIECE + 1), bias_of_tile[half], lane);
         uint32_t segment = 0;
+        [[maybe_unused]] int64_t bias_n0 = -1;  // whose bias is there
         for (int item = blockIdx.x; item < t.items; item += gridDim.x) {
             const Item i = item_of<T, FORM>(t, item);
             const int64_t m0 = i.m0 + quarter * 32, n0 = i.n0 + half * COLUMNS;
-            if (FORM == FORWARD && t.epilogue.bias != nullptr) {
+            if (FORM == FORWARD && t.epilogue.bias != nullptr && n0 != bias_n0) {
                 // the half's columns, by the four warps of the half
+                bias_n0 = n0;
                 asm volatile("bar.sync %0, %1;" ::"r"(1 + half), "n"(EPILOGUE_WARPS / 2 * 32) : "memory");
                 for (int c = quarter * 32 + lane; c < COLUMNS; c += EPILOGUE_WARPS / 2 * 32)
                     bias_of_tile[half][c] = n0 + c < t.N ? widen(t.epilogue.bias[n0 + c]) : 0.f;
