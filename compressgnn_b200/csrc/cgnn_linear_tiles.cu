@@ -45,15 +45,15 @@ struct Shape {
     static constexpr bool ASYNC = WHOLE && !SPLIT;
     static constexpr int PLANES = SPLIT ? 3 : 1;
     static constexpr int BN = SPLIT ? 128 : 256;
-    static constexpr int BK = SPLIT || FORM == WEIGHT ? 32 : 64;
+    static constexpr int BK = SPLIT || (FORM == WEIGHT && !WHOLE) ? 32 : 64;
     static constexpr int A_PLANE = BM * BK * 2, B_PLANE = BN * BK * 2;
     static constexpr int STAGE = PLANES * (A_PLANE + B_PLANE);
-    static constexpr int STAGES = !SPLIT && FORM == WEIGHT ? 7 : 4;
-    static constexpr int AHEAD = FORM == WEIGHT ? 2 : 1;  // of a group's own chunks
+    static constexpr int STAGES = SPLIT || FORM != WEIGHT || WHOLE ? 4 : 7;
+    static constexpr int AHEAD = 1;  // of a group's own chunks
     static constexpr int SEGMENT = SPLIT ? 256 / BK : 1 << 30;  // chunks of BK that an accumulator takes
     static constexpr int GROUPS = SPLIT && FORM == WEIGHT ? 1 : 2, MEMBERS = PRODUCERS / GROUPS;  // producers that fill a stage
     static constexpr int A_UNITS = BM * BK / 8 / MEMBERS, B_UNITS = FORM == WEIGHT ? BN * BK / 8 / MEMBERS : 0;
-    static constexpr int MASK_SLOT = ASYNC && FORM != FORWARD ? A_UNITS * MEMBERS * 4 : 0;  // a word of the mask for each unit
+    static constexpr int MASK_SLOT = ASYNC && FORM != FORWARD ? A_UNITS * MEMBERS : 0;  // a word of the mask for four units of a row
     static constexpr int STAGING = EPILOGUE_WARPS * 32 * (PIECE + 1) * 4;
     static constexpr int SUMS = FORM == WEIGHT ? 16 * BM * 4 : 0;  // of the columns
     static constexpr int SHARED = STAGES * (STAGE + MASK_SLOT) + STAGING + SUMS + 1024;
@@ -359,14 +359,15 @@ __device__ __forceinline__ Item item_of(const Tiles<T> &t, int item) {
     i.k1 = min(t.K, i.k0 + t.k_per_item);
     return i;
 }
-template <typename T, int FORM>
+template <typename T, int FORM, bool WHOLE>
 __device__ __forceinline__ int chunks_of(const Tiles<T> &t, int item) {
+    using S = Shape<T, FORM, WHOLE>;
     int64_t k = t.K;
     if (FORM == WEIGHT) {
         const int64_t k0 = item / (t.tiles_m * t.tiles_n) * t.k_per_item;
         k = min(k, k0 + t.k_per_item) - k0;
     }
-    return (int)((k + Tile<T, FORM>::BK - 1) / Tile<T, FORM>::BK);
+    return (int)((k + S::BK - 1) / S::BK);
 }
 
 // One element by fp32 arithmetic: where an operand is infinite, no number or beyond bf16's range, its parts say nothing.
@@ -613,7 +614,7 @@ struct Producer {
         if (item >= t.items) return;
         const Item i = item_of<T, FORM>(t, item);
         chunk = 0;
-        chunks = chunks_of<T, FORM>(t, item);
+        chunks = chunks_of<T, FORM, WHOLE>(t, item);
         if constexpr (FORM == WEIGHT) {
             const int64_t row = i.k0 + p / A_ACROSS, column = i.m0 + p % A_ACROSS * 8;
             const int64_t b_row = i.k0 + p / B_ACROSS, b_column = i.n0 + p % B_ACROSS * 8;
@@ -677,9 +678,9 @@ struct Producer {
             if constexpr (FORM != FORWARD) {
                 const uint8_t *word = bytes ? mask : t.mask;
                 const int64_t word_down = bytes ? mask_step : 0;
-                if (masked)
+                if (masked && p % 4 == 0)
 #pragma unroll
-                    for (int u = 0; u < S::A_UNITS; ++u, word += word_down) copy4(masks + (u * MEMBERS + p) * 4, word, bytes != 0);
+                    for (int u = 0; u < S::A_UNITS; ++u, word += word_down) copy4(masks + u * MEMBERS + p, word, bytes != 0);
             }
         } else {
 #pragma unroll
@@ -687,7 +688,7 @@ struct Producer {
                 const int there = u * A_DOWN < rows ? bytes : 0;
                 copy16(stage + a_place(u), there ? a + u * a_step : t.a, there);
                 if constexpr (FORM != FORWARD)
-                    if (masked) copy4(masks + (u * MEMBERS + p) * 4, there ? mask + u * mask_step : t.mask, there != 0);
+                    if (masked && p % 4 == 0) copy4(masks + u * MEMBERS + p, there ? mask + u * mask_step : t.mask, there != 0);
             }
         }
         if constexpr (FORM == WEIGHT) {
@@ -772,13 +773,14 @@ struct Producer {
         if constexpr (FORM != FORWARD) {
             const bool summed = FORM == WEIGHT && t.column_sums != nullptr;
             if (!masked && !summed) return;
+            __syncwarp();  // a word of the mask was copied by one of four
             Unit<T> x[S::A_UNITS + S::B_UNITS];
 #pragma unroll
             for (int u = 0; u < S::A_UNITS; ++u) {
                 T *const at = reinterpret_cast<T *>(stage + a_place(u));
                 x[u].load_whole(at);
                 if (masked) {
-                    x[u].keep(bits_of(*reinterpret_cast<const uint32_t *>(masks + (u * MEMBERS + p) * 4)));
+                    x[u].keep(bits_of(*reinterpret_cast<const uint32_t *>(masks + u * MEMBERS + p / 4 * 4)));
                     uint4 planes[S::PLANES];
                     x[u].planes(planes);
                     store_shared(shared_address(at), planes[0]);
@@ -874,7 +876,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 ++segment;
             };
             int before = 0;  // segments ahead of the last
-            if constexpr (MANY) before = (chunks_of<T, FORM>(t, item) - 1) / S::SEGMENT;
+            if constexpr (MANY) before = (chunks_of<T, FORM, WHOLE>(t, item) - 1) / S::SEGMENT;
             if (before == 0) {
                 const uint32_t buffer = await();
 #pragma unroll 1
@@ -924,7 +926,7 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
         if (group == 1 && ahead.more()) ahead.next();
         uint32_t s = group, parity = 1;  // of the stage that the group fills next
         bool alive = true;
-        int item = blockIdx.x, chunk = 0, chunks = chunks_of<T, FORM>(t, item);
+        int item = blockIdx.x, chunk = 0, chunks = chunks_of<T, FORM, WHOLE>(t, item);
         const auto await = [&] {
             if (alive) alive = __all_sync(0xffffffffu, barrier_wait(&empty[s], parity, polls, &given_up));
         };
@@ -960,7 +962,7 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
             }
             chunk = 0;
             item += gridDim.x;
-            if (FORM == WEIGHT && item < t.items) chunks = chunks_of<T, FORM>(t, item);
+            if (FORM == WEIGHT && item < t.items) chunks = chunks_of<T, FORM, WHOLE>(t, item);
         };
         if constexpr (S::ASYNC) {
             if (direct) {
@@ -1035,10 +1037,10 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
             const bool leads = leader_of_warp();
             uint32_t s = 0, parity = 0, buffer = 0, buffer_parity = 1, issued = 0;
             bool alive = true;
-            int chunks = chunks_of<T, FORM>(t, blockIdx.x);
+            int chunks = chunks_of<T, FORM, WHOLE>(t, blockIdx.x);
             for (int item = blockIdx.x; alive && item < t.items; item += gridDim.x) {
                 const int64_t n0 = item_of<T, FORM>(t, item).n0;
-                if (FORM == WEIGHT) chunks = chunks_of<T, FORM>(t, item);
+                if (FORM == WEIGHT) chunks = chunks_of<T, FORM, WHOLE>(t, item);
                 const int columns = (int)min((int64_t)BN, (t.N - n0 + 15) / 16 * 16);
                 const uint32_t descriptor = base | (uint32_t)(columns / 8) << 17;
                 int of_segment = 0;
@@ -1092,7 +1094,7 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
             // -------------------------------------------------------------- the weight's images
             uint32_t round = 0;
             bool alive = true;
-            const int chunks = chunks_of<T, FORM>(t, 0);
+            const int chunks = chunks_of<T, FORM, WHOLE>(t, 0);
             for (int item = blockIdx.x; alive && item < t.items; item += gridDim.x) {
                 const int64_t n0 = item_of<T, FORM>(t, item).n0;
                 const uint32_t rows = (uint32_t)min((int64_t)BN, (t.N - n0 + 15) / 16 * 16);
