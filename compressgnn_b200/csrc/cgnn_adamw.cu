@@ -195,40 +195,64 @@ __device__ __forceinline__ int scale_exponent(uint32_t largest_bits) {
 }
 __device__ __forceinline__ float power_of_two(int exponent) { return __uint_as_float((uint32_t)(exponent + 127) << 23); }
 
-// |size| (at most 448) rounded to an e4m3 number, up with the probability that 16 random bits allow: a normal number loses
-// the lower 20 bits of its fraction after they were added to, one below 2^-6 is a multiple of 2^-9.
-// What is not finite becomes NaN.
-__device__ __forceinline__ float rounded_up_or_down(float size, uint32_t random16) {
-    const uint32_t bits = __float_as_uint(size);
-    const float upper = __uint_as_float((bits + (random16 << 4)) & 0xfff00000u);
-    const float lower = __fmul_rn(floorf(__fadd_rn(__fmul_rn(size, 512.f), __fmul_rn((float)random16, 1.f / 65536.f))), 1.f / 512.f);
-    const float rounded = bits >= 0x3c800000u ? upper : lower;
-    return bits > 0x43e00000u ? __uint_as_float(0x7fffffffu) : rounded;
-}
-
-// Four values as codes; at_least: what a value above zero is not rounded below.
-__device__ __forceinline__ uint32_t codes_of(const float (&x)[4], float inverse, const uint32_t (&random16)[4], float at_least) {
+// Four values as codes: |x| * inverse, at most 448, rounded to an e4m3 number, up with the probability that 16 random bits
+// allow.  A normal number loses the lower 20 bits of its fraction after they were added to, one below 2^-6 is a multiple of
+// 2^-9.  ROOT: a value above zero is not rounded to zero.  `plain`: every value of the warp is finite; others become NaN.
+template <bool ROOT>
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[4], float inverse, const uint32_t (&random16)[4], bool plain) {
     uint32_t codes = 0;
+    float rounded[4];
+    bool small = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float size = __fmul_rn(fabsf(x[k]), inverse);
+        small = small || size < 1.f / 64.f;
+        rounded[k] = __uint_as_float((__float_as_uint(size) + (random16[k] << 4)) & 0xfff00000u);
+    }
+    if (small || !plain) {  // few blocks have such values
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float size = __fmul_rn(fabsf(x[k]), inverse);
+            if (size < 1.f / 64.f) {
+                const float steps = floorf(__fadd_rn(__fmul_rn(size, 512.f), __fmul_rn((float)random16[k], 1.f / 65536.f)));
+                rounded[k] = __fmul_rn(ROOT && size > 0.f ? fmaxf(steps, 1.f) : steps, 1.f / 512.f);
+            }
+            if (__float_as_uint(size) > 0x43e00000u) rounded[k] = __uint_as_float(0x7fffffffu);
+        }
+    }
 #pragma unroll
     for (int k = 0; k < 4; k += 2) {
-        float2 two;
-        float *const y = &two.x;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float size = __fmul_rn(fabsf(x[k + j]), inverse);
-            float r = rounded_up_or_down(size, random16[k + j]);
-            if (at_least > 0.f && size > 0.f && r < at_least) r = at_least;
-            y[j] = copysignf(r, x[k + j]);
-        }
+        const float2 two = ROOT ? make_float2(rounded[k], rounded[k + 1])
+                                : make_float2(copysignf(rounded[k], x[k]), copysignf(rounded[k + 1], x[k + 1]));
         codes |= (uint32_t)__nv_cvt_float2_to_fp8x2(two, __NV_SATFINITE, __NV_E4M3) << (8 * k);
     }
     return codes;
 }
 
-__device__ __forceinline__ uint32_t finite_bits(float x) {
-    const uint32_t bits = __float_as_uint(x) & 0x7fffffffu;
-    return bits < 0x7f800000u ? bits : 0u;
+__device__ __forceinline__ uint32_t size_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t size_bits(double) { return 0u; }
+// The largest of a block's eight values a lane, of the finite ones where there are others.
+__device__ __forceinline__ uint32_t largest_of(const float (&x)[2][4], bool &plain) {
+    uint32_t largest = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) largest = max(largest, size_bits(x[e / 4][e % 4]));
+    largest = __reduce_max_sync(0xffffffffu, largest);
+    if (largest >= 0x7f800000u) {
+        plain = false;
+        largest = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t bits = size_bits(x[e / 4][e % 4]);
+            largest = max(largest, bits < 0x7f800000u ? bits : 0u);
+        }
+        largest = __reduce_max_sync(0xffffffffu, largest);
+    }
+    return largest;
 }
+
+// (The quotient goes into the parameter only, whose rounding is far above its two last bits.)
+__device__ __forceinline__ float quotient(float a, float b) { return __fdividef(a, b); }
+__device__ __forceinline__ double quotient(double a, double b) { return a / b; }
 
 template <typename T, bool EIGHT, int CAP>
 __global__ void __launch_bounds__(ADAM_THREADS) adamw_kernel(const __grid_constant__ Table<CAP> table, const Step set) {
@@ -305,7 +329,6 @@ __global__ void __launch_bounds__(ADAM_THREADS) adamw_kernel(const __grid_consta
             }
         }
         A root[2][4];
-        uint32_t largest_m = 0, largest_r = 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -314,25 +337,21 @@ __global__ void __launch_bounds__(ADAM_THREADS) adamw_kernel(const __grid_consta
                 m[u][k] = plus(times(m[u][k], b1), times(gk, c1));
                 v[u][k] = plus(times(v[u][k], b2), times(times(gk, gk), c2));
                 root[u][k] = root_of(v[u][k]);
-                p[u][k] = plus(times(p[u][k], keep), times(rate, m[u][k] / plus(times(root[u][k], inverse_root2), eps)));
-                if constexpr (EIGHT) {
-                    largest_m = max(largest_m, finite_bits(m[u][k]));
-                    largest_r = max(largest_r, finite_bits(root[u][k]));
-                }
+                p[u][k] = plus(times(p[u][k], keep), times(rate, quotient(m[u][k], plus(times(root[u][k], inverse_root2), eps))));
             }
 #pragma unroll
         for (int u = 0; u < 2; ++u) store4<T>(static_cast<T *>(e.param), whole, at[u], e.n, p[u]);
         if constexpr (EIGHT) {
-            const int m_exponent = scale_exponent(__reduce_max_sync(0xffffffffu, largest_m));
-            const int r_exponent = scale_exponent(__reduce_max_sync(0xffffffffu, largest_r));
+            bool plain = true;
+            const int m_exponent = scale_exponent(largest_of(m, plain)), r_exponent = scale_exponent(largest_of(root, plain));
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const uint4 w = words((uint64_t)at[u] >> 2);
                 const uint32_t low[4] = {w.x & 0xffffu, w.y & 0xffffu, w.z & 0xffffu, w.w & 0xffffu};
                 const uint32_t high[4] = {w.x >> 16, w.y >> 16, w.z >> 16, w.w >> 16};
-                store_codes(static_cast<uint8_t *>(e.first), whole, at[u], e.n, codes_of(m[u], power_of_two(-m_exponent), low, 0.f));
+                store_codes(static_cast<uint8_t *>(e.first), whole, at[u], e.n, codes_of<false>(m[u], power_of_two(-m_exponent), low, plain));
                 store_codes(static_cast<uint8_t *>(e.second), whole, at[u], e.n,
-                            codes_of(root[u], power_of_two(-r_exponent), high, 1.f / 512.f));
+                            codes_of<true>(root[u], power_of_two(-r_exponent), high, plain));
             }
             if (lane == 0) {
                 e.first_scale[group] = power_of_two(m_exponent);

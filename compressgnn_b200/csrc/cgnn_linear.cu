@@ -220,11 +220,17 @@ int small_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
 template <typename T>
 constexpr bool HAS_TILES = sizeof(T) < 8;
 
-// Whether a call goes to the tensor cores: from 3e8 multiplications (fp32) and 8e7 (16 bits) on.  Us by tiles / by single
-// elements: fp32 forward 10,000 x 256 -> 128 25 / 37, 10,000 x 128 -> 64 21 / 14; bf16 10,000 x 128 -> 64 13 / 16, 40,000 x
-// 64 -> 64 19 / 21, 10,000 x 64 -> 64 12 / 11.
+// Whether a call goes to the tensor cores: by its number of multiplications, earlier where rows are whole vectors and where one
+// contraction is long (a tile of single elements takes it alone).  Us by tiles / by single elements, forward + input gradient +
+// weight gradient: fp32 10,000 x 64 -> 64 (4e7) 47 / 48, 20,000 x 64 -> 64 54 / 64, 2708 x 64 -> 64 46 / 38;
+// 40,000 x 64 -> 47 (1e8) 72 / 92, 20,000 x 64 -> 47 60 / 61; 32 x 4096 -> 64 112 / 195;
+// bf16 2708 x 64 -> 64 (1e7) 38 / 40, 1024 x 64 -> 64 38 / 40, 256 x 64 -> 64 30 / 37; 20,000 x 64 -> 47 (6e7) 70 / 66.
 bool by_tiles(int dtype, int64_t rows, int64_t in, int64_t out) {
-    return dtype != CGNN_F64 && in > 0 && (double)rows * (double)in * (double)out >= (dtype == CGNN_F32 ? 3e8 : 8e7);
+    if (dtype == CGNN_F64 || in <= 0) return false;
+    const double products = (double)rows * (double)in * (double)out;
+    const bool whole = in % 8 == 0 && out % 8 == 0;
+    if (std::max(in, out) >= 1024 && products >= 4e6) return true;
+    return products >= (dtype == CGNN_F32 ? (whole ? 4e7 : 1e8) : whole ? 4e6 : 6e7);
 }
 
 std::atomic<int> wait_limit{WAIT_LIMIT};
