@@ -178,6 +178,19 @@ __device__ __forceinline__ void tmem_load16(uint32_t address, float (&v)[16]) {
         for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
     }
 }
+// Thirty-two columns of one accumulator.
+__device__ __forceinline__ void tmem_load32(uint32_t address, float (&v)[2][16]) {
+    uint32_t r[16], q[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : CGNN_SIXTEEN(r), CGNN_SIXTEEN(q)
+        : "r"(address), "r"(address + 16)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[0][i] = __uint_as_float(r[i]), v[1][i] = __uint_as_float(q[i]);
+}
 // Eight columns, with the small products'.
 __device__ __forceinline__ void tmem_load8(uint32_t address, float (&v)[8]) {
     uint32_t r[8], q[8];
@@ -435,7 +448,7 @@ __device__ __forceinline__ void store16(T *p, int left, bool wide, const float (
 // The epilogue of one warp: 32 rows, a row a lane as they lie in the accumulators, PIECE columns at a time.  Rows of whole vectors are
 // read and written by their lane, a sector or two at once; of others the results go through shared memory, from where
 // neighbouring lanes take neighbouring columns.
-template <typename T, int FORM>
+template <typename T, int FORM, bool DROP>
 struct Finish {
     const Tiles<T> &t;
     float *const staging;  // [32][PIECE + 1]
@@ -449,7 +462,7 @@ struct Finish {
 
     __device__ __forceinline__ Finish(const Tiles<T> &t_, float *staging_, const float *bias_, int lane_)
         : t(t_), staging(staging_), bias(bias_), lane(lane_),
-          words(FORM == FORWARD && t_.epilogue.drop.threshold ? t_.epilogue.drop.key() : 0) {}
+          words(DROP ? t_.epilogue.drop.key() : 0) {}
 
     __device__ __forceinline__ void begin(int64_t m0, int64_t n0_) {
         m = m0 + lane;
@@ -516,8 +529,8 @@ struct Finish {
                         through &= ~(1u << k);
                     }
             }
-            const uint32_t threshold = t.epilogue.drop.threshold;
-            if (threshold) {
+            if constexpr (DROP) {
+                const uint32_t threshold = t.epilogue.drop.threshold;
                 const float scale = (float)t.epilogue.drop.scale;
                 const uint64_t block = (uint64_t)(first + c) >> 2;
                 const int ahead = (int)((first + c) & 3);  // not zero: the rows do not begin with a block of words
@@ -791,8 +804,9 @@ struct Producer {
     }
 };
 
-// MANY: fp32 contractions of more than one segment, whose sums take registers that the others keep.
-template <typename T, int FORM, bool WHOLE, bool MANY>
+// MANY: fp32 contractions of more than one segment, whose sums take registers that the others keep.  DROP: a forward pass with
+// dropout, whose instructions the others do without (they are read again for every sixteen columns).
+template <typename T, int FORM, bool WHOLE, bool MANY, bool DROP>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ Tiles<T> t) {
     using S = Shape<T, FORM, WHOLE>;
     constexpr int BN = S::BN, BK = S::BK, STAGES = S::STAGES, PLANES = S::PLANES;
@@ -839,8 +853,11 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         // ------------------------------------------------------------------ accumulators to results
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(EPILOGUE_REGISTERS));
         constexpr int COLUMNS = BN / 2;  // of a warp's half of the tile
+        // Read from the accumulators at once.  (Two pieces make two copies of what follows, which costs more than it gives where that
+        // is much: 2.45 M x 128 -> 256 bf16 forward 712 us for 450, input gradient 314 for 330.)
+        constexpr int TURN = S::SPLIT || FORM == FORWARD ? PIECE : 2 * PIECE;
         const int quarter = warp & 3, half = warp >> 2;
-        Finish<T, FORM> finish(t, staging + warp * 32 * (PIECE + 1), bias_of_tile[half], lane);
+        Finish<T, FORM, DROP> finish(t, staging + warp * 32 * (PIECE + 1), bias_of_tile[half], lane);
         uint32_t segment = 0;
         [[maybe_unused]] int64_t bias_n0 = -1;  // whose bias is there
         for (int item = blockIdx.x; item < t.items; item += gridDim.x) {
@@ -880,12 +897,19 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             if (before == 0) {
                 const uint32_t buffer = await();
 #pragma unroll 1
-                for (int c = 0; c < COLUMNS; c += PIECE) {
-                    float x[PIECE], added[PIECE];
-                    if (c < pieces_end) finish.fetch(c, added);
-                    if (alive) tmem_load16<S::SPLIT>(rows + buffer * 256 + c, x);
-                    if (c + PIECE == COLUMNS) release(buffer);
-                    if (c < pieces_end) finish.piece(x, added, i, c, alive);
+                for (int c = 0; c < COLUMNS; c += TURN) {
+                    float x[TURN / PIECE][PIECE], added[TURN / PIECE][PIECE];
+#pragma unroll
+                    for (int q = 0; q < TURN / PIECE; ++q)
+                        if (c + q * PIECE < pieces_end) finish.fetch(c + q * PIECE, added[q]);
+                    if (alive) {
+                        if constexpr (TURN == PIECE) tmem_load16<S::SPLIT>(rows + buffer * 256 + c, x[0]);
+                        else tmem_load32(rows + buffer * 256 + c, x);
+                    }
+                    if (c + TURN == COLUMNS) release(buffer);
+#pragma unroll
+                    for (int q = 0; q < TURN / PIECE; ++q)
+                        if (c + q * PIECE < pieces_end) finish.piece(x[q], added[q], i, c + q * PIECE, alive);
                 }
             } else if constexpr (MANY) {
                 float sum[COLUMNS];
@@ -1143,13 +1167,20 @@ size_t packed_bytes(int64_t N, int64_t K) {
     return (size_t)ceil_div(N, S::BN) * (size_t)ceil_div(K, S::BK) * S::PLANES * S::B_PLANE;
 }
 
-template <typename T, int FORM, bool WHOLE, bool MANY>
+template <typename T, int FORM, bool WHOLE, bool MANY, bool DROP>
 int launch_as(const Tiles<T> &t, cudaStream_t stream) {
     using S = Shape<T, FORM, WHOLE>;
-    CGNN_CUDA(cudaFuncSetAttribute(tile_kernel<T, FORM, WHOLE, MANY>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SHARED));
-    tile_kernel<T, FORM, WHOLE, MANY><<<(unsigned)std::min(t.items, SMS), THREADS, S::SHARED, stream>>>(t);
+    auto *const kernel = tile_kernel<T, FORM, WHOLE, MANY, DROP>;
+    CGNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SHARED));
+    kernel<<<(unsigned)std::min(t.items, SMS), THREADS, S::SHARED, stream>>>(t);
     CGNN_LAUNCH_CHECK();
     return CGNN_OK;
+}
+template <typename T, int FORM, bool WHOLE, bool MANY>
+int launch_dropping(const Tiles<T> &t, cudaStream_t stream) {
+    if constexpr (FORM == FORWARD)
+        if (t.epilogue.drop.threshold) return launch_as<T, FORM, WHOLE, MANY, true>(t, stream);
+    return launch_as<T, FORM, WHOLE, MANY, false>(t, stream);
 }
 
 template <typename T, int FORM>
@@ -1164,8 +1195,8 @@ int launch(Tiles<T> &t, int64_t splits, cudaStream_t stream) {
                        (!Tile<T, FORM>::SPLIT || ((FORM == WEIGHT ? t.M : t.K) % 8 == 0 && (FORM != WEIGHT || t.N % 8 == 0)));
     if constexpr (Tile<T, FORM>::SPLIT)
         if (t.k_per_item > Tile<T, FORM>::SEGMENT * Tile<T, FORM>::BK)
-            return whole ? launch_as<T, FORM, true, true>(t, stream) : launch_as<T, FORM, false, true>(t, stream);
-    return whole ? launch_as<T, FORM, true, false>(t, stream) : launch_as<T, FORM, false, false>(t, stream);
+            return whole ? launch_dropping<T, FORM, true, true>(t, stream) : launch_dropping<T, FORM, false, true>(t, stream);
+    return whole ? launch_dropping<T, FORM, true, false>(t, stream) : launch_dropping<T, FORM, false, false>(t, stream);
 }
 
 template <typename T, int FORM>
