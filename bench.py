@@ -933,7 +933,19 @@ def cpu_gcn_epoch(data, width, classes=47, hidden=128, bits=16, epochs=3):
             "sample": f"whole graph, {epochs} epochs after one warm-up epoch (none of them a refresh epoch)"}
 
 
-def measure_gcn(graph, e_orig, steps, warmup, world, rank, device, widths=(16, 64, 256, 1024)):
+GCN_OPTIMIZERS = {"adam": "torch.optim.Adam(lr=1e-3, fused=True)", "adamw": "optim.AdamW(lr=1e-3, weight_decay=0)",
+                  "adamw8": "optim.AdamW(lr=1e-3, weight_decay=0, state_bits=8)"}
+
+
+def gcn_optimizer(name, params):
+    import torch
+    from compressgnn_b200 import optim
+    if name == "adam":
+        return torch.optim.Adam(params, lr=1e-3, fused=True)  # one kernel for all parameters
+    return optim.AdamW(params, lr=1e-3, weight_decay=0.0, state_bits=8 if name == "adamw8" else 32)
+
+
+def measure_gcn(graph, e_orig, steps, warmup, world, rank, device, widths=(16, 64, 256, 1024), optimizer="adam"):
     """Config 5: end-to-end 2-layer GCN with propagation and transformation compression
     (use_transformation=True, H=16, refresh_interval=5) on the config-2 graph (already on `device`),
     47 uniform classes, input feature width swept over 16/64/256/1024.  A step = one training epoch
@@ -956,7 +968,7 @@ def measure_gcn(graph, e_orig, steps, warmup, world, rank, device, widths=(16, 6
         torch.manual_seed(5)
         model = GCN(width, 47, hidden_features=128, param_H=16, dropout=0.3, use_transformation=True,
                     refresh_interval=5, num_layers=2).to(device)
-        opt = torch.optim.Adam(model.parameters(), lr=1e-3, fused=True)  # one kernel for all parameters
+        opt = gcn_optimizer(optimizer, model.parameters())
         # N > 1: column-sharded from 512 input columns up (shares the parameters of `model`), a replica on
         # every rank below that, where the collectives of a sharded epoch cost more than the shards save
         net, sharded = cdist.place_model(model, width, dist.group.WORLD if world > 1 else None)
@@ -1006,7 +1018,7 @@ def measure_gcn(graph, e_orig, steps, warmup, world, rank, device, widths=(16, 6
             "scaling": "strong", "higher_is_better": False, "dtype": "f32", "data": "synthetic",
             "config": {"workload": "gcn: 2-layer GCN, propagation + transformation compression, config-2 graph",
                        "nodes": n, "orig_edges": e_orig, "rules": graph.rule_cnt, "levels": graph.step, "classes": 47,
-                       "hidden": 128, "bits": 16, "refresh_interval": 5, "optimizer": "torch.optim.Adam(lr=1e-3, fused=True)",
+                       "hidden": 128, "bits": 16, "refresh_interval": 5, "optimizer": GCN_OPTIMIZERS[optimizer],
                        "compressor": COMPRESS,
                        "parallelism": f"{world} GPU(s), graph replicated; inputs of 512 columns and more: feature "
                                       "columns of every layer sharded; narrower inputs: one replica per GPU, no "
@@ -1027,7 +1039,7 @@ def run_gcn(args):
         cpu = cpu_gcn_epoch(data, 256)
     graph = data.edge_index
     graph.to(device)
-    report = measure_gcn(graph, e_orig, args.steps, args.warmup, world, rank, device)
+    report = measure_gcn(graph, e_orig, args.steps, args.warmup, world, rank, device, optimizer=args.optimizer)
     if world > 1:
         dist.destroy_process_group()
     if rank != 0:
@@ -1079,6 +1091,7 @@ def main():
     ap.add_argument("--impl", choices=["cgnn", "reference"], default="cgnn")
     ap.add_argument("--workload", choices=sorted(WORKLOADS) + ["cluster", "gcn", "compress", "sample"],
                     default="propagation")
+    ap.add_argument("--optimizer", choices=sorted(GCN_OPTIMIZERS), default="adam", help="of the gcn workload's epochs")
     ap.add_argument("--cluster-nodes", type=int, default=2450000)
     ap.add_argument("--graph", choices=sorted(WORKLOADS), default="propagation",
                     help="graph of the compress and sample workloads")

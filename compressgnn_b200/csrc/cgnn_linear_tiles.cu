@@ -875,6 +875,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         Finish<T, FORM, DROP> finish(t, staging + warp * 32 * (PIECE + 1), bias_of_tile[half], lane);
         uint32_t segment = 0;
         [[maybe_unused]] int64_t bias_n0 = -1;  // whose bias is there
+        bool alive = true;  // A warp that gave up a wait has lost count: it takes nothing and releases nothing from then on.
         for (int item = blockIdx.x; item < t.items; item += gridDim.x) {
             const Item i = item_of<T, FORM>(t, item);
             const int64_t m0 = i.m0 + quarter * 32, n0 = i.n0 + half * COLUMNS;
@@ -894,17 +895,16 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             const uint32_t rows = tmem + ((uint32_t)(quarter * 32) << 16) + half * COLUMNS;
             const int pieces_end = m0 < t.M ? (int)min((int64_t)COLUMNS, t.N - n0) : 0;  // (the same for the warp)
             finish.begin(m0, n0);
-            bool alive = true;
             const auto await = [&] {
                 const uint32_t buffer = segment & 1;
-                alive = __all_sync(0xffffffffu, barrier_wait(&sums_full[buffer], segment >> 1 & 1, polls, &given_up)) && alive;
+                if (alive) alive = __all_sync(0xffffffffu, barrier_wait(&sums_full[buffer], segment >> 1 & 1, polls, &given_up));
                 fence_after();
                 return buffer;
             };
             const auto release = [&](uint32_t buffer) {
                 fence_before();
                 __syncwarp();
-                if (lane == 0) barrier_arrive(&sums_empty[buffer]);
+                if (alive && lane == 0) barrier_arrive(&sums_empty[buffer]);
                 ++segment;
             };
             int before = 0;  // segments ahead of the last

@@ -147,6 +147,65 @@ def test_linear_with_what_follows(dtype, rows, inner, outer, relu, p, added):
     check_linear(x, weight, rand(outer, dtype=dtype, seed=3), relu, p, residual, what=f"relu {relu} p {p}")
 
 
+# Calls that go to the tensor cores: their edges in rows and both widths, contractions of one chunk and of several segments, more
+# tiles than multiprocessors, and weight gradients of few and of many splits.
+TILE_SIZES = [(40000, 64, 72), (9001, 257, 129), (130, 1024, 1024), (129, 2051, 33), (1, 2048, 2056), (20000, 40, 136), (70001, 33, 47),
+              (3000, 1030, 17), (5000, 300, 300), (150000, 16, 24), (19000, 128, 256), (300000, 8, 24), (2500, 512, 1000)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows, inner, outer", TILE_SIZES)
+@pytest.mark.parametrize("relu, p, added", [(False, 0.0, False), (True, 0.3, True)])
+def test_linear_on_tiles(dtype, rows, inner, outer, relu, p, added):
+    x = rand(rows, inner, dtype=dtype, seed=1, offset=0.2)
+    weight = rand(outer, inner, dtype=dtype, seed=2, scale=inner**-0.5)
+    check_linear(x, weight, rand(outer, dtype=dtype, seed=3, scale=0.1), relu, p,
+                 rand(rows, outer, dtype=dtype, seed=4) if added else None, what=f"{rows}x{inner}x{outer}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_linear_on_tiles_strides(dtype):
+    rows, weight, bias = 40000, rand(72, 64, dtype=dtype, seed=2, scale=0.1), rand(72, dtype=dtype, seed=3)
+    base = rand(rows, 104, dtype=dtype, seed=1)
+    # rows on vectors, on vectors of other lengths, between vectors, far apart, backwards in memory, on one place
+    for x in (base[:, 8:72], base[:, 4:68], base[:, 3:67], rand(rows, 100, dtype=dtype, seed=4)[:, :64], base[::3, :64].repeat(3, 1),
+              rand(64, rows, dtype=dtype, seed=5).t(), rand(1, 64, dtype=dtype, seed=6).expand(rows, 64), base[1:, 32:96]):
+        check_linear(x.detach(), weight.detach(), bias.detach(), True, 0.25, what=str(x.stride()))
+    odd = rand(rows * 64 + 1, dtype=dtype, seed=7)[1:].view(rows, 64)
+    oddly = rand(72 * 64 + 1, dtype=dtype, seed=8, scale=0.1)[1:].view(72, 64)
+    check_linear(odd, oddly, bias.detach(), True, residual=rand(rows * 72 + 1, dtype=dtype, seed=9)[1:].view(rows, 72), what="odd addresses")
+    check_linear(base[:, :64].detach().clone(), rand(64, 72, dtype=dtype, seed=10, scale=0.1).t().detach(), what="transposed weight")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("polls", [0, 1])
+def test_linear_waits_that_run_out(dtype, polls):
+    """A kernel that gives up a wait leaves NaN for what it has not computed and says so; the next one is as ever."""
+    x, w, b = (t.requires_grad_() for t in (rand(30000, 96, dtype=dtype, seed=1), rand(128, 96, dtype=dtype, seed=2, scale=0.1),
+                                             rand(128, dtype=dtype, seed=3)))
+    grad = rand(30000, 128, dtype=dtype, seed=4)
+
+    def both():
+        y = rt.linear(x, w, b, "relu")  # (a dropped element would be a zero all the same)
+        return [y.detach(), *torch.autograd.grad(y, (x, w, b), grad)]
+    want = both()
+    assert rt.device_status() == 0
+    before = rt.lib().cgnn_linear_wait_limit(polls)
+    try:
+        got = both()
+        torch.cuda.synchronize()
+    finally:
+        rt.lib().cgnn_linear_wait_limit(before)
+    assert rt.device_status() == 2
+    lost = [torch.isnan(g) for g in got]
+    assert any(nan.any() for nan in lost)
+    for g, v, nan in zip(got, want, lost):
+        assert nan.all() if polls == 0 else torch.equal(g[~nan], v[~nan])
+    for g, v in zip(both(), want):
+        assert torch.equal(g, v)
+    assert rt.device_status() == 0
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [40, 6000])
 def test_linear_strides_and_dimensions(dtype, rows):
@@ -188,7 +247,7 @@ def test_linear_of_nothing(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows", [300, 20000])
+@pytest.mark.parametrize("rows", [300, 40000])
 def test_linear_infinities_and_nan(dtype, rows):
     """They reach the outputs that they have a part in, as the formula says, and no others."""
     x, w = rand(rows, 70, dtype=dtype, seed=1), rand(50, 70, dtype=dtype, seed=2)
