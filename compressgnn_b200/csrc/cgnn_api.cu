@@ -107,7 +107,7 @@ cudaError_t pool_alloc(void **ptr, size_t bytes, cudaStream_t stream) {
 namespace cgnn {
 int sample_status(int *out);  // cgnn_sample.cu
 int loss_status(int *out);    // cgnn_loss.cu
-int linear_status(int *out);  // cgnn_linear.cu
+int linear_status(int *out);  // cgnn_linear_tiles.cu
 }
 
 extern "C" {

@@ -12,15 +12,6 @@
 
 namespace cgnn {
 
-static __device__ int g_linear_status = 0;
-
-int linear_status(int *out) {
-    const int zero = 0;
-    CGNN_CUDA(cudaMemcpyFromSymbol(out, g_linear_status, sizeof(int)));
-    CGNN_CUDA(cudaMemcpyToSymbol(g_linear_status, &zero, sizeof(int)));
-    return CGNN_OK;
-}
-
 namespace {
 
 // ---------------------------------------------------------------------------------------------
@@ -235,13 +226,6 @@ bool by_tiles(int dtype, int64_t rows, int64_t in, int64_t out) {
 
 std::atomic<int> wait_limit{WAIT_LIMIT};
 
-int status_address(int **out) {
-    void *p = nullptr;
-    CGNN_CUDA(cudaGetSymbolAddress(&p, g_linear_status));
-    *out = static_cast<int *>(p);
-    return CGNN_OK;
-}
-
 template <typename F>
 size_t bytes_of_type(int dtype, F &&call) {
     switch (dtype) {
@@ -263,12 +247,7 @@ int forward(const Call &c, const void *weight, const void *bias, const void *res
     e.relu = relu;
     e.drop = drop;
     if constexpr (HAS_TILES<T>)
-        if (tiles) {
-            int *status;
-            const int rc = status_address(&status);
-            if (rc != CGNN_OK) return rc;
-            return tiles_forward<T>(c, static_cast<const T *>(weight), e, static_cast<T *>(y), scratch, wait_limit.load(), status, stream);
-        }
+        if (tiles) return tiles_forward<T>(c, static_cast<const T *>(weight), e, static_cast<T *>(y), scratch, wait_limit.load(), stream);
     return small_forward<T>(c, static_cast<const T *>(weight), e, static_cast<T *>(y), stream);
 }
 
@@ -276,14 +255,10 @@ template <typename T>
 int backward(const Call &c, const void *weight, const void *mask, const void *grad, double scale, void *dx, void *dweight, void *dbias,
              void *scratch, bool tiles, cudaStream_t stream) {
     if constexpr (HAS_TILES<T>)
-        if (tiles) {
-            int *status;
-            const int rc = status_address(&status);
-            if (rc != CGNN_OK) return rc;
+        if (tiles)
             return tiles_backward<T>(c, static_cast<const T *>(weight), static_cast<const T *>(grad), static_cast<const uint8_t *>(mask),
                                      scale, static_cast<T *>(dx), static_cast<T *>(dweight), static_cast<T *>(dbias), scratch,
-                                     wait_limit.load(), status, stream);
-        }
+                                     wait_limit.load(), stream);
     return small_backward<T>(c, static_cast<const T *>(weight), static_cast<const T *>(grad), static_cast<const uint8_t *>(mask),
                              scale, static_cast<T *>(dx), static_cast<T *>(dweight), static_cast<T *>(dbias), scratch, stream);
 }

@@ -73,12 +73,11 @@ static int join(const Acc<T> *parts, int64_t splits, int64_t n, double scale, T 
 template <typename T>
 size_t tiles_forward_bytes(int64_t in, int64_t out);
 template <typename T>
-int tiles_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T *y, void *scratch, int polls, int *status,
-                  cudaStream_t stream);
+int tiles_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T *y, void *scratch, int polls, cudaStream_t stream);
 template <typename T>
 size_t tiles_backward_bytes(int64_t rows, int64_t in, int64_t out);
 template <typename T>
 int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t *mask, double scale, T *dx, T *dweight, T *dbias,
-                   void *scratch, int polls, int *status, cudaStream_t stream);
+                   void *scratch, int polls, cudaStream_t stream);
 
 }  // namespace cgnn

@@ -20,6 +20,16 @@
 #include "cgnn_linear.cuh"
 
 namespace cgnn {
+
+static __device__ int g_linear_status = 0;
+
+int linear_status(int *out) {
+    const int zero = 0;
+    CGNN_CUDA(cudaMemcpyFromSymbol(out, g_linear_status, sizeof(int)));
+    CGNN_CUDA(cudaMemcpyToSymbol(g_linear_status, &zero, sizeof(int)));
+    return CGNN_OK;
+}
+
 namespace {
 
 constexpr int BM = 128;
@@ -80,7 +90,6 @@ struct Tiles {
     float scale;
     Epilogue<T> epilogue;         // FORWARD
     int polls;
-    int *status;
 };
 
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -1158,7 +1167,7 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (threadIdx.x == 0 && given_up) atomicOr(t.status, STATUS_WAIT_EXPIRED);
+    if (threadIdx.x == 0 && given_up) atomicOr(&g_linear_status, STATUS_WAIT_EXPIRED);
     if (warp == MMA_WARP) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLUMNS) : "memory");
@@ -1232,8 +1241,7 @@ size_t tiles_forward_bytes(int64_t in, int64_t out) {
 }
 
 template <typename T>
-int tiles_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T *y, void *scratch, int polls, int *status,
-                  cudaStream_t stream) {
+int tiles_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T *y, void *scratch, int polls, cudaStream_t stream) {
     uint8_t *const packed = static_cast<uint8_t *>(scratch);
     int rc = pack<T, FORWARD>(weight, c.in, c.out, c.in, packed, stream);
     if (rc != CGNN_OK) return rc;
@@ -1250,7 +1258,6 @@ int tiles_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T
     if (epilogue.residual != nullptr) t.out_whole = t.out_whole && whole_rows(epilogue.residual, c.out, sizeof(T));
     t.epilogue = epilogue;
     t.polls = polls;
-    t.status = status;
     return launch<T, FORWARD>(t, 1, stream);
 }
 
@@ -1273,7 +1280,7 @@ size_t tiles_backward_bytes(int64_t rows, int64_t in, int64_t out) {
 
 template <typename T>
 int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t *mask, double scale, T *dx, T *dweight, T *dbias,
-                   void *scratch, int polls, int *status, cudaStream_t stream) {
+                   void *scratch, int polls, cudaStream_t stream) {
     uint8_t *const packed = static_cast<uint8_t *>(scratch);
     Tiles<T> t{};
     t.a = grad;
@@ -1282,7 +1289,6 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
     t.mask_pitch = mask_pitch(c.out);
     t.scale = (float)scale;
     t.polls = polls;
-    t.status = status;
     if (dx != nullptr) {
         int rc = pack<T, INPUT>(weight, c.in, c.in, c.out, packed, stream);
         if (rc != CGNN_OK) return rc;
@@ -1319,9 +1325,9 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
 
 #define CGNN_TILES_OF(T)                                                                                                        \
     template size_t tiles_forward_bytes<T>(int64_t, int64_t);                                                                   \
-    template int tiles_forward<T>(const Call &, const T *, const Epilogue<T> &, T *, void *, int, int *, cudaStream_t);         \
+    template int tiles_forward<T>(const Call &, const T *, const Epilogue<T> &, T *, void *, int, cudaStream_t);                \
     template size_t tiles_backward_bytes<T>(int64_t, int64_t, int64_t);                                                         \
-    template int tiles_backward<T>(const Call &, const T *, const T *, const uint8_t *, double, T *, T *, T *, void *, int, int *, \
+    template int tiles_backward<T>(const Call &, const T *, const T *, const uint8_t *, double, T *, T *, T *, void *, int, \
                                    cudaStream_t);
 CGNN_TILES_OF(float)
 CGNN_TILES_OF(__nv_bfloat16)

@@ -8,7 +8,7 @@ from . import runtime as _native
 class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay; ``weight_decay=0`` is Adam), as ``torch.optim.AdamW`` computes it.
 
-    ``max_norm``: the gradients of all groups are clipped by their common 2-norm, which ``step`` leaves in ``grad_norm``
+    ``max_norm`` (not a group's): the gradients of all groups are clipped by their common 2-norm, which ``step`` leaves in ``grad_norm``
     (a float32 tensor on the device); the gradients themselves are not changed.
     ``state_bits=8``: moments of tensors with ``least_8bit`` elements or more are held in 8 bits, 4 bytes a float32
     parameter less to keep and 12 less to move a step; smaller ones, and float64, keep theirs in full.  ``seed`` is the key
@@ -16,6 +16,8 @@ class AdamW(torch.optim.Optimizer):
 
     ``lr`` may be a CUDA tensor of one float32.  The steps taken are counted on the device, so a step can be captured into
     a CUDA graph once the state exists (after one step outside of the capture)."""
+
+    grad_norm = None
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, state_bits=32,
                  least_8bit=4096, seed=0):
@@ -29,9 +31,9 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("max_norm must not be negative")
         if state_bits not in (8, 32):
             raise ValueError("Supported state_bits: 8, 32")
-        self.grad_norm = None
-        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits))
-        self.max_norm, self.least_8bit, self.seed = max_norm, least_8bit, seed
+        # (all of it in the defaults: they are what a copy of an optimiser takes along)
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, max_norm=max_norm,
+                                      state_bits=state_bits, least_8bit=least_8bit, seed=seed))
 
     def _begin(self, params):
         """State for parameters that have none yet: ``(group, parameter)`` pairs."""
@@ -42,7 +44,7 @@ class AdamW(torch.optim.Optimizer):
             state = self.state[p]
             state["step"] = step
             wide = torch.float64 if p.dtype == torch.float64 else torch.float32
-            if group["state_bits"] == 8 and p.numel() >= self.least_8bit and wide == torch.float32:
+            if group["state_bits"] == 8 and p.numel() >= group["least_8bit"] and wide == torch.float32:
                 blocks = (p.numel() + 255) // 256
                 for name in ("exp_avg", "exp_avg_sq"):  # (the second holds the root)
                     state[name] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
@@ -57,6 +59,9 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        max_norm, seed = self.defaults["max_norm"], int(self.defaults["seed"])
+        if max_norm is not None:
+            self.grad_norm = None  # (of a step without a gradient)
         calls, fresh = {}, []
         for group in self.param_groups:
             for p in group["params"]:
@@ -69,7 +74,7 @@ class AdamW(torch.optim.Optimizer):
                 if not self.state[p]:
                     fresh.append((group, p))
                 calls.setdefault((p.device, tuple(group["betas"]), group["eps"]), []).append((group, p))
-        if self.max_norm is not None and len(calls) > 1:
+        if max_norm is not None and len(calls) > 1:
             raise RuntimeError("AdamW: with max_norm all parameters lie on one device and share betas and eps")
         for device in {p.device for _, p in fresh}:
             self._begin([(group, p) for group, p in fresh if p.device == device])
@@ -78,9 +83,9 @@ class AdamW(torch.optim.Optimizer):
             norm = _native.adamw_step(
                 [p for _, p in members], [p.grad.contiguous() for _, p in members], [s["exp_avg"] for s in states],
                 [s["exp_avg_sq"] for s in states], [s["step"] for s in states], [group["lr"] for group, _ in members], betas, eps,
-                [group["weight_decay"] for group, _ in members], self.max_norm, [s.get("exp_avg_scale") for s in states],
-                [s.get("exp_avg_sq_scale") for s in states], self.seed + (number << 32))
-            if self.max_norm is not None:
+                [group["weight_decay"] for group, _ in members], max_norm, [s.get("exp_avg_scale") for s in states],
+                [s.get("exp_avg_sq_scale") for s in states], seed + (number << 32))
+            if max_norm is not None:
                 self.grad_norm = norm
         return loss
 

@@ -7,8 +7,12 @@ core's is within the same: fp32 operands go in as three bf16 numbers whose remai
 out are at most 2 * 2^-24 of the term, and every 16 terms of a product are added to the sum with a truncation of at most 2 U for
 the alignment of each of at most 17 summands, 34 / 16 a term in n, which a bound of n alone would not take in; so
 those sums count ``3 n``."""
+import copy
 import math
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -171,6 +175,8 @@ def test_linear_on_tiles_strides(dtype):
     for x in (base[:, 8:72], base[:, 4:68], base[:, 3:67], rand(rows, 100, dtype=dtype, seed=4)[:, :64], base[::3, :64].repeat(3, 1),
               rand(64, rows, dtype=dtype, seed=5).t(), rand(1, 64, dtype=dtype, seed=6).expand(rows, 64), base[1:, 32:96]):
         check_linear(x.detach(), weight.detach(), bias.detach(), True, 0.25, what=str(x.stride()))
+    # rows on vectors that end inside one
+    check_linear(base[:, 8:68].detach(), weight[:, :60].contiguous().detach(), bias.detach(), True, 0.25, what="60 of 104")
     odd = rand(rows * 64 + 1, dtype=dtype, seed=7)[1:].view(rows, 64)
     oddly = rand(72 * 64 + 1, dtype=dtype, seed=8, scale=0.1)[1:].view(72, 64)
     check_linear(odd, oddly, bias.detach(), True, residual=rand(rows * 72 + 1, dtype=dtype, seed=9)[1:].view(rows, 72), what="odd addresses")
@@ -396,6 +402,46 @@ def test_linear_replayed_and_on_other_streams():
     [t.join() for t in threads]
     for got in results.values():
         assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_linear_traced():
+    w, b = rand(72, 64, seed=2), rand(72, seed=3)
+    traced = torch.jit.trace(lambda a: rt.linear(a, w, b, "relu"), (rand(2000, 64, seed=1),))
+    x = rand(3000, 64, seed=4).requires_grad_()
+    y = traced(x)
+    assert torch.equal(y, rt.linear(x, w, b, "relu"))
+    grads = [torch.autograd.grad(f(x).square().sum(), x)[0] for f in (traced, lambda a: rt.linear(a, w, b, "relu"))]
+    assert torch.equal(*grads)
+
+
+FIRST = """
+import sys, torch
+sys.path.insert(0, {root!r})
+from compressgnn_b200 import runtime as rt
+x, w, b = (torch.randn(*s, device="cuda").requires_grad_() for s in ((30000, 64), (72, 64), (72,)))
+p, g, m, v = (torch.randn(5000, device="cuda") for _ in range(4))
+v.square_()
+steps = [torch.zeros((), dtype=torch.int64, device="cuda")]
+grad, before = torch.randn(30000, 72, device="cuda"), p.clone()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = rt.linear(x, w, b, "relu", 0.0)
+    grads = torch.autograd.grad(y, (x, w, b), grad)
+    rt.adamw_step([p], [g], [m], [v], steps, max_norm=1.0)
+graph.replay()
+torch.cuda.synchronize()
+y = y.detach().clone()
+assert torch.equal(y, rt.linear(x, w, b, "relu").detach()) and int(steps[0]) == 1 and not torch.equal(p, before)
+z = rt.linear(x, w, b, "relu")
+assert all(torch.equal(a, c) for a, c in zip(grads, torch.autograd.grad(z, (x, w, b), grad)))
+"""
+
+
+def test_first_calls_inside_a_capture():
+    root = Path(__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", FIRST.format(root=str(root))], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_linear_refuses():
@@ -780,6 +826,24 @@ def test_optimiser_state_is_saved_and_loaded(bits, dtype, tmp_path):
     for p, q in zip(model.parameters(), other.parameters()):
         assert torch.equal(p, q) and int(opt2.state[q]["step"]) == 4
         assert opt2.state[q]["exp_avg"].dtype == opt.state[p]["exp_avg"].dtype
+
+
+def test_optimiser_is_copied_whole():
+    model = small_model()
+    opt = optim.AdamW(model.parameters(), max_norm=0.5, state_bits=8, least_8bit=100, seed=7)
+    gradients(model, 3)
+    opt.step()
+    other = copy.deepcopy((model, opt))
+    for m, o in ((model, opt), other):
+        gradients(m, 20)
+        o.step()
+    for p, q in zip(model.parameters(), other[0].parameters()):
+        assert torch.equal(p, q)
+    assert torch.equal(opt.grad_norm, other[1].grad_norm)
+    for p in model.parameters():
+        p.grad = None
+    opt.step()
+    assert opt.grad_norm is None
 
 
 def test_optimiser_with_8_bits_follows_the_one_with_32():
