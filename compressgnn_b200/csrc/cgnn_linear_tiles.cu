@@ -48,7 +48,8 @@ constexpr int PIECE = 16;          // columns that a warp of the epilogue takes 
 // HBM wants 35 KB on their way to each multiprocessor.  16-bit operands are copied asynchronously to where the tensor core
 // reads them, as many stages early as there are, or AHEAD where somebody looks at them on their way.  fp32 ones go through
 // registers, by two groups of producers that take every other chunk: a warp's wait for one load is a wait for its latest, so that
-// loads further ahead by the same warps did not help (4 chunks ahead 180 us, 1 chunk 178; two groups TWO_GROUPS_US).
+// loads further ahead by the same warps did not help (325,557 x
+// 256 -> 128 forward: 4 chunks ahead 180 us, 1 chunk 178, two groups 157).
 template <typename T, int FORM, bool WHOLE>
 struct Shape {
     static constexpr bool SPLIT = sizeof(T) == 4;
@@ -456,7 +457,8 @@ __device__ __forceinline__ void store16(T *p, int left, bool wide, const float (
 }
 
 // What few warps come to stands in functions of its own: what all of them read again and again has to fit the instruction caches
-// (2.45 M x 128 -> 256 bf16 forward with these and the dropout inside: 450 us, without: INSIDE_US).
+// (2.45 M x 128 -> 256 bf16 forward with these and the dropout inside: 450 us,
+// without 386).
 
 // Rows of no whole vectors: what the lanes left in `staging` ([32][PIECE + 1]) by neighbouring lanes for neighbouring columns.
 template <typename O>
@@ -1091,6 +1093,12 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
                 if (FORM == WEIGHT) chunks = chunks_of<T, FORM, WHOLE>(t, item);
                 const int columns = (int)min((int64_t)BN, (t.N - n0 + 15) / 16 * 16);
                 const uint32_t descriptor = base | (uint32_t)(columns / 8) << 17;
+                // Of a whole tile the planes h and m of B lie behind each other in shared memory as the two accumulators do in theirs: one
+                // product of twice the columns gives hh and hm, another mh and mm, and reads A once.  (Reading the operands
+                // bounds products of 128 columns, at some 108 cycles for 64.  100,000 x 1024 -> 1024: forward 1344 us with six
+                // products, 1279 with these; input gradient 1182, 1071.)
+                [[maybe_unused]] const bool both = columns == BN;
+                [[maybe_unused]] constexpr uint32_t descriptor_of_both = base | (uint32_t)(2 * BN / 8) << 17;
                 int of_segment = 0;
                 for (int chunk = 0; alive && chunk < chunks; ++chunk) {
                     const uint32_t accumulator = tmem + buffer * 256, small = accumulator + 128;
@@ -1107,8 +1115,15 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
                         for (int k = 0; k < BK / 16; ++k) {
                             const uint32_t ak = a + k * STEP, bk = b + k * STEP;
                             const bool add = !fresh || k > 0;
-                            multiply<UPPER>(accumulator, ak, bk, descriptor, add);
-                            if constexpr (S::SPLIT) {
+                            if constexpr (!S::SPLIT) {
+                                multiply<UPPER>(accumulator, ak, bk, descriptor, add);
+                            } else if (both) {
+                                multiply<UPPER>(accumulator, ak, bk, descriptor_of_both, add);
+                                multiply<UPPER>(accumulator, ak + AP, bk, descriptor_of_both, true);
+                                multiply<UPPER>(small, ak, bk + 2 * BP, descriptor, true);
+                                multiply<UPPER>(small, ak + 2 * AP, bk, descriptor, true);
+                            } else {
+                                multiply<UPPER>(accumulator, ak, bk, descriptor, add);
                                 multiply<UPPER>(small, ak, bk + BP, descriptor, add);
                                 multiply<UPPER>(small, ak + AP, bk, descriptor, true);
                                 multiply<UPPER>(small, ak, bk + 2 * BP, descriptor, true);
