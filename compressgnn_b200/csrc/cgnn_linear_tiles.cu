@@ -8,9 +8,15 @@
 //
 // fp32 operands become three bf16 numbers each, high + middle + low (8 bits of the fraction apiece, 24 together), and a
 // product six: hh, hm, mh, hl, lh, mm; what is left out is below 2^-23 of a term.  A tensor core adds to its fp32
-// accumulator with truncation, so that the error grows with the number of additions: hh has an accumulator of its own, the five
-// small ones share another, and after 256 terms both are added to fp32 registers and begin anew.  Six products at
-// the bf16 rate are 275 TFLOP/s of fp32, where the fp32 pipes have 72.
+// accumulator with truncation, so that the error grows with the number of additions: hh has an accumulator of its own, the
+// five small ones share another, and after 256 terms both are added to fp32 registers and begin
+// anew (325,557 x 256 -> 128: outputs 1.5e-7 of their size from 64 bits, the fp32 pipes' 1.8e-7).  Six products at the bf16
+// rate are 275 TFLOP/s of fp32, where the fp32 pipes have 72.
+//
+// What it takes, us: 325,557 x 256 -> 128 fp32 forward 161 (floor 78, by products and by bytes alike; the library's product on
+// the fp32 pipes 579), input gradient 190 (462), weight gradient 187 (638); 100,000 x 1024 -> 1024 forward 1253 (763).  In bf16,
+// where bytes bound it: 2.45 M x 128 -> 256 forward 390 (floor 287, the library's product without anything behind it 281), input
+// gradient 320 (294), weight gradient 456 (291, and 507 for the bias' in torch); 16,384 x 4096 -> 4096 forward 430 (333; 354).
 //
 // Operands lie in shared memory in the swizzled layout that the tensor core reads.  The streamed ones are masked and split on
 // their way there.  The weight is laid out and split once a call by a kernel of its own, as the images of shared memory
@@ -41,15 +47,15 @@ constexpr int THREADS = (MMA_WARP + 4) * 32;
 constexpr int EPILOGUE_REGISTERS = 112, PRODUCER_REGISTERS = 112, OTHER_REGISTERS = 32;
 constexpr int SMS = 148;
 constexpr int TMEM_COLUMNS = 512;  // two buffers of 256
-constexpr int PIECE = 16;          // columns that a warp of the epilogue takes through shared memory at once
+constexpr int PIECE = 16;          // columns that a warp of the epilogue takes at once
 
 // A stage holds BK of the contraction: rows of BK 16-bit elements (FORWARD, INPUT), or BK rows of panels of 64 (WEIGHT).
 //
 // HBM wants 35 KB on their way to each multiprocessor.  16-bit operands are copied asynchronously to where the tensor core
 // reads them, as many stages early as there are, or AHEAD where somebody looks at them on their way.  fp32 ones go through
 // registers, by two groups of producers that take every other chunk: a warp's wait for one load is a wait for its latest, so that
-// loads further ahead by the same warps did not help (325,557 x
-// 256 -> 128 forward: 4 chunks ahead 180 us, 1 chunk 178, two groups 157).
+// loads further ahead by the same warps did not help (325,557 x 256 -> 128 forward: 4 chunks ahead 180 us, 1 chunk 178,
+// two groups 157; weight gradient: one group of four units a thread 197, two groups of eight 213).
 template <typename T, int FORM, bool WHOLE>
 struct Shape {
     static constexpr bool SPLIT = sizeof(T) == 4;
@@ -1094,9 +1100,9 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
                 const int columns = (int)min((int64_t)BN, (t.N - n0 + 15) / 16 * 16);
                 const uint32_t descriptor = base | (uint32_t)(columns / 8) << 17;
                 // Of a whole tile the planes h and m of B lie behind each other in shared memory as the two accumulators do in theirs: one
-                // product of twice the columns gives hh and hm, another mh and mm, and reads A once.  (Reading the operands
-                // bounds products of 128 columns, at some 108 cycles for 64.  100,000 x 1024 -> 1024: forward 1344 us with six
-                // products, 1279 with these; input gradient 1182, 1071.)
+                // product of twice the columns gives hh and hm and reads A once.  (Reading the operands bounds products of 128
+                // columns, at some 108 cycles for 64.  The same for mh and mm would put mh into the accumulator of hh: no faster,
+                // for twice the error.)
                 [[maybe_unused]] const bool both = columns == BN;
                 [[maybe_unused]] constexpr uint32_t descriptor_of_both = base | (uint32_t)(2 * BN / 8) << 17;
                 int of_segment = 0;
@@ -1119,12 +1125,11 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
                                 multiply<UPPER>(accumulator, ak, bk, descriptor, add);
                             } else if (both) {
                                 multiply<UPPER>(accumulator, ak, bk, descriptor_of_both, add);
-                                multiply<UPPER>(accumulator, ak + AP, bk, descriptor_of_both, true);
-                                multiply<UPPER>(small, ak, bk + 2 * BP, descriptor, true);
-                                multiply<UPPER>(small, ak + 2 * AP, bk, descriptor, true);
                             } else {
                                 multiply<UPPER>(accumulator, ak, bk, descriptor, add);
                                 multiply<UPPER>(small, ak, bk + BP, descriptor, add);
+                            }
+                            if constexpr (S::SPLIT) {
                                 multiply<UPPER>(small, ak + AP, bk, descriptor, true);
                                 multiply<UPPER>(small, ak, bk + 2 * BP, descriptor, true);
                                 multiply<UPPER>(small, ak + 2 * AP, bk, descriptor, true);

@@ -3,10 +3,9 @@
 Tolerances count roundings, from ``U``, half a step of the sums (2^-24; for fp64 2^-53), and ``half_step``, that of a result's type.
 
 A product of ``n`` terms is off by at most ``(n + 32) U sum|a b|``: an fp32 sum one after the other makes n roundings.  A tensor
-core's is within the same: fp32 operands go in as three bf16 numbers whose remainder is at most 2^-24 of them, the products left
-out are at most 2 * 2^-24 of the term, and every 16 terms of a product are added to the sum with a truncation of at most 2 U for
-the alignment of each of at most 17 summands, 34 / 16 a term in n, which a bound of n alone would not take in; so
-those sums count ``3 n``."""
+core's: fp32 operands go in as three bf16 numbers whose remainder is at most 2^-24 of them, the products left out are at
+most 2 * 2^-24 of the term, and every 16 terms are added to their sum with a truncation of at most 2 U for the alignment of
+each of 17 summands: 34 / 16 a term (the parts of lower order add 2^-8 of that).  So those sums count ``3 n``."""
 import copy
 import math
 import subprocess
