@@ -1077,9 +1077,15 @@ c10::optional<Tensor> adamw_step(const std::vector<Tensor> &params, const std::v
                                  const std::vector<c10::optional<Tensor>> &rate_tensors, const std::vector<double> &decays, double beta1,
                                  double beta2, double eps, const c10::optional<double> &max_norm, int64_t seed) {
     const size_t n = params.size();
-    TORCH_CHECK(grads.size() == n && firsts.size() == n && seconds.size() == n && steps.size() == n && first_scales.size() == n &&
-                    second_scales.size() == n && rates.size() == n && rate_tensors.size() == n && decays.size() == n,
+    // (of scales none at all, of rates one for all)
+    TORCH_CHECK(grads.size() == n && firsts.size() == n && seconds.size() == n && steps.size() == n &&
+                    (first_scales.size() == n || first_scales.empty()) && (second_scales.size() == n || second_scales.empty()) &&
+                    (rates.size() == n || rates.size() == 1) && rate_tensors.size() == rates.size() &&
+                    (decays.size() == n || decays.size() == 1),
                 "adamw_step: as many gradients, moments, steps, scales and rates as parameters are needed");
+    const auto scale_of = [](const std::vector<c10::optional<Tensor>> &scales, size_t i) {
+        return scales.empty() || !scales[i].has_value() ? Tensor() : *scales[i];
+    };
     // (the library's bounds, before anything is looked at: a list without tensors is checked too)
     TORCH_CHECK(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adamw_step: the betas must lie in [0, 1)");
     TORCH_CHECK(eps >= 0.0, "adamw_step: eps must not be negative");
@@ -1104,22 +1110,23 @@ c10::optional<Tensor> adamw_step(const std::vector<Tensor> &params, const std::v
         TORCH_CHECK(m.scalar_type() == v.scalar_type() && (eight ? dtype != CGNN_F64 : m.scalar_type() == sum_type(p)),
                     "adamw_step: moments are float32 (float64 beside float64 parameters) or, with scales, float8_e4m3fn");
         TORCH_CHECK(t.scalar_type() == at::kLong && t.numel() == 1, "adamw_step: the steps taken are one int64 for each parameter");
-        TORCH_CHECK(eight == (first_scales[i].has_value() && first_scales[i]->defined()) &&
-                        eight == (second_scales[i].has_value() && second_scales[i]->defined()),
+        const Tensor first_scale = scale_of(first_scales, i), second_scale = scale_of(second_scales, i);
+        TORCH_CHECK(eight == first_scale.defined() && eight == second_scale.defined(),
                     "adamw_step: moments of 8 bits come with scales, others without");
         cgnn_adamw_tensor &e = list[i];
-        e.lr = rates[i];
-        e.weight_decay = decays[i];
+        const size_t rate_at = rates.size() == 1 ? 0 : i;
+        e.lr = rates[rate_at];
+        e.weight_decay = decays[decays.size() == 1 ? 0 : i];
         e.device_lr = nullptr;
         TORCH_CHECK(e.lr >= 0.0 && e.weight_decay >= 0.0, "adamw_step: lr and weight_decay must not be negative");
-        if (rate_tensors[i].has_value()) {
-            const Tensor &rate = *rate_tensors[i];
+        if (rate_tensors[rate_at].has_value()) {
+            const Tensor &rate = *rate_tensors[rate_at];
             TORCH_CHECK(rate.device() == device && rate.scalar_type() == at::kFloat && rate.numel() == 1,
                         "adamw_step: a learning rate in a tensor is one float32 on the parameters' device");
             e.device_lr = rate.const_data_ptr<float>();
         }
         if (eight)
-            for (const Tensor &s : {*first_scales[i], *second_scales[i]})
+            for (const Tensor &s : {first_scale, second_scale})
                 TORCH_CHECK(s.device() == device && s.scalar_type() == at::kFloat && s.is_contiguous() && s.numel() == (p.numel() + 255) / 256,
                             "adamw_step: a moment has one float32 scale for each block of 256 elements");
         for (const Tensor *w : {&p, &m, &v, &t}) written.add(*w);
@@ -1129,11 +1136,11 @@ c10::optional<Tensor> adamw_step(const std::vector<Tensor> &params, const std::v
         e.exp_avg_sq = data(v);
         e.exp_avg_scale = e.exp_avg_sq_scale = nullptr;
         if (eight) {
-            written.add(*first_scales[i]);
-            written.add(*second_scales[i]);
+            written.add(first_scale);
+            written.add(second_scale);
             // (of an empty tensor: no scales, which are not looked at, but moments of 8 bits all the same)
-            e.exp_avg_scale = static_cast<float *>(p.numel() ? data(*first_scales[i]) : data(t));
-            e.exp_avg_sq_scale = static_cast<float *>(p.numel() ? data(*second_scales[i]) : data(t));
+            e.exp_avg_scale = static_cast<float *>(p.numel() ? data(first_scale) : data(t));
+            e.exp_avg_sq_scale = static_cast<float *>(p.numel() ? data(second_scale) : data(t));
         }
         e.step = t.data_ptr<int64_t>();
         e.n = p.numel();

@@ -723,14 +723,15 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr=1e-3, betas=(0.9,
     ``max_norm``: the gradients are taken times ``min(1, max_norm / (norm + 1e-6))`` with the 2-norm of all of them, which is
     returned (a float32 tensor; None without ``max_norm``); they are not written."""
     params = list(params)
-    none = [None] * len(params)
-    rates = list(lr) if isinstance(lr, (list, tuple)) else [lr] * len(params)
-    decays = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * len(params)
+    rates, decays = ([v] if not isinstance(v, (list, tuple)) else list(v) for v in (lr, weight_decay))
+    for given, name in ((lr, "lr"), (weight_decay, "weight_decay")):  # (one number goes for all)
+        _require(not isinstance(given, (list, tuple)) or len(given) == len(params),
+                 f"adamw_step: as many values of {name} as parameters are needed")
     beta1, beta2 = betas
     seed, _ = _seed_args(int(seed))
     return ops().adamw_step(params, list(grads), list(exp_avgs), list(exp_avg_sqs), list(steps),
-                            none if exp_avg_scales is None else list(exp_avg_scales),
-                            none if exp_avg_sq_scales is None else list(exp_avg_sq_scales),
+                            [] if exp_avg_scales is None else list(exp_avg_scales),
+                            [] if exp_avg_sq_scales is None else list(exp_avg_sq_scales),
                             [0.0 if torch.is_tensor(r) else float(r) for r in rates],
                             [r if torch.is_tensor(r) else None for r in rates], [float(d) for d in decays],
                             float(beta1), float(beta2), float(eps), None if max_norm is None else float(max_norm), seed)
