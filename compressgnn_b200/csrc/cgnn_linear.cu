@@ -236,12 +236,12 @@ size_t bytes_of_type(int dtype, F &&call) {
 }
 
 template <typename T>
-int forward(const Call &c, const void *weight, const void *bias, const void *residual, int relu, const Drop &drop, void *y, void *mask,
-            void *scratch, bool tiles, cudaStream_t stream) {
+int forward(const Call &c, const void *weight, const void *bias, const void *residual, int relu, double p, const Drop &drop, void *y,
+            void *mask, void *scratch, bool tiles, cudaStream_t stream) {
     Epilogue<T> e{};
     e.bias = static_cast<const T *>(bias);
     e.residual = static_cast<const T *>(residual);
-    e.mask = relu || drop.threshold ? static_cast<uint8_t *>(mask) : nullptr;
+    e.mask = relu || p > 0.0 ? static_cast<uint8_t *>(mask) : nullptr;  // (of a p below 2^-32, which drops nothing, too)
     e.mask_pitch = mask_pitch(c.out);
     e.width = c.out;
     e.relu = relu;
@@ -302,10 +302,10 @@ int cgnn_linear(int dtype, int64_t rows, int64_t in, int64_t out, int64_t stride
     const Drop drop = Drop::of(p, seed, device_seed);
     const bool tiles = by_tiles(dtype, rows, in, out);
     switch (dtype) {
-        case CGNN_F32: return forward<float>(c, weight, bias, residual, relu, drop, y, mask, scratch, tiles, stream);
-        case CGNN_F64: return forward<double>(c, weight, bias, residual, relu, drop, y, mask, scratch, tiles, stream);
-        case CGNN_BF16: return forward<__nv_bfloat16>(c, weight, bias, residual, relu, drop, y, mask, scratch, tiles, stream);
-        default: return forward<__half>(c, weight, bias, residual, relu, drop, y, mask, scratch, tiles, stream);
+        case CGNN_F32: return forward<float>(c, weight, bias, residual, relu, p, drop, y, mask, scratch, tiles, stream);
+        case CGNN_F64: return forward<double>(c, weight, bias, residual, relu, p, drop, y, mask, scratch, tiles, stream);
+        case CGNN_BF16: return forward<__nv_bfloat16>(c, weight, bias, residual, relu, p, drop, y, mask, scratch, tiles, stream);
+        default: return forward<__half>(c, weight, bias, residual, relu, p, drop, y, mask, scratch, tiles, stream);
     }
 }
 

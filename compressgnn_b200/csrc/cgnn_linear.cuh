@@ -9,7 +9,7 @@ namespace cgnn {
 // y = x W^T, dx = z W, dW = z^T x.
 enum Form : int { FORWARD, INPUT, WEIGHT };
 
-constexpr int64_t WIDEST = (int64_t)1 << 30;  // most columns of a matrix
+constexpr int64_t WIDEST = (int64_t)1 << 28;  // a matrix has fewer columns
 constexpr int WAIT_LIMIT = 1 << 20;           // polls of a barrier in shared memory
 
 struct Call {

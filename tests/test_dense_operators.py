@@ -64,7 +64,7 @@ def _adamw(count=1, beta1=0.9, beta2=0.999, eps=1e-8, max_norm=-1.0, scratch=64,
     return _lib.lib().cgnn_adamw(None if none else ctypes.byref(t), count, beta1, beta2, eps, max_norm, 0, None, scratch, room, None)
 
 
-HUGE = 2**30
+HUGE = 2**28
 REFUSED = [
     (_linear, dict(dtype=4), b"unknown dtype"), (_linear, dict(dtype=-1), b"unknown dtype"), (_linear, dict(rows=-1), b"negative"),
     (_linear, dict(inner=-1), b"negative"), (_linear, dict(outer=-1), b"negative"), (_linear, dict(stride=-1), b"negative"),

@@ -306,11 +306,45 @@ def test_linear_is_deterministic_and_rows_do_not_touch_each_other(dtype):
         assert torch.equal(rt.linear(other, w, b)[30000:], y[30000:])
 
 
+def test_linear_beyond_32_bits():
+    """More elements than 32 bits count, in the output, its mask and gradient, and in the input."""
+    rows, last = 2_200_000, slice(2_199_900, None)
+    x = torch.ones(rows, 16, dtype=BF16, device="cuda")
+    x[last] = rand(100, 16, dtype=BF16, seed=1)
+    w = rand(1000, 16, dtype=BF16, seed=2)
+    x.requires_grad_()
+    y = rt.linear(x, w, None, "relu")
+    assert y.numel() > 2**31
+    with torch.no_grad():
+        z = x[last].double() @ w.double().t()
+        within(y[last].detach(), z.clamp(min=0), terms(16, 2.0**-24) * (x[last].double().abs() @ w.double().abs().t()) +
+               half_step(BF16) * z.abs() + least(BF16), "the last rows")
+        assert torch.equal(y[1000], y[0]) and torch.equal(y[2_000_000], y[0])
+    dx, = torch.autograd.grad(y.sum(), x)
+    want = (y[last].detach() > 0).double() @ w.double()
+    within(dx[last], want, terms(1000, 2.0**-24) * w.double().abs().sum(0) + half_step(BF16) * want.abs() + least(BF16), "dx")
+    del y, dx
+    wide = torch.zeros(rows, 1000, dtype=BF16, device="cuda")
+    wide[-1], wide[0] = 2.0, 1.0
+    v = rand(16, 1000, dtype=BF16, seed=3).requires_grad_()
+    y = rt.linear(wide, v)
+    with torch.no_grad():
+        assert torch.equal(y[1], torch.zeros_like(y[1]))
+        within(y[-1], 2 * v.double().sum(1), terms(1000, 2.0**-24) * 2 * v.double().abs().sum(1) + half_step(BF16) * y[-1].double().abs() +
+               least(BF16), "wide")
+    dv, = torch.autograd.grad(y, v, torch.ones_like(y))
+    assert torch.equal(dv, torch.full_like(dv, 3.0))
+
+
 def test_linear_dropout_is_the_dropout_operators():
     for shape, outer in (((300, 40), 31), ((20000, 64), 128), ((20000, 64), 47)):
         x, w = rand(*shape, seed=1), rand(outer, shape[1], seed=2)
         dropped = rt.linear(x, w, dropout=0.4, seed=77) == 0
         assert torch.equal(dropped, rt.dropout(torch.ones(shape[0], outer, device="cuda"), 0.4, seed=77) == 0)
+    for rows in (50, 20000):  # a probability that drops nothing
+        a, b = (rand(rows, 64, seed=3).requires_grad_() for _ in range(2))
+        y, z = rt.linear(a, w, dropout=1e-12), rt.linear(b, w)
+        assert torch.equal(y, z) and torch.equal(torch.autograd.grad(y.sum(), a)[0], torch.autograd.grad(z.sum(), b)[0])
     key = torch.tensor([77], device="cuda")
     assert torch.equal(rt.linear(x, w, dropout=0.4, seed=key), rt.linear(x, w, dropout=0.4, seed=77))
     torch.manual_seed(3)
@@ -701,6 +735,26 @@ def test_step_replayed_and_on_other_streams():
             assert torch.equal(p, q) and int(opt.state[p]["step"]) == 4
             assert torch.equal(opt.state[p]["exp_avg"].view(torch.uint8), eager.state[q]["exp_avg"].view(torch.uint8))
         assert torch.equal(opt.grad_norm, eager.grad_norm)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_step_beyond_32_bits(eight):
+    n, tail = 2**31 + 5000, 4096
+    p, g = (torch.full((n,), v, dtype=BF16, device="cuda") for v in (0.5, 0.01))
+    p[-tail:], g[-tail:] = rand(tail, dtype=BF16, seed=1), rand(tail, dtype=BF16, seed=2, scale=0.01)
+    part = p[-tail:].clone()
+    if eight:
+        first, second = (torch.zeros(n, dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2))
+        scales = [[torch.ones((n + 255) // 256, device="cuda")] for _ in range(2)]
+    else:
+        first, second = (torch.zeros(n, device="cuda") for _ in range(2))
+        scales = [None, None]
+    rt.adamw_step([p], [g], [first], [second], step_count(1, 0), exp_avg_scales=scales[0], exp_avg_sq_scales=scales[1])
+    one = [torch.zeros(tail, device="cuda") for _ in range(2)]
+    rt.adamw_step([part], [g[-tail:].clone()], [one[0]], [one[1]], step_count(1, 0))
+    assert torch.equal(p[-tail:], part) and bool((p[:-tail] == p[0]).all())
+    if not eight:
+        assert torch.equal(first[-tail:], one[0]) and torch.equal(second[-tail:], one[1])
 
 
 def test_steps_beside_each_other():
