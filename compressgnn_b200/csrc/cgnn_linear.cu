@@ -20,6 +20,11 @@ namespace {
 constexpr int TM = 32, TN = 64, TK = 16, TILE_THREADS = 128;
 constexpr int TILE_WAVE = 148 * 4;
 
+// Groups of TILE_THREADS that share a block's terms where blocks are few: one group is one warp to each of an SM's four
+// schedulers, and its own instructions bound it.  4 groups of fp32 (2 of fp64: what they stage is what static shared memory holds).
+template <typename A>
+constexpr int GROUPS = 16 / (int)sizeof(A);
+
 // C[m, n] = sum over k of A(m, k) B(n, k).  A: x, or z (masked); B: the weight, its transpose, or x.
 template <typename T>
 struct Small {
@@ -35,23 +40,28 @@ struct Small {
     Epilogue<T> epilogue;         // FORWARD
 };
 
-template <typename T, int FORM>
-__global__ void __launch_bounds__(TILE_THREADS) small_kernel(const Small<T> s) {
+template <typename T, int FORM, int GROUPS>
+__global__ void __launch_bounds__(GROUPS *TILE_THREADS) small_kernel(const Small<T> s) {
     using A = Acc<T>;
-    __shared__ A as[TK][TM + 1], bs[TK][TN + 1];
+    __shared__ A as_of[GROUPS][TK][TM + 1];
+    __shared__ A bs_of[GROUPS][TK][TN + 1];
+    const int group = GROUPS > 1 ? threadIdx.x / TILE_THREADS : 0, thread = GROUPS > 1 ? threadIdx.x % TILE_THREADS : threadIdx.x;
+    auto &as = as_of[group];
+    auto &bs = bs_of[group];
     const int64_t tiles_n = (s.N + TN - 1) / TN > 0 ? (s.N + TN - 1) / TN : 1;
     const int64_t m0 = (blockIdx.x / tiles_n) * TM, n0 = (blockIdx.x % tiles_n) * TN;
     const int64_t k_begin = (int64_t)blockIdx.y * s.k_per_split, k_end = min(s.K, k_begin + s.k_per_split);
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;  // columns tx + 16 j, rows ty * 4 + i
+    const int tx = thread % 16, ty = thread / 16;  // columns tx + 16 j, rows ty * 4 + i
     A acc[4][4], sum = A(0);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = A(0);
     constexpr bool A_ALONG_K = FORM != WEIGHT, B_ALONG_K = FORM == FORWARD;
-    for (int64_t k0 = k_begin; k0 < k_end; k0 += TK) {
+    for (int64_t stage = k_begin; stage < k_end; stage += GROUPS * TK) {
+        const int64_t k0 = stage + group * TK;  // (may lie behind the end: zeros)
 #pragma unroll
-        for (int i = threadIdx.x; i < TM * TK; i += TILE_THREADS) {
+        for (int i = thread; i < TM * TK; i += TILE_THREADS) {
             const int m = A_ALONG_K ? i / TK : i % TM, k = A_ALONG_K ? i % TK : i / TM;
             A v = A(0);
             if (m0 + m < s.M && k0 + k < k_end) {
@@ -64,7 +74,7 @@ __global__ void __launch_bounds__(TILE_THREADS) small_kernel(const Small<T> s) {
             as[k][m] = v;
         }
 #pragma unroll
-        for (int i = threadIdx.x; i < TN * TK; i += TILE_THREADS) {
+        for (int i = thread; i < TN * TK; i += TILE_THREADS) {
             const int n = B_ALONG_K ? i / TK : i % TN, k = B_ALONG_K ? i % TK : i / TN;
             bs[k][n] = n0 + n < s.N && k0 + k < k_end ? A(widen(s.b[(n0 + n) * s.b_n + (k0 + k) * s.b_k])) : A(0);
         }
@@ -85,6 +95,22 @@ __global__ void __launch_bounds__(TILE_THREADS) small_kernel(const Small<T> s) {
                 for (int j = 0; j < 4; ++j) acc[i][j] = fused(av[i], bv[j], acc[i][j]);
         }
         __syncthreads();
+    }
+    if constexpr (GROUPS > 1) {  // (the last stage's barrier is behind every thread: its place is free)
+        static_assert(FORM != WEIGHT, "column sums are not joined");
+        static_assert(16 * TILE_THREADS <= GROUPS * TK * (TN + 1), "a group's sums are wider than the stages");
+        A *const sums = &bs_of[0][0][0];
+        for (int g = 1; g < GROUPS; ++g) {
+            if (group == g)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sums[i * TILE_THREADS + thread] = acc[i / 4][i % 4];
+            __syncthreads();
+            if (group == 0)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[i / 4][i % 4] += sums[i * TILE_THREADS + thread];
+            __syncthreads();
+        }
+        if (group > 0) return;
     }
     const bool whole = gridDim.y == 1;
     if (FORM == WEIGHT && s.column_sums != nullptr && n0 == 0 && threadIdx.x < TM && m0 + threadIdx.x < s.M) {
@@ -135,12 +161,23 @@ int64_t small_splits(int64_t rows, int64_t in, int64_t out) {
     return std::max<int64_t>(1, std::min<int64_t>(TILE_WAVE / std::max<int64_t>(1, small_tiles(out, in)), rows / (8 * TK)));
 }
 
+// Whether groups share a block's terms: while no SM has a second block, and where there are stages to share.  Us by groups / by
+// one: fp32 1 x 560 -> 544 forward 22.6 / 28.7, input gradient 19.4 / 38.9, bf16 24.6 / 39.0 and 21.1 / 43.0;
+// 1000 x 301 -> 47 (32 tiles) 14.4 / 18.5, its input gradient (160 tiles) 10.3 / 8.2; 10,000 x 64 -> 47 (313) 12.3 / 10.3;
+// 2708 x 16 -> 7 (one stage) 6.2 / 5.4.
+bool shared_terms(int64_t tiles, int64_t terms) { return tiles <= 148 && terms > 2 * TK; }
+
 template <typename T, int FORM>
 int small_product(Small<T> &s, int64_t splits, cudaStream_t stream) {
     const int64_t tiles = small_tiles(s.M, s.N);
     CGNN_REQUIRE(tiles < (1ll << 31), "linear: grid too large");
     s.k_per_split = ceil_div(ceil_div(std::max<int64_t>(s.K, 1), splits), TK) * TK;
-    small_kernel<T, FORM><<<dim3((unsigned)tiles, (unsigned)splits), TILE_THREADS, 0, stream>>>(s);
+    const dim3 grid((unsigned)tiles, (unsigned)splits);
+    constexpr int groups = FORM == WEIGHT ? 1 : GROUPS<Acc<T>>;
+    if (groups > 1 && shared_terms(tiles, s.K))
+        small_kernel<T, FORM, groups><<<grid, groups * TILE_THREADS, 0, stream>>>(s);
+    else
+        small_kernel<T, FORM, 1><<<grid, TILE_THREADS, 0, stream>>>(s);
     CGNN_LAUNCH_CHECK();
     return CGNN_OK;
 }
@@ -214,7 +251,7 @@ constexpr bool HAS_TILES = sizeof(T) < 8;
 // Whether a call goes to the tensor cores: by its number of multiplications, earlier where rows are whole vectors and where one
 // contraction is long (a tile of single elements takes it alone).  Us by tiles / by single elements, forward + input gradient +
 // weight gradient: fp32 10,000 x 64 -> 64 (4e7) 47 / 48, 20,000 x 64 -> 64 54 / 64, 2708 x 64 -> 64 46 / 38;
-// 40,000 x 64 -> 47 (1e8) 72 / 92, 20,000 x 64 -> 47 60 / 61; 32 x 4096 -> 64 112 / 195;
+// 40,000 x 64 -> 47 (1e8) 72 / 92, 20,000 x 64 -> 47 60 / 61; 32 x 4096 -> 64 107 / 140;
 // bf16 2708 x 64 -> 64 (1e7) 38 / 40, 1024 x 64 -> 64 38 / 40, 256 x 64 -> 64 30 / 37; 20,000 x 64 -> 47 (6e7) 70 / 66.
 bool by_tiles(int dtype, int64_t rows, int64_t in, int64_t out) {
     if (dtype == CGNN_F64 || in <= 0) return false;
