@@ -182,6 +182,67 @@ int small_product(Small<T> &s, int64_t splits, cudaStream_t stream) {
     return CGNN_OK;
 }
 
+// ---------------------------------------------------------------------------------------------
+// the bias' gradient alone: column sums of z, for which neither x nor the weight is looked at
+// ---------------------------------------------------------------------------------------------
+constexpr int COLUMN_WARPS = 8, COLUMN_UNROLL = 8;
+constexpr int64_t COLUMN_BLOCKS = 148 * 8, COLUMN_ROWS = COLUMN_WARPS * COLUMN_UNROLL;  // rows: of a block, at least
+
+int64_t column_splits(int64_t rows, int64_t out) {
+    return std::max<int64_t>(1, std::min<int64_t>(COLUMN_BLOCKS / ceil_div(out, 32), rows / COLUMN_ROWS));
+}
+
+size_t column_bytes(int64_t rows, int64_t out) {
+    const int64_t splits = column_splits(rows, out);
+    return splits == 1 ? 0 : (size_t)splits * (size_t)out * sizeof(double);
+}
+
+// A lane has a column, a warp every eighth row with COLUMN_UNROLL of them on their way.  The grid's second dimension splits the rows:
+// parts[blockIdx.y, column], or, of one split, the sums themselves.  HBM bounds it, with fp64 sums too.
+template <typename T>
+__global__ void __launch_bounds__(COLUMN_WARPS * 32) columns_kernel(const T *grad, const uint8_t *mask, int64_t mask_pitch, int64_t rows,
+                                                                    int64_t rows_per_split, int64_t width, double scale, double *parts,
+                                                                    T *out) {
+    __shared__ double sums[COLUMN_WARPS][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c0 = (int64_t)blockIdx.x * 32, c = c0 + lane;
+    const int64_t end = min(rows, ((int64_t)blockIdx.y + 1) * rows_per_split);
+    double s = 0.0;
+    if (c < width) {
+        for (int64_t row = (int64_t)blockIdx.y * rows_per_split + warp; row < end; row += COLUMN_ROWS) {
+            T v[COLUMN_UNROLL];
+            uint32_t keep[COLUMN_UNROLL];
+#pragma unroll
+            for (int u = 0; u < COLUMN_UNROLL; ++u) {
+                const int64_t r = row + u * COLUMN_WARPS;
+                v[u] = r < end ? grad[r * width + c] : narrow<T>(Acc<T>(0));
+                // (a row of the mask is whole 64-bit words)
+                keep[u] = mask != nullptr && r < end ? *reinterpret_cast<const uint32_t *>(mask + r * mask_pitch + c0 / 8) : 0xffffffffu;
+            }
+#pragma unroll
+            for (int u = 0; u < COLUMN_UNROLL; ++u)
+                if (keep[u] >> lane & 1) s += (double)widen(v[u]);
+        }
+    }
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (warp > 0 || c >= width) return;
+#pragma unroll
+    for (int w = 1; w < COLUMN_WARPS; ++w) s += sums[w][lane];
+    if (gridDim.y == 1) out[c] = narrow<T>((Acc<T>)(s * scale));
+    else parts[blockIdx.y * width + c] = s;
+}
+
+template <typename T>
+int column_sums(const Call &c, const T *grad, const uint8_t *mask, double scale, T *dbias, void *scratch, cudaStream_t stream) {
+    const int64_t splits = column_splits(c.rows, c.out);
+    double *const parts = static_cast<double *>(scratch);
+    columns_kernel<T><<<dim3((unsigned)ceil_div(c.out, 32), (unsigned)splits), COLUMN_WARPS * 32, 0, stream>>>(
+        grad, mask, mask_pitch(c.out), c.rows, ceil_div(c.rows, splits), c.out, scale, parts, dbias);
+    CGNN_LAUNCH_CHECK();
+    return splits == 1 ? CGNN_OK : join(parts, splits, c.out, scale, dbias, stream);
+}
+
 size_t small_backward_bytes(int64_t acc_bytes, int64_t rows, int64_t in, int64_t out) {
     const int64_t splits = small_splits(rows, in, out);
     return splits == 1 ? 0 : (size_t)splits * (size_t)out * (size_t)(in + 1) * (size_t)acc_bytes;
@@ -226,22 +287,22 @@ int small_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
         const int rc = small_product<T, INPUT>(s, 1, stream);
         if (rc != CGNN_OK) return rc;
     }
-    if (dweight == nullptr && dbias == nullptr) return CGNN_OK;
+    if (dweight == nullptr) return CGNN_OK;
     s.a_m = 1;
     s.a_k = c.out;
     s.b = static_cast<const T *>(c.x);
     s.b_n = 1;
     s.b_k = c.stride;
     s.M = c.out;
-    s.N = dweight != nullptr ? c.in : 0;  // (without columns only the sums of z are formed)
+    s.N = c.in;
     s.K = c.rows;
     const int64_t splits = small_splits(c.rows, c.in, c.out);
     A *const parts = static_cast<A *>(scratch), *const sums = parts + splits * c.out * c.in;
     s.out = splits == 1 ? static_cast<void *>(dweight) : parts;
     s.column_sums = dbias == nullptr ? nullptr : splits == 1 ? static_cast<void *>(dbias) : sums;
     int rc = small_product<T, WEIGHT>(s, splits, stream);
-    if (rc == CGNN_OK && splits > 1 && dweight != nullptr) rc = join<T>(parts, splits, c.out * c.in, scale, dweight, stream);
-    if (rc == CGNN_OK && splits > 1 && dbias != nullptr) rc = join<T>(sums, splits, c.out, scale, dbias, stream);
+    if (rc == CGNN_OK && splits > 1) rc = join(parts, splits, c.out * c.in, scale, dweight, stream);
+    if (rc == CGNN_OK && splits > 1 && dbias != nullptr) rc = join(sums, splits, c.out, scale, dbias, stream);
     return rc;
 }
 
@@ -291,6 +352,12 @@ int forward(const Call &c, const void *weight, const void *bias, const void *res
 template <typename T>
 int backward(const Call &c, const void *weight, const void *mask, const void *grad, double scale, void *dx, void *dweight, void *dbias,
              void *scratch, bool tiles, cudaStream_t stream) {
+    if (dweight == nullptr && dbias != nullptr) {  // (behind it on the stream the input's gradient takes the scratch anew)
+        const int rc = column_sums<T>(c, static_cast<const T *>(grad), static_cast<const uint8_t *>(mask), scale, static_cast<T *>(dbias),
+                                      scratch, stream);
+        if (rc != CGNN_OK) return rc;
+        dbias = nullptr;
+    }
     if constexpr (HAS_TILES<T>)
         if (tiles)
             return tiles_backward<T>(c, static_cast<const T *>(weight), static_cast<const T *>(grad), static_cast<const uint8_t *>(mask),
@@ -348,9 +415,10 @@ int cgnn_linear(int dtype, int64_t rows, int64_t in, int64_t out, int64_t stride
 
 size_t cgnn_linear_backward_scratch_bytes(int dtype, int64_t rows, int64_t in, int64_t out) {
     if (dtype < CGNN_F32 || dtype > CGNN_F16 || rows <= 0 || in < 0 || out <= 0 || in >= WIDEST || out >= WIDEST) return 0;
+    const size_t columns = column_bytes(rows, out);
     if (by_tiles(dtype, rows, in, out))
-        return bytes_of_type(dtype, [&](auto zero) { return tiles_backward_bytes<decltype(zero)>(rows, in, out); });
-    return small_backward_bytes(dtype == CGNN_F64 ? 8 : 4, rows, in, out);
+        return std::max(columns, bytes_of_type(dtype, [&](auto zero) { return tiles_backward_bytes<decltype(zero)>(rows, in, out); }));
+    return std::max(columns, small_backward_bytes(dtype == CGNN_F64 ? 8 : 4, rows, in, out));
 }
 
 int cgnn_linear_backward(int dtype, int64_t rows, int64_t in, int64_t out, int64_t stride, const void *x, const void *weight,

@@ -53,18 +53,18 @@ struct Epilogue {
 };
 
 // out[i] = scale * the sum over the splits, in their order.
-template <typename T>
-static __global__ void __launch_bounds__(256) join_kernel(const Acc<T> *parts, int64_t splits, int64_t n, double scale, T *out) {
+template <typename T, typename P>
+static __global__ void __launch_bounds__(256) join_kernel(const P *parts, int64_t splits, int64_t n, double scale, T *out) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
-    Acc<T> sum = parts[i];
+    P sum = parts[i];
     for (int64_t s = 1; s < splits; ++s) sum += parts[s * n + i];
-    out[i] = narrow<T>(sum * (Acc<T>)scale);
+    out[i] = narrow<T>((Acc<T>)(sum * (P)scale));
 }
 
-template <typename T>
-static int join(const Acc<T> *parts, int64_t splits, int64_t n, double scale, T *out, cudaStream_t stream) {
-    join_kernel<T><<<(unsigned)ceil_div(n, 256), 256, 0, stream>>>(parts, splits, n, scale, out);
+template <typename T, typename P>
+static int join(const P *parts, int64_t splits, int64_t n, double scale, T *out, cudaStream_t stream) {
+    join_kernel<T, P><<<(unsigned)ceil_div(n, 256), 256, 0, stream>>>(parts, splits, n, scale, out);
     CGNN_LAUNCH_CHECK();
     return CGNN_OK;
 }

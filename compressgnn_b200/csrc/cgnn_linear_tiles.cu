@@ -1322,7 +1322,7 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
         rc = launch<T, INPUT>(t, 1, stream);
         if (rc != CGNN_OK) return rc;
     }
-    if (dweight == nullptr && dbias == nullptr) return CGNN_OK;
+    if (dweight == nullptr) return CGNN_OK;
     int64_t per_split;
     const int64_t splits = weight_splits<T>(c.rows, c.in, c.out, &per_split);
     float *const parts = reinterpret_cast<float *>(align_up((size_t)packed + packed_bytes<T>(c.in, c.out), 32));
@@ -1334,12 +1334,12 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
     t.N = c.in;
     t.K = c.rows;
     t.k_per_item = per_split;
-    t.partial = splits > 1 || dweight == nullptr;
+    t.partial = splits > 1;
     set_out(t, t.partial ? static_cast<void *>(parts) : dweight, c.in, t.partial ? sizeof(float) : sizeof(T));
     t.column_sums = dbias != nullptr ? sums : nullptr;
     int rc = launch<T, WEIGHT>(t, splits, stream);
-    if (rc == CGNN_OK && t.partial && dweight != nullptr) rc = join<T>(parts, splits, c.out * c.in, scale, dweight, stream);
-    if (rc == CGNN_OK && dbias != nullptr) rc = join<T>(sums, splits, c.out, scale, dbias, stream);
+    if (rc == CGNN_OK && t.partial) rc = join(parts, splits, c.out * c.in, scale, dweight, stream);
+    if (rc == CGNN_OK && dbias != nullptr) rc = join(sums, splits, c.out, scale, dbias, stream);
     return rc;
 }
 

@@ -422,7 +422,8 @@ int cgnn_cross_entropy_backward(int dtype, int64_t rows, int64_t classes, int64_
  *             the backward pass reads; may be null; not written where neither is asked for
  *   scratch   cgnn_linear_scratch_bytes(), 16-byte aligned; its contents do not matter; the same for the backward pass
  * Backward: grad: dense [rows, out]; mask: as written, or null where there was neither; p: of the forward call.  dx (dense
- * [rows, in]), dweight, dbias: each may be null.  Sums over rows are added up in a fixed order.
+ * [rows, in]), dweight, dbias: each may be null.  x is looked at for dweight only and the weight for dx only; they may be null
+ * otherwise.  Sums over rows are added up in a fixed order.
  * A kernel that waits for its own copies or products gives up after a number of polls; it writes NaN for what it has not
  * computed and sets status bit 2.  cgnn_linear_wait_limit sets that number as cgnn_cross_entropy_wait_limit does. */
 size_t cgnn_linear_mask_bytes(int64_t rows, int64_t out);
