@@ -117,13 +117,29 @@ __device__ __forceinline__ bool barrier_poll(uint64_t *barrier, uint32_t parity)
                  : "memory");
     return done != 0;
 }
-// Waits for the phase of that parity; gives up after `polls`, or when another thread of the block has.
-__device__ __forceinline__ bool barrier_wait(uint64_t *barrier, uint32_t parity, int polls, volatile int *given_up) {
-    for (int i = 0; i < polls; ++i) {
-        if (barrier_poll(barrier, parity)) return true;
-        if (*given_up) return false;
-    }
-    *given_up = 1;
+// What the warps of a block know of each other's waits.
+struct Waits {
+    int given_up;
+    int computed;  // what `compute_again` has come through
+    uint32_t again[EPILOGUE_WARPS][4];  // of a warp's item: rows with an element in that piece of columns that is to be computed again
+};
+// Waits for the phase of that parity; gives up after `polls`, or when another thread of the block has.  PATIENT: not while a warp is
+// computing elements again, which the others may have to wait for.
+template <bool PATIENT>
+__device__ __forceinline__ bool barrier_wait(uint64_t *barrier, uint32_t parity, int polls, volatile Waits *waits) {
+    [[maybe_unused]] int seen = 0;
+    do {
+        for (int i = 0; i < polls; ++i) {
+            if (barrier_poll(barrier, parity)) return true;
+            if (waits->given_up) return false;
+        }
+        if constexpr (PATIENT) {
+            const int now = waits->computed;
+            if (now == seen) break;
+            seen = now;
+        }
+    } while (PATIENT);
+    waits->given_up = 1;
     return false;
 }
 __device__ __forceinline__ void bulk_copy(uint32_t to, const void *from, uint32_t bytes, uint64_t *barrier) {
@@ -399,21 +415,6 @@ __device__ __forceinline__ int chunks_of(const Tiles<T> &t, int item) {
     return (int)((k + S::BK - 1) / S::BK);
 }
 
-// One element by fp32 arithmetic.
-template <typename T, int FORM>
-__device__ __forceinline__ float single_element(const Tiles<T> &t, int64_t m, int64_t n, int64_t k0, int64_t k1) {
-    float sum = 0.f;
-#pragma unroll 1
-    for (int64_t k = k0; k < k1; ++k) {
-        const int64_t row = FORM == WEIGHT ? k : m, column = FORM == WEIGHT ? m : k;
-        float a = widen(t.a[row * t.a_stride + column]);
-        if (FORM != FORWARD && t.mask != nullptr && !(t.mask[row * t.mask_pitch + column / 8] >> (column % 8) & 1)) a = 0.f;
-        sum = fmaf(a, widen(FORM == FORWARD ? t.b[n * t.b_stride + k] : t.b[k * t.b_stride + n]), sum);
-        if (sum != sum) break;
-    }
-    return sum;
-}
-
 // Sixteen neighbouring elements of a row, on a boundary of 32 bytes (fp32, wide) or 16.
 __device__ __forceinline__ void load16(const float *p, int left, bool, float (&y)[16]) {
 #pragma unroll
@@ -480,12 +481,83 @@ template <typename T>
 __device__ __noinline__ void read_row(float *staging, const T *row, int left) {
     for (int k = 0; k < PIECE; ++k) staging[k] = k < left ? widen(row[k]) : 0.f;
 }
-// The elements of a lane's row that are no finite numbers, computed again by fp32 arithmetic: where an operand is infinite, no number
-// or beyond bf16's range, its parts say nothing.
+// Elements of a warp's 32 x 64 of an item computed again by fp32 arithmetic and written over: where an operand is infinite, no
+// number or beyond bf16's range, its parts say nothing.  PIECE columns at once: of few rows one row after the other, its terms by all
+// lanes (one infinity in an incoming gradient makes a row of the weight's gradient infinite, of as many terms as there are
+// nodes); of more than 8 every lane its own.  (Not a function of its own: around a call the fp32 forward pass spilled registers, 191 us for 161.)
 template <typename T, int FORM>
-__device__ __noinline__ void compute_again(const Tiles<T> &t, float *staging, int64_t m, int64_t n, int left, int64_t k0, int64_t k1) {
-    for (int c = 0; c < PIECE && c < left; ++c)
-        if (!(fabsf(staging[c]) <= 3.402823466e38f)) staging[c] = single_element<T, FORM>(t, m, n + c, k0, k1);
+__device__ __forceinline__ void compute_again(const Tiles<T> &t, int item, Waits *waits) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Item i = item_of<T, FORM>(t, item);
+    const int64_t m0 = i.m0 + (warp & 3) * 32, n0 = i.n0 + (warp >> 2) * (Tile<T, FORM>::BN / 2);
+    for (int p = 0; p < Tile<T, FORM>::BN / 2 / PIECE; ++p) {
+        uint32_t rows = waits->again[warp][p];
+        __syncwarp();
+        if (lane == 0) waits->again[warp][p] = 0;
+        const int64_t n = n0 + p * PIECE;
+        const int left = (int)min(t.N - n, (int64_t)PIECE);
+        const bool own = __popc(rows) > 8;
+        while (rows) {
+            const int64_t m = m0 + (own ? lane : __ffs(rows) - 1);
+            const bool mine = !own || (rows >> lane & 1);
+            float sum[PIECE];
+#pragma unroll
+            for (int c = 0; c < PIECE; ++c) sum[c] = 0.f;
+#pragma unroll 1
+            for (int64_t first = i.k0; first < i.k1; first += own ? 1 : 32) {
+                const int64_t k = first + (own ? 0 : lane);
+                bool lost = false;  // every column's sum is no number any more, and stays none
+                if (k < i.k1 && mine) {
+                    const int64_t row = FORM == WEIGHT ? k : m, column = FORM == WEIGHT ? m : k;
+                    const T *const from = FORM == FORWARD ? t.b + n * t.b_stride + k : t.b + k * t.b_stride + n;
+                    float a = widen(t.a[row * t.a_stride + column]), b[PIECE];
+#pragma unroll
+                    for (int c = 0; c < PIECE; ++c) b[c] = c < left ? widen(from[FORM == FORWARD ? c * t.b_stride : c]) : 0.f;
+                    if (FORM != FORWARD && t.mask != nullptr && !(t.mask[row * t.mask_pitch + column / 8] >> (column % 8) & 1)) a = 0.f;
+                    lost = true;
+#pragma unroll
+                    for (int c = 0; c < PIECE; ++c) {
+                        sum[c] = fmaf(a, b[c], sum[c]);
+                        lost = lost && (sum[c] != sum[c] || c >= left);
+                    }
+                }
+                if (own ? __all_sync(0xffffffffu, lost || !mine) : __any_sync(0xffffffffu, lost)) break;
+                if (lane == 0 && first % 1024 < 32) atomicAdd(&waits->computed, 1);
+            }
+            if (!own) {  // every lane's sums to the first lane's: half of the columns each time, with the other half's lane
+#pragma unroll
+                for (int half = PIECE / 2; half > 0; half >>= 1)
+#pragma unroll
+                    for (int c = 0; c < half; ++c) {
+                        const bool upper = lane & (2 * half);
+                        const float kept = upper ? sum[c + half] : sum[c], given = upper ? sum[c] : sum[c + half];
+                        sum[c] = kept + __shfl_xor_sync(0xffffffffu, given, 2 * half);
+                    }
+                sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 1);
+                sum[0] = __shfl_sync(0xffffffffu, sum[0], 2 * lane & 31);  // column n + lane
+            }
+            uint32_t bits = 0;
+            [[maybe_unused]] Philox words(FORM == FORWARD ? t.epilogue.drop.key() : 0);
+#pragma unroll
+            for (int c = 0; c < PIECE; ++c)
+                if (own ? mine && c < left : c == 0 && lane < left) {
+                    const int64_t column = n + (own ? c : lane);
+                    float y = sum[c];
+                    if constexpr (FORM == FORWARD) bits |= (uint32_t)t.epilogue.element(y, m, column, words) << c;
+                    else if (!(FORM == WEIGHT && t.partial)) y *= t.scale;
+                    if (FORM == WEIGHT && t.partial) static_cast<float *>(t.out)[(i.split * t.M + m) * t.N + column] = y;
+                    else static_cast<T *>(t.out)[m * t.N + column] = narrow<T>(y);
+                }
+            if constexpr (FORM == FORWARD)
+                if (t.epilogue.mask != nullptr) {
+                    const uint32_t of_row = __ballot_sync(0xffffffffu, bits & 1);
+                    if (own ? mine : lane == 0)
+                        *reinterpret_cast<uint16_t *>(t.epilogue.mask + m * t.epilogue.mask_pitch + n / 8) = (uint16_t)(own ? bits : of_row);
+                }
+            rows = own ? 0 : rows & (rows - 1);
+        }
+    }
+    if (lane == 0) atomicAdd(&waits->computed, 1);
 }
 
 // The epilogue of one warp: 32 rows, a row a lane as they lie in the accumulators, PIECE columns at a time.  Rows of whole vectors are
@@ -497,14 +569,15 @@ struct Finish {
     float *const staging;  // [32][PIECE + 1]
     const float *const bias;
     const int lane;
+    Waits *const waits;
     Philox words;
     // of the present item
     int64_t m, n0, first;  // the lane's row, the first column, and the output's element that they are
     int columns;           // from there on, none for a row that is not there
     uint64_t passed;       // a bit for each column, 64 a turn
 
-    __device__ __forceinline__ Finish(const Tiles<T> &t_, float *staging_, const float *bias_, int lane_)
-        : t(t_), staging(staging_), bias(bias_), lane(lane_),
+    __device__ __forceinline__ Finish(const Tiles<T> &t_, float *staging_, const float *bias_, int lane_, Waits *waits_)
+        : t(t_), staging(staging_), bias(bias_), lane(lane_), waits(waits_),
           words(DROP ? t_.epilogue.drop.key() : 0) {}
 
     __device__ __forceinline__ void begin(int64_t m0, int64_t n0_) {
@@ -538,14 +611,7 @@ struct Finish {
             float none = 0.f;  // zero unless one of them is no finite number
 #pragma unroll
             for (int k = 0; k < PIECE; ++k) none = fmaf(y[k], 0.f, none);
-            if (none != 0.f && alive) {
-                float *const row = staging + lane * (PIECE + 1);
-#pragma unroll
-                for (int k = 0; k < PIECE; ++k) row[k] = y[k];
-                compute_again<T, FORM>(t, row, m, n0 + c, left, i.k0, i.k1);
-#pragma unroll
-                for (int k = 0; k < PIECE; ++k) y[k] = row[k];
-            }
+            if (none != 0.f && left > 0 && alive) atomicOr(&waits->again[threadIdx.x >> 5][c / PIECE], 1u << lane);
         }
         if (!alive) {
 #pragma unroll
@@ -845,7 +911,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t full[STAGES], empty[STAGES], sums_full[2], sums_empty[2], drained;
     __shared__ uint32_t tmem_base;
-    __shared__ int given_up;
+    __shared__ Waits waits;
     __shared__ __align__(16) float bias_of_tile[2][BN / 2];
     uint8_t *const stages = raw + (1024 - shared_address(raw) % 1024) % 1024;  // groups of eight swizzled rows lie on 1024 bytes
     [[maybe_unused]] uint8_t *const masks = stages + STAGES * S::STAGE;
@@ -866,7 +932,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             barrier_init(&sums_empty[b], EPILOGUE_WARPS);
         }
         barrier_init(&drained, 1);
-        given_up = 0;
+        waits.given_up = waits.computed = 0;
+        for (int k = 0; k < EPILOGUE_WARPS * 4; ++k) waits.again[k / 4][k % 4] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == MMA_WARP) {
@@ -889,7 +956,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         // is much: 2.45 M x 128 -> 256 bf16 forward 712 us for 450, input gradient 314 for 330.)
         constexpr int TURN = S::SPLIT || FORM == FORWARD ? PIECE : 2 * PIECE;
         const int quarter = warp & 3, half = warp >> 2;
-        Finish<T, FORM, DROP> finish(t, staging + warp * 32 * (PIECE + 1), bias_of_tile[half], lane);
+        Finish<T, FORM, DROP> finish(t, staging + warp * 32 * (PIECE + 1), bias_of_tile[half], lane, &waits);
         uint32_t segment = 0;
         [[maybe_unused]] int64_t bias_n0 = -1;  // whose bias is there
         bool alive = true;  // A warp that gave up a wait has lost count: it takes nothing and releases nothing from then on.
@@ -914,7 +981,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             finish.begin(m0, n0);
             const auto await = [&] {
                 const uint32_t buffer = segment & 1;
-                if (alive) alive = __all_sync(0xffffffffu, barrier_wait(&sums_full[buffer], segment >> 1 & 1, polls, &given_up));
+                if (alive) alive = __all_sync(0xffffffffu, barrier_wait<S::SPLIT>(&sums_full[buffer], segment >> 1 & 1, polls, &waits));
                 fence_after();
                 return buffer;
             };
@@ -970,6 +1037,11 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     if (c < pieces_end) finish.piece(x, added, i, c, alive);
                 }
             }
+            if constexpr (S::SPLIT) {  // (the accumulators have gone back already)
+                static_assert(COLUMNS / PIECE == 4, "an item's pieces have a word each");
+                __syncwarp();
+                if (__any_sync(0xffffffffu, waits.again[warp][lane & 3] != 0)) compute_again<T, FORM>(t, item, &waits);
+            }
         }
     } else if (warp < MMA_WARP) {
         // ------------------------------------------------------------------ operands to shared memory
@@ -984,7 +1056,7 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
         bool alive = true;
         int item = blockIdx.x, chunk = 0, chunks = chunks_of<T, FORM, WHOLE>(t, item);
         const auto await = [&] {
-            if (alive) alive = __all_sync(0xffffffffu, barrier_wait(&empty[s], parity, polls, &given_up));
+            if (alive) alive = __all_sync(0xffffffffu, barrier_wait<S::SPLIT>(&empty[s], parity, polls, &waits));
         };
         const auto filled = [&](uint32_t stage) {
             fence_to_async();
@@ -1008,7 +1080,7 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
                         float total = 0.f;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) total += column_parts[r * BM + p];
-                        if (*(volatile int *)&given_up) total = __uint_as_float(0x7fffffffu);
+                        if (*(volatile int *)&waits.given_up) total = __uint_as_float(0x7fffffffu);
                         t.column_sums[i.split * t.M + i.m0 + p] = total;
                     }
                     asm volatile("bar.sync 3, %0;" ::"n"(PRODUCERS) : "memory");
@@ -1109,8 +1181,8 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
                 for (int chunk = 0; alive && chunk < chunks; ++chunk) {
                     const uint32_t accumulator = tmem + buffer * 256, small = accumulator + 128;
                     const bool fresh = of_segment == 0, last = ++of_segment == S::SEGMENT || chunk + 1 == chunks;
-                    bool good = !fresh || barrier_wait(&sums_empty[buffer], buffer_parity, polls, &given_up);
-                    good = good && barrier_wait(&full[s], parity, polls, &given_up);
+                    bool good = !fresh || barrier_wait<S::SPLIT>(&sums_empty[buffer], buffer_parity, polls, &waits);
+                    good = good && barrier_wait<S::SPLIT>(&full[s], parity, polls, &waits);
                     alive = __all_sync(0xffffffffu, good);
                     if (!alive) break;
                     fence_after();
@@ -1152,7 +1224,7 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
             for (; alive && issued > 0; --issued) {  // the last reports have come in
                 if (s == 0) s = STAGES, parity ^= 1;
                 --s;
-                alive = __all_sync(0xffffffffu, barrier_wait(&empty[s], parity, polls, &given_up));
+                alive = __all_sync(0xffffffffu, barrier_wait<S::SPLIT>(&empty[s], parity, polls, &waits));
             }
             if (!alive && leads) {  // products that are still under way read shared memory and write the accumulators
                 commit(&drained);
@@ -1169,7 +1241,7 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
                 const uint8_t *image = t.packed + (n0 / BN) * chunks * PLANES * S::B_PLANE;
                 for (int chunk = 0; alive && chunk < chunks; ++chunk, ++round, image += PLANES * S::B_PLANE) {
                     const uint32_t s = round % STAGES;
-                    alive = barrier_wait(&empty[s], (round / STAGES & 1) ^ 1, polls, &given_up);
+                    alive = barrier_wait<S::SPLIT>(&empty[s], (round / STAGES & 1) ^ 1, polls, &waits);
                     if (!alive) break;
                     const uint32_t to = shared_address(stages) + s * S::STAGE + PLANES * S::A_PLANE;
                     barrier_expect(&full[s], rows * (BK * 2) * PLANES);
@@ -1187,7 +1259,7 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (threadIdx.x == 0 && given_up) atomicOr(&g_linear_status, STATUS_WAIT_EXPIRED);
+    if (threadIdx.x == 0 && waits.given_up) atomicOr(&g_linear_status, STATUS_WAIT_EXPIRED);
     if (warp == MMA_WARP) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLUMNS) : "memory");

@@ -80,3 +80,119 @@ def test_gradients_with_a_frozen_weight(dtype, rows):
     dx, beside = torch.autograd.grad(rt.linear(x, w, b), (x, b), grad)
     assert torch.equal(alone, grad.double().sum(0).to(dtype)) and torch.equal(alone, beside)
     assert torch.equal(dx, (grad.double() @ w.double()).to(dtype))
+
+
+# ---------------------------------------------------------------------------------------------
+# infinities and NaN
+# ---------------------------------------------------------------------------------------------
+def terms(n, dtype=F32):
+    """Half steps of an fp32 sum of n terms on the tensor cores, of the sum of their sizes: n roundings of a sum, and 2 n for the
+    truncations of every sixteen and the parts left out of fp32's three."""
+    return (3 * n + 32) * (2.0**-53 if dtype == F64 else 2.0**-24)
+
+
+def compare(got, want, bound, what):
+    """64-bit results with what fp32 makes of them: NaN and infinities in their places, the others within their bound."""
+    narrowed = want.float()
+    assert torch.equal(torch.isnan(got), torch.isnan(narrowed)), f"{what}: NaN"
+    sure = torch.isinf(want)  # (a large finite sum may lie on either side of the type's end)
+    assert torch.equal(got[sure], narrowed[sure]), f"{what}: infinities"
+    ordinary = torch.isfinite(want) & (want.abs() < 2.0**126)
+    excess = ((got.double() - want).abs() - bound)[ordinary]
+    assert excess.numel() == 0 or excess.max() <= 0, f"{what}: over its bound by {excess.max():.3e}"
+
+
+def finite(t):
+    return torch.nan_to_num(t.double(), 0.0, 0.0, 0.0).abs()
+
+
+BAD = [float("inf"), float("-inf"), float("nan"), torch.finfo(F32).max]
+
+
+@pytest.mark.parametrize("which", ["grad", "x", "weight"])
+@pytest.mark.parametrize("rows, inner, outer", [(20000, 256, 4096), (300000, 72, 136), (3001, 1030, 301)])
+@pytest.mark.parametrize("relu", [False, True])
+def test_gradients_with_numbers_that_are_not_finite(which, rows, inner, outer, relu):
+    """They reach the elements that they have a part in and no others, whatever a multiprocessor's further tiles wait for meanwhile."""
+    x, w, b = rand(rows, inner, seed=1), rand(outer, inner, seed=2, scale=inner**-0.5), rand(outer, seed=3)
+    grad = rand(rows, outer, seed=4)
+    activation = "relu" if relu else None
+
+    def both():
+        leaves = [t.detach().clone().requires_grad_() for t in (x, w, b)]
+        y = rt.linear(*leaves, activation)
+        return [y.detach(), *torch.autograd.grad(y, leaves, grad)]
+    clean = both()
+    held = {"grad": grad, "x": x, "weight": w}[which]
+    places = [(held.size(0) // 2 + 3 * i, held.size(1) - 1 - 37 * i) for i in range(len(BAD))]
+    for place, bad in zip(places, BAD):
+        held[place] = bad
+    assert rt.device_status() == 0
+    y, dx, dw, db = both()
+    assert rt.device_status() == 0
+    z = x.double() @ w.double().t() + b.double()
+    sizes = finite(x) @ finite(w).t() + b.double().abs()
+    got_z = rt.linear(x, w, b)
+    compare(got_z, z, (terms(inner) + 2.0**-24) * sizes + 2.0**-149, "z")
+    assert torch.equal(y, torch.where(got_z <= 0, 0.0, got_z) if relu else got_z) or \
+        torch.equal(torch.isnan(y), torch.isnan(got_z)) and torch.equal(y[~torch.isnan(y)], torch.where(got_z <= 0, 0.0, got_z)[~torch.isnan(y)]
+                                                                        if relu else got_z[~torch.isnan(y)])
+    g = torch.where(got_z <= 0, 0.0, grad.double()) if relu else grad.double()
+    del z, sizes
+    compare(dx, g @ w.double(), terms(outer) * (finite(g) @ finite(w)) + 2.0**-149, "dx")
+    compare(dw, g.t() @ x.double(), terms(rows) * (finite(g).t() @ finite(x)) + 2.0**-149, "dweight")
+    compare(db, g.sum(0), terms(rows) * finite(g).sum(0) + 2.0**-149, "dbias")
+    # what has no part in them is what it was, to the bit
+    rows_of, columns_of = (torch.ones(held.size(d), dtype=torch.bool, device="cuda") for d in (0, 1))
+    for r, c in places:
+        rows_of[r] = columns_of[c] = False
+    if which == "grad":
+        assert torch.equal(dx[rows_of], clean[1][rows_of]) and torch.equal(dw[columns_of], clean[2][columns_of])
+        assert torch.equal(db[columns_of], clean[3][columns_of]) and torch.equal(y, clean[0])
+    elif which == "x":
+        assert torch.equal(y[rows_of], clean[0][rows_of]) and torch.equal(dx[rows_of], clean[1][rows_of])
+
+
+@pytest.mark.parametrize("columns", [128, 131])
+@pytest.mark.parametrize("p, added", [(0.0, False), (0.25, True)])
+def test_forward_with_numbers_that_are_not_finite_and_what_follows(columns, p, added):
+    x, w, b = rand(40000, 96, seed=1), rand(columns, 96, seed=2, scale=0.1), rand(columns, seed=3)
+    residual = rand(40000, columns, seed=5) if added else None
+    x[5, 0], x[20000, 95], x[39999, 50], x[39998, 50] = BAD
+    y = rt.linear(x, w, b, "relu", p, residual, seed=7)
+    z = rt.linear(x, w, b)
+    want = torch.where(z <= 0, 0.0, z)
+    if p:
+        kept = rt.dropout(torch.ones_like(z), p, seed=7) != 0
+        want = torch.where(kept, want * (1 / (1 - p)), 0.0)
+    if added:
+        want = want + residual
+    assert torch.equal(y.isnan(), want.isnan())
+    assert torch.equal(y[~y.isnan()], want[~y.isnan()])
+    # the mask, by the gradient of a constant: what the ReLU and the dropout let through
+    one = torch.zeros(columns, device="cuda", requires_grad=True)
+    g = rand(40000, columns, seed=6)
+    db, = torch.autograd.grad(rt.linear(x, w, b + one, "relu", p, residual, seed=7), one, g)
+    passed = ~(z <= 0) & (kept if p else True)
+    exact = torch.where(passed, g, 0.0).double().sum(0) / (1 - p)
+    assert ((db.double() - exact).abs() <= terms(40000) * g.double().abs().sum(0)).all()
+    assert rt.device_status() == 0
+
+
+def test_waits_go_on_while_elements_are_computed_again():
+    """A row of 4096 sums over 20,000 nodes by lanes takes milliseconds, a wait of 2^14 polls some tenths of one: the tiles behind the
+    row's wait for as long as it takes."""
+    x, grad = rand(20000, 4096, seed=1), rand(20000, 4096, seed=2)
+    w = torch.zeros(4096, 4096, device="cuda", requires_grad=True)
+    before = rt.lib().cgnn_linear_wait_limit(1 << 14)
+    try:
+        clean, = torch.autograd.grad(rt.linear(x, w), w, grad)
+        assert rt.device_status() == 0
+        grad[777, 1000] = float("inf")
+        got, = torch.autograd.grad(rt.linear(x, w), w, grad)
+        assert rt.device_status() == 0
+    finally:
+        rt.lib().cgnn_linear_wait_limit(before)
+    others = torch.arange(4096, device="cuda") != 1000
+    assert torch.equal(got[others], clean[others])
+    assert torch.equal(got[1000], torch.copysign(torch.full_like(got[1000], float("inf")), x[777]))
