@@ -1367,7 +1367,7 @@ template <typename T>
 size_t tiles_backward_bytes(int64_t rows, int64_t in, int64_t out) {
     int64_t per_split;
     const int64_t splits = weight_splits<T>(rows, in, out, &per_split);
-    return packed_bytes<T>(in, out) + (size_t)splits * out * (in + 1) * sizeof(float) + 64;
+    return packed_bytes<T>(in, out) + (size_t)splits * out * ((splits > 1 ? in : 0) + 1) * sizeof(float) + 64;
 }
 
 template <typename T>
@@ -1398,7 +1398,7 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
     int64_t per_split;
     const int64_t splits = weight_splits<T>(c.rows, c.in, c.out, &per_split);
     float *const parts = reinterpret_cast<float *>(align_up((size_t)packed + packed_bytes<T>(c.in, c.out), 32));
-    float *const sums = parts + splits * c.out * c.in;
+    float *const sums = splits > 1 ? parts + splits * c.out * c.in : parts;
     t.b = static_cast<const T *>(c.x);
     t.b_stride = c.stride;
     t.packed = nullptr;
