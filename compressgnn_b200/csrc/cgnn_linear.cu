@@ -387,7 +387,7 @@ size_t cgnn_linear_mask_bytes(int64_t rows, int64_t out) { return rows <= 0 || o
 size_t cgnn_linear_scratch_bytes(int dtype, int64_t rows, int64_t in, int64_t out) {
     if (dtype < CGNN_F32 || dtype > CGNN_F16 || rows <= 0 || in <= 0 || out <= 0 || in >= WIDEST || out >= WIDEST) return 0;
     if (!by_tiles(dtype, rows, in, out)) return 0;
-    return bytes_of_type(dtype, [&](auto zero) { return tiles_forward_bytes<decltype(zero)>(in, out); });
+    return bytes_of_type(dtype, [&](auto zero) { return tiles_forward_bytes<decltype(zero)>(rows, in, out); });
 }
 
 int cgnn_linear(int dtype, int64_t rows, int64_t in, int64_t out, int64_t stride, const void *x, const void *weight, const void *bias,

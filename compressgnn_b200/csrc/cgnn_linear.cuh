@@ -71,7 +71,7 @@ static int join(const P *parts, int64_t splits, int64_t n, double scale, T *out,
 
 // The products on the tensor cores (fp32, bf16, fp16).
 template <typename T>
-size_t tiles_forward_bytes(int64_t in, int64_t out);
+size_t tiles_forward_bytes(int64_t rows, int64_t in, int64_t out);
 template <typename T>
 int tiles_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T *y, void *scratch, int polls, cudaStream_t stream);
 template <typename T>

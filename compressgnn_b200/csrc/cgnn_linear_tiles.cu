@@ -49,6 +49,12 @@ constexpr int SMS = 148;
 constexpr int TMEM_COLUMNS = 512;  // two buffers of 256
 constexpr int PIECE = 16;          // columns that a warp of the epilogue takes at once
 
+// Terms of 16-bit operands that an accumulator takes: its truncations lose 1e-7 of a sum of one sign for every sixteen, so 5e-5 of so
+// many (half a step of fp16 is 4.9e-4; 300,000 terms in one accumulator were 2e-3 off).  Longer contractions add up in fp32
+// in memory, a segment after the other (weight gradients without the bias' in bf16: 2.45 M x 128 -> 256 310 us, in one accumulator
+// 292; 16,384 x 4096 -> 4096 496 and 470).
+constexpr int LONGEST = 8192;
+
 // A stage holds BK of the contraction: rows of BK 16-bit elements (FORWARD, INPUT), or BK rows of panels of 64 (WEIGHT).
 //
 // HBM wants 35 KB on their way to each multiprocessor.  16-bit operands are copied asynchronously to where the tensor core
@@ -67,7 +73,7 @@ struct Shape {
     static constexpr int STAGE = PLANES * (A_PLANE + B_PLANE);
     static constexpr int STAGES = SPLIT || FORM != WEIGHT || WHOLE ? 4 : 7;
     static constexpr int AHEAD = 1;  // of a group's own chunks
-    static constexpr int SEGMENT = SPLIT ? 256 / BK : 1 << 30;  // chunks of BK that an accumulator takes
+    static constexpr int SEGMENT = (SPLIT ? 256 : LONGEST) / BK;  // chunks of BK that an accumulator takes
     static constexpr int GROUPS = SPLIT && FORM == WEIGHT ? 1 : 2, MEMBERS = PRODUCERS / GROUPS;  // producers that fill a stage
     static constexpr int A_UNITS = BM * BK / 8 / MEMBERS, B_UNITS = FORM == WEIGHT ? BN * BK / 8 / MEMBERS : 0;
     static constexpr int MASK_SLOT = ASYNC && FORM != FORWARD ? A_UNITS * MEMBERS : 0;  // a word of the mask for four units of a row
@@ -93,6 +99,8 @@ struct Tiles {
     int out_whole, out_wide;      // rows of the output and the residual lie on vectors of 8 elements, of 32 bytes
     void *out;                    // [M, N] of T, or (WEIGHT of several splits) [splits, M, N] of fp32
     int partial;
+    float *running;               // contractions of more than LONGEST, 16 bits: [M, N] (WEIGHT: of each split) of fp32
+    int running_whole;            // its rows lie on vectors of 8
     float *column_sums;           // WEIGHT: [splits, M]
     float scale;
     Epilogue<T> epilogue;         // FORWARD
@@ -680,6 +688,31 @@ struct Finish {
         if (FORM == WEIGHT && t.partial) write(static_cast<float *>(t.out) + i.split * t.M * t.N, c, left, y);
         else write(static_cast<T *>(t.out), c, left, y);
     }
+    // Columns c .. c + PIECE of the item's sum over the segments before, added or left for the next.  (A lane comes back to its own.)
+    __device__ __forceinline__ void add_running(const float *sums, int c, float (&x)[PIECE]) {
+        const float *const p = sums + first + c;
+        const int left = columns - c;
+        float before[PIECE];
+        if (t.running_whole) {
+            load16(p, left, true, before);
+        } else {
+#pragma unroll
+            for (int k = 0; k < PIECE; ++k) before[k] = k < left ? p[k] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < PIECE; ++k) x[k] += before[k];
+    }
+    __device__ __forceinline__ void leave_running(float *sums, int c, const float (&x)[PIECE]) {
+        float *const p = sums + first + c;
+        const int left = columns - c;
+        if (t.running_whole) {
+            store16(p, left, true, x);
+        } else {
+#pragma unroll
+            for (int k = 0; k < PIECE; ++k)
+                if (k < left) p[k] = x[k];
+        }
+    }
     template <typename O>
     __device__ __forceinline__ void write(O *out, int c, int left, const float (&y)[PIECE]) {
         if (t.out_whole) {
@@ -902,7 +935,7 @@ struct Producer {
     }
 };
 
-// MANY: fp32 contractions of more than one segment, whose sums take registers that the others keep.  DROP: a forward pass with
+// MANY: contractions of more than one segment: in fp32 their sums take registers that the others keep.  DROP: a forward pass with
 // dropout, whose instructions the others do without (they are read again for every sixteen columns).
 template <typename T, int FORM, bool WHOLE, bool MANY, bool DROP>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ Tiles<T> t) {
@@ -993,7 +1026,23 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             };
             int before = 0;  // segments ahead of the last
             if constexpr (MANY) before = (chunks_of<T, FORM, WHOLE>(t, item) - 1) / S::SEGMENT;
-            if (before == 0) {
+            if constexpr (MANY && !S::SPLIT) {
+                float *const running = t.running + (FORM == WEIGHT ? i.split * t.M * t.N : 0);
+                for (int s = 0; s <= before; ++s) {
+                    const uint32_t buffer = await();
+#pragma unroll 1
+                    for (int c = 0; c < COLUMNS; c += PIECE) {
+                        float x[PIECE], added[PIECE];
+                        if (s == before && c < pieces_end) finish.fetch(c, added);
+                        if (alive) tmem_load16<false>(rows + buffer * 256 + c, x);
+                        if (c + PIECE == COLUMNS) release(buffer);
+                        if (c >= pieces_end) continue;
+                        if (s > 0) finish.add_running(running, c, x);
+                        if (s < before) finish.leave_running(running, c, x);
+                        else finish.piece(x, added, i, c, alive);
+                    }
+                }
+            } else if (before == 0) {
                 const uint32_t buffer = await();
 #pragma unroll 1
                 for (int c = 0; c < COLUMNS; c += TURN) {
@@ -1309,9 +1358,8 @@ int launch(Tiles<T> &t, int64_t splits, cudaStream_t stream) {
     // (fp32 units are loaded at once, and are there or not)
     const bool whole = whole_rows(t.a, t.a_stride, sizeof(T)) && (FORM != WEIGHT || whole_rows(t.b, t.b_stride, sizeof(T))) &&
                        (!Tile<T, FORM>::SPLIT || ((FORM == WEIGHT ? t.M : t.K) % 8 == 0 && (FORM != WEIGHT || t.N % 8 == 0)));
-    if constexpr (Tile<T, FORM>::SPLIT)
-        if (t.k_per_item > Tile<T, FORM>::SEGMENT * Tile<T, FORM>::BK)
-            return whole ? launch_dropping<T, FORM, true, true>(t, stream) : launch_dropping<T, FORM, false, true>(t, stream);
+    if (t.k_per_item > Tile<T, FORM>::SEGMENT * Tile<T, FORM>::BK)
+        return whole ? launch_dropping<T, FORM, true, true>(t, stream) : launch_dropping<T, FORM, false, true>(t, stream);
     return whole ? launch_dropping<T, FORM, true, false>(t, stream) : launch_dropping<T, FORM, false, false>(t, stream);
 }
 
@@ -1327,9 +1375,24 @@ int pack(const T *weight, int64_t in, int64_t N, int64_t K, uint8_t *packed, cud
 
 }  // namespace
 
+// Whether sums over the segments lie in memory, [rows, columns] of them.
 template <typename T>
-size_t tiles_forward_bytes(int64_t in, int64_t out) {
-    return packed_bytes<T>(out, in);
+static bool in_segments(int64_t terms) {
+    return !Tile<T, FORWARD>::SPLIT && terms > LONGEST;
+}
+template <typename T>
+static size_t running_bytes(int64_t rows, int64_t columns, int64_t terms) {
+    return in_segments<T>(terms) ? (size_t)rows * columns * sizeof(float) + 32 : 0;
+}
+template <typename T>
+static void set_running(Tiles<T> &t, void *behind) {
+    t.running = reinterpret_cast<float *>(align_up((size_t)behind, 32));
+    t.running_whole = t.N % 8 == 0;
+}
+
+template <typename T>
+size_t tiles_forward_bytes(int64_t rows, int64_t in, int64_t out) {
+    return packed_bytes<T>(out, in) + running_bytes<T>(rows, out, in);
 }
 
 template <typename T>
@@ -1348,6 +1411,7 @@ int tiles_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T
     t.K = t.k_per_item = c.in;
     set_out(t, y, c.out, sizeof(T));
     if (epilogue.residual != nullptr) t.out_whole = t.out_whole && whole_rows(epilogue.residual, c.out, sizeof(T));
+    set_running(t, packed + packed_bytes<T>(c.out, c.in));
     t.epilogue = epilogue;
     t.polls = polls;
     return launch<T, FORWARD>(t, 1, stream);
@@ -1367,7 +1431,10 @@ template <typename T>
 size_t tiles_backward_bytes(int64_t rows, int64_t in, int64_t out) {
     int64_t per_split;
     const int64_t splits = weight_splits<T>(rows, in, out, &per_split);
-    return packed_bytes<T>(in, out) + (size_t)splits * out * ((splits > 1 ? in : 0) + 1) * sizeof(float) + 64;
+    // (the input's gradient and then the weight's take what is behind the weight's image)
+    const bool parts = splits > 1 || in_segments<T>(per_split);
+    const size_t of_weight = (size_t)splits * out * ((parts ? in : 0) + 1) * sizeof(float) + 64;
+    return packed_bytes<T>(in, out) + std::max(of_weight, running_bytes<T>(rows, in, out));
 }
 
 template <typename T>
@@ -1391,6 +1458,7 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
         t.N = c.in;
         t.K = t.k_per_item = c.out;
         set_out(t, dx, c.in, sizeof(T));
+        set_running(t, packed + packed_bytes<T>(c.in, c.out));
         rc = launch<T, INPUT>(t, 1, stream);
         if (rc != CGNN_OK) return rc;
     }
@@ -1398,7 +1466,7 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
     int64_t per_split;
     const int64_t splits = weight_splits<T>(c.rows, c.in, c.out, &per_split);
     float *const parts = reinterpret_cast<float *>(align_up((size_t)packed + packed_bytes<T>(c.in, c.out), 32));
-    float *const sums = splits > 1 ? parts + splits * c.out * c.in : parts;
+    float *const sums = splits > 1 || in_segments<T>(per_split) ? parts + splits * c.out * c.in : parts;
     t.b = static_cast<const T *>(c.x);
     t.b_stride = c.stride;
     t.packed = nullptr;
@@ -1408,6 +1476,7 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
     t.k_per_item = per_split;
     t.partial = splits > 1;
     set_out(t, t.partial ? static_cast<void *>(parts) : dweight, c.in, t.partial ? sizeof(float) : sizeof(T));
+    set_running(t, parts);  // (of several splits the parts themselves)
     t.column_sums = dbias != nullptr ? sums : nullptr;
     int rc = launch<T, WEIGHT>(t, splits, stream);
     if (rc == CGNN_OK && t.partial) rc = join(parts, splits, c.out * c.in, scale, dweight, stream);
@@ -1416,7 +1485,7 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
 }
 
 #define CGNN_TILES_OF(T)                                                                                                        \
-    template size_t tiles_forward_bytes<T>(int64_t, int64_t);                                                                   \
+    template size_t tiles_forward_bytes<T>(int64_t, int64_t, int64_t);                                                                   \
     template int tiles_forward<T>(const Call &, const T *, const Epilogue<T> &, T *, void *, int, cudaStream_t);                \
     template size_t tiles_backward_bytes<T>(int64_t, int64_t, int64_t);                                                         \
     template int tiles_backward<T>(const Call &, const T *, const T *, const uint8_t *, double, T *, T *, T *, void *, int, \

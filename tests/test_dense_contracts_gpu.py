@@ -196,3 +196,75 @@ def test_waits_go_on_while_elements_are_computed_again():
     others = torch.arange(4096, device="cuda") != 1000
     assert torch.equal(got[others], clean[others])
     assert torch.equal(got[1000], torch.copysign(torch.full_like(got[1000], float("inf")), x[777]))
+
+
+# ---------------------------------------------------------------------------------------------
+# long contractions of 16-bit operands
+# ---------------------------------------------------------------------------------------------
+def positive(*shape, dtype, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.rand(*shape, device="cuda", generator=gen).mul_(0.2).add_(0.1).to(dtype)
+
+
+def within_one_rounding(got, want, what):
+    """One rounding of the result.  In front of it an accumulator takes up to 8192 terms in 512 additions, each off by at most two steps
+    of 2^-23 of a sum that is half of the last on average (together 2^-14), and no more than 64 such sums are added."""
+    relative = ((got.double() - want) / want).abs().max()
+    assert relative <= torch.finfo(got.dtype).eps / 2 + 2.0**-14 + 64 * 2.0**-24, f"{what}: {relative:.3e}"
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows, inner, outer", [(300000, 2048, 1280), (300001, 2045, 1277), (700000, 64, 128), (9000, 2048, 1280)])
+def test_weight_gradients_of_one_sign_over_many_rows(dtype, rows, inner, outer):
+    """In one split and in many: sums that only grow keep their last digits."""
+    x, grad = positive(rows, inner, dtype=dtype, seed=1), positive(rows, outer, dtype=dtype, seed=2)
+    w = torch.zeros(outer, inner, dtype=dtype, device="cuda", requires_grad=True)
+    b = torch.zeros(outer, dtype=dtype, device="cuda", requires_grad=True)
+    dw, db = torch.autograd.grad(rt.linear(x, w, b), (w, b), grad)
+    some = torch.arange(0, inner, max(1, inner // 61), device="cuda")
+    within_one_rounding(dw[:, some], grad.double().t() @ x[:, some].double(), "dweight")
+    if dtype == BF16 or rows < 300000:  # (fp16 ends at 65504)
+        within_one_rounding(db, grad.double().sum(0), "dbias")
+    assert rt.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows, terms_, columns", [(256, 400000, 128), (300, 100001, 131), (20000, 8200, 40)])
+def test_products_of_one_sign_and_many_terms(dtype, rows, terms_, columns):
+    x, w = positive(rows, terms_, dtype=dtype, seed=1), positive(columns, terms_, dtype=dtype, seed=2)
+    b, residual = positive(columns, dtype=dtype, seed=3), positive(rows, columns, dtype=dtype, seed=4)
+    want = x.double() @ w.double().t()
+    within_one_rounding(rt.linear(x, w), want, "forward")
+    within_one_rounding(rt.linear(x, w, b, "relu", residual=residual), want + b.double() + residual.double(), "with what follows")
+    # the same contraction in the gradient of an input
+    leaf = torch.zeros(rows, columns, dtype=dtype, device="cuda", requires_grad=True)
+    dx, = torch.autograd.grad(rt.linear(leaf, w.t().contiguous()), leaf, x)
+    within_one_rounding(dx, want, "dx")
+    assert rt.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows, inner, outer", [(20011, 1200, 2056), (20011, 1203, 2055), (140, 20011, 136), (140, 20008, 131), (131, 136, 20011)])
+@pytest.mark.parametrize("relu, p", [(False, 0.0), (True, 0.5)])
+def test_whole_numbers_over_several_segments(dtype, rows, inner, outer, relu, p):
+    """Sums of few terms, among them those at the ends of segments and of the contraction: exact."""
+    x, w = torch.zeros(rows, inner, dtype=dtype, device="cuda"), torch.zeros(outer, inner, dtype=dtype, device="cuda")
+    grad = torch.zeros(rows, outer, dtype=dtype, device="cuda")
+    for t, d in ((x, 0), (x, 1), (w, 0), (w, 1), (grad, 0), (grad, 1)):
+        for i, at in enumerate((0, 63, 64, 4095, 8191, 8192, 8193, 16383, 16384, t.size(d) - 1)):
+            if at < t.size(d):
+                part = whole(t.size(1 - d), dtype=dtype, seed=7 * i + d, largest=3)
+                t[at].copy_(part) if d == 0 else t[:, at].copy_(part)
+    b = whole(outer, dtype=dtype, seed=5)
+    for t in (x, w, b):
+        t.requires_grad_()
+    y = rt.linear(x, w, b, "relu" if relu else None, p, seed=11)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), grad)
+    with torch.no_grad():
+        z = x.double() @ w.double().t() + b.double()
+        factor = torch.where(z > 0, 1.0, 0.0) if relu else torch.ones_like(z)
+        if p:
+            factor = factor * (rt.dropout(torch.ones_like(y), p, seed=11) != 0) * 2
+        g = grad.double() * factor
+        for got, want in ((y, z * factor), (dx, g @ w.double()), (dw, g.t() @ x.double()), (db, g.sum(0))):
+            assert torch.equal(got, want.to(dtype))
