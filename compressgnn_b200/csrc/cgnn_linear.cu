@@ -35,7 +35,6 @@ struct Small {
     int64_t mask_pitch;
     int64_t k_per_split;
     void *out;                    // FORWARD, INPUT: [M, N] of T; WEIGHT: [splits, M, N] sums, or, of one split, T
-    void *column_sums;            // WEIGHT: [splits, M] sums of A over k, or of one split T; may be null
     double scale;
     Epilogue<T> epilogue;         // FORWARD
 };
@@ -52,7 +51,7 @@ __global__ void __launch_bounds__(GROUPS *TILE_THREADS) small_kernel(const Small
     const int64_t m0 = (blockIdx.x / tiles_n) * TM, n0 = (blockIdx.x % tiles_n) * TN;
     const int64_t k_begin = (int64_t)blockIdx.y * s.k_per_split, k_end = min(s.K, k_begin + s.k_per_split);
     const int tx = thread % 16, ty = thread / 16;  // columns tx + 16 j, rows ty * 4 + i
-    A acc[4][4], sum = A(0);
+    A acc[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -79,9 +78,6 @@ __global__ void __launch_bounds__(GROUPS *TILE_THREADS) small_kernel(const Small
             bs[k][n] = n0 + n < s.N && k0 + k < k_end ? A(widen(s.b[(n0 + n) * s.b_n + (k0 + k) * s.b_k])) : A(0);
         }
         __syncthreads();
-        if (FORM == WEIGHT && threadIdx.x < TM)
-#pragma unroll
-            for (int k = 0; k < TK; ++k) sum += as[k][threadIdx.x];
 #pragma unroll
         for (int k = 0; k < TK; ++k) {
             A av[4], bv[4];
@@ -97,7 +93,6 @@ __global__ void __launch_bounds__(GROUPS *TILE_THREADS) small_kernel(const Small
         __syncthreads();
     }
     if constexpr (GROUPS > 1) {  // (the last stage's barrier is behind every thread: its place is free)
-        static_assert(FORM != WEIGHT, "column sums are not joined");
         static_assert(16 * TILE_THREADS <= GROUPS * TK * (TN + 1), "a group's sums are wider than the stages");
         A *const sums = &bs_of[0][0][0];
         for (int g = 1; g < GROUPS; ++g) {
@@ -113,11 +108,6 @@ __global__ void __launch_bounds__(GROUPS *TILE_THREADS) small_kernel(const Small
         if (group > 0) return;
     }
     const bool whole = gridDim.y == 1;
-    if (FORM == WEIGHT && s.column_sums != nullptr && n0 == 0 && threadIdx.x < TM && m0 + threadIdx.x < s.M) {
-        const int64_t m = m0 + threadIdx.x;
-        if (whole) static_cast<T *>(s.column_sums)[m] = narrow<T>(sum * (A)s.scale);
-        else static_cast<A *>(s.column_sums)[blockIdx.y * s.M + m] = sum;
-    }
     if constexpr (FORM == FORWARD) {
         Philox words(s.epilogue.drop.key());
 #pragma unroll
@@ -183,11 +173,11 @@ int small_product(Small<T> &s, int64_t splits, cudaStream_t stream) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// the bias' gradient alone: column sums of z, for which neither x nor the weight is looked at
+// the bias' gradient by itself: column sums of z, for which neither x nor the weight is looked at
 // ---------------------------------------------------------------------------------------------
-constexpr int COLUMN_WARPS = 8, COLUMN_UNROLL = 8;
-constexpr int64_t COLUMN_BLOCKS = 148 * 8, COLUMN_ROWS = COLUMN_WARPS * COLUMN_UNROLL;  // rows: of a block, at least
+constexpr int64_t COLUMN_BLOCKS = 148 * 8;
 
+// None of fewer rows than a block has on their way.
 int64_t column_splits(int64_t rows, int64_t out) {
     return std::max<int64_t>(1, std::min<int64_t>(COLUMN_BLOCKS / ceil_div(out, 32), rows / COLUMN_ROWS));
 }
@@ -197,55 +187,19 @@ size_t column_bytes(int64_t rows, int64_t out) {
     return splits == 1 ? 0 : (size_t)splits * (size_t)out * sizeof(double);
 }
 
-// A lane has a column, a warp every eighth row with COLUMN_UNROLL of them on their way.  The grid's second dimension splits the rows:
-// parts[blockIdx.y, column], or, of one split, the sums themselves.  HBM bounds it, with fp64 sums too.
-template <typename T>
-__global__ void __launch_bounds__(COLUMN_WARPS * 32) columns_kernel(const T *grad, const uint8_t *mask, int64_t mask_pitch, int64_t rows,
-                                                                    int64_t rows_per_split, int64_t width, double scale, double *parts,
-                                                                    T *out) {
-    __shared__ double sums[COLUMN_WARPS][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t c0 = (int64_t)blockIdx.x * 32, c = c0 + lane;
-    const int64_t end = min(rows, ((int64_t)blockIdx.y + 1) * rows_per_split);
-    double s = 0.0;
-    if (c < width) {
-        for (int64_t row = (int64_t)blockIdx.y * rows_per_split + warp; row < end; row += COLUMN_ROWS) {
-            T v[COLUMN_UNROLL];
-            uint32_t keep[COLUMN_UNROLL];
-#pragma unroll
-            for (int u = 0; u < COLUMN_UNROLL; ++u) {
-                const int64_t r = row + u * COLUMN_WARPS;
-                v[u] = r < end ? grad[r * width + c] : narrow<T>(Acc<T>(0));
-                // (a row of the mask is whole 64-bit words)
-                keep[u] = mask != nullptr && r < end ? *reinterpret_cast<const uint32_t *>(mask + r * mask_pitch + c0 / 8) : 0xffffffffu;
-            }
-#pragma unroll
-            for (int u = 0; u < COLUMN_UNROLL; ++u)
-                if (keep[u] >> lane & 1) s += (double)widen(v[u]);
-        }
-    }
-    sums[warp][lane] = s;
-    __syncthreads();
-    if (warp > 0 || c >= width) return;
-#pragma unroll
-    for (int w = 1; w < COLUMN_WARPS; ++w) s += sums[w][lane];
-    if (gridDim.y == 1) out[c] = narrow<T>((Acc<T>)(s * scale));
-    else parts[blockIdx.y * width + c] = s;
-}
-
 template <typename T>
 int column_sums(const Call &c, const T *grad, const uint8_t *mask, double scale, T *dbias, void *scratch, cudaStream_t stream) {
     const int64_t splits = column_splits(c.rows, c.out);
     double *const parts = static_cast<double *>(scratch);
-    columns_kernel<T><<<dim3((unsigned)ceil_div(c.out, 32), (unsigned)splits), COLUMN_WARPS * 32, 0, stream>>>(
+    columns_kernel<T, T><<<dim3((unsigned)ceil_div(c.out, 32), (unsigned)splits), COLUMN_WARPS * 32, 0, stream>>>(
         grad, mask, mask_pitch(c.out), c.rows, ceil_div(c.rows, splits), c.out, scale, parts, dbias);
     CGNN_LAUNCH_CHECK();
-    return splits == 1 ? CGNN_OK : join(parts, splits, c.out, scale, dbias, stream);
+    return splits == 1 ? CGNN_OK : join_columns(parts, splits, c.out, scale, dbias, stream);
 }
 
 size_t small_backward_bytes(int64_t acc_bytes, int64_t rows, int64_t in, int64_t out) {
     const int64_t splits = small_splits(rows, in, out);
-    return splits == 1 ? 0 : (size_t)splits * (size_t)out * (size_t)(in + 1) * (size_t)acc_bytes;
+    return splits == 1 ? 0 : (size_t)splits * (size_t)out * (size_t)in * (size_t)acc_bytes;
 }
 
 template <typename T>
@@ -266,8 +220,8 @@ int small_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T
 }
 
 template <typename T>
-int small_backward(const Call &c, const T *weight, const T *grad, const uint8_t *mask, double scale, T *dx, T *dweight, T *dbias,
-                   void *scratch, cudaStream_t stream) {
+int small_backward(const Call &c, const T *weight, const T *grad, const uint8_t *mask, double scale, T *dx, T *dweight, void *scratch,
+                   cudaStream_t stream) {
     using A = Acc<T>;
     Small<T> s{};
     s.a = grad;
@@ -297,13 +251,10 @@ int small_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
     s.N = c.in;
     s.K = c.rows;
     const int64_t splits = small_splits(c.rows, c.in, c.out);
-    A *const parts = static_cast<A *>(scratch), *const sums = parts + splits * c.out * c.in;
+    A *const parts = static_cast<A *>(scratch);
     s.out = splits == 1 ? static_cast<void *>(dweight) : parts;
-    s.column_sums = dbias == nullptr ? nullptr : splits == 1 ? static_cast<void *>(dbias) : sums;
-    int rc = small_product<T, WEIGHT>(s, splits, stream);
-    if (rc == CGNN_OK && splits > 1) rc = join(parts, splits, c.out * c.in, scale, dweight, stream);
-    if (rc == CGNN_OK && splits > 1 && dbias != nullptr) rc = join(sums, splits, c.out, scale, dbias, stream);
-    return rc;
+    const int rc = small_product<T, WEIGHT>(s, splits, stream);
+    return rc == CGNN_OK && splits > 1 ? join(parts, splits, c.out * c.in, scale, dweight, stream) : rc;
 }
 
 template <typename T>
@@ -352,7 +303,10 @@ int forward(const Call &c, const void *weight, const void *bias, const void *res
 template <typename T>
 int backward(const Call &c, const void *weight, const void *mask, const void *grad, double scale, void *dx, void *dweight, void *dbias,
              void *scratch, bool tiles, cudaStream_t stream) {
-    if (dweight == nullptr && dbias != nullptr) {  // (behind it on the stream the input's gradient takes the scratch anew)
+    // The tensor core path sums the columns on their way to the weight's gradient.  By single elements that is a kernel of its own (sums
+    // beside the products: 200,000 x 16 -> 7 weight gradient with the bias' 103 us, without 95; apart 105 and 85; 2708 x 16 -> 7
+    // 38 and 34, apart 34 and 28).  Behind it on the stream the other gradients take the scratch anew.
+    if (dbias != nullptr && (dweight == nullptr || !tiles)) {
         const int rc = column_sums<T>(c, static_cast<const T *>(grad), static_cast<const uint8_t *>(mask), scale, static_cast<T *>(dbias),
                                       scratch, stream);
         if (rc != CGNN_OK) return rc;
@@ -364,7 +318,7 @@ int backward(const Call &c, const void *weight, const void *mask, const void *gr
                                      scale, static_cast<T *>(dx), static_cast<T *>(dweight), static_cast<T *>(dbias), scratch,
                                      wait_limit.load(), stream);
     return small_backward<T>(c, static_cast<const T *>(weight), static_cast<const T *>(grad), static_cast<const uint8_t *>(mask),
-                             scale, static_cast<T *>(dx), static_cast<T *>(dweight), static_cast<T *>(dbias), scratch, stream);
+                             scale, static_cast<T *>(dx), static_cast<T *>(dweight), scratch, stream);
 }
 
 int check_call(int dtype, const Call &c, double p) {

@@ -78,7 +78,7 @@ struct Shape {
     static constexpr int A_UNITS = BM * BK / 8 / MEMBERS, B_UNITS = FORM == WEIGHT ? BN * BK / 8 / MEMBERS : 0;
     static constexpr int MASK_SLOT = ASYNC && FORM != FORWARD ? A_UNITS * MEMBERS : 0;  // a word of the mask for four units of a row
     static constexpr int STAGING = EPILOGUE_WARPS * 32 * (PIECE + 1) * 4;
-    static constexpr int SUMS = FORM == WEIGHT ? 16 * BM * 4 : 0;  // of the columns
+    static constexpr int SUMS = FORM == WEIGHT ? PRODUCER_WARPS * BM * 8 : 0;  // of the columns
     static constexpr int SHARED = STAGES * (STAGE + MASK_SLOT) + STAGING + SUMS + 1024;
     static_assert(SHARED + (FORM == FORWARD ? 2048 : 512) <= 232448 && (SPLIT || 2 * (AHEAD + 1) <= STAGES), "a block has 227 KB");
 };
@@ -101,7 +101,7 @@ struct Tiles {
     int partial;
     float *running;               // contractions of more than LONGEST, 16 bits: [M, N] (WEIGHT: of each split) of fp32
     int running_whole;            // its rows lie on vectors of 8
-    float *column_sums;           // WEIGHT: [splits, M]
+    double *column_sums;          // WEIGHT: [splits, M]
     float scale;
     Epilogue<T> epilogue;         // FORWARD
     int polls;
@@ -727,6 +727,24 @@ struct Finish {
     }
 };
 
+// Eight LongSums, two at a time.
+struct LongSums {
+    float2 high[4] = {}, low[4] = {};
+    __device__ __forceinline__ static float2 difference(float2 a, float2 b) { return __ffma2_rn(b, make_float2(-1.f, -1.f), a); }
+    __device__ __forceinline__ void add(const float (&x)[8]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 v = make_float2(x[2 * k], x[2 * k + 1]), s = __fadd2_rn(high[k], v), part = difference(s, high[k]);
+            low[k] = __fadd2_rn(low[k], __fadd2_rn(difference(high[k], difference(s, part)), difference(v, part)));
+            high[k] = s;
+        }
+    }
+    __device__ __forceinline__ double value(int k) const {
+        const float h = k % 2 ? high[k / 2].y : high[k / 2].x;
+        return isfinite(h) ? (double)h + (double)(k % 2 ? low[k / 2].y : low[k / 2].x) : (double)h;
+    }
+};
+
 // The units of a producer: a thread has the same place in every chunk of its group.  WHOLE: rows lie on vectors of 8 elements;
 // units of other rows are loaded an element at a time.
 template <typename T, int FORM, bool WHOLE>
@@ -877,18 +895,23 @@ struct Producer {
         }
         next_own();
     }
-    __device__ __forceinline__ void add_columns(const Unit<T> (&x)[S::A_UNITS + S::B_UNITS], float (&columns)[8]) const {
-        float sum[8];
+    // (Of the 16-bit types eight rows in fp32 first, which lose nothing that their result would keep.)
+    __device__ __forceinline__ void add_columns(const Unit<T> (&x)[S::A_UNITS + S::B_UNITS], LongSums &columns) const {
+        if constexpr (S::SPLIT) {
 #pragma unroll
-        for (int u = 0; u < S::A_UNITS; ++u)
+            for (int u = 0; u < S::A_UNITS; ++u) columns.add(x[u].v);
+        } else {
+            float sum[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) sum[k] = u == 0 ? x[u].value(k) : sum[k] + x[u].value(k);
+            for (int u = 0; u < S::A_UNITS; ++u)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) columns[k] += sum[k];
+                for (int k = 0; k < 8; ++k) sum[k] = u == 0 ? x[u].value(k) : sum[k] + x[u].value(k);
+            columns.add(sum);
+        }
     }
     // Units to their planes in a stage.
     __device__ __forceinline__ void store(Unit<T> (&x)[S::A_UNITS + S::B_UNITS], const uint32_t (&keep)[S::A_UNITS], uint32_t stage,
-                                          float (&columns)[8]) const {
+                                          LongSums &columns) const {
         if constexpr (FORM != FORWARD) {
             if (masked)
 #pragma unroll
@@ -913,7 +936,7 @@ struct Producer {
         }
     }
     // 16-bit units of A that have arrived in their stage: those of the mask go, and the others are added up.
-    __device__ __forceinline__ void mend(uint8_t *stage, const uint8_t *masks, float (&columns)[8]) const {
+    __device__ __forceinline__ void mend(uint8_t *stage, const uint8_t *masks, LongSums &columns) const {
         if constexpr (FORM != FORWARD) {
             const bool summed = FORM == WEIGHT && t.column_sums != nullptr;
             if (!masked && !summed) return;
@@ -949,7 +972,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     uint8_t *const stages = raw + (1024 - shared_address(raw) % 1024) % 1024;  // groups of eight swizzled rows lie on 1024 bytes
     [[maybe_unused]] uint8_t *const masks = stages + STAGES * S::STAGE;
     float *const staging = reinterpret_cast<float *>(masks + STAGES * S::MASK_SLOT);
-    [[maybe_unused]] float *const column_parts = staging + S::STAGING / 4;
+    [[maybe_unused]] double *const column_parts = reinterpret_cast<double *>(staging + S::STAGING / 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // 16-bit operands that nobody looks at on their way: their copies report to the barriers themselves, each thread's.
     const bool direct = S::ASYNC && (FORM == FORWARD || t.mask == nullptr) && (FORM != WEIGHT || t.column_sums == nullptr);
@@ -1096,9 +1119,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         // ------------------------------------------------------------------ operands to shared memory
 asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
         const int group = (threadIdx.x - EPILOGUE_WARPS * 32) / S::MEMBERS, p = (threadIdx.x - EPILOGUE_WARPS * 32) % S::MEMBERS;
-        float columns[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) columns[k] = 0.f;
+        LongSums columns;
         Producer<T, FORM, WHOLE> ahead(t, p);
         if (group == 1 && ahead.more()) ahead.next();
         uint32_t s = group, parity = 1;  // of the stage that the group fills next
@@ -1123,19 +1144,22 @@ asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
                 const Item i = item_of<T, FORM>(t, item);
                 if (i.n0 == 0) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) column_parts[(group * (S::MEMBERS / 16) + p / 16) * BM + p % 16 * 8 + k] = columns[k];
+                    for (int k = 0; k < 8; ++k) {  // (a warp's halves have the same columns)
+                        double sum = columns.value(k);
+                        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                        if (lane < 16) column_parts[(warp - EPILOGUE_WARPS) * BM + lane * 8 + k] = sum;
+                    }
                     asm volatile("bar.sync 3, %0;" ::"n"(PRODUCERS) : "memory");
                     if (group == 0 && p < BM && i.m0 + p < t.M) {
-                        float total = 0.f;
+                        double total = 0.0;
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) total += column_parts[r * BM + p];
-                        if (*(volatile int *)&waits.given_up) total = __uint_as_float(0x7fffffffu);
+                        for (int r = 0; r < PRODUCER_WARPS; ++r) total += column_parts[r * BM + p];
+                        if (*(volatile int *)&waits.given_up) total = __longlong_as_double(0x7fffffffffffffffll);
                         t.column_sums[i.split * t.M + i.m0 + p] = total;
                     }
                     asm volatile("bar.sync 3, %0;" ::"n"(PRODUCERS) : "memory");
                 }
-#pragma unroll
-                for (int k = 0; k < 8; ++k) columns[k] = 0.f;
+                columns = LongSums();
             }
             chunk = 0;
             item += gridDim.x;
@@ -1433,7 +1457,7 @@ size_t tiles_backward_bytes(int64_t rows, int64_t in, int64_t out) {
     const int64_t splits = weight_splits<T>(rows, in, out, &per_split);
     // (the input's gradient and then the weight's take what is behind the weight's image)
     const bool parts = splits > 1 || in_segments<T>(per_split);
-    const size_t of_weight = (size_t)splits * out * ((parts ? in : 0) + 1) * sizeof(float) + 64;
+    const size_t of_weight = (size_t)splits * out * ((parts ? in : 0) * sizeof(float) + sizeof(double)) + 64;
     return packed_bytes<T>(in, out) + std::max(of_weight, running_bytes<T>(rows, in, out));
 }
 
@@ -1465,8 +1489,8 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
     if (dweight == nullptr) return CGNN_OK;
     int64_t per_split;
     const int64_t splits = weight_splits<T>(c.rows, c.in, c.out, &per_split);
-    float *const parts = reinterpret_cast<float *>(align_up((size_t)packed + packed_bytes<T>(c.in, c.out), 32));
-    float *const sums = splits > 1 || in_segments<T>(per_split) ? parts + splits * c.out * c.in : parts;
+    double *const sums = reinterpret_cast<double *>(align_up((size_t)packed + packed_bytes<T>(c.in, c.out), 32));
+    float *const parts = reinterpret_cast<float *>(align_up((size_t)(sums + splits * c.out), 32));
     t.b = static_cast<const T *>(c.x);
     t.b_stride = c.stride;
     t.packed = nullptr;
@@ -1480,7 +1504,7 @@ int tiles_backward(const Call &c, const T *weight, const T *grad, const uint8_t 
     t.column_sums = dbias != nullptr ? sums : nullptr;
     int rc = launch<T, WEIGHT>(t, splits, stream);
     if (rc == CGNN_OK && t.partial) rc = join(parts, splits, c.out * c.in, scale, dweight, stream);
-    if (rc == CGNN_OK && dbias != nullptr) rc = join(sums, splits, c.out, scale, dbias, stream);
+    if (rc == CGNN_OK && dbias != nullptr) rc = join_columns(sums, splits, c.out, scale, dbias, stream);
     return rc;
 }
 

@@ -268,3 +268,26 @@ def test_whole_numbers_over_several_segments(dtype, rows, inner, outer, relu, p)
         g = grad.double() * factor
         for got, want in ((y, z * factor), (dx, g @ w.double()), (dw, g.t() @ x.double()), (db, g.sum(0))):
             assert torch.equal(got, want.to(dtype))
+
+
+# ---------------------------------------------------------------------------------------------
+# the bias' gradient
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, inner, outer", [(325557, 256, 128), (2708, 128, 64), (40000, 64, 72), (200000, 16, 7), (9001, 257, 129),
+                                                (700, 2048, 1), (20000, 1024, 2048)])
+@pytest.mark.parametrize("p", [0.0, 0.3])
+def test_bias_gradient_is_summed_in_64_bits(dtype, rows, inner, outer, p):
+    """fp32: one rounding, of the result.  16 bits: eight rows may be added in fp32 before, seven roundings of them."""
+    x, w = rand(rows, inner, dtype=dtype, seed=1), rand(outer, inner, dtype=dtype, seed=2).requires_grad_()
+    b = rand(outer, dtype=dtype, seed=3).requires_grad_()
+    grad = rand(rows, outer, dtype=dtype, seed=4)
+    dw, beside = torch.autograd.grad(rt.linear(x, w, b, None, p, seed=5), (w, b), grad)
+    alone, = torch.autograd.grad(rt.linear(x, w.detach(), b, None, p, seed=5), b, grad)
+    kept = rt.dropout(torch.ones_like(grad), p, seed=5) != 0 if p else torch.ones_like(grad, dtype=torch.bool)
+    terms_of = torch.where(kept, grad, 0).double() / (1 - p)
+    want, size = terms_of.sum(0), terms_of.abs().sum(0)
+    # (64-bit sums of 10^5 terms and a factor, here and there: 2^-36 of the sizes at most; a product with the factor in 64 bits)
+    bound = torch.finfo(dtype).eps / 2 * want.abs() + 2.0**-36 * size + (7 * 2.0**-24 * size if dtype in (BF16, F16) else 0.0)
+    for got, what in ((beside, "beside the weight's"), (alone, "alone")):
+        assert ((got.double() - want).abs() <= bound).all(), (what, float(((got.double() - want).abs() - bound).max()))
