@@ -960,32 +960,36 @@ Tensor cross_entropy_autograd(const Tensor &logits, const Tensor &target_in, int
 // a dense layer as one product
 // ---------------------------------------------------------------------------------------------
 struct LinearBackward : public Node {
-    SavedVariable x_, weight_, mask_;
+    SavedVariable x_, weight_, mask_;  // the input where the weight has a gradient, the weight where the input has one
     int dtype = 0;
-    bool masked = false;
     double p = 0.0;
-    at::TensorOptions weight_options;
+    std::vector<int64_t> sizes;  // of the input
+    int64_t rows = 0, in = 0, out = 0;
+    at::TensorOptions options;
     variable_list apply(variable_list &&grads) override {
         Tensor dx, dw, db, dresidual;
         {
             at::NoGradGuard no_grad;
             const Tensor incoming = materialized(*this, grads[0]);
             const c10::cuda::OptionalCUDAGuard guard(incoming.device());
-            // both of them, needed or not: one that was modified in place since the forward pass is an error
-            const Tensor x_in = x_.unpack(), weight = weight_.unpack().contiguous();
-            const Tensor mask = masked ? mask_.unpack().contiguous() : Tensor();
-            const int64_t in = weight.size(1), out = weight.size(0);
-            if (task_should_compute_output(0)) dx = at::empty(x_in.sizes(), x_in.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
-            if (task_should_compute_output(1)) dw = at::empty({out, in}, weight_options);
-            if (task_should_compute_output(2)) db = at::empty({out}, weight_options);
+            // all that was kept, needed this time or not: one that was modified in place since the forward pass is an error
+            const Tensor x_in = x_.unpack(), weight = dense(weight_.unpack()), mask = dense(mask_.unpack());
+            if (task_should_compute_output(0)) dx = at::empty(sizes, options);
+            if (task_should_compute_output(1)) dw = at::empty({out, in}, options);
+            if (task_should_compute_output(2)) db = at::empty({out}, options);
             if (dx.defined() || dw.defined() || db.defined()) {
                 const Tensor grad = incoming.contiguous();
-                const Rows x(x_in);
-                const int64_t rows = out ? grad.numel() / out : x.rows;
+                Tensor x;
+                int64_t stride = in;
+                if (x_in.defined()) {
+                    const Rows of_x(x_in);
+                    x = of_x.held;
+                    stride = of_x.stride;
+                }
                 const size_t bytes = cgnn_linear_backward_scratch_bytes(dtype, rows, in, out);
-                const Tensor scratch = at::empty({(int64_t)bytes}, weight_options.dtype(at::kByte));
-                check(cgnn_linear_backward(dtype, rows, in, out, x.stride, data(x.held), data(weight), data(mask), data(grad), p,
-                                           data(dx), data(dw), data(db), data(scratch), bytes, current_stream(grad)));
+                const Tensor scratch = at::empty({(int64_t)bytes}, options.dtype(at::kByte));
+                check(cgnn_linear_backward(dtype, rows, in, out, stride, data(x), data(weight), data(mask), data(grad), p, data(dx),
+                                           data(dw), data(db), data(scratch), bytes, current_stream(grad)));
             }
             if (task_should_compute_output(3)) dresidual = incoming;
         }
@@ -1021,13 +1025,13 @@ Tensor linear_autograd(const Tensor &x_in, const Tensor &weight, const c10::opti
     refuse_foreign_leaves("linear", {x_in, weight, bias, residual});
     const bool differentiated = torch::autograd::compute_requires_grad(x_in, weight, bias, residual);
     const bool masked = differentiated && (relu || p > 0.0);
+    const auto plain = x_in.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
+    const int64_t rows = c10::multiply_integers(sizes.begin(), sizes.end() - 1);
     Tensor y, mask;
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        const auto plain = x_in.options().requires_grad(false);
         const Rows x(x_in);
-        y = at::empty(sizes, plain.memory_format(at::MemoryFormat::Contiguous));
-        const int64_t rows = out ? y.numel() / out : 0;
+        y = at::empty(sizes, plain);
         if (masked) mask = at::empty({(int64_t)cgnn_linear_mask_bytes(rows, out)}, plain.dtype(at::kByte));
         const size_t bytes = cgnn_linear_scratch_bytes(dtype, rows, in, out);
         const Tensor scratch = at::empty({(int64_t)bytes}, plain.dtype(at::kByte));
@@ -1038,12 +1042,15 @@ Tensor linear_autograd(const Tensor &x_in, const Tensor &weight, const c10::opti
     if (differentiated) {
         auto node = new_node<LinearBackward>();
         node->dtype = dtype;
-        node->masked = masked;
         node->p = p;
-        node->weight_options = weight.options().requires_grad(false);
-        node->x_ = SavedVariable(x_in, false);
-        node->weight_ = SavedVariable(weight, false);
-        node->mask_ = SavedVariable(mask, false);
+        node->sizes = x_in.sizes().vec();
+        node->rows = rows;
+        node->in = in;
+        node->out = out;
+        node->options = plain;
+        if (weight.requires_grad()) node->x_ = SavedVariable(x_in, false);
+        if (x_in.requires_grad()) node->weight_ = SavedVariable(weight, false);
+        if (masked) node->mask_ = SavedVariable(mask, false);
         node->set_next_edges(torch::autograd::collect_next_edges(x_in, weight, bias, residual));
         torch::autograd::set_history(y, node);
     }

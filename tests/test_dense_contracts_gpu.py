@@ -82,6 +82,44 @@ def test_gradients_with_a_frozen_weight(dtype, rows):
     assert torch.equal(dx, (grad.double() @ w.double()).to(dtype))
 
 
+@pytest.mark.parametrize("activation, p", [(None, 0.0), ("relu", 0.25)])
+def test_what_no_gradient_needs_is_not_kept(activation, p):
+    """The input is there for the weight's gradient and the weight for the input's, as torch's layer has it: otherwise they may be
+    changed, or given back, in front of the backward pass."""
+    def tensors_():
+        return [rand(*shape, seed=i) for i, shape in enumerate([(300, 7, 64), (48, 64), (48,)])]
+    grad = rand(300, 7, 48, seed=5)
+    for which in ((0,), (1,), (2,), (0, 2), (1, 2)):
+        leaves = [t.requires_grad_(i in which) for i, t in enumerate(tensors_())]
+        every = [t.requires_grad_() for t in tensors_()]
+        want = torch.autograd.grad(rt.linear(*every, activation, p, seed=4), every, grad)
+        y = rt.linear(*leaves, activation, p, seed=4)
+        with torch.no_grad():
+            if 0 not in which:
+                leaves[1].fill_(7.0)
+            if 1 not in which:
+                leaves[0].fill_(7.0)
+        got = torch.autograd.grad(y, [leaves[i] for i in which], grad)
+        assert all(torch.equal(g, want[i]) for g, i in zip(got, which))
+    # what is needed is kept, and a change of it refused
+    for changed, wanted in ((0, 1), (1, 0)):
+        leaves = [t.requires_grad_(i == wanted) for i, t in enumerate(tensors_())]
+        y = rt.linear(*leaves, activation, p, seed=4)
+        with torch.no_grad():
+            leaves[changed].add_(1.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    # nor does a frozen layer hold its input's memory
+    x, w, b = tensors_()
+    b.requires_grad_()
+    inner = torch.zeros(1 << 20, 64, device="cuda")
+    y = rt.linear(inner, w, b, activation, p, seed=4)
+    held = torch.cuda.memory_allocated()
+    inner = None
+    assert held - torch.cuda.memory_allocated() >= 256 << 20
+    assert torch.autograd.grad(y, b, torch.ones_like(y))[0].shape == b.shape
+
+
 # ---------------------------------------------------------------------------------------------
 # infinities and NaN
 # ---------------------------------------------------------------------------------------------
