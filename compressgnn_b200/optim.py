@@ -8,16 +8,20 @@ from . import runtime as _native
 class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay; ``weight_decay=0`` is Adam), as ``torch.optim.AdamW`` computes it.
 
-    ``max_norm`` (not a group's): the gradients of all groups are clipped by their common 2-norm, which ``step`` leaves in ``grad_norm``
+    ``max_norm``: the gradients of all groups are clipped by their common 2-norm, which ``step`` leaves in ``grad_norm``
     (a float32 tensor on the device); the gradients themselves are not changed.
     ``state_bits=8``: moments of tensors with ``least_8bit`` elements or more are held in 8 bits, 4 bytes a float32
     parameter less to keep and 12 less to move a step; smaller ones, and float64, keep theirs in full.  ``seed`` is the key
     of their stochastic rounding.
 
+    The groups hold ``max_norm`` and ``seed`` as they hold the rest, so a schedule may set them and a loaded state brings its own; but
+    there is one of each, and groups that differ in them are refused.
+
     ``lr`` may be a CUDA tensor of one float32.  The steps taken are counted on the device, so a step can be captured into
     a CUDA graph once the state exists (after one step outside of the capture)."""
 
     grad_norm = None
+    _COMMON = ("max_norm", "seed")
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, state_bits=32,
                  least_8bit=4096, seed=0):
@@ -53,13 +57,22 @@ class AdamW(torch.optim.Optimizer):
                 for name in ("exp_avg", "exp_avg_sq"):
                     state[name] = torch.zeros(p.shape, dtype=wide, device=p.device)
 
+    def add_param_group(self, group):
+        for name in self._COMMON:
+            common = self.param_groups[0][name] if self.param_groups else self.defaults[name]
+            if group.setdefault(name, common) != common:
+                raise ValueError(f"AdamW: {name} is common to all groups")
+        super().add_param_group(group)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        max_norm, seed = self.defaults["max_norm"], int(self.defaults["seed"])
+        max_norm, seed = (self.param_groups[0][name] for name in self._COMMON)
+        if any((group["max_norm"], group["seed"]) != (max_norm, seed) for group in self.param_groups):
+            raise RuntimeError("AdamW: max_norm and seed are common to all groups, set them in each")
         if max_norm is not None:
             self.grad_norm = None  # (of a step without a gradient)
         calls, fresh = {}, []
@@ -84,7 +97,7 @@ class AdamW(torch.optim.Optimizer):
                 [p for _, p in members], [p.grad.contiguous() for _, p in members], [s["exp_avg"] for s in states],
                 [s["exp_avg_sq"] for s in states], [s["step"] for s in states], [group["lr"] for group, _ in members], betas, eps,
                 [group["weight_decay"] for group, _ in members], max_norm, [s.get("exp_avg_scale") for s in states],
-                [s.get("exp_avg_sq_scale") for s in states], seed + (number << 32))
+                [s.get("exp_avg_sq_scale") for s in states], int(seed) + (number << 32))
             if max_norm is not None:
                 self.grad_norm = norm
         return loss
