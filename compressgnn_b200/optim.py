@@ -103,7 +103,14 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """(The base class casts a parameter's state to its type: the moments keep theirs, and the count stays whole.)"""
+        """(The base class casts a parameter's state to its type: the moments keep theirs, and the count stays whole.)  A state of another
+        optimiser, ``torch.optim.AdamW`` among them, is refused: its groups lack settings, its counts are fractions on the host."""
+        ours = all(set(self.defaults) <= set(group) for group in state_dict["param_groups"])
+        for state in filter(None, state_dict["state"].values()):
+            step = state.get("step")
+            ours = ours and "exp_avg" in state and "exp_avg_sq" in state and torch.is_tensor(step) and step.dtype == torch.int64
+        if not ours:
+            raise ValueError("AdamW: this is the state of another optimiser")
         super().load_state_dict(state_dict)
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         ours = [p for group in self.param_groups for p in group["params"]]

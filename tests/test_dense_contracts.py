@@ -54,3 +54,18 @@ def test_a_loaded_state_brings_its_norm_and_seed(monkeypatch):
     opt.param_groups[0]["max_norm"] = 0.5
     opt.step()
     assert seen == [(0.25, 9), (0.5, 9)]
+
+
+def test_a_state_of_another_optimiser_is_refused():
+    p = parameter()
+    p.grad = torch.ones(3)
+    theirs = torch.optim.AdamW([p])
+    opt = optim.AdamW([p], lr=0.5)
+    with pytest.raises(ValueError, match="another optimiser"):
+        opt.load_state_dict(theirs.state_dict())  # before its first step: the groups
+    theirs.step()
+    state = theirs.state_dict()
+    state["param_groups"] = opt.state_dict()["param_groups"]
+    with pytest.raises(ValueError, match="another optimiser"):
+        opt.load_state_dict(state)
+    assert not opt.state and opt.param_groups[0]["lr"] == 0.5
