@@ -1060,19 +1060,29 @@ Tensor linear_autograd(const Tensor &x_in, const Tensor &weight, const c10::opti
 // ---------------------------------------------------------------------------------------------
 // one optimiser step over many tensors
 // ---------------------------------------------------------------------------------------------
-// The places that a step writes: no two of its tensors may share memory.
+// The places that a step writes: no two of its tensors may share memory, nor one of them with what it reads.
 struct Places {
-    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-    void add(const Tensor &t) {
+    using Span = std::pair<uintptr_t, uintptr_t>;
+    std::vector<Span> written, read;
+    static Span span_of(const Tensor &t) {
+        const uintptr_t first = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+        return {first, first + t.nbytes()};
+    }
+    void writes(const Tensor &t) {
         TORCH_CHECK(!t.is_inference() || c10::InferenceMode::is_enabled(), "adamw_step: an inference tensor is written in inference mode only");
-        if (!t.numel()) return;
-        const uintptr_t first = reinterpret_cast<uintptr_t>(t.data_ptr());
-        spans.push_back({first, first + t.nbytes()});
+        if (t.numel()) written.push_back(span_of(t));
+    }
+    void reads(const Tensor &t) {
+        if (t.numel()) read.push_back(span_of(t));
     }
     bool apart() {
-        std::sort(spans.begin(), spans.end());
-        for (size_t i = 1; i < spans.size(); ++i)
-            if (spans[i].first < spans[i - 1].second) return false;
+        std::sort(written.begin(), written.end());
+        for (size_t i = 1; i < written.size(); ++i)
+            if (written[i].first < written[i - 1].second) return false;
+        for (const Span &r : read) {  // (the first written one that ends behind its beginning)
+            const auto next = std::partition_point(written.begin(), written.end(), [&](const Span &w) { return w.second <= r.first; });
+            if (next != written.end() && next->first < r.second) return false;
+        }
         return true;
     }
 };
@@ -1101,8 +1111,9 @@ c10::optional<Tensor> adamw_step(const std::vector<Tensor> &params, const std::v
     const auto device = params[0].device();
     TORCH_CHECK(device.is_cuda(), "compressgnn_b200 runs on CUDA tensors only (no CPU optimiser path)");
     std::vector<cgnn_adamw_tensor> list(n);
-    Places written;
-    written.spans.reserve(6 * n);
+    Places places;
+    places.written.reserve(6 * n);
+    places.read.reserve(2 * n);
     for (size_t i = 0; i < n; ++i) {
         const Tensor &p = params[i], &g = grads[i], &m = firsts[i], &v = seconds[i], &t = steps[i];
         const int dtype = row_dtype(p, "adamw_step");
@@ -1131,20 +1142,22 @@ c10::optional<Tensor> adamw_step(const std::vector<Tensor> &params, const std::v
             TORCH_CHECK(rate.device() == device && rate.scalar_type() == at::kFloat && rate.numel() == 1,
                         "adamw_step: a learning rate in a tensor is one float32 on the parameters' device");
             e.device_lr = rate.const_data_ptr<float>();
+            places.reads(rate);
         }
         if (eight)
             for (const Tensor &s : {first_scale, second_scale})
                 TORCH_CHECK(s.device() == device && s.scalar_type() == at::kFloat && s.is_contiguous() && s.numel() == (p.numel() + 255) / 256,
                             "adamw_step: a moment has one float32 scale for each block of 256 elements");
-        for (const Tensor *w : {&p, &m, &v, &t}) written.add(*w);
+        for (const Tensor *w : {&p, &m, &v, &t}) places.writes(*w);
+        places.reads(g);
         e.param = data(p);
         e.grad = data(g);
         e.exp_avg = data(m);
         e.exp_avg_sq = data(v);
         e.exp_avg_scale = e.exp_avg_sq_scale = nullptr;
         if (eight) {
-            written.add(first_scale);
-            written.add(second_scale);
+            places.writes(first_scale);
+            places.writes(second_scale);
             // (of an empty tensor: no scales, which are not looked at, but moments of 8 bits all the same)
             e.exp_avg_scale = static_cast<float *>(p.numel() ? data(first_scale) : data(t));
             e.exp_avg_sq_scale = static_cast<float *>(p.numel() ? data(second_scale) : data(t));
@@ -1153,7 +1166,7 @@ c10::optional<Tensor> adamw_step(const std::vector<Tensor> &params, const std::v
         e.n = p.numel();
         e.dtype = dtype;
     }
-    TORCH_CHECK(written.apart(), "adamw_step: parameters, moments, scales and steps must not share memory");
+    TORCH_CHECK(places.apart(), "adamw_step: parameters, moments, scales and steps must not share memory, nor with gradients and rates");
     const c10::cuda::OptionalCUDAGuard guard(device);
     at::AutoDispatchBelowADInplaceOrView below;
     Tensor norm, scratch;

@@ -449,7 +449,7 @@ int cgnn_linear_wait_limit(int polls);
  *   max_norm    clip = min(1, max_norm / (norm + 1e-6)) with the 2-norm of all gradients; negative: clip = 1
  *   norm        one float for that norm (written with max_norm >= 0 only); may be null
  *   scratch     cgnn_adamw_scratch_bytes(), 8-byte aligned, needed with max_norm >= 0; its contents do not matter
- * The list lies in host memory and is read before the call returns.  No two of its tensors may share memory. */
+ * The list lies in host memory and is read before the call returns.  What is written shares no memory with anything else of the list. */
 typedef struct {
     void *param;
     const void *grad;

@@ -329,3 +329,32 @@ def test_bias_gradient_is_summed_in_64_bits(dtype, rows, inner, outer, p):
     bound = torch.finfo(dtype).eps / 2 * want.abs() + 2.0**-36 * size + (7 * 2.0**-24 * size if dtype in (BF16, F16) else 0.0)
     for got, what in ((beside, "beside the weight's"), (alone, "alone")):
         assert ((got.double() - want).abs() <= bound).all(), (what, float(((got.double() - want).abs() - bound).max()))
+
+
+# ---------------------------------------------------------------------------------------------
+# an optimiser step
+# ---------------------------------------------------------------------------------------------
+def test_a_step_reads_nothing_that_it_writes():
+    """Warps take what they read and write in any order: a gradient that lies over a moment, or the rate in a parameter, is refused."""
+    n = 5000
+    held = rand(3 * n, seed=1)
+    p, m, v, g = rand(n, seed=2), torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda"), rand(n, seed=3)
+
+    def step(p=p, g=g, m=m, v=v, **more):
+        t = torch.zeros((), dtype=torch.int64, device="cuda")
+        return rt.adamw_step([p, rand(5)], [g, rand(5)], [m, torch.zeros(5, device="cuda")], [v, torch.zeros(5, device="cuda")],
+                             [t, torch.zeros((), dtype=torch.int64, device="cuda")], **more)
+    parts = held[:n], held[n - 1:2 * n - 1], held[2 * n:]
+    before = held.clone()
+    for wrong in (dict(g=parts[0], m=parts[1]), dict(g=parts[1], v=parts[0]), dict(g=parts[0], p=parts[1]), dict(g=held[:n], p=held[:n]),
+                  dict(p=parts[0], lr=held[:1]), dict(v=parts[0], lr=held[n - 1])):
+        with pytest.raises(RuntimeError, match="share memory"):
+            step(**wrong)
+    assert torch.equal(held, before)
+    # beside each other, and read twice
+    step(p=held[:n], g=held[n:2 * n], m=held[2 * n:])
+    rate = torch.tensor(1e-3, device="cuda")
+    two = [rand(n, seed=5), rand(n, seed=5)]
+    rt.adamw_step(two, [g, g], [torch.zeros(n, device="cuda") for _ in two], [torch.zeros(n, device="cuda") for _ in two],
+                  list(torch.zeros(2, dtype=torch.int64, device="cuda")), lr=[rate, rate])
+    assert torch.equal(*two)
