@@ -7,7 +7,8 @@
 //   WEIGHT   A = z^T,          B = x^T      contraction over the nodes, which is split over the blocks and joined afterwards
 //
 // fp32 operands become three bf16 numbers each, high + middle + low (8 bits of the fraction apiece, 24 together), and a
-// product six: hh, hm, mh, hl, lh, mm; what is left out is below 2^-23 of a term.  A tensor core adds to its fp32
+// product six: hh, hm, mh, hl, lh, mm; what is left out is below 2^-23 of a term, or, of an operand below 2^-110, the rest beyond a
+// multiple of 2^-133, bf16's least number.  A tensor core adds to its fp32
 // accumulator with truncation, so that the error grows with the number of additions: hh has an accumulator of its own, the
 // five small ones share another, and after 256 terms both are added to fp32 registers and begin
 // anew (325,557 x 256 -> 128: outputs 1.5e-7 of their size from 64 bits, the fp32 pipes' 1.8e-7).  Six products at the bf16

@@ -692,8 +692,9 @@ def linear(input, weight, bias=None, activation=None, dropout=0.0, residual=None
 
     ``input``: float32, float64, bfloat16 or float16, ``[..., in]``; rows of a matrix may lie apart.  ``weight``
     ``[out, in]``, ``bias`` ``[out]`` or None and ``residual`` (of the output's shape, or None) have its type.  Products are
-    added up in float32 (float64 for float64) and rounded once; float32 is computed to its last digits whatever torch's
-    switches for TF32 say.  ``activation``: None or ``"relu"``.  ``dropout``: the probability of the dropout that
+    added up in float32 (float64 for float64) and rounded once; float32 operands keep their 24 binary digits whatever torch's
+    switches for TF32 say (in calls for the tensor cores those below 2^-110, 8e-34, are taken to the nearest multiple of
+    2^-133).  ``activation``: None or ``"relu"``.  ``dropout``: the probability of the dropout that
     follows; its mask is ``runtime.dropout``'s for the same ``seed``.  What the backward pass needs to know of the
     output is one bit for each element; the output itself is not kept."""
     _require(activation in (None, "relu"), "Supported activations: None, relu")

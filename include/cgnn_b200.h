@@ -417,7 +417,8 @@ int cgnn_cross_entropy_backward(int dtype, int64_t rows, int64_t classes, int64_
 /* A dense layer as one product: y[r,:] = residual[r,:] + dropout(act(x[r,:] weight^T + bias)), act = ReLU or nothing, the dropout
  * that of cgnn_dropout on y.  weight: [out, in]; bias ([out]) and residual ([rows, out]) may be null; row r of x begins at
  * x + r * stride elements; everything else is dense.  All of one type; products are added up in fp32 (fp64 for fp64) and
- * a result is rounded once.  fp32 products are exact to fp32's last digits (no TF32).
+ * a result is rounded once.  fp32 operands keep their 24 binary digits (no TF32), but where a call is large enough for the tensor
+ * cores, one below 2^-110 is taken to the nearest multiple of 2^-133.
  *   mask      cgnn_linear_mask_bytes(), 8-byte aligned: a bit for each element of y that the ReLU and the dropout let through, what
  *             the backward pass reads; may be null; not written where neither is asked for
  *   scratch   cgnn_linear_scratch_bytes(), 16-byte aligned; its contents do not matter; the same for the backward pass

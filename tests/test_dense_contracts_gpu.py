@@ -332,6 +332,34 @@ def test_bias_gradient_is_summed_in_64_bits(dtype, rows, inner, outer, p):
 
 
 # ---------------------------------------------------------------------------------------------
+# fp32 operands near the end of their range
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows, inner, outer", [(40000, 64, 72), (3000, 1030, 301), (200, 16, 7)])
+@pytest.mark.parametrize("exponent", [-100, -109, -112, -118, -124, -130])
+def test_small_fp32_operands(rows, inner, outer, exponent):
+    """Operands are off by 2^-134 at most, half of bf16's least number, beyond what they are off elsewhere; sums by half a step of 2^-149
+    an addition.  By single elements nothing is lost beyond that half step."""
+    tiles = rows * inner * outer >= 4e7
+    x, w, grad = rand(rows, inner, seed=1, scale=2.0**exponent), rand(outer, inner, seed=2), rand(rows, outer, seed=3)
+
+    def check(got, a, b, n, what):
+        a, b = a.double(), b.double()
+        bound = terms(n) * (a.abs() @ b.abs()) + (3 * n + 32) * 2.0**-149
+        if tiles:
+            bound += 2.0**-134 * b.abs().sum(0)
+        excess = ((got.double() - a @ b).abs() - bound).max()
+        assert excess <= 0, f"{what}: {excess:.3e}"
+    check(rt.linear(x, w), x, w.t(), inner, "y")
+    v = torch.zeros(outer, inner, device="cuda", requires_grad=True)
+    dw, = torch.autograd.grad(rt.linear(x, v), v, grad)
+    check(dw.t(), x.t(), grad, rows, "dweight")
+    small, leaf = grad * 2.0**exponent, torch.zeros(rows, inner, device="cuda", requires_grad=True)
+    dx, = torch.autograd.grad(rt.linear(leaf, w), leaf, small)
+    check(dx, small, w, outer, "dx")
+    assert rt.device_status() == 0
+
+
+# ---------------------------------------------------------------------------------------------
 # an optimiser step
 # ---------------------------------------------------------------------------------------------
 def test_a_step_reads_nothing_that_it_writes():
