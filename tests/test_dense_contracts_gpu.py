@@ -309,6 +309,96 @@ def test_whole_numbers_over_several_segments(dtype, rows, inner, outer, relu, p)
 
 
 # ---------------------------------------------------------------------------------------------
+# every term, once
+# ---------------------------------------------------------------------------------------------
+LONG = [(325557, 256, 128), (70001, 301, 173), (300000, 72, 136), (150000, 8, 520), (40017, 1030, 47), (2708, 128, 64), (9001, 257, 129)]
+
+
+def products_of(x, w, b, grad, activation=None, p=0.0):
+    """An output, its gradients, and what all of them are in 64 bits."""
+    leaves = [t.detach().clone().requires_grad_() for t in (x, w, b)]
+    y = rt.linear(*leaves, activation, p, seed=6)
+    got = [y.detach(), *torch.autograd.grad(y, leaves, grad)]
+    assert rt.device_status() == 0
+    x, w, b, g = (t.double() for t in (x, w, b, grad))
+    z = x @ w.t() + b
+    passed = torch.where(z > 0, 1.0, 0.0) if activation else torch.ones_like(z)
+    if p:
+        passed = passed * (rt.dropout(torch.ones_like(grad), p, seed=6) != 0) / (1 - p)
+    g = g * passed
+    return got, [z * passed, g @ w, g.t() @ x, g.sum(0)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, inner, outer", LONG)
+@pytest.mark.parametrize("activation, p", [(None, 0.0), ("relu", 0.5)])
+def test_whole_numbers_come_out_to_the_bit(dtype, rows, inner, outer, activation, p):
+    """Sums of whole numbers up to 4, at most 2 * 4 * 325,557 of them: exact in fp32 whatever their order, and rounded once.  A term
+    that is lost, or counted twice, at the end of a split or anywhere else, shows."""
+    x, w, b = whole(rows, inner, dtype=dtype, seed=1), whole(outer, inner, dtype=dtype, seed=2), whole(outer, dtype=dtype, seed=3)
+    got, want = products_of(x, w, b, whole(rows, outer, dtype=dtype, seed=4), activation, p)
+    for a, e, name in zip(got, want, ("y", "dx", "dweight", "dbias")):
+        assert e.abs().max() < 2**24
+        assert torch.equal(a, e.to(dtype)), name
+
+
+@pytest.mark.parametrize("rows, inner, outer", LONG)
+def test_a_single_term_has_all_of_fp32s_digits(rows, inner, outer):
+    """One product an element, of numbers with digits in all three bf16 parts.  Left out are three products of parts, together
+    below 2^-23 of it (parts of 2^-9 and 2^-17 at most: 2 * 2^-26 + 2^-34); the accumulators and their sum truncate or round five times
+    by 2^-23 at most; the result as written."""
+    few = 2.0**-23 * 6 + 2.0**-24
+    gen = torch.Generator(device="cuda").manual_seed(1)
+
+    def odd(*shape):
+        """1 to 2 in size, the last digit set."""
+        digits = torch.randint(0, 1 << 22, shape, device="cuda", generator=gen) * 2 + 1
+        sign = torch.randint(0, 2, shape, device="cuda", generator=gen) * 2 - 1
+        return (sign * (1 + digits.double() * 2.0**-23)).float()
+    w, grad = odd(outer, inner), odd(rows, outer)
+    at = torch.randint(0, inner, (rows,), device="cuda", generator=gen)
+    of = torch.randint(0, outer, (rows,), device="cuda", generator=gen)
+    values = odd(rows)
+    x = torch.zeros(rows, inner, device="cuda").scatter_(1, at[:, None], values[:, None])
+    want = values.double()[:, None] * w.double().t()[at]
+    y = rt.linear(x, w)
+    assert ((y.double() - want).abs() <= few * want.abs()).all()
+    thin = torch.zeros(rows, outer, device="cuda").scatter_(1, of[:, None], values[:, None])
+    leaf = torch.zeros(rows, inner, device="cuda", requires_grad=True)
+    dx, = torch.autograd.grad(rt.linear(leaf, w), leaf, thin)
+    want = values.double()[:, None] * w.double()[of]
+    assert ((dx.double() - want).abs() <= few * want.abs()).all()
+    for row in (0, rows // 2, rows - 1):
+        x = torch.zeros(rows, inner, device="cuda")
+        x[row] = odd(inner)
+        v = torch.zeros(outer, inner, device="cuda", requires_grad=True)
+        dw, = torch.autograd.grad(rt.linear(x, v), v, grad)
+        want = grad[row].double()[:, None] * x[row].double()
+        assert ((dw.double() - want).abs() <= few * want.abs()).all()
+    assert rt.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows, inner, outer", LONG + [(100000, 1024, 256)])
+@pytest.mark.parametrize("activation, p", [(None, 0.0), ("relu", 0.3)])
+def test_errors_do_not_grow_with_the_number_of_rows(dtype, rows, inner, outer, activation, p):
+    """Over all elements (root mean squares): an accumulator takes 16 terms an addition and truncates it, half a step of 2^-23 of the sum
+    so far on average; of fp32 it takes 256 terms, whose 16 additions lose at most 8 steps of 2^-23 of a sum that is 0.7 of the last on
+    average: 6.7e-7, by one sign within the 256 and by any from one 256 to the next.  Of 16 bits it takes 8192, 512 additions, 2.1e-5; the
+    rounding of the result is half a step at most."""
+    x, w, b = rand(rows, inner, dtype=dtype, seed=1), rand(outer, inner, dtype=dtype, seed=2), rand(outer, dtype=dtype, seed=3)
+    got, want = products_of(x, w, b, rand(rows, outer, dtype=dtype, seed=4), activation, p)
+    if activation:  # (a sum next to zero may lie on its other side in fp32: its gradient's terms are those that the kernel took)
+        passed = (got[0] != 0).double() / (1 - p)
+        g = rand(rows, outer, dtype=dtype, seed=4).double() * passed
+        want[1:] = [g @ w.double(), g.t() @ x.double(), g.sum(0)]
+    bound = 6.7e-7 if dtype == F32 else torch.finfo(dtype).eps / 2 + 2.1e-5
+    for a, e, name in zip(got, want, ("y", "dx", "dweight", "dbias")):
+        off = float(((a.double() - e).square().mean() / e.square().mean()).sqrt())
+        assert off <= bound, f"{name}: {off:.3e} of {bound:.3e}"
+
+
+# ---------------------------------------------------------------------------------------------
 # the bias' gradient
 # ---------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", TYPES)
