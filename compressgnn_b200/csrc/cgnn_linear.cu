@@ -175,11 +175,9 @@ int small_product(Small<T> &s, int64_t splits, cudaStream_t stream) {
 // ---------------------------------------------------------------------------------------------
 // the bias' gradient by itself: column sums of z, for which neither x nor the weight is looked at
 // ---------------------------------------------------------------------------------------------
-constexpr int64_t COLUMN_BLOCKS = 148 * 8;
-
-// None of fewer rows than a block has on their way.
+// Splits of the rows: some blocks for every multiprocessor, and none of fewer rows than a block has on their way.
 int64_t column_splits(int64_t rows, int64_t out) {
-    return std::max<int64_t>(1, std::min<int64_t>(COLUMN_BLOCKS / ceil_div(out, 32), rows / COLUMN_ROWS));
+    return std::max<int64_t>(1, std::min<int64_t>(148 * 4 / ceil_div(out, 256), rows / (COLUMN_UNROLL * 8)));
 }
 
 size_t column_bytes(int64_t rows, int64_t out) {
@@ -187,14 +185,22 @@ size_t column_bytes(int64_t rows, int64_t out) {
     return splits == 1 ? 0 : (size_t)splits * (size_t)out * sizeof(double);
 }
 
-template <typename T>
-int column_sums(const Call &c, const T *grad, const uint8_t *mask, double scale, T *dbias, void *scratch, cudaStream_t stream) {
-    const int64_t splits = column_splits(c.rows, c.out);
+template <typename T, int VW>
+int column_sums_by(const Call &c, const T *grad, const uint8_t *mask, double scale, T *dbias, void *scratch, cudaStream_t stream) {
+    const int64_t splits = column_splits(c.rows, c.out), vectors = ceil_div(c.out, VW);
+    const int across = columns_across(vectors);
     double *const parts = static_cast<double *>(scratch);
-    columns_kernel<T, T><<<dim3((unsigned)ceil_div(c.out, 32), (unsigned)splits), COLUMN_WARPS * 32, 0, stream>>>(
-        grad, mask, mask_pitch(c.out), c.rows, ceil_div(c.rows, splits), c.out, scale, parts, dbias);
+    columns_kernel<T, T, VW><<<dim3((unsigned)ceil_div(vectors, 1 << across), (unsigned)splits), COLUMN_THREADS, 0, stream>>>(
+        grad, mask, mask_pitch(c.out), c.rows, ceil_div(c.rows, splits), c.out, across, scale, parts, dbias);
     CGNN_LAUNCH_CHECK();
     return splits == 1 ? CGNN_OK : join_columns(parts, splits, c.out, scale, dbias, stream);
+}
+
+template <typename T>
+int column_sums(const Call &c, const T *grad, const uint8_t *mask, double scale, T *dbias, void *scratch, cudaStream_t stream) {
+    constexpr int VW = 16 / sizeof(T);
+    return c.out % VW == 0 && (uintptr_t)grad % 16 == 0 ? column_sums_by<T, VW>(c, grad, mask, scale, dbias, scratch, stream)
+                                                        : column_sums_by<T, 1>(c, grad, mask, scale, dbias, scratch, stream);
 }
 
 size_t small_backward_bytes(int64_t acc_bytes, int64_t rows, int64_t in, int64_t out) {

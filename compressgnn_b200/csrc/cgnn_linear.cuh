@@ -1,6 +1,8 @@
 // What the kernels of a dense layer share.
 #pragma once
 
+#include <type_traits>
+
 #include "cgnn_dropout.cuh"
 #include "cgnn_rows.cuh"
 
@@ -89,51 +91,79 @@ struct LongSum<double> {
     __device__ __forceinline__ double value() const { return sum; }
 };
 
-// Column sums of x [rows, width], of the elements that `mask` has a bit for (null: all).  A lane has a column, a warp every eighth row
-// with COLUMN_UNROLL of them on their way; the grid's second dimension splits the rows: parts[blockIdx.y, column], or, of one
-// split, scale times the sums themselves.
-constexpr int COLUMN_WARPS = 8, COLUMN_UNROLL = 8;
-constexpr int64_t COLUMN_ROWS = COLUMN_WARPS * COLUMN_UNROLL;
+// Column sums of x [rows, width], of the elements that `mask` has a bit for (null: all).  A thread has VW neighbouring columns, 2^across
+// neighbouring threads a row, each of them COLUMN_UNROLL rows on their way; the grid's second dimension splits the rows:
+// parts[blockIdx.y, column], or, of one split, scale times the sums themselves.  (16-bit types: eight rows in fp32 first, which lose nothing that
+// their result would keep.)  By vectors of 16 bytes HBM bounds it: 2.45 M x 256 bf16 216 us (floor 192; by a column a lane, two bytes an
+// access, 1072), 325,557 x 256 fp32 78 (51).
+constexpr int COLUMN_THREADS = 256, COLUMN_UNROLL = 8;
 
-template <typename T, typename X>
-static __global__ void __launch_bounds__(COLUMN_WARPS * 32) columns_kernel(const X *x, const uint8_t *mask, int64_t mask_pitch, int64_t rows,
-                                                                           int64_t rows_per_split, int64_t width, double scale,
-                                                                           double *parts, T *out) {
-    __shared__ double sums[COLUMN_WARPS][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t c0 = (int64_t)blockIdx.x * 32, c = c0 + lane;
+template <typename T, typename X, int VW>
+static __global__ void __launch_bounds__(COLUMN_THREADS) columns_kernel(const X *x, const uint8_t *mask, int64_t mask_pitch, int64_t rows,
+                                                                        int64_t rows_per_split, int64_t width, int across, double scale,
+                                                                        double *parts, T *out) {
+    __shared__ double sums[COLUMN_THREADS * VW];
+    const int down = threadIdx.x >> across, step = COLUMN_THREADS >> across;
+    const int64_t first = ((int64_t)blockIdx.x << across) * VW, c = first + (threadIdx.x & ((1 << across) - 1)) * VW;
     const int64_t end = min(rows, ((int64_t)blockIdx.y + 1) * rows_per_split);
-    LongSum<Acc<X>> sum;
-    if (c < width) {
-        for (int64_t row = (int64_t)blockIdx.y * rows_per_split + warp; row < end; row += COLUMN_ROWS) {
-            Acc<X> v[COLUMN_UNROLL];
-            uint32_t keep[COLUMN_UNROLL];
+    LongSum<Acc<X>> sum[VW];
+    // (The last rows by a loop of their own: with a test at each load the compiler has them wait for each other.)
+    const auto take = [&](int64_t row, [[maybe_unused]] auto all) {
+        Vec<X, VW> v[COLUMN_UNROLL];
+        uint32_t keep[COLUMN_UNROLL];
+#pragma unroll
+        for (int u = 0; u < COLUMN_UNROLL; ++u) {
+            const int64_t r = row + u * step;
+            v[u] = decltype(all)::value || r < end ? vec_load<X, VW>(x + r * width + c) : vec_zero<X, VW>();
+            keep[u] = 0xffu;
+        }
+        if (mask != nullptr)
 #pragma unroll
             for (int u = 0; u < COLUMN_UNROLL; ++u) {
-                const int64_t r = row + u * COLUMN_WARPS;
-                v[u] = r < end ? widen(x[r * width + c]) : Acc<X>(0);
-                // (a row of the mask is whole 64-bit words)
-                keep[u] = mask != nullptr && r < end ? *reinterpret_cast<const uint32_t *>(mask + r * mask_pitch + c0 / 8) : 0xffffffffu;
+                const int64_t r = row + u * step;
+                if (decltype(all)::value || r < end) keep[u] = mask[r * mask_pitch + c / 8] >> (c % 8);  // (VW divides 8)
             }
+        [[maybe_unused]] Acc<X> of_eight[VW];
 #pragma unroll
-            for (int u = 0; u < COLUMN_UNROLL; ++u) sum.add(keep[u] >> lane & 1 ? v[u] : Acc<X>(0));
+        for (int u = 0; u < COLUMN_UNROLL; ++u) {
+            Acc<X> y[VW];
+            widen_all<X, VW>(v[u], y);
+#pragma unroll
+            for (int k = 0; k < VW; ++k) {
+                if (!(keep[u] >> k & 1)) y[k] = Acc<X>(0);
+                if constexpr (sizeof(X) == 2) of_eight[k] = u == 0 ? y[k] : of_eight[k] + y[k];
+                else sum[k].add(y[k]);
+            }
         }
-    }
-    double s = sum.value();
-    sums[warp][lane] = s;
-    __syncthreads();
-    if (warp > 0 || c >= width) return;
+        if constexpr (sizeof(X) == 2)
 #pragma unroll
-    for (int w = 1; w < COLUMN_WARPS; ++w) s += sums[w][lane];
-    if (gridDim.y == 1) out[c] = narrow<T>((Acc<T>)(s * scale));
-    else parts[blockIdx.y * width + c] = s;
+            for (int k = 0; k < VW; ++k) sum[k].add(of_eight[k]);
+    };
+    if (c < width) {
+        int64_t row = (int64_t)blockIdx.y * rows_per_split + down;
+        for (; row + (COLUMN_UNROLL - 1) * step < end; row += step * COLUMN_UNROLL) take(row, std::true_type());
+        if (row < end) take(row, std::false_type());
+    }
+#pragma unroll
+    for (int k = 0; k < VW; ++k) sums[threadIdx.x * VW + k] = sum[k].value();
+    __syncthreads();
+    const int columns = VW << across;  // of the block, a thread each (256 at most)
+    if (threadIdx.x >= columns || first + threadIdx.x >= width) return;
+    double s = 0.0;
+    for (int d = 0; d < step; ++d) s += sums[d * columns + threadIdx.x];
+    if (gridDim.y == 1) out[first + threadIdx.x] = narrow<T>((Acc<T>)(s * scale));
+    else parts[blockIdx.y * width + first + threadIdx.x] = s;
 }
+
+// Threads for a row of the matrix, 8 to 32 (as a power of two).
+__host__ __forceinline__ int columns_across(int64_t vectors) { return vectors > 16 ? 5 : vectors > 8 ? 4 : 3; }
 
 // out[c] = scale * the sum of column c over the splits, in a fixed order.
 template <typename T>
 static int join_columns(const double *parts, int64_t splits, int64_t width, double scale, T *out, cudaStream_t stream) {
-    columns_kernel<T, double><<<(unsigned)ceil_div(width, 32), COLUMN_WARPS * 32, 0, stream>>>(parts, nullptr, 0, splits, splits, width, scale,
-                                                                                                  nullptr, out);
+    constexpr int across = 3;  // (few rows: as many of them at once as there can be)
+    columns_kernel<T, double, 1><<<(unsigned)ceil_div(width, 1 << across), COLUMN_THREADS, 0, stream>>>(
+        parts, nullptr, 0, splits, splits, width, across, scale, nullptr, out);
     CGNN_LAUNCH_CHECK();
     return CGNN_OK;
 }

@@ -70,6 +70,21 @@ def test_bias_gradient_alone_looks_at_the_incoming_one_only(dtype, rows, inner, 
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, outer", [(1, 8), (7, 16), (64, 24), (65, 136), (5000, 264), (100000, 16), (30011, 1032)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_bias_gradient_alone_of_rows_on_any_address(dtype, rows, outer, masked):
+    """Rows of whole vectors, on their boundary and an element behind it."""
+    mask, bits = random_mask(rows, outer, 2) if masked else (None, torch.ones(rows, outer, dtype=torch.bool, device="cuda"))
+    for ahead in (0, 1):
+        held = whole(rows * outer + ahead, dtype=dtype, seed=1)
+        grad = held[ahead:].view(rows, outer)
+        dbias = torch.empty(outer, dtype=dtype, device="cuda")
+        backward(None, None, mask, grad, 0.5 if masked else 0.0, dbias=dbias, inner=3)
+        want = torch.where(bits, grad, 0).double().sum(0) * (2 if masked else 1)
+        assert torch.equal(dbias, want.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [50, 40000])
 def test_gradients_with_a_frozen_weight(dtype, rows):
     x, w, b = whole(rows, 64, dtype=dtype, seed=1), whole(72, 64, dtype=dtype, seed=2), whole(72, dtype=dtype, seed=3)
