@@ -310,8 +310,8 @@ template <typename T>
 int backward(const Call &c, const void *weight, const void *mask, const void *grad, double scale, void *dx, void *dweight, void *dbias,
              void *scratch, bool tiles, cudaStream_t stream) {
     // The tensor core path sums the columns on their way to the weight's gradient.  By single elements that is a kernel of its own (sums
-    // beside the products: 200,000 x 16 -> 7 weight gradient with the bias' 103 us, without 95; apart 105 and 85; 2708 x 16 -> 7
-    // 38 and 34, apart 34 and 28).  Behind it on the stream the other gradients take the scratch anew.
+    // beside the products: 200,000 x 16 -> 7 weight gradient with the bias' 103 us, without 95; apart 92 and 86; 2708 x 16 -> 7
+    // 38 and 34, apart 35 and 28).  Behind it on the stream the other gradients take the scratch anew.
     if (dbias != nullptr && (dweight == nullptr || !tiles)) {
         const int rc = column_sums<T>(c, static_cast<const T *>(grad), static_cast<const uint8_t *>(mask), scale, static_cast<T *>(dbias),
                                       scratch, stream);

@@ -14,10 +14,11 @@
 // anew (325,557 x 256 -> 128: outputs 1.5e-7 of their size from 64 bits, the fp32 pipes' 1.8e-7).  Six products at the bf16
 // rate are 275 TFLOP/s of fp32, where the fp32 pipes have 72.
 //
-// What it takes, us: 325,557 x 256 -> 128 fp32 forward 161 (floor 78, by products and by bytes alike; the library's product on
-// the fp32 pipes 579), input gradient 190 (462), weight gradient 187 (638); 100,000 x 1024 -> 1024 forward 1253 (763).  In bf16,
-// where bytes bound it: 2.45 M x 128 -> 256 forward 390 (floor 287, the library's product without anything behind it 281), input
-// gradient 320 (294), weight gradient 456 (291, and 507 for the bias' in torch); 16,384 x 4096 -> 4096 forward 430 (333; 354).
+// What it takes, us (a few per cent more or less from one card to the next): 325,557 x 256 -> 128 fp32 forward 159 (floor 78, by
+// products and by bytes alike; the library's product and bias on the fp32 pipes 585), input gradient 177 (467), weight gradient with the
+// bias' 185 (641 and 203); 100,000 x 1024 -> 1024 forward 1232 (floor 763; 3858).  In bf16: 2.45 M x 128 -> 256, which bytes bound,
+// forward 407 (floor 287; 283), input gradient 312 (300), weight gradient with the bias' 398 (312 and 492); 16,384 x 4096 -> 4096 forward
+// 409 (floor 333; 343), input gradient 441 (331), weight gradient 517, with the bias' 900 (349 and 51).
 //
 // Operands lie in shared memory in the swizzled layout that the tensor core reads.  The streamed ones are masked and split on
 // their way there.  The weight is laid out and split once a call by a kernel of its own, as the images of shared memory
@@ -493,7 +494,7 @@ __device__ __noinline__ void read_row(float *staging, const T *row, int left) {
 // Elements of a warp's 32 x 64 of an item computed again by fp32 arithmetic and written over: where an operand is infinite, no
 // number or beyond bf16's range, its parts say nothing.  PIECE columns at once: of few rows one row after the other, its terms by all
 // lanes (one infinity in an incoming gradient makes a row of the weight's gradient infinite, of as many terms as there are
-// nodes); of more than 8 every lane its own.  (Not a function of its own: around a call the fp32 forward pass spilled registers, 191 us for 161.)
+// nodes); of more than 8 every lane its own.  (Not a function of its own: around a call the fp32 forward pass spilled registers, 191 us for 159.)
 template <typename T, int FORM>
 __device__ __forceinline__ void compute_again(const Tiles<T> &t, int item, Waits *waits) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -1118,7 +1119,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         }
     } else if (warp < MMA_WARP) {
         // ------------------------------------------------------------------ operands to shared memory
-asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGISTERS));
         const int group = (threadIdx.x - EPILOGUE_WARPS * 32) / S::MEMBERS, p = (threadIdx.x - EPILOGUE_WARPS * 32) % S::MEMBERS;
         LongSums columns;
         Producer<T, FORM, WHOLE> ahead(t, p);
@@ -1442,7 +1443,9 @@ int tiles_forward(const Call &c, const T *weight, const Epilogue<T> &epilogue, T
     return launch<T, FORWARD>(t, 1, stream);
 }
 
-// Splits of the rows of a weight gradient: what gives every multiprocessor one item, and none of fewer than four chunks.
+// Splits of the rows of a weight gradient: as many as leave each multiprocessor one item at most, and none of fewer rows than 8 chunks of
+// whole vectors (256 rows in fp32, 512 in 16 bits).  From 75 tiles up that is one split: up to 147 leave multiprocessors without an
+// item, more take turns.
 template <typename T>
 static int64_t weight_splits(int64_t rows, int64_t in, int64_t out, int64_t *rows_per_split) {
     using S = Tile<T, WEIGHT>;

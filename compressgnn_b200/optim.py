@@ -10,14 +10,14 @@ class AdamW(torch.optim.Optimizer):
 
     ``max_norm``: the gradients of all groups are clipped by their common 2-norm, which ``step`` leaves in ``grad_norm``
     (a float32 tensor on the device); the gradients themselves are not changed.
-    ``state_bits=8``: moments of tensors with ``least_8bit`` elements or more are held in 8 bits, 4 bytes a float32
+    ``state_bits=8``: moments of tensors with ``least_8bit`` elements or more are held in 8 bits, 6 bytes a float32
     parameter less to keep and 12 less to move a step; smaller ones, and float64, keep theirs in full.  ``seed`` is the key
     of their stochastic rounding.
 
     The groups hold ``max_norm`` and ``seed`` as they hold the rest, so a schedule may set them and a loaded state brings its own; but
     there is one of each, and groups that differ in them are refused.
 
-    ``lr`` may be a CUDA tensor of one float32.  The steps taken are counted on the device, so a step can be captured into
+    Parameters are contiguous.  ``lr`` may be a CUDA tensor of one float32.  The steps taken are counted on the device, so a step can be captured into
     a CUDA graph once the state exists (after one step outside of the capture)."""
 
     grad_norm = None
