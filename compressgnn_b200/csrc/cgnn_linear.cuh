@@ -81,7 +81,7 @@ struct LongSum {
         low += (high - (s - part)) + (x - part);
         high = s;
     }
-    // (of an infinity nothing is lost, but the second number says NaN)
+    // (Of an infinity nothing is lost, but the second number says NaN.  A sum beyond fp32's range on the way is infinite, as in fp32.)
     __device__ __forceinline__ double value() const { return isfinite(high) ? (double)high + (double)low : (double)high; }
 };
 template <>

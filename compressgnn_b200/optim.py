@@ -58,7 +58,7 @@ class AdamW(torch.optim.Optimizer):
                     state[name] = torch.zeros(p.shape, dtype=wide, device=p.device)
 
     def add_param_group(self, group):
-        for name in self._COMMON:
+        for name in self._COMMON if isinstance(group, dict) else ():  # (the base class refuses others)
             common = self.param_groups[0][name] if self.param_groups else self.defaults[name]
             if group.setdefault(name, common) != common:
                 raise ValueError(f"AdamW: {name} is common to all groups")
